@@ -1,0 +1,576 @@
+// Causal grouped-query attention over the 8-bit cache (quant_cache.cu): bfloat16 queries, keys and values as whole numbers with one float32
+// scale a (token, kv head), head size HEAD_DIM (a compile-time multiple of 16 up to 256; the library is built per head size).
+//
+//   score of query i and key j = scale * ks_j * sum_c q_ic kc_jc,   out_ic = sum_j (p_ij vs_j) vc_jc / sum_j p_ij
+//
+// The whole numbers are exact in bfloat16, so the products run on bfloat16 tensor cores (mma.sync m16n8k16, float32 sums) as if the cache
+// were bfloat16, and a key's scale is multiplied to its scores, a value's to its probabilities, in float32; maxima, sums and outputs are
+// float32.  One rounding comes in: p vs to bfloat16 (8 bits; each weight is off by at most 2^-8 of itself, as in the attention over a
+// bfloat16 cache) because the other operand is bfloat16.
+//
+// The products are turned around: S^T = K Q^T and O^T = V^T P^T, keys and channels in the 16 rows of an instruction, queries in its 8
+// columns.  A decoding request has the G query heads of a kv head as its queries, mostly 4 to 8: so an instruction is full, and an element of
+// the cache is widened once for all of them.
+//   K: ldmatrix on bytes gives a lane four neighbouring channels of one key, which are taken as k indices 2q, 2q + 1, 2q + 8, 2q + 9 (a sum does
+//      not mind the order of its terms; the queries' fragments take the same order);
+//   V: ldmatrix.trans on bytes gives a lane two neighbouring channels of two keys; the even channel goes to row r of the instruction, the odd
+//      one to row r + 8, so a lane ends with two neighbouring output channels of a query;
+//   P: the scores' fragment, rounded, is turned by movmatrix.
+// Rows of shared memory are an odd number of 16-byte units long, so the eight rows of an ldmatrix lie in different banks.
+#include "common.cuh"
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<multiple of 16>"
+#endif
+
+using bf16 = __nv_bfloat16;
+
+namespace {
+
+constexpr int HD = HEAD_DIM;
+static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 in [16, 256]");
+constexpr int CHUNKS = HD / 16;                    // 16-byte units of a row
+constexpr int STRIDE = (CHUNKS | 1) * 16;          // bytes between rows of shared memory
+constexpr int KEYS = 16;                           // keys that a warp works on at a time
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int TILE = WARPS * KEYS;                 // keys of a block's step
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Params {
+    const bf16* q; bf16* out;
+    const int8_t* k; const int8_t* v; const float* k_scale; const float* v_scale;
+    const int* cu_q; const int* q_start; const int* kv_len; const int* table;
+    const float* sink;              // float32 [nh] or null: one more term exp(sink) of a row's denominator
+    float* part_o; float* part_ml;  // results of key slices: [request][kv head][slice][16][HD] and [..][2]
+    int max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests;
+    int per, slices;                // key slices: tiles of each, most of them that any request has
+    float scale_log2;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+    const int n = there ? 16 : 0;   // 0: nothing is read, zeros are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+    const int n = there ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// Two signed bytes of r (chosen by SEL) as bfloat16.  With u the byte's low seven bits, 0x4300 | u is 128 + u, and 0x4300 | (byte & 128) is 128
+// or, with the sign bit in the exponent's lowest place, 256: their difference is the byte's value.
+template <int SEL>
+__device__ __forceinline__ uint32_t widen2(uint32_t r) {
+    const uint32_t w = __byte_perm(r, 0x43434343u, SEL);
+    const uint32_t t = w & 0xff7fff7fu, c = w & 0xff80ff80u;
+    uint32_t d;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(t), "r"(c));
+    return d;
+}
+
+// What a warp keeps of 8 * NB queries: of block nb a lane holds columns 2 (lane & 3) and the next.
+template <int NB>
+struct Queries {
+    uint32_t qf[CHUNKS][NB][2];
+    float o[CHUNKS][NB][4];      // channels 16 mb + 2 (lane / 4) (entries 0, 1) and the next (2, 3) of the lane's two queries
+    float m[NB][2], l[NB][2];    // l: this lane's keys only
+    int pos[NB][2], lo[NB][2];   // position and first visible key; pos < 0: no such query
+};
+
+// Queries row0 .. of the stacked rows (row = token * G + head of the group) of a request whose first token is `tok`.
+template <int NB>
+__device__ __forceinline__ void load_queries(const Params& p, Queries<NB>& s, int tok, int g, int row0, int n_rows, int q_pos0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int row = row0 + 8 * nb + (lane >> 2);
+        const int t = row / p.G;
+        const bf16* src = p.q + ((size_t)(tok + t) * p.nh + g * p.G + (row - t * p.G)) * HD + 4 * (lane & 3);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const uint2 v = row < n_rows ? *reinterpret_cast<const uint2*>(src + 16 * c) : make_uint2(0, 0);
+            s.qf[c][nb][0] = v.x; s.qf[c][nb][1] = v.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int col = row0 + 8 * nb + 2 * (lane & 3) + e;
+            s.pos[nb][e] = col < n_rows ? q_pos0 + col / p.G : -1;
+            s.lo[nb][e] = col < n_rows ? bw::first_visible(s.pos[nb][e], p.window, p.chunk) : 0;
+            s.m[nb][e] = -INFINITY; s.l[nb][e] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) s.o[c][nb][0] = s.o[c][nb][1] = s.o[c][nb][2] = s.o[c][nb][3] = 0.f;
+    }
+}
+
+// Sixteen keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page.
+template <int NB>
+__device__ __forceinline__ void sixteen_keys(Queries<NB>& s, uint32_t k_rows, uint32_t v_rows, const float* ks, const float* vs, int key0,
+                                             unsigned there, bool need_mask, float scale_log2) {
+    const int lane = threadIdx.x & 31, r = lane >> 2;
+    // matrices of an ldmatrix: keys 0-7 and 8-15 of one 16-byte unit, then of the next
+    const uint32_t at = (uint32_t)(((lane & 7) + 8 * ((lane >> 3) & 1)) * STRIDE);
+    float sc[NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c += 2) {
+        uint32_t f[4];
+        // (an odd last unit: its second pair of matrices reads the first's again)
+        ldsm4(k_rows + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (c + i >= CHUNKS) break;
+            const uint32_t a[4] = {widen2<0x4140>(f[2 * i]), widen2<0x4140>(f[2 * i + 1]), widen2<0x4342>(f[2 * i]), widen2<0x4342>(f[2 * i + 1])};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma(sc[nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
+        }
+    }
+    const float k0 = ks[r] * scale_log2, k1 = ks[r + 8] * scale_log2, v0 = vs[r], v1 = vs[r + 8];
+    uint32_t pf[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        float t[4] = {sc[nb][0] * k0, sc[nb][1] * k0, sc[nb][2] * k1, sc[nb][3] * k1};
+        bool seen[4] = {true, true, true, true};
+        if (need_mask) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int kp = key0 + r + 8 * (i >> 1), e = i & 1;
+                seen[i] = kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> (r + 8 * (i >> 1)) & 1);
+                if (!seen[i]) t[i] = -INFINITY;
+            }
+        }
+        float mx[2] = {fmaxf(t[0], t[2]), fmaxf(t[1], t[3])}, corr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+            const float m_new = fmaxf(s.m[nb][e], mx[e]);
+            mx[e] = m_new == -INFINITY ? 0.f : m_new;
+            corr[e] = exp2f(s.m[nb][e] - mx[e]);        // nothing seen so far: 0
+            s.m[nb][e] = m_new;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = exp2f(t[i] - mx[i & 1]);
+        s.l[nb][0] = s.l[nb][0] * corr[0] + (t[0] + t[2]);
+        s.l[nb][1] = s.l[nb][1] * corr[1] + (t[1] + t[3]);
+        // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
+        const float w[4] = {seen[0] ? t[0] * v0 : 0.f, seen[1] ? t[1] * v0 : 0.f, seen[2] ? t[2] * v1 : 0.f, seen[3] ? t[3] * v1 : 0.f};
+        pf[nb][0] = turn8x8(bw::pack_bf16x2(w[0], w[1]));
+        pf[nb][1] = turn8x8(bw::pack_bf16x2(w[2], w[3]));
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            s.o[c][nb][0] *= corr[0]; s.o[c][nb][1] *= corr[1]; s.o[c][nb][2] *= corr[0]; s.o[c][nb][3] *= corr[1];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c += 2) {
+        uint32_t f[4];
+        ldsm4_t(v_rows + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (c + i >= CHUNKS) break;
+            const uint32_t a[4] = {widen2<0x4240>(f[2 * i]), widen2<0x4341>(f[2 * i]), widen2<0x4240>(f[2 * i + 1]), widen2<0x4341>(f[2 * i + 1])};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, pf[nb][0], pf[nb][1]);
+        }
+    }
+}
+
+// The row (page, kv head, place) that holds a key; -1: none (behind the request's last token, or its page is not held).
+__device__ __forceinline__ int key_row(const Params& p, const int* bt, int g, int key, int kv_len) {
+    if (key >= kv_len) return -1;
+    const int blk = key / p.page_size;
+    if (blk >= p.max_blocks) return -1;
+    const int page = bt[blk];
+    return page >= 0 && page < p.num_pages ? (page * p.nkv + g) * p.page_size + (key - blk * p.page_size) : -1;
+}
+
+constexpr int STAGE = 2 * KEYS * STRIDE + 2 * KEYS * 4;     // K, V, their scales
+// Sixteen keys into a stage, by one warp; `row`: key_row of key lane & 15 in every lane.
+__device__ __forceinline__ void fetch(const Params& p, uint8_t* stage, int row) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t k_to = smem_u32(stage), v_to = k_to + KEYS * STRIDE;
+#pragma unroll
+    for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
+        const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
+        const int rw = __shfl_sync(0xffffffffu, row, key & 15);
+        if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
+        const size_t off = rw >= 0 ? (size_t)rw * HD + 16 * c : 0;
+        cp_async16(k_to + key * STRIDE + 16 * c, p.k + off, rw >= 0);
+        cp_async16(v_to + key * STRIDE + 16 * c, p.v + off, rw >= 0);
+    }
+    cp_async4(k_to + 2 * KEYS * STRIDE + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + (row >= 0 ? row : 0), row >= 0);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few queries
+// All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
+// with a ring of its own, and are joined at the end.  Slices are equally long for every request; how many of them a request has follows
+// from its length on the device, so the same launch serves a captured step whatever the lengths become.
+constexpr int STAGES = 4;
+constexpr int SMEM_RING = WARPS * STAGES * STAGE;
+constexpr int JOIN_LD = HD + 8;
+constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD) * 4;
+constexpr int SMEM_KEYS = SMEM_RING > SMEM_JOIN ? SMEM_RING : SMEM_JOIN;
+
+struct Walk { int first, tiles, per, live; };   // in tiles of TILE keys: where it begins, how many, of a slice; slices that have any
+__device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last) {
+    Walk w;
+    w.first = bw::first_visible(q_pos0, p.window, p.chunk) / TILE;
+    w.tiles = last / TILE + 1 - w.first;
+    // (a request that is longer than the plan was made for gets longer slices, not more of them)
+    w.per = max(p.per, (w.tiles + p.slices - 1) / p.slices);
+    w.live = (w.tiles + w.per - 1) / w.per;
+    return w;
+}
+
+__device__ __forceinline__ void write_row(const Params& p, size_t token, int head, int c, float4 v, float L) {
+    // (a row that sees nothing is zeros; a sum that is no number stays one)
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (L == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<uint2*>(p.out + (token * p.nh + head) * HD + c) =
+        make_uint2(bw::pack_bf16x2(v.x * inv, v.y * inv), bw::pack_bf16x2(v.z * inv, v.w * inv));
+}
+__device__ __forceinline__ float sink_term(const Params& p, int head, float M) { return p.sink ? exp2f(p.sink[head] * LOG2E - M) : 0.f; }
+
+template <int NB>
+__global__ void __launch_bounds__(THREADS)
+few_kernel(Params p) {
+    BW_PDL_TRIGGER();
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int slice = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    BW_PDL_WAIT();
+    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
+    if (n_tok <= 0 || n_rows > 8 * NB || (NB == 2 && n_rows <= 8)) return;
+    const int q_pos0 = p.q_start[r], last = q_pos0 + n_tok - 1, kv_len = p.kv_len[r];
+    const Walk walk = walk_of(p, q_pos0, last);
+    if (slice >= walk.live) return;
+    const int t0 = walk.first + slice * walk.per, t1 = min(walk.first + walk.tiles, t0 + walk.per);
+    const int* bt = p.table + (size_t)r * p.max_blocks;
+    uint8_t* ring = smem + warp * STAGES * STAGE;
+    // the row of this lane's key of the next tile that is fetched: looked up a tile ahead of its use
+    int next = key_row(p, bt, g, t0 * TILE + warp * KEYS + (lane & 15), kv_len);
+    unsigned there[STAGES];
+    auto feed = [&](int t, int st) {
+        if (t < t1) {
+            there[st] = __ballot_sync(0xffffffffu, next >= 0) & 0xffffu;
+            fetch(p, ring + st * STAGE, next);
+            next = t + 1 < t1 ? key_row(p, bt, g, (t + 1) * TILE + warp * KEYS + (lane & 15), kv_len) : -1;
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st) feed(t0 + st, st);
+    Queries<NB> s;
+    load_queries<NB>(p, s, tok, g, 0, n_rows, q_pos0);
+    const int see_all = bw::first_visible(last, p.window, p.chunk);      // from here on every query of the segment sees keys up to q_pos0
+    for (int t = t0; t < t1; t += STAGES) {
+#pragma unroll
+        for (int st = 0; st < STAGES; ++st) {
+            if (t + st >= t1) break;
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();
+            feed(t + st + STAGES - 1, (st + STAGES - 1) % STAGES);
+            const uint8_t* at = ring + st * STAGE;
+            const int key0 = (t + st) * TILE + warp * KEYS;
+            if (key0 <= last) {
+                const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
+                const bool need_mask = there[st] != 0xffffu || key0 + KEYS - 1 > q_pos0 || key0 < see_all;
+                sixteen_keys<NB>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, there[st], need_mask, p.scale_log2);
+            }
+            __syncwarp();
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    // the warps' shares joined through shared memory (over the rings)
+    float* ms = reinterpret_cast<float*>(smem);
+    float* ls = ms + WARPS * 16;
+    float* os = ls + WARPS * 16;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float l = s.l[nb][e];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int col = 8 * nb + 2 * (lane & 3) + e;
+            if ((lane >> 2) == 0) { ms[warp * 16 + col] = s.m[nb][e]; ls[warp * 16 + col] = l; }
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+                *reinterpret_cast<float2*>(os + (warp * 16 + col) * JOIN_LD + 16 * c + 2 * (lane >> 2)) = make_float2(s.o[c][nb][e], s.o[c][nb][2 + e]);
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < n_rows * (HD / 4); idx += THREADS) {
+        const int row = idx / (HD / 4), c = (idx - row * (HD / 4)) * 4;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, ms[w * 16 + row]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float mw = ms[w * 16 + row], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+            const float4 v = *reinterpret_cast<const float4*>(os + (w * 16 + row) * JOIN_LD + c);
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+            L += ls[w * 16 + row] * f;
+        }
+        if (walk.live == 1) {
+            const int t = row / p.G, head = g * p.G + row - t * p.G;
+            write_row(p, (size_t)(tok + t), head, c, acc, L + sink_term(p, head, M));
+        } else {
+            const size_t at = (((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
+            *reinterpret_cast<float4*>(p.part_o + at * HD + c) = acc;
+            if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+        }
+    }
+}
+
+// Joins the slices of every request that has more than one: a block per (row, kv head, request), groups of HD / 4 threads that take every
+// so many-th slice, then the groups' sums in order: the same sum whatever ran beside it.
+constexpr int QUADS = HD / 4;
+constexpr int JOIN_GROUPS = 256 / QUADS;
+__global__ void __launch_bounds__(256)
+join_kernel(Params p) {
+    BW_PDL_TRIGGER();
+    BW_PDL_WAIT();
+    const int row = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
+    if (n_tok <= 0 || n_rows > 16 || row >= n_rows) return;
+    const int q_pos0 = p.q_start[r];
+    const int live = walk_of(p, q_pos0, q_pos0 + n_tok - 1).live;
+    if (live <= 1) return;
+    __shared__ float4 red[JOIN_GROUPS][QUADS];
+    __shared__ float red_l[JOIN_GROUPS];
+    const size_t base = ((size_t)r * p.nkv + g) * p.slices * 16 + row;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+    float M = -INFINITY;
+    for (int i = 0; i < live; ++i) M = fmaxf(M, ml[base + (size_t)i * 16].x);
+    const int group = threadIdx.x / QUADS, quad = threadIdx.x - group * QUADS;
+    if (group < JOIN_GROUPS) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+        for (int i = group; i < live; i += JOIN_GROUPS) {
+            const float2 x = ml[base + (size_t)i * 16];
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+            const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + (size_t)i * 16) * HD)[quad];
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+            L += x.y * f;
+        }
+        red[group][quad] = acc;
+        if (quad == 0) red_l[group] = L;
+    }
+    __syncthreads();
+    if (threadIdx.x < QUADS) {
+        float4 acc = red[0][threadIdx.x];
+        float L = red_l[0];
+        for (int i = 1; i < JOIN_GROUPS; ++i) {
+            const float4 v = red[i][threadIdx.x];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            L += red_l[i];
+        }
+        const int t = row / p.G, head = g * p.G + row - t * p.G;
+        write_row(p, (size_t)(tok + t), head, 4 * threadIdx.x, acc, L + sink_term(p, head, M));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many queries
+// Portions of prompts: 64 rows of one (request, kv head) a block, sixteen a warp; the warps share the keys that the block fetches, 64 at a time
+// in a ring, and walk them up to the causal diagonal.
+constexpr int MANY = 16;                                   // requests with many rows that one launch takes
+struct Portions { int n; int request[MANY]; int first[MANY + 1]; };   // first: the block index of each one's first 64 rows
+constexpr int ROWS = 16 * WARPS;
+constexpr int RING = 2;
+constexpr int SMEM_MANY = RING * WARPS * STAGE + 64;
+
+__global__ void __launch_bounds__(THREADS)
+many_kernel(Params p, Portions work) {
+    BW_PDL_TRIGGER();
+    extern __shared__ __align__(16) uint8_t smem[];
+    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.x;
+    int i = 0;
+    while (i + 1 < work.n && (int)blockIdx.y >= work.first[i + 1]) ++i;
+    BW_PDL_WAIT();
+    const int r = work.request[i];
+    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, all_rows = n_tok * p.G;
+    // the latest rows first: they have the most keys
+    const int row0 = (work.first[i + 1] - 1 - (int)blockIdx.y) * ROWS;
+    if (row0 >= all_rows) return;
+    const int q_pos0 = p.q_start[r], kv_len = p.kv_len[r];
+    const int* bt = p.table + (size_t)r * p.max_blocks;
+    const int mine = row0 + 16 * warp, last_row = min(all_rows, row0 + ROWS) - 1;
+    const int first_pos = q_pos0 + row0 / p.G, last_pos = q_pos0 + last_row / p.G;
+    const int t0 = bw::first_visible(first_pos, p.window, p.chunk) / TILE, t1 = last_pos / TILE + 1;
+    auto feed = [&](int t) {
+        if (t < t1) {
+            const int st = (t - t0) % RING;
+            const int row = key_row(p, bt, g, t * TILE + warp * KEYS + (lane & 15), kv_len);
+            const unsigned b = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            if (lane == 0) there[st * WARPS + warp] = b;
+            fetch(p, smem + (st * WARPS + warp) * STAGE, row);
+        }
+        cp_async_commit();
+    };
+    feed(t0);
+    Queries<2> s;
+    load_queries<2>(p, s, tok, g, mine, all_rows, q_pos0);
+    const int my_first = q_pos0 + mine / p.G, my_last = q_pos0 + min(last_row, mine + 15) / p.G;
+    const int see_all = bw::first_visible(my_last, p.window, p.chunk);
+    for (int t = t0; t < t1; ++t) {
+        feed(t + 1);
+        cp_async_wait<1>();
+        __syncthreads();
+        const int st = (t - t0) % RING;
+        if (mine <= last_row) {
+            for (int w = 0; w < WARPS; ++w) {
+                const int key0 = t * TILE + w * KEYS;
+                if (key0 > my_last) break;
+                const uint8_t* at = smem + (st * WARPS + w) * STAGE;
+                const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
+                const unsigned ok = there[st * WARPS + w];
+                const bool need_mask = ok != 0xffffu || key0 + KEYS - 1 > my_first || key0 < see_all;
+                sixteen_keys<2>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask, p.scale_log2);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float l = s.l[nb][e];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int row = mine + 8 * nb + 2 * (lane & 3) + e;
+            if (row > last_row) continue;
+            const int t = row / p.G, head = g * p.G + row - t * p.G;
+            l += sink_term(p, head, s.m[nb][e]);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            bf16* dst = p.out + ((size_t)(tok + t) * p.nh + head) * HD + 2 * (lane >> 2);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+                *reinterpret_cast<uint32_t*>(dst + 16 * c) = bw::pack_bf16x2(s.o[c][nb][e] * inv, s.o[c][nb][2 + e] * inv);
+        }
+    }
+}
+
+}  // namespace
+
+// Key slices of the requests with at most 16 rows: how many tiles of TILE keys a slice has (*per) so that the slices of all requests fill
+// the GPU about once, and the most slices of any request (the return value; 0: there is no such request).  Lengths are the host's: of the
+// step, or, for a step that is captured, the longest that may come (`bound` > 0: for every request).
+BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound,
+                                   int* per) {
+    if (requests < 0 || G <= 0 || nkv <= 0 || !per) return BW_ERR_BAD_ARG;
+    long long most = 0, total = 0;
+    auto tiles_of = [&](int r) -> long long {
+        if (q_len[r] <= 0 || (long long)q_len[r] * G > 16) return 0;
+        const long long first = bound > 0 ? 0 : bw::first_visible(q_start[r], window, chunk), end = bound > 0 ? bound : (long long)q_start[r] + q_len[r];
+        long long n = (end - 1) / TILE + 1 - first / TILE;
+        if (bound > 0) {      // wherever the token stands, it sees no more than this
+            long long span = bound;
+            if (window > 0 && window + q_len[r] < span) span = window + q_len[r];
+            if (chunk > 0 && chunk + q_len[r] < span) span = chunk + q_len[r];
+            const long long m = (span + TILE - 1) / TILE + 1;
+            if (m < n) n = m;
+        }
+        return n;
+    };
+    for (int r = 0; r < requests; ++r) {
+        const long long n = tiles_of(r);
+        total += n;
+        if (n > most) most = n;
+    }
+    *per = 1;
+    if (most == 0) return 0;
+    const long long room = 2LL * bw::num_sms();          // blocks that run at once
+    long long lo = 1, hi = most;
+    while (lo < hi) {
+        const long long mid = (lo + hi) / 2;
+        long long blocks = 0;
+        for (int r = 0; r < requests; ++r) blocks += (tiles_of(r) + mid - 1) / mid;
+        if (blocks * nkv <= room) hi = mid; else lo = mid + 1;
+    }
+    *per = (int)lo;
+    return (int)((most + lo - 1) / lo);
+}
+
+// q, out: bfloat16 [tokens][nh][HD]; lengths on the host (q_len, h_q_start) as in bw_attention_q8_plan, per and slices as it gave them; part_o,
+// part_ml: room for requests * nkv * slices * 16 rows of HD and of 2 floats, where slices > 1.
+BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
+                              const int* cu_q, const int* q_start, const int* kv_len, const int* table, int max_blocks, const int* h_q_len,
+                              int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, float scale,
+                              const float* sink, int per, int slices, float* part_o, float* part_ml, void* stream) {
+    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || per <= 0) return BW_ERR_BAD_ARG;
+    if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v) & 15) || (slices > 1 && (!part_o || !part_ml))) return BW_ERR_BAD_ARG;
+    if ((long long)num_pages * nkv * page_size > 0x7fffffffll || nkv > 65535 || requests > 65535) return BW_ERR_UNSUPPORTED;
+    const int G = nh / nkv;
+    Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, part_o, part_ml,
+             max_blocks, nh, nkv, G, page_size, num_pages, window > 0 ? window : 0, chunk > 0 ? chunk : 0, requests, per, slices, scale * LOG2E};
+    cudaStream_t s = (cudaStream_t)stream;
+    static bool few1_done[bw::MAX_DEVICES], few2_done[bw::MAX_DEVICES], many_done[bw::MAX_DEVICES];
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<1>, SMEM_KEYS, few1_done); e != cudaSuccess) return (int)e;
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<2>, SMEM_KEYS, few2_done); e != cudaSuccess) return (int)e;
+    if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
+    Portions work{};
+    int most_rows = 0;
+    bool few1 = false, few2 = false;
+    auto flush = [&]() -> int {
+        if (!work.n) return 0;
+        if (work.first[work.n] > 65535) return BW_ERR_UNSUPPORTED;
+        bw::launch(many_kernel, dim3((unsigned)nkv, (unsigned)work.first[work.n]), dim3(THREADS), SMEM_MANY, s, p, work);
+        BW_LAUNCH_CHECK();
+        work = Portions{};
+        return 0;
+    };
+    for (int r = 0; r < requests; ++r) {
+        const long long rows = (long long)h_q_len[r] * G;
+        if (rows <= 0) continue;
+        if (rows <= 16) {
+            (rows <= 8 ? few1 : few2) = true;
+            if (rows > most_rows) most_rows = (int)rows;
+            continue;
+        }
+        if (rows > 0x7fffffffll / 2) return BW_ERR_UNSUPPORTED;
+        work.request[work.n] = r;
+        work.first[work.n + 1] = work.first[work.n] + (int)((rows + ROWS - 1) / ROWS);
+        if (++work.n == MANY) if (const int e = flush()) return e;
+    }
+    if (const int e = flush()) return e;
+    if (!most_rows) return 0;
+    if (slices < 1) return BW_ERR_BAD_ARG;
+    const dim3 grid((unsigned)slices, (unsigned)nkv, (unsigned)requests);
+    if (few1) { bw::launch(few_kernel<1>, grid, dim3(THREADS), SMEM_KEYS, s, p); BW_LAUNCH_CHECK(); }
+    if (few2) { bw::launch(few_kernel<2>, grid, dim3(THREADS), SMEM_KEYS, s, p); BW_LAUNCH_CHECK(); }
+    if (slices > 1) {
+        bw::launch(join_kernel, dim3((unsigned)most_rows, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
+        BW_LAUNCH_CHECK();
+    }
+    return 0;
+}

@@ -1381,6 +1381,176 @@ def _loaded_libs():
 
 # ------------------------------------------------------------------ norm after a sublayer, stream sums
 
+# ------------------------------------------------------------------ the 8-bit cache of keys and values
+
+class QuantPages:
+    """Pages of keys and values held in 8 bits: ``k`` and ``v`` int8 [num_pages, nkv, page_size, head_dim], whole numbers of -127 to 127, and
+    ``k_scale``, ``v_scale`` float32 [num_pages, nkv, page_size], one scale per (token, kv head): a channel's value is number * scale.
+    Views of a pool are fine as long as each is contiguous."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @property
+    def shape(self):
+        return self.k.shape
+
+
+QUANT_MAX_HEAD_DIM = 256
+
+
+def check_quant_supported(head_dim: int, group: int = 1) -> None:
+    """Raises for a geometry that the kernels of the 8-bit cache do not take (known when a model is built)."""
+    if head_dim <= 0 or head_dim % 16 or head_dim > QUANT_MAX_HEAD_DIM:
+        raise KernelError(f"8-bit cache: head sizes in steps of 16 up to {QUANT_MAX_HEAD_DIM}, got {head_dim}")
+    if group > MAX_GROUP_BF16:
+        raise KernelError(f"8-bit cache: {group} query heads per kv head exceed the attention kernels' limit of {MAX_GROUP_BF16}")
+
+
+def _quant_pages(pages: QuantPages, block_table: torch.Tensor, what: str):
+    if pages.k.dim() != 4 or pages.v.shape != pages.k.shape:
+        raise KernelError(f"{what}: keys and values must be [num_pages, nkv, page_size, head_dim]")
+    num_pages, nkv, page_size, hd = pages.k.shape
+    if pages.k_scale.shape != (num_pages, nkv, page_size) or pages.v_scale.shape != pages.k_scale.shape:
+        raise KernelError(f"{what}: scales must be [num_pages, nkv, page_size]")
+    _dev(pages.k, "k", torch.int8); _dev(pages.v, "v", torch.int8)
+    _dev(pages.k_scale, "k_scale", torch.float32); _dev(pages.v_scale, "v_scale", torch.float32)
+    _dev(block_table, "block_table", torch.int32)
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be [requests, blocks]")
+    check_quant_supported(hd)
+    return num_pages, nkv, page_size, hd
+
+
+def _same_device(what: str, *tensors) -> None:
+    # a kernel runs on the current device, on its current stream: operands elsewhere would be read over the bus or not at all
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{here}")
+
+
+_QUANT_APPEND_ARGS = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_int, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_void_p]
+_QUANT_READ_ARGS = [c_void_p] * 9 + [c_int] * 8 + [c_void_p]
+
+
+def quant_append(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch.Tensor, block_table: torch.Tensor, pages: QuantPages,
+                 nh: int, table: Optional[torch.Tensor] = None, paired: bool = False, append: bool = True) -> torch.Tensor:
+    """:func:`rope_append` for an 8-bit cache: rotates the q and k heads of ``qkv`` [T, (nh + 2 nkv) * head_dim] (float32 or bfloat16; or float32 planes
+    [S, T, width] of :func:`gemm_tc_planes`, added while they are read) by ``table`` (float32 [T, rotary_dim] of :func:`rope_table`; None: no
+    rotation), returns q [T, nh * head_dim] in bfloat16 and writes the rotated keys and the values to the pages of the tokens'
+    positions.  A row (head_dim channels of one token and kv head) with largest magnitude a gets the scale a / 127 and the numbers
+    x * (127 / a), rounded to nearest; one with a below 2^-110 becomes zeros; one that holds an infinity or NaN reads back as NaN.  A token
+    whose position has no page (-1 in the block table, or beyond it) is not written.  Two tokens of one call must not have the
+    same request and position.  ``paired``: the q and k heads are in the order of :func:`rotary_row_order`."""
+    n_planes, plane_stride = 1, 0
+    if qkv.dim() == 3:
+        if qkv.dtype != torch.float32 or not qkv.shape[0]:
+            raise KernelError("quant_append: planes are float32 [S, T, width]")
+        n_planes, plane_stride = qkv.shape[0], qkv.stride(0)
+        qkv = qkv[0]
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_append")
+    _dev(qkv, "qkv"); _dev(positions, "positions", torch.int32); _dev(req_of_token, "req_of_token", torch.int32)
+    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+        raise KernelError(f"quant_append: qkv must be [T, (nh + 2 nkv) * head_dim = {(nh + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
+    T = qkv.shape[0]
+    if positions.numel() != T or req_of_token.numel() != T:
+        raise KernelError("quant_append: one position and one request per token")
+    rd = 0
+    if table is not None:
+        _dev(table, "table", torch.float32)
+        if table.dim() != 2 or table.shape[0] != T or table.shape[1] % 2 or table.shape[1] > hd:
+            raise KernelError("quant_append: the cos/sin table must be [T, rotary_dim], rotary_dim even and at most the head size")
+        rd = table.shape[1]
+    _same_device("quant_append", qkv, positions, req_of_token, block_table, table, pages.k, pages.v, pages.k_scale, pages.v_scale)
+    q = torch.empty((T, nh * hd), dtype=torch.bfloat16, device=qkv.device)
+    if T == 0:
+        return q
+    fn = _fn("quant_cache", "bw_quant_append", _QUANT_APPEND_ARGS)
+    _check(fn(_ptr(qkv), _code(qkv, "qkv"), n_planes, plane_stride, _ptr(table) if rd else None, rd, int(paired), _ptr(q), nh, _ptr(pages.k),
+              _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(positions), _ptr(req_of_token), _ptr(block_table), T,
+              block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, hd, int(append), _stream()), "quant_append")
+    return q
+
+
+def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.Tensor, block_table: torch.Tensor,
+               out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values that an 8-bit cache holds, [n, nkv, head_dim] each in ``out_dtype`` (bfloat16 or float32): row i is position
+    ``positions[i]`` of request ``req_of_token[i]`` (a row of the block table).  Zeros where no page is held."""
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_read")
+    _dev(positions, "positions", torch.int32); _dev(req_of_token, "req_of_token", torch.int32)
+    n = positions.numel()
+    if req_of_token.numel() != n:
+        raise KernelError("quant_read: one request per position")
+    _same_device("quant_read", positions, req_of_token, block_table, pages.k, pages.v, pages.k_scale, pages.v_scale)
+    k = torch.empty((n, nkv, hd), dtype=out_dtype, device=pages.k.device)
+    v = torch.empty_like(k)
+    code = _code(k, "out")
+    if n == 0:
+        return k, v
+    fn = _fn("quant_cache", "bw_quant_read", _QUANT_READ_ARGS)
+    _check(fn(_ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(positions), _ptr(req_of_token), _ptr(block_table),
+              _ptr(k), _ptr(v), code, n, block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, hd, _stream()), "quant_read")
+    return k, v
+
+
+_ATTN_Q8_PLAN_ARGS = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]
+_ATTN_Q8_ARGS = [c_void_p] * 10 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]
+
+
+def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torch.Tensor, nh: int, scale: float, window: Optional[int] = None,
+                    chunk: Optional[int] = None, sink: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_attention` over an 8-bit cache (which already holds this step's keys and values): bfloat16 queries [T, nh * head_dim],
+    bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
+    held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator."""
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_attention")
+    _dev(q, "q", torch.bfloat16)
+    if nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
+        raise KernelError("quant_attention: q must be [T, nh * head_dim] with nh a multiple of the kv heads")
+    G, R = nh // nkv, batch.R
+    check_quant_supported(hd, G)
+    _check_sink(sink, nh)
+    cu_q, q_start, kv_len = (_dev(t, n, torch.int32) for t, n in ((batch.cu_q, "cu_q"), (batch.q_start, "q_start"), (batch.kv_len, "kv_len")))
+    if q.shape[0] != batch.T or block_table.shape[0] < R or cu_q.numel() < R + 1 or q_start.numel() < R or kv_len.numel() < R \
+            or len(batch.h_q_len) < R or len(batch.h_q_start) < R or sum(batch.h_q_len[:R]) != batch.T:
+        raise KernelError("quant_attention: the batch's segments, the queries and the block table do not fit together")
+    _same_device("quant_attention", q, cu_q, q_start, kv_len, block_table, sink, pages.k, pages.v, pages.k_scale, pages.v_scale)
+    out = torch.empty_like(q)
+    if batch.T == 0:
+        return out
+    window, chunk = int(window or 0), int(chunk or 0)
+    h_len, h_start = (c_int * R)(*batch.h_q_len[:R]), (c_int * R)(*batch.h_q_start[:R])
+    macros = attention_q8_macros(hd)
+    per = c_int(1)
+    slices = _fn("attention_q8", "bw_attention_q8_plan", _ATTN_Q8_PLAN_ARGS, macros=macros)(
+        h_len, h_start, R, G, nkv, window, chunk, int(batch.static_bound or 0), ctypes.byref(per))
+    if slices < 0:
+        _check(slices, "quant_attention")
+    part_o = part_ml = None
+    if slices > 1:
+        rows = R * nkv * slices * 16
+        part_o = torch.empty((rows, hd), dtype=torch.float32, device=q.device)
+        part_ml = torch.empty((rows, 2), dtype=torch.float32, device=q.device)
+    fn = _fn("attention_q8", "bw_attention_q8", _ATTN_Q8_ARGS, macros=macros)
+    _check(fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start),
+              _ptr(kv_len), _ptr(block_table), block_table.shape[1], h_len, R, nh, nkv, page_size, num_pages, window, chunk, float(scale),
+              _ptr(sink), per.value, slices, _ptr(part_o), _ptr(part_ml), _stream()), "quant_attention")
+    return out
+
+
+_ATTN_Q8_MACROS = {}
+
+
+def attention_q8_macros(hd: int) -> dict:
+    """The build of the attention over an 8-bit cache for this head size."""
+    macros = _ATTN_Q8_MACROS.get(hd)
+    if macros is None:
+        macros = _ATTN_Q8_MACROS[hd] = {"HEAD_DIM": hd}
+    return macros
+
+
 def rmsnorm_add(x: torch.Tensor, w: torch.Tensor, eps: float, stream: torch.Tensor) -> torch.Tensor:
     """``stream += x / rms(x) * w`` row by row (float32 [T, H] both): the norm that follows a sublayer."""
     _dev(x, "x", torch.float32); _dev(w, "w"); _dev(stream, "stream", torch.float32)

@@ -1,0 +1,313 @@
+"""The 8-bit cache on the GPU: rows written and read back, and attention over them, against a plain 64-bit implementation."""
+import math
+import random
+
+import pytest
+import torch
+
+from blackwellllm_b200.engine.batch import StepBatch
+from blackwellllm_b200.kernels import ops
+from plain_quant import attention, attention_bound, quantize, rotate, row_index
+
+pytestmark = pytest.mark.gpu
+
+
+def _cuda(t, dtype=None):
+    return t.to("cuda", dtype) if dtype else t.cuda()
+
+
+class Case:
+    """Requests with segments (tokens, first position, length) over a pool whose pages lie in random order."""
+
+    def __init__(self, segments, nkv, hd, page, seed, gone=(), extra=3):
+        g = torch.Generator().manual_seed(seed)
+        self.segments, self.nkv, self.hd, self.page = segments, nkv, hd, page
+        R = len(segments)
+        blocks = [-(-total // page) for _, _, total in segments]
+        count = sum(blocks)
+        self.num_pages = count + extra
+        order = torch.randperm(self.num_pages, generator=g)[:count].tolist()
+        self.table = torch.full((R, max(blocks + [1]) + 1), -1, dtype=torch.int32)
+        for r, n in enumerate(blocks):
+            for b in range(n):
+                self.table[r, b] = order.pop()
+        for r, b in gone:
+            self.table[r, b] = -1
+        lens = torch.tensor([n for n, _, _ in segments])
+        self.cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)])
+        self.T = int(self.cu[-1])
+        self.req = torch.repeat_interleave(torch.arange(R), lens)
+        self.start = torch.tensor([a for _, a, _ in segments])
+        self.total = torch.tensor([t for _, _, t in segments])
+        self.pos = torch.arange(self.T) - self.cu[:-1][self.req] + self.start[self.req]
+        self.gen = g
+
+    def fill(self, loud=True):
+        """A pool full of rows: what the segments' requests hold, and leftovers."""
+        shape = (self.num_pages, self.nkv, self.page, self.hd)
+        got = []
+        for which in range(2):
+            x = torch.randn(shape, generator=self.gen, dtype=torch.float64)
+            if loud and which == 0:
+                x[..., ::7] *= 5.0
+            codes, scale = quantize(x * torch.exp(torch.randn(shape[:3] + (1,), generator=self.gen, dtype=torch.float64)))
+            got += [codes.to(torch.int8), scale.float()]
+        self.k, self.k_scale, self.v, self.v_scale = got
+        return self
+
+    def empty(self):
+        shape = (self.num_pages, self.nkv, self.page, self.hd)
+        self.k, self.v = torch.full(shape, 77, dtype=torch.int8), torch.full(shape, -77, dtype=torch.int8)
+        self.k_scale, self.v_scale = torch.full(shape[:3], 3.0), torch.full(shape[:3], 5.0)
+        return self
+
+    def pages(self):
+        return ops.QuantPages(self.k.cuda(), self.v.cuda(), self.k_scale.cuda(), self.v_scale.cuda())
+
+    def batch(self, bound=None):
+        i32 = torch.int32
+        z = self.start.to("cuda", i32)
+        return StepBatch(T=self.T, R=len(self.segments), token_ids=self.pos.to("cuda", i32), positions=self.pos.to("cuda", i32),
+                         req_of_token=self.req.to("cuda", i32), cu_q=self.cu.to("cuda", i32), q_start=z, kv_len=self.total.to("cuda", i32),
+                         state_slot=z, logit_rows=z, block_tables={0: self.table.cuda()}, h_q_start=self.start.tolist(),
+                         h_q_len=[n for n, _, _ in self.segments], h_kv_len=self.total.tolist(), static_bound=bound)
+
+    def check_attention(self, nh, window=0, chunk=0, sink=None, scale=None, bound=None, pages=None):
+        q = torch.randn(self.T, nh * self.hd, generator=self.gen).to(torch.bfloat16)
+        scale = self.hd ** -0.5 if scale is None else scale
+        b = self.batch(bound)
+        got = ops.quant_attention(q.cuda(), pages or self.pages(), b, b.block_tables[0], nh, scale, window or None, chunk or None,
+                                  None if sink is None else sink.cuda())
+        want, mass, score_abs = attention(q.view(self.T, nh, self.hd), self.k, self.v, self.k_scale, self.v_scale, self.cu, self.start, self.total,
+                                          self.table, scale, window, chunk, sink)
+        tol = attention_bound(want, mass, score_abs, self.hd)
+        got = got.cpu().double().view_as(want)
+        assert torch.isfinite(got).all()
+        over = ((got - want).abs() / tol).max().item()
+        assert over <= 1.0, f"error {over:.2f} times the bound"
+        return got
+
+
+# ------------------------------------------------------------------------------------------------ writing and reading back
+@pytest.mark.parametrize("hd,rd,page", [(128, 128, 16), (64, 64, 8), (64, 32, 16), (80, 80, 24), (256, 64, 16), (16, 16, 1), (96, 12, 5),
+                                        (128, 0, 64), (144, 6, 16)])
+@pytest.mark.parametrize("source", ["float32", "bfloat16", "planes", "paired"])
+def test_append_then_read(hd, rd, page, source):
+    nh, nkv = 6, 2
+    c = Case([(5, 3, 8), (1, 40, 41), (0, 0, 1), (17, 0, 17)], nkv, hd, page, seed=hd * 100 + rd + page, gone=[(0, 4 // page)]).empty()
+    width = (nh + 2 * nkv) * hd
+    x = torch.randn(c.T, width, generator=c.gen)
+    x[:, ::11] *= 9.0
+    planes = None
+    if source == "bfloat16":
+        x = x.to(torch.bfloat16).float()
+    if source == "planes":
+        planes = torch.randn(3, c.T, width, generator=c.gen)
+        x = (planes[0] + planes[1]) + planes[2]
+    angle = torch.rand(c.T, rd // 2, generator=c.gen, dtype=torch.float64) * 6
+    turns = torch.cat([angle.cos(), angle.sin()], dim=1).float() if rd else None
+    pages, table = c.pages(), c.table.cuda()
+    pos, req = _cuda(c.pos, torch.int32), _cuda(c.req, torch.int32)
+    fed = planes.cuda() if planes is not None else x.cuda().to(torch.bfloat16) if source == "bfloat16" else x.cuda()
+    q = ops.quant_append(fed, pos, req, table, pages, nh, table=None if turns is None else turns.cuda(), paired=source == "paired")
+    heads = x.double().view(c.T, nh + 2 * nkv, hd)
+    cos, sin = (turns.double().chunk(2, dim=1) if rd else (torch.zeros(c.T, 0), torch.zeros(c.T, 0)))
+    turned = rotate(heads[:, :nh + nkv], cos, sin, paired=source == "paired")
+    # a rotated channel is two products and a sum in float32: 2^-22 of the magnitudes; then one rounding to bfloat16
+    size = rotate(heads[:, :nh + nkv].abs(), cos.abs(), -sin.abs(), paired=source == "paired").abs() + turned.abs()
+    want_q = turned[:, :nh]
+    err = (q.cpu().double().view_as(want_q) - want_q).abs()
+    assert (err <= 2.0 ** -8 * want_q.abs() + 2.0 ** -21 * size[:, :nh]).all()
+    page_of, slot = row_index(c.pos, c.req, c.table, page)
+    held = page_of >= 0
+    assert not held.all() and held.any()
+    for name, rows, rough in (("k", turned[:, nh:], size[:, nh:]), ("v", heads[:, nh + nkv:], heads[:, nh + nkv:].abs())):
+        codes, scale = getattr(pages, name).cpu(), getattr(pages, name + "_scale").cpu().double()
+        _, want_s = quantize(rows)
+        got_s = scale[page_of[held], :, slot[held]]
+        # the largest magnitude is off by what the rotation is off, the division by half a step
+        slack = 2.0 ** -21 * rough.amax(-1)
+        assert ((got_s - want_s[held]).abs() <= 2.0 ** -24 * want_s[held] + slack[held] / 127).all()
+        got = codes[page_of[held], :, slot[held]].double() * got_s[..., None]
+        # a number is within half a scale of the value; the factor, the product and the scale are each rounded (127 steps of 2^-24, in scales)
+        assert ((got - rows[held]).abs() <= 0.5 * (1 + 2.0 ** -14) * got_s[..., None] + 2 * slack[held][..., None]).all()
+        # what no token of the step owns is as it was
+        mark = torch.ones(codes.shape[0], codes.shape[2], dtype=torch.bool)
+        mark[page_of[held], slot[held]] = False
+        left = codes.transpose(1, 2)[mark]
+        assert (left == (77 if name == "k" else -77)).all()
+        assert (scale.transpose(1, 2)[mark] == (3.0 if name == "k" else 5.0)).all()
+    # read back: the number times its scale, one rounding
+    for dtype, u in ((torch.float32, 2.0 ** -24), (torch.bfloat16, 2.0 ** -8)):
+        for got, name in zip(ops.quant_read(pages, pos, req, table, dtype), ("k", "v")):
+            codes, scale = getattr(pages, name).cpu().double(), getattr(pages, name + "_scale").cpu().double()
+            want = torch.zeros(c.T, nkv, hd, dtype=torch.float64)
+            want[held] = codes[page_of[held], :, slot[held]] * scale[page_of[held], :, slot[held]][..., None]
+            # (float32: the product itself is rounded once; bfloat16: that and the rounding to it)
+            assert ((got.cpu().double() - want).abs() <= (u + 2.0 ** -24) * want.abs()).all()
+
+
+def test_append_without_writing():
+    c = Case([(3, 0, 3)], 2, 64, 16, seed=1).empty()
+    pages = c.pages()
+    x = torch.randn(3, (4 + 4) * 64, generator=c.gen).cuda()
+    q = ops.quant_append(x, _cuda(c.pos, torch.int32), _cuda(c.req, torch.int32), c.table.cuda(), pages, 4, append=False)
+    assert torch.equal(q, x[:, :256].to(torch.bfloat16))
+    assert (pages.k == 77).all() and (pages.v == -77).all() and (pages.k_scale == 3).all() and (pages.v_scale == 5).all()
+
+
+def test_rows_at_the_ends_of_the_range():
+    """Zeros, tiny and huge rows, infinities and NaN: nothing overflows, and what is no number stays none."""
+    hd, nh, nkv = 64, 1, 1
+    x = torch.ones(8, hd)
+    x[0] = 0.0
+    x[1] = 1e-40
+    x[2] = 2.0 ** -109
+    x[3] = 3.3e38
+    x[4, 5] = math.inf
+    x[5, 63] = math.nan
+    x[6] = -0.0
+    x[7, 1:] = 1e-30
+    c = Case([(8, 0, 8)], nkv, hd, 4, seed=2).empty()
+    pages = c.pages()
+    rows = torch.cat([torch.zeros(8, hd), x, x.flip(0)], dim=1).cuda()
+    pos, req, table = _cuda(c.pos, torch.int32), _cuda(c.req, torch.int32), c.table.cuda()
+    ops.quant_append(rows, pos, req, table, pages, nh)
+    k, v = (t.cpu()[:, 0] for t in ops.quant_read(pages, pos, req, table, torch.float32))
+    for got, want in ((k, x), (v, x.flip(0))):
+        for a, b in zip(got, want):
+            if not torch.isfinite(b).all():
+                assert torch.isnan(a).all()
+            else:
+                most = b.abs().max().item()
+                # (tiny rows are zeros; else half a scale, and the product's rounding)
+                tol = 2.0 ** -110 if most < 2.0 ** -110 else most / 127 * 0.5 * (1 + 2.0 ** -20)
+                assert torch.isfinite(a).all() and (a.double() - b.double()).abs().max().item() <= tol
+
+
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("hd", [128, 64, 80, 256, 16, 96])
+@pytest.mark.parametrize("nh,nkv,page", [(8, 2, 16), (7, 1, 8), (16, 1, 24), (3, 3, 64), (10, 2, 1)])
+def test_attention_few_queries(hd, nh, nkv, page):
+    segs = [(1, 0, 1), (1, 15, 16), (1, 63, 64), (1, 64, 65), (1, 300, 301), (0, 5, 5), (2 if nh // nkv <= 8 else 1, 130, 132 if nh // nkv <= 8 else 131)]
+    Case(segs, nkv, hd, page, seed=hd + nh + page).fill().check_attention(nh)
+
+
+@pytest.mark.parametrize("hd", [128, 64, 80, 256, 192])
+@pytest.mark.parametrize("nh,nkv,page", [(8, 2, 16), (7, 1, 8), (16, 1, 24), (4, 4, 64)])
+def test_attention_portions(hd, nh, nkv, page):
+    segs = [(37, 0, 37), (1, 70, 71), (19, 111, 130), (130, 5, 135), (3, 200, 203)]
+    Case(segs, nkv, hd, page, seed=hd * 3 + nh + page).fill().check_attention(nh)
+
+
+@pytest.mark.parametrize("window,chunk", [(1, 0), (17, 0), (64, 0), (100, 0), (0, 32), (50, 64), (0, 1)])
+def test_attention_windows_and_chunks(window, chunk):
+    segs = [(1, 299, 300), (40, 90, 130), (2, 63, 65), (25, 0, 25)]
+    c = Case(segs, 2, 64, 16, seed=window * 7 + chunk).fill()
+    c.check_attention(6, window, chunk)
+    c.check_attention(6, window, chunk, bound=512)
+
+
+def test_attention_sink():
+    c = Case([(1, 99, 100), (30, 10, 40), (1, 0, 1)], 2, 128, 16, seed=5).fill()
+    c.check_attention(8, sink=torch.linspace(-3, 6, 8))
+
+
+@pytest.mark.parametrize("count", [33, 40])
+def test_attention_more_portions_than_one_launch_takes(count):
+    Case([(18 + i % 3, i, 18 + i % 3 + i) for i in range(count)], 1, 64, 16, seed=count).fill().check_attention(2)
+
+
+def test_attention_slices_are_joined_in_order():
+    """One request, long: many slices; the same inputs give the same bits, also beside other requests of the same plan."""
+    c = Case([(1, 5000, 5001)], 1, 128, 16, seed=9).fill()
+    b, pages = c.batch(), c.pages()
+    q = torch.randn(1, 4 * 128, generator=c.gen).to(torch.bfloat16).cuda()
+    outs = [ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.088) for _ in range(5)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    c.check_attention(4)
+
+
+def test_attention_pages_that_are_gone():
+    """Keys whose pages are not held are not seen; a row that sees none is zeros, in both kernels."""
+    c = Case([(1, 40, 41), (20, 12, 32), (1, 20, 21), (18, 0, 18)], 2, 64, 16, seed=11,
+             gone=[(0, 1), (1, 0), (2, 0), (2, 1), (3, 0), (3, 1)]).fill()
+    got = c.check_attention(6)
+    # (positions 12 to 15 of the second request see its first page alone, which is gone)
+    empty = torch.zeros(c.T, dtype=torch.bool)
+    empty[1:5] = empty[21:] = True
+    assert (got[empty] == 0).all() and (got[~empty] != 0).any(-1).all()
+
+
+def test_attention_leaves_out_what_is_no_number_where_it_is_not_seen():
+    """Scales that are NaN behind a request's last token, in other requests' pages and in a later token of the same tile."""
+    c = Case([(1, 20, 21), (30, 0, 30)], 1, 64, 16, seed=13).fill()
+    page = c.page
+    free = [p for p in range(c.num_pages) if p not in c.table.tolist()[0] + c.table.tolist()[1]]
+    c.k_scale[free], c.v_scale[free] = math.nan, math.nan
+    for r, total in ((0, 21), (1, 30)):
+        last = int(c.table[r, (total - 1) // page])
+        c.k_scale[last, :, total % page:] = math.nan
+        c.v_scale[last, :, total % page:] = math.inf
+    c.check_attention(4)
+    # a key of position 25 is no number: the tokens before it do not see that, the ones from it on do
+    p25 = int(c.table[1, 25 // page])
+    c.k_scale[p25, :, 25 % page] = math.nan
+    c.v_scale[p25, :, 25 % page] = math.nan
+    b = c.batch()
+    q = torch.randn(c.T, 4 * 64, generator=c.gen).to(torch.bfloat16).cuda()
+    got = ops.quant_attention(q, c.pages(), b, b.block_tables[0], 4, 0.125).float()
+    assert torch.isfinite(got[:26]).all() and torch.isnan(got[26:]).all()
+
+
+def test_attention_in_a_graph_of_any_length():
+    """A captured decode step replays with other lengths, on the bound that it was captured for."""
+    c = Case([(1, 700, 701), (1, 3, 4), (1, 64, 65)], 2, 128, 16, seed=17).fill()
+    b = c.batch(bound=1024)
+    pages = c.pages()
+    q = torch.zeros(c.T, 8 * 128, dtype=torch.bfloat16, device="cuda")
+    ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.088)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.088)
+    for starts in ([700, 3, 64], [0, 250, 1], [63, 64, 63]):
+        starts = [min(s, int(t) - 1) for s, t in zip(starts, c.total)]
+        b.q_start.copy_(torch.tensor(starts)); b.kv_len.copy_(torch.tensor(starts) + 1)
+        fresh = torch.randn(c.T, 8 * 128, generator=c.gen).to(torch.bfloat16)
+        q.copy_(fresh)
+        graph.replay()
+        want, mass, score_abs = attention(fresh.view(3, 8, 128), c.k, c.v, c.k_scale, c.v_scale, c.cu, starts, [s + 1 for s in starts], c.table, 0.088)
+        tol = attention_bound(want, mass, score_abs, 128)
+        assert ((out.cpu().double().view_as(want) - want).abs() <= tol).all()
+
+
+def test_refusals():
+    c = Case([(1, 3, 4)], 2, 64, 16, seed=1).fill()
+    pages, b = c.pages(), c.batch()
+    table = b.block_tables[0]
+    q = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q.float(), pages, b, table, 4, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q, pages, b, table, 3, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(torch.zeros(2, 4 * 64, dtype=torch.bfloat16, device="cuda"), pages, b, table, 4, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q, ops.QuantPages(pages.k, pages.v, pages.k_scale[:, :1], pages.v_scale), b, table, 4, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q, ops.QuantPages(pages.k.float(), pages.v, pages.k_scale, pages.v_scale), b, table, 4, 0.1)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q, pages, b, table, 4, 0.1, sink=torch.zeros(3, device="cuda"))
+    with pytest.raises(ops.KernelError):      # 34 query heads to a kv head
+        ops.quant_attention(torch.zeros(1, 34 * 64, dtype=torch.bfloat16, device="cuda"), pages, b, table, 34, 0.1)
+    x = torch.zeros(1, 8 * 64, device="cuda")
+    with pytest.raises(ops.KernelError):
+        ops.quant_append(x[:, :-1].contiguous(), b.positions, b.req_of_token, table, pages, 4)
+    with pytest.raises(ops.KernelError):
+        ops.quant_append(x, b.positions, b.req_of_token, table, pages, 4, table=torch.zeros(1, 63, device="cuda"))
+    with pytest.raises(ops.KernelError):
+        ops.quant_append(x.half(), b.positions, b.req_of_token, table, pages, 4)
+    with pytest.raises(ops.KernelError):
+        ops.quant_read(pages, b.positions, b.req_of_token[:0], table)
+    with pytest.raises(ops.KernelError):
+        ops.quant_read(pages, b.positions, b.req_of_token, table, torch.float16)
