@@ -10,7 +10,7 @@ import math
 import os
 import threading
 from collections import OrderedDict
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -67,6 +67,14 @@ def _dev(t: torch.Tensor, name: str, dtype=None, contiguous=True):
     if contiguous and not t.is_contiguous():
         raise KernelError(f"{name} must be contiguous")
     return t
+
+
+def _same_device(what: str, *tensors) -> None:
+    # a kernel runs on the current device, on its current stream: operands elsewhere would be read over the bus or not at all
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{here}")
 
 
 def _code(t: torch.Tensor, name: str) -> int:
@@ -829,6 +837,46 @@ def log_prob(logits: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
     return out
 
 
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_log_probs` returns, per row of logits."""
+    log_prob: torch.Tensor       # float32 [R]: ln P(target)
+    entropy: torch.Tensor        # float32 [R]: of the row's distribution, in nats
+    rank: torch.Tensor           # int32 [R]: how many tokens stand before the target (0: it is the most probable one)
+    top_ids: torch.Tensor        # int32 [R, top], the most probable first; ties to the lowest id
+    top_log_probs: torch.Tensor  # float32 [R, top]
+
+
+TOKEN_LOG_PROBS_MAX_TOP = 32
+_TOKEN_PROBS_ARGS = [c_void_p] * 7 + [c_int, c_int, c_int, c_ll, c_void_p]
+
+
+def token_log_probs(logits: torch.Tensor, target: torch.Tensor, top: int = 0) -> TokenLogProbs:
+    """Log probability, rank, entropy and the ``top`` (at most 32) most probable tokens of every row of float32 ``logits`` [R, V] (rows may be
+    apart), in one pass over them.  ``target`` int32 [R]; one outside [0, V) stands for none: log probability NaN, rank -1.  A row without a
+    distribution (a NaN or +infinity among its logits, or nothing but -infinity) gets NaN, and -1 for rank and ids."""
+    _dev(logits, "logits", torch.float32, contiguous=False)
+    if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise KernelError("token_log_probs: logits must be [R, V] with contiguous rows that do not overlap")
+    R, V = logits.shape
+    _dev(target, "target", torch.int32)
+    if target.numel() != R:
+        raise KernelError("token_log_probs: one target per row")
+    if not 0 <= top <= min(TOKEN_LOG_PROBS_MAX_TOP, V):
+        raise KernelError(f"token_log_probs: top must be 0 to {TOKEN_LOG_PROBS_MAX_TOP} and at most the row's {V} tokens, got {top}")
+    _same_device("token_log_probs", logits, target)
+    # one allocation: three numbers and two lists a row
+    both = torch.empty(R * (3 + 2 * top), dtype=torch.float32, device=logits.device)
+    ints = both.view(torch.int32)
+    got = TokenLogProbs(both[:R], both[R:2 * R], ints[2 * R:3 * R], ints[3 * R:(3 + top) * R].view(R, top), both[(3 + top) * R:].view(R, top))
+    if R == 0:
+        return got
+    fn = _fn("token_probs", "bw_token_probs", _TOKEN_PROBS_ARGS)
+    at = both.data_ptr()
+    _check(fn(logits.data_ptr(), target.data_ptr(), at, at + 4 * R, at + 8 * R, at + 12 * R, at + 4 * (3 + top) * R, R, V, top,
+              logits.stride(0) if R > 1 else V, _stream()), "token_log_probs")
+    return got
+
+
 # ------------------------------------------------------------------ dispatch
 
 _GEMM_TC_ARGS = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_ll, c_ll, c_int, c_int,
@@ -1422,14 +1470,6 @@ def _quant_pages(pages: QuantPages, block_table: torch.Tensor, what: str):
         raise KernelError(f"{what}: the block table must be [requests, blocks]")
     check_quant_supported(hd)
     return num_pages, nkv, page_size, hd
-
-
-def _same_device(what: str, *tensors) -> None:
-    # a kernel runs on the current device, on its current stream: operands elsewhere would be read over the bus or not at all
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{here}")
 
 
 _QUANT_APPEND_ARGS = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_int, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_void_p]
