@@ -33,7 +33,7 @@ constexpr int CHUNKS = HD / 16;                    // 16-byte units of a row
 constexpr int STRIDE = (CHUNKS | 1) * 16;          // bytes between rows of shared memory
 constexpr int KEYS = 16;                           // keys that a warp works on at a time
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int TILE = WARPS * KEYS;                 // keys of a block's step
+constexpr int TILE = 128;                          // keys that slices are counted in: a step of a block's warps, or two
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
@@ -76,6 +76,12 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Two signed bytes of r (chosen by SEL) as bfloat16.  With u the byte's low seven bits, 0x4300 | u is 128 + u, and 0x4300 | (byte & 128) is 128
@@ -124,77 +130,114 @@ __device__ __forceinline__ void load_queries(const Params& p, Queries<NB>& s, in
     }
 }
 
-// Sixteen keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page.
-template <int NB>
-__device__ __forceinline__ void sixteen_keys(Queries<NB>& s, uint32_t k_rows, uint32_t v_rows, const float* ks, const float* vs, int key0,
-                                             unsigned there, bool need_mask, float scale_log2) {
+// 16 KG keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page.  KG groups of sixteen keys
+// go side by side: a group's products are a chain, and a warp has little else to do meanwhile.
+// The reference m of a query's exponents follows its largest score lazily: as long as no score is more than 8 above it (a factor of 256) it
+// stays, so most steps need one vote instead of a maximum over the lanes and a pass over the outputs.  Weights stay below 2^8, and what they
+// are divided by has the same reference.
+template <int NB, int KG>
+__device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint32_t v_rows, const float* ks, const float* vs, int key0,
+                                          unsigned there, bool need_mask, float scale_log2) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
     // matrices of an ldmatrix: keys 0-7 and 8-15 of one 16-byte unit, then of the next
     const uint32_t at = (uint32_t)(((lane & 7) + 8 * ((lane >> 3) & 1)) * STRIDE);
-    float sc[NB][4];
+    float sc[KG][NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+    for (int h = 0; h < KG; ++h)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) sc[h][nb][0] = sc[h][nb][1] = sc[h][nb][2] = sc[h][nb][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t f[4];
-        // (an odd last unit: its second pair of matrices reads the first's again)
-        ldsm4(k_rows + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (c + i >= CHUNKS) break;
-            const uint32_t a[4] = {widen2<0x4140>(f[2 * i]), widen2<0x4140>(f[2 * i + 1]), widen2<0x4342>(f[2 * i]), widen2<0x4342>(f[2 * i + 1])};
+        for (int h = 0; h < KG; ++h) {
+            uint32_t f[4];
+            // (an odd last unit: its second pair of matrices reads the first's again)
+            ldsm4(k_rows + h * KEYS * STRIDE + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) mma(sc[nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
-        }
-    }
-    const float k0 = ks[r] * scale_log2, k1 = ks[r + 8] * scale_log2, v0 = vs[r], v1 = vs[r + 8];
-    uint32_t pf[NB][2];
+            for (int i = 0; i < 2; ++i) {
+                if (c + i >= CHUNKS) break;
+                const uint32_t a[4] = {widen2<0x4140>(f[2 * i]), widen2<0x4140>(f[2 * i + 1]), widen2<0x4342>(f[2 * i]), widen2<0x4342>(f[2 * i + 1])};
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        float t[4] = {sc[nb][0] * k0, sc[nb][1] * k0, sc[nb][2] * k1, sc[nb][3] * k1};
-        bool seen[4] = {true, true, true, true};
-        if (need_mask) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int kp = key0 + r + 8 * (i >> 1), e = i & 1;
-                seen[i] = kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> (r + 8 * (i >> 1)) & 1);
-                if (!seen[i]) t[i] = -INFINITY;
+                for (int nb = 0; nb < NB; ++nb) mma(sc[h][nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
             }
         }
-        float mx[2] = {fmaxf(t[0], t[2]), fmaxf(t[1], t[3])}, corr[2];
+    }
+    float most[NB][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
-            const float m_new = fmaxf(s.m[nb][e], mx[e]);
-            mx[e] = m_new == -INFINITY ? 0.f : m_new;
-            corr[e] = exp2f(s.m[nb][e] - mx[e]);        // nothing seen so far: 0
-            s.m[nb][e] = m_new;
+    for (int nb = 0; nb < NB; ++nb) most[nb][0] = most[nb][1] = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < KG; ++h) {
+        const float k0 = ks[16 * h + r] * scale_log2, k1 = ks[16 * h + r + 8] * scale_log2;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float t = sc[h][nb][i] * (i < 2 ? k0 : k1);
+                if (need_mask) {
+                    const int j = 16 * h + r + 8 * (i >> 1), kp = key0 + j, e = i & 1;
+                    if (!(kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> j & 1))) t = -INFINITY;
+                }
+                sc[h][nb][i] = t;
+                most[nb][i & 1] = fmaxf(most[nb][i & 1], t);
+            }
         }
+    }
+    bool grown = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = exp2f(t[i] - mx[i & 1]);
-        s.l[nb][0] = s.l[nb][0] * corr[0] + (t[0] + t[2]);
-        s.l[nb][1] = s.l[nb][1] * corr[1] + (t[1] + t[3]);
-        // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
-        const float w[4] = {seen[0] ? t[0] * v0 : 0.f, seen[1] ? t[1] * v0 : 0.f, seen[2] ? t[2] * v1 : 0.f, seen[3] ? t[3] * v1 : 0.f};
-        pf[nb][0] = turn8x8(bw::pack_bf16x2(w[0], w[1]));
-        pf[nb][1] = turn8x8(bw::pack_bf16x2(w[2], w[3]));
+    for (int nb = 0; nb < NB; ++nb) grown |= most[nb][0] > s.m[nb][0] + 8.f || most[nb][1] > s.m[nb][1] + 8.f;
+    if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            s.o[c][nb][0] *= corr[0]; s.o[c][nb][1] *= corr[1]; s.o[c][nb][2] *= corr[0]; s.o[c][nb][3] *= corr[1];
+        for (int nb = 0; nb < NB; ++nb) {
+            float corr[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float mx = most[nb][e];
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float m_new = fmaxf(s.m[nb][e], mx);
+                corr[e] = m_new == -INFINITY ? 0.f : ex2(s.m[nb][e] - m_new);     // nothing seen so far: 0
+                s.m[nb][e] = m_new;
+                s.l[nb][e] *= corr[e];
+            }
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                s.o[c][nb][0] *= corr[0]; s.o[c][nb][1] *= corr[1]; s.o[c][nb][2] *= corr[0]; s.o[c][nb][3] *= corr[1];
+            }
+        }
+    }
+    uint32_t pf[KG][NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const float ref[2] = {s.m[nb][0] == -INFINITY ? 0.f : s.m[nb][0], s.m[nb][1] == -INFINITY ? 0.f : s.m[nb][1]};
+#pragma unroll
+        for (int h = 0; h < KG; ++h) {
+            const float v0 = vs[16 * h + r], v1 = vs[16 * h + r + 8];
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float t = ex2(sc[h][nb][i] - ref[i & 1]);
+                s.l[nb][i & 1] += t;
+                // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
+                w[i] = need_mask && sc[h][nb][i] == -INFINITY ? 0.f : t * (i < 2 ? v0 : v1);
+            }
+            pf[h][nb][0] = turn8x8(bw::pack_bf16x2(w[0], w[1]));
+            pf[h][nb][1] = turn8x8(bw::pack_bf16x2(w[2], w[3]));
         }
     }
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t f[4];
-        ldsm4_t(v_rows + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
+    for (int h = 0; h < KG; ++h) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (c + i >= CHUNKS) break;
-            const uint32_t a[4] = {widen2<0x4240>(f[2 * i]), widen2<0x4341>(f[2 * i]), widen2<0x4240>(f[2 * i + 1]), widen2<0x4341>(f[2 * i + 1])};
+        for (int c = 0; c < CHUNKS; c += 2) {
+            uint32_t f[4];
+            ldsm4_t(v_rows + h * KEYS * STRIDE + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, pf[nb][0], pf[nb][1]);
+            for (int i = 0; i < 2; ++i) {
+                if (c + i >= CHUNKS) break;
+                const uint32_t a[4] = {widen2<0x4240>(f[2 * i]), widen2<0x4341>(f[2 * i]), widen2<0x4240>(f[2 * i + 1]), widen2<0x4341>(f[2 * i + 1])};
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, pf[h][nb][0], pf[h][nb][1]);
+            }
         }
     }
 }
@@ -208,32 +251,42 @@ __device__ __forceinline__ int key_row(const Params& p, const int* bt, int g, in
     return page >= 0 && page < p.num_pages ? (page * p.nkv + g) * p.page_size + (key - blk * p.page_size) : -1;
 }
 
-constexpr int STAGE = 2 * KEYS * STRIDE + 2 * KEYS * 4;     // K, V, their scales
-// Sixteen keys into a stage, by one warp; `row`: key_row of key lane & 15 in every lane.
+// 16 KG keys into a stage (rows of K, of V, their scales), by one warp; `row`: key_row of key lane (of lane & 15 with KG 1) in every lane.
+template <int KG> constexpr int STAGE = 2 * KG * KEYS * (STRIDE + 4);
+template <int KG>
 __device__ __forceinline__ void fetch(const Params& p, uint8_t* stage, int row) {
+    constexpr int N = KG * KEYS;
     const int lane = threadIdx.x & 31;
-    const uint32_t k_to = smem_u32(stage), v_to = k_to + KEYS * STRIDE;
+    const uint32_t k_to = smem_u32(stage), v_to = k_to + N * STRIDE, s_to = v_to + N * STRIDE;
 #pragma unroll
-    for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
+    for (int i = 0; i < (N * CHUNKS + 31) / 32; ++i) {
         const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
-        const int rw = __shfl_sync(0xffffffffu, row, key & 15);
-        if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
+        const int rw = __shfl_sync(0xffffffffu, row, key & (N - 1));
+        if ((N * CHUNKS) % 32 && key >= N) break;
         const size_t off = rw >= 0 ? (size_t)rw * HD + 16 * c : 0;
         cp_async16(k_to + key * STRIDE + 16 * c, p.k + off, rw >= 0);
         cp_async16(v_to + key * STRIDE + 16 * c, p.v + off, rw >= 0);
     }
-    cp_async4(k_to + 2 * KEYS * STRIDE + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + (row >= 0 ? row : 0), row >= 0);
+    const int from = row >= 0 ? row : 0;
+    if constexpr (KG == 1) {
+        cp_async4(s_to + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + from, row >= 0);
+    } else {
+        cp_async4(s_to + 4 * lane, p.k_scale + from, row >= 0);
+        cp_async4(s_to + 4 * (lane + N), p.v_scale + from, row >= 0);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- few queries
 // All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
 // with a ring of its own, and are joined at the end.  Slices are equally long for every request; how many of them a request has follows
 // from its length on the device, so the same launch serves a captured step whatever the lengths become.
-constexpr int STAGES = 4;
-constexpr int SMEM_RING = WARPS * STAGES * STAGE;
+// Queries in registers beside two groups of keys: up to 256 channels of queries (one block of eight of up to 256, two of up to 128).
+template <int NB> constexpr int FEW_KG = NB * HD <= 256 ? 2 : 1;
+constexpr int STAGES = 3;
+template <int NB> constexpr int SMEM_RING = WARPS * STAGES * STAGE<FEW_KG<NB>>;
 constexpr int JOIN_LD = HD + 8;
 constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD) * 4;
-constexpr int SMEM_KEYS = SMEM_RING > SMEM_JOIN ? SMEM_RING : SMEM_JOIN;
+template <int NB> constexpr int SMEM_FEW = SMEM_RING<NB> > SMEM_JOIN ? SMEM_RING<NB> : SMEM_JOIN;
 
 struct Walk { int first, tiles, per, live; };   // in tiles of TILE keys: where it begins, how many, of a slice; slices that have any
 __device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last) {
@@ -270,37 +323,39 @@ few_kernel(Params p) {
     if (slice >= walk.live) return;
     const int t0 = walk.first + slice * walk.per, t1 = min(walk.first + walk.tiles, t0 + walk.per);
     const int* bt = p.table + (size_t)r * p.max_blocks;
-    uint8_t* ring = smem + warp * STAGES * STAGE;
-    // the row of this lane's key of the next tile that is fetched: looked up a tile ahead of its use
-    int next = key_row(p, bt, g, t0 * TILE + warp * KEYS + (lane & 15), kv_len);
+    constexpr int KG = FEW_KG<NB>, N = KG * KEYS;      // keys of a warp's step
+    constexpr unsigned ALL = N == 32 ? 0xffffffffu : (1u << (N & 31)) - 1;
+    uint8_t* ring = smem + warp * STAGES * STAGE<KG>;
+    // a warp's steps: every fourth N keys of the slice
+    const int first = t0 * TILE + warp * N, end = min(t1 * TILE, last + 1);
+    // the row of this lane's key of the next step that is fetched: looked up a step ahead of its use
+    int next = first < end ? key_row(p, bt, g, first + (lane & (N - 1)), kv_len) : -1;
     unsigned there[STAGES];
-    auto feed = [&](int t, int st) {
-        if (t < t1) {
-            there[st] = __ballot_sync(0xffffffffu, next >= 0) & 0xffffu;
-            fetch(p, ring + st * STAGE, next);
-            next = t + 1 < t1 ? key_row(p, bt, g, (t + 1) * TILE + warp * KEYS + (lane & 15), kv_len) : -1;
+    auto feed = [&](int key0, int st) {
+        if (key0 < end) {
+            there[st] = __ballot_sync(0xffffffffu, next >= 0) & ALL;
+            fetch<KG>(p, ring + st * STAGE<KG>, next);
+            next = key0 + WARPS * N < end ? key_row(p, bt, g, key0 + WARPS * N + (lane & (N - 1)), kv_len) : -1;
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) feed(t0 + st, st);
+    for (int st = 0; st < STAGES - 1; ++st) feed(first + st * WARPS * N, st);
     Queries<NB> s;
     load_queries<NB>(p, s, tok, g, 0, n_rows, q_pos0);
     const int see_all = bw::first_visible(last, p.window, p.chunk);      // from here on every query of the segment sees keys up to q_pos0
-    for (int t = t0; t < t1; t += STAGES) {
+    for (int base = first; base < end; base += STAGES * WARPS * N) {
 #pragma unroll
         for (int st = 0; st < STAGES; ++st) {
-            if (t + st >= t1) break;
+            const int key0 = base + st * WARPS * N;
+            if (key0 >= end) break;
             cp_async_wait<STAGES - 2>();
             __syncwarp();
-            feed(t + st + STAGES - 1, (st + STAGES - 1) % STAGES);
-            const uint8_t* at = ring + st * STAGE;
-            const int key0 = (t + st) * TILE + warp * KEYS;
-            if (key0 <= last) {
-                const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
-                const bool need_mask = there[st] != 0xffffu || key0 + KEYS - 1 > q_pos0 || key0 < see_all;
-                sixteen_keys<NB>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, there[st], need_mask, p.scale_log2);
-            }
+            feed(key0 + (STAGES - 1) * WARPS * N, (st + STAGES - 1) % STAGES);
+            const uint32_t at = smem_u32(ring + st * STAGE<KG>);
+            const float* sc = reinterpret_cast<const float*>(ring + st * STAGE<KG> + 2 * N * STRIDE);
+            const bool need_mask = there[st] != ALL || key0 + N - 1 > q_pos0 || key0 < see_all;
+            some_keys<NB, KG>(s, at, at + N * STRIDE, sc, sc + N, key0, there[st], need_mask, p.scale_log2);
             __syncwarp();
         }
     }
@@ -405,13 +460,14 @@ constexpr int MANY = 16;                                   // requests with many
 struct Portions { int n; int request[MANY]; int first[MANY + 1]; };   // first: the block index of each one's first 64 rows
 constexpr int ROWS = 16 * WARPS;
 constexpr int RING = 2;
-constexpr int SMEM_MANY = RING * WARPS * STAGE + 64;
+constexpr int MANY_TILE = WARPS * KEYS;                    // keys of a block's step
+constexpr int SMEM_MANY = RING * WARPS * STAGE<1> + 64;
 
 __global__ void __launch_bounds__(THREADS)
 many_kernel(Params p, Portions work) {
     BW_PDL_TRIGGER();
     extern __shared__ __align__(16) uint8_t smem[];
-    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE);
+    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE<1>);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.x;
     int i = 0;
     while (i + 1 < work.n && (int)blockIdx.y >= work.first[i + 1]) ++i;
@@ -425,14 +481,14 @@ many_kernel(Params p, Portions work) {
     const int* bt = p.table + (size_t)r * p.max_blocks;
     const int mine = row0 + 16 * warp, last_row = min(all_rows, row0 + ROWS) - 1;
     const int first_pos = q_pos0 + row0 / p.G, last_pos = q_pos0 + last_row / p.G;
-    const int t0 = bw::first_visible(first_pos, p.window, p.chunk) / TILE, t1 = last_pos / TILE + 1;
+    const int t0 = bw::first_visible(first_pos, p.window, p.chunk) / MANY_TILE, t1 = last_pos / MANY_TILE + 1;
     auto feed = [&](int t) {
         if (t < t1) {
             const int st = (t - t0) % RING;
-            const int row = key_row(p, bt, g, t * TILE + warp * KEYS + (lane & 15), kv_len);
+            const int row = key_row(p, bt, g, t * MANY_TILE + warp * KEYS + (lane & 15), kv_len);
             const unsigned b = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
             if (lane == 0) there[st * WARPS + warp] = b;
-            fetch(p, smem + (st * WARPS + warp) * STAGE, row);
+            fetch<1>(p, smem + (st * WARPS + warp) * STAGE<1>, row);
         }
         cp_async_commit();
     };
@@ -448,13 +504,13 @@ many_kernel(Params p, Portions work) {
         const int st = (t - t0) % RING;
         if (mine <= last_row) {
             for (int w = 0; w < WARPS; ++w) {
-                const int key0 = t * TILE + w * KEYS;
+                const int key0 = t * MANY_TILE + w * KEYS;
                 if (key0 > my_last) break;
-                const uint8_t* at = smem + (st * WARPS + w) * STAGE;
+                const uint8_t* at = smem + (st * WARPS + w) * STAGE<1>;
                 const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
                 const unsigned ok = there[st * WARPS + w];
                 const bool need_mask = ok != 0xffffu || key0 + KEYS - 1 > my_first || key0 < see_all;
-                sixteen_keys<2>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask, p.scale_log2);
+                some_keys<2, 1>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask, p.scale_log2);
             }
         }
         __syncthreads();
@@ -509,7 +565,8 @@ BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int req
     }
     *per = 1;
     if (most == 0) return 0;
-    const long long room = 2LL * bw::num_sms();          // blocks that run at once
+    constexpr int at_once = (227 * 1024) / (SMEM_FEW<1> + 1024);
+    const long long room = (long long)(at_once < 4 ? at_once : 4) * bw::num_sms();          // blocks that run at once
     long long lo = 1, hi = most;
     while (lo < hi) {
         const long long mid = (lo + hi) / 2;
@@ -535,8 +592,8 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
              max_blocks, nh, nkv, G, page_size, num_pages, window > 0 ? window : 0, chunk > 0 ? chunk : 0, requests, per, slices, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
     static bool few1_done[bw::MAX_DEVICES], few2_done[bw::MAX_DEVICES], many_done[bw::MAX_DEVICES];
-    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<1>, SMEM_KEYS, few1_done); e != cudaSuccess) return (int)e;
-    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<2>, SMEM_KEYS, few2_done); e != cudaSuccess) return (int)e;
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<1>, SMEM_FEW<1>, few1_done); e != cudaSuccess) return (int)e;
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<2>, SMEM_FEW<2>, few2_done); e != cudaSuccess) return (int)e;
     if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
     Portions work{};
     int most_rows = 0;
@@ -566,8 +623,8 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
     const dim3 grid((unsigned)slices, (unsigned)nkv, (unsigned)requests);
-    if (few1) { bw::launch(few_kernel<1>, grid, dim3(THREADS), SMEM_KEYS, s, p); BW_LAUNCH_CHECK(); }
-    if (few2) { bw::launch(few_kernel<2>, grid, dim3(THREADS), SMEM_KEYS, s, p); BW_LAUNCH_CHECK(); }
+    if (few1) { bw::launch(few_kernel<1>, grid, dim3(THREADS), SMEM_FEW<1>, s, p); BW_LAUNCH_CHECK(); }
+    if (few2) { bw::launch(few_kernel<2>, grid, dim3(THREADS), SMEM_FEW<2>, s, p); BW_LAUNCH_CHECK(); }
     if (slices > 1) {
         bw::launch(join_kernel, dim3((unsigned)most_rows, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
         BW_LAUNCH_CHECK();
