@@ -3,21 +3,30 @@
 //
 //   score of query i and key j = scale * ks_j * sum_c q_ic kc_jc,   out_ic = sum_j (p_ij vs_j) vc_jc / sum_j p_ij
 //
-// The whole numbers are exact in bfloat16, so the products run on bfloat16 tensor cores (mma.sync m16n8k16, float32 sums) as if the cache
-// were bfloat16, and a key's scale is multiplied to its scores, a value's to its probabilities, in float32; maxima, sums and outputs are
-// float32.  One rounding comes in: p vs to bfloat16 (8 bits; each weight is off by at most 2^-8 of itself, as in the attention over a
-// bfloat16 cache) because the other operand is bfloat16.
+// The whole numbers are widened to float16, in which they are exact, and the products run on the tensor cores (mma.sync m16n8k16, float32
+// sums).  A byte b of two's complement with its top bit turned over is u = b + 128, and 0x6400 | u is the float16 1024 + u: one byte
+// permutation makes two.  For V 1152 is subtracted from it; for K it is left in and 1152 times the sum of the query's channels comes off the score
+// (which is then off by at most a few 2^-24 of 1152 sum |q|, a few 1e-7 of the largest score that such a key can have).
+//   Queries: a row is multiplied by a power of two that brings its largest channel to 2^14 up to 2^15, so that bfloat16's eight bits
+//      fit float16's eleven whatever the row's size (channels below 2^-31 of the largest lose bits); the power comes off the score.
+//   Weights: with the value's scale inside the exponent, w_ij = 2^(t_ij + log2 vs_j - m_i), t the score in powers of two.  The reference m follows
+//      the largest t + log2 vs, so what counts most is near 1 and float16 rounds each weight by at most 2^-11 of itself, or of 2^-14: never
+//      more than 2^-25 of the largest.  The denominator is the sum of w / vs in float32.  A value's scale of 0 counts as 2^-100 (its
+//      whole numbers are zeros).
+// Everything else is float32: scores, references, sums, outputs.
 //
-// The products are turned around: S^T = K Q^T and O^T = V^T P^T, keys and channels in the 16 rows of an instruction, queries in its 8
+// The products are turned around: S^T = K Q^T and O^T = V^T W^T, keys and channels in the 16 rows of an instruction, queries in its 8
 // columns.  A decoding request has the G query heads of a kv head as its queries, mostly 4 to 8: so an instruction is full, and an element of
 // the cache is widened once for all of them.
 //   K: ldmatrix on bytes gives a lane four neighbouring channels of one key, which are taken as k indices 2q, 2q + 1, 2q + 8, 2q + 9 (a sum does
 //      not mind the order of its terms; the queries' fragments take the same order);
 //   V: ldmatrix.trans on bytes gives a lane two neighbouring channels of two keys; the even channel goes to row r of the instruction, the odd
 //      one to row r + 8, so a lane ends with two neighbouring output channels of a query;
-//   P: the scores' fragment, rounded, is turned by movmatrix.
-// Rows of shared memory are an odd number of 16-byte units long, so the eight rows of an ldmatrix lie in different banks.
+//   W: the scores' fragment, rounded, is turned by movmatrix.
+// The eight rows of an ldmatrix lie in different banks: 16-byte units are permuted by the row's number where a row is 64, 128 or 256 bytes,
+// else rows are an odd number of units apart.
 #include "common.cuh"
+#include <cuda_fp16.h>
 
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=<multiple of 16>"
@@ -30,11 +39,15 @@ namespace {
 constexpr int HD = HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 in [16, 256]");
 constexpr int CHUNKS = HD / 16;                    // 16-byte units of a row
-constexpr int STRIDE = (CHUNKS | 1) * 16;          // bytes between rows of shared memory
+constexpr bool PERMUTED = HD == 64 || HD == 128 || HD == 256;
+constexpr int STRIDE = PERMUTED ? HD : (CHUNKS | 1) * 16;      // bytes between rows of shared memory
+// where unit c of row r lies in its row
+__device__ __forceinline__ int unit(int r, int c) { return PERMUTED ? c ^ (HD == 64 ? r >> 1 & 3 : r & 7) : c; }
 constexpr int KEYS = 16;                           // keys that a warp works on at a time
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int TILE = 128;                          // keys that slices are counted in: a step of a block's warps, or two
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LEAST_SCALE = 7.888609052210118e-31f;   // 2^-100
 
 struct Params {
     const bf16* q; bf16* out;
@@ -68,7 +81,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -84,14 +97,29 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Two signed bytes of r (chosen by SEL) as bfloat16.  With u the byte's low seven bits, 0x4300 | u is 128 + u, and 0x4300 | (byte & 128) is 128
-// or, with the sign bit in the exponent's lowest place, 256: their difference is the byte's value.
-template <int SEL>
-__device__ __forceinline__ uint32_t widen2(uint32_t r) {
-    const uint32_t w = __byte_perm(r, 0x43434343u, SEL);
-    const uint32_t t = w & 0xff7fff7fu, c = w & 0xff80ff80u;
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two bytes of r (chosen by SEL), each 128 too large, as float16: 1024 more than they are, or themselves less 128.
+template <int SEL> __device__ __forceinline__ uint32_t raised2(uint32_t r) { return __byte_perm(r, 0x64646464u, SEL); }
+template <int SEL> __device__ __forceinline__ uint32_t widen2(uint32_t r) {
     uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(t), "r"(c));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(raised2<SEL>(r)), "r"(0x64806480u));
+    return d;
+}
+constexpr uint32_t TOP_BITS = 0x80808080u;
+constexpr float RAISED = 1152.f;
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
 
@@ -101,6 +129,7 @@ struct Queries {
     uint32_t qf[CHUNKS][NB][2];
     float o[CHUNKS][NB][4];      // channels 16 mb + 2 (lane / 4) (entries 0, 1) and the next (2, 3) of the lane's two queries
     float m[NB][2], l[NB][2];    // l: this lane's keys only
+    float off[NB][2], mul[NB][2];   // a score in powers of two is (product + off) * mul * key's scale
     int pos[NB][2], lo[NB][2];   // position and first visible key; pos < 0: no such query
 };
 
@@ -113,13 +142,39 @@ __device__ __forceinline__ void load_queries(const Params& p, Queries<NB>& s, in
         const int row = row0 + 8 * nb + (lane >> 2);
         const int t = row / p.G;
         const bf16* src = p.q + ((size_t)(tok + t) * p.nh + g * p.G + (row - t * p.G)) * HD + 4 * (lane & 3);
+        unsigned most = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint2 v = row < n_rows ? *reinterpret_cast<const uint2*>(src + 16 * c) : make_uint2(0, 0);
             s.qf[c][nb][0] = v.x; s.qf[c][nb][1] = v.y;
+            most = max(max(most, max(v.x & 0x7fffu, v.x >> 16 & 0x7fffu)), max(v.y & 0x7fffu, v.y >> 16 & 0x7fffu));
         }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // the largest channel's exponent; tiny rows as if it were 2^-112, one with an infinity or NaN as it is
+        unsigned ex = max(most >> 7, 15u);
+        if (ex == 255) ex = 141;
+        const float up = __uint_as_float((268 - ex) << 23), down = __uint_as_float((ex - 14) << 23);
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t v = s.qf[c][nb][i];
+                const uint32_t h = pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                sum += f.x + f.y;
+                s.qf[c][nb][i] = h;
+            }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            // (the lanes that hold the query of column 2 (lane & 3) + e)
+            const int holder = 4 * (2 * (lane & 3) + e);
+            s.off[nb][e] = -RAISED * __shfl_sync(0xffffffffu, sum, holder);
+            s.mul[nb][e] = __shfl_sync(0xffffffffu, down, holder) * p.scale_log2;
             const int col = row0 + 8 * nb + 2 * (lane & 3) + e;
             s.pos[nb][e] = col < n_rows ? q_pos0 + col / p.G : -1;
             s.lo[nb][e] = col < n_rows ? bw::first_visible(s.pos[nb][e], p.window, p.chunk) : 0;
@@ -130,17 +185,18 @@ __device__ __forceinline__ void load_queries(const Params& p, Queries<NB>& s, in
     }
 }
 
-// 16 KG keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page.  KG groups of sixteen keys
-// go side by side: a group's products are a chain, and a warp has little else to do meanwhile.
-// The reference m of a query's exponents follows its largest score lazily: as long as no score is more than 8 above it (a factor of 256) it
-// stays, so most steps need one vote instead of a maximum over the lanes and a pass over the outputs.  Weights stay below 2^8, and what they
-// are divided by has the same reference.
+// 16 KG keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page (what lies in the rows
+// of the others is left over: whole numbers, and scales of any kind).  KG groups of sixteen keys go side by side: a group's products
+// are a chain, and a warp has little else to do meanwhile.
+// The reference follows its largest lazily: as long as nothing is more than 8 above it (a factor of 256) it stays, so most steps need one
+// vote instead of a maximum over the lanes and a pass over the outputs.
 template <int NB, int KG>
 __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint32_t v_rows, const float* ks, const float* vs, int key0,
-                                          unsigned there, bool need_mask, float scale_log2) {
+                                          unsigned there, bool need_mask) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
     // matrices of an ldmatrix: keys 0-7 and 8-15 of one 16-byte unit, then of the next
-    const uint32_t at = (uint32_t)(((lane & 7) + 8 * ((lane >> 3) & 1)) * STRIDE);
+    const int row = (lane & 7) + 8 * (lane >> 3 & 1), more = lane >> 4;
+    const uint32_t at = (uint32_t)(row * STRIDE);
     float sc[KG][NB][4];
 #pragma unroll
     for (int h = 0; h < KG; ++h)
@@ -148,37 +204,47 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
         for (int nb = 0; nb < NB; ++nb) sc[h][nb][0] = sc[h][nb][1] = sc[h][nb][2] = sc[h][nb][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c += 2) {
+        // (an odd last unit: its second pair of matrices reads the first's again)
+        const uint32_t col = at + 16 * unit(row, c + 1 < CHUNKS ? c + more : c);
 #pragma unroll
         for (int h = 0; h < KG; ++h) {
             uint32_t f[4];
-            // (an odd last unit: its second pair of matrices reads the first's again)
-            ldsm4(k_rows + h * KEYS * STRIDE + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
+            ldsm4(k_rows + h * KEYS * STRIDE + col, f);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (c + i >= CHUNKS) break;
-                const uint32_t a[4] = {widen2<0x4140>(f[2 * i]), widen2<0x4140>(f[2 * i + 1]), widen2<0x4342>(f[2 * i]), widen2<0x4342>(f[2 * i + 1])};
+                const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
+                const uint32_t a[4] = {raised2<0x4140>(x), raised2<0x4140>(y), raised2<0x4342>(x), raised2<0x4342>(y)};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) mma(sc[h][nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
             }
         }
     }
-    float most[NB][2];
+    float most[NB][2], per_v[KG][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) most[nb][0] = most[nb][1] = -INFINITY;
 #pragma unroll
     for (int h = 0; h < KG; ++h) {
-        const float k0 = ks[16 * h + r] * scale_log2, k1 = ks[16 * h + r + 8] * scale_log2;
+        float kk[2], lv[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            kk[i] = ks[16 * h + r + 8 * i];
+            const float v = vs[16 * h + r + 8 * i], v1 = v < LEAST_SCALE ? LEAST_SCALE : v;      // (NaN stays)
+            lv[i] = lg2(v1);
+            per_v[h][i] = reciprocal(v1);
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float t = sc[h][nb][i] * (i < 2 ? k0 : k1);
+                const int e = i & 1;
+                float t = fmaf((sc[h][nb][i] + s.off[nb][e]) * s.mul[nb][e], kk[i >> 1], lv[i >> 1]);
                 if (need_mask) {
-                    const int j = 16 * h + r + 8 * (i >> 1), kp = key0 + j, e = i & 1;
+                    const int j = 16 * h + r + 8 * (i >> 1), kp = key0 + j;
                     if (!(kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> j & 1))) t = -INFINITY;
                 }
                 sc[h][nb][i] = t;
-                most[nb][i & 1] = fmaxf(most[nb][i & 1], t);
+                most[nb][e] = fmaxf(most[nb][e], t);
             }
         }
     }
@@ -206,37 +272,37 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
             }
         }
     }
-    uint32_t pf[KG][NB][2];
+    uint32_t wf[KG][NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const float ref[2] = {s.m[nb][0] == -INFINITY ? 0.f : s.m[nb][0], s.m[nb][1] == -INFINITY ? 0.f : s.m[nb][1]};
 #pragma unroll
         for (int h = 0; h < KG; ++h) {
-            const float v0 = vs[16 * h + r], v1 = vs[16 * h + r + 8];
             float w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float t = ex2(sc[h][nb][i] - ref[i & 1]);
-                s.l[nb][i & 1] += t;
+                w[i] = ex2(sc[h][nb][i] - ref[i & 1]);
                 // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
-                w[i] = need_mask && sc[h][nb][i] == -INFINITY ? 0.f : t * (i < 2 ? v0 : v1);
+                s.l[nb][i & 1] += need_mask && sc[h][nb][i] == -INFINITY ? 0.f : w[i] * per_v[h][i >> 1];
             }
-            pf[h][nb][0] = turn8x8(bw::pack_bf16x2(w[0], w[1]));
-            pf[h][nb][1] = turn8x8(bw::pack_bf16x2(w[2], w[3]));
+            wf[h][nb][0] = turn8x8(pack_f16x2(w[0], w[1]));
+            wf[h][nb][1] = turn8x8(pack_f16x2(w[2], w[3]));
         }
     }
 #pragma unroll
-    for (int h = 0; h < KG; ++h) {
+    for (int c = 0; c < CHUNKS; c += 2) {
+        const uint32_t col = at + 16 * unit(row, c + 1 < CHUNKS ? c + more : c);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) {
+        for (int h = 0; h < KG; ++h) {
             uint32_t f[4];
-            ldsm4_t(v_rows + h * KEYS * STRIDE + at + 16 * (c + 1 < CHUNKS ? c + (lane >> 4) : c), f);
+            ldsm4_t(v_rows + h * KEYS * STRIDE + col, f);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (c + i >= CHUNKS) break;
-                const uint32_t a[4] = {widen2<0x4240>(f[2 * i]), widen2<0x4341>(f[2 * i]), widen2<0x4240>(f[2 * i + 1]), widen2<0x4341>(f[2 * i + 1])};
+                const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
+                const uint32_t a[4] = {widen2<0x4240>(x), widen2<0x4341>(x), widen2<0x4240>(y), widen2<0x4341>(y)};
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, pf[h][nb][0], pf[h][nb][1]);
+                for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, wf[h][nb][0], wf[h][nb][1]);
             }
         }
     }
@@ -251,42 +317,89 @@ __device__ __forceinline__ int key_row(const Params& p, const int* bt, int g, in
     return page >= 0 && page < p.num_pages ? (page * p.nkv + g) * p.page_size + (key - blk * p.page_size) : -1;
 }
 
-// 16 KG keys into a stage (rows of K, of V, their scales), by one warp; `row`: key_row of key lane (of lane & 15 with KG 1) in every lane.
+// 16 KG keys into a stage (rows of K, of V, their scales), by one warp.  What is held is looked up a step ahead of its use (`find`).
+// WHOLE: pages are a multiple of sixteen keys long, so sixteen keys are one stretch of memory and need one look-up; places behind the
+// request's last token are read with the others (and masked).  Otherwise every lane looks up a key of its own.
 template <int KG> constexpr int STAGE = 2 * KG * KEYS * (STRIDE + 4);
-template <int KG>
-__device__ __forceinline__ void fetch(const Params& p, uint8_t* stage, int row) {
-    constexpr int N = KG * KEYS;
-    const int lane = threadIdx.x & 31;
-    const uint32_t k_to = smem_u32(stage), v_to = k_to + N * STRIDE, s_to = v_to + N * STRIDE;
+template <int KG, bool WHOLE>
+struct Feed {
+    static constexpr int N = KG * KEYS;
+    int row[WHOLE ? KG : 1];
+    __device__ __forceinline__ void find(const Params& p, const int* bt, int g, int key0, int end, int kv_len) {
+        if constexpr (WHOLE) {
 #pragma unroll
-    for (int i = 0; i < (N * CHUNKS + 31) / 32; ++i) {
-        const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
-        const int rw = __shfl_sync(0xffffffffu, row, key & (N - 1));
-        if ((N * CHUNKS) % 32 && key >= N) break;
-        const size_t off = rw >= 0 ? (size_t)rw * HD + 16 * c : 0;
-        cp_async16(k_to + key * STRIDE + 16 * c, p.k + off, rw >= 0);
-        cp_async16(v_to + key * STRIDE + 16 * c, p.v + off, rw >= 0);
+            for (int h = 0; h < KG; ++h) row[h] = key0 + 16 * h < end ? key_row(p, bt, g, key0 + 16 * h, kv_len) : -1;
+        } else {
+            row[0] = key0 < end ? key_row(p, bt, g, key0 + (threadIdx.x & (N - 1)), kv_len) : -1;
+        }
     }
-    const int from = row >= 0 ? row : 0;
-    if constexpr (KG == 1) {
-        cp_async4(s_to + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + from, row >= 0);
-    } else {
-        cp_async4(s_to + 4 * lane, p.k_scale + from, row >= 0);
-        cp_async4(s_to + 4 * (lane + N), p.v_scale + from, row >= 0);
+    // which keys are held, as bits
+    __device__ __forceinline__ unsigned fetch(const Params& p, uint8_t* stage) const {
+        const int lane = threadIdx.x & 31;
+        const uint32_t k_to = smem_u32(stage), v_to = k_to + N * STRIDE, s_to = v_to + N * STRIDE;
+        if constexpr (WHOLE) {
+            unsigned got = 0;
+#pragma unroll
+            for (int h = 0; h < KG; ++h) {
+                if (row[h] < 0) continue;        // (uniform)
+                got |= 0xffffu << (16 * h);
+                const int8_t* k_from = p.k + (size_t)row[h] * HD + 16 * lane;
+                const int8_t* v_from = p.v + (size_t)row[h] * HD + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
+                    const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
+                    if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
+                    const uint32_t to = (16 * h + key) * STRIDE + 16 * unit(key, c);
+                    cp_async16(k_to + to, k_from + 512 * i, true);
+                    cp_async16(v_to + to, v_from + 512 * i, true);
+                }
+                cp_async4(s_to + 4 * ((lane < 16 ? 0 : N - 16) + 16 * h + lane), (lane < 16 ? p.k_scale : p.v_scale) + row[h] + (lane & 15), true);
+            }
+            return got;
+        } else {
+            const unsigned got = __ballot_sync(0xffffffffu, row[0] >= 0);
+#pragma unroll
+            for (int i = 0; i < (N * CHUNKS + 31) / 32; ++i) {
+                const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
+                const int rw = __shfl_sync(0xffffffffu, row[0], key & (N - 1));
+                if ((N * CHUNKS) % 32 && key >= N) break;
+                const size_t off = rw >= 0 ? (size_t)rw * HD + 16 * c : 0;
+                const uint32_t to = key * STRIDE + 16 * unit(key, c);
+                cp_async16(k_to + to, p.k + off, rw >= 0);
+                cp_async16(v_to + to, p.v + off, rw >= 0);
+            }
+            const int from = row[0] >= 0 ? row[0] : 0;
+            if constexpr (KG == 1) {
+                cp_async4(s_to + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + from, row[0] >= 0);
+            } else {
+                cp_async4(s_to + 4 * lane, p.k_scale + from, row[0] >= 0);
+                cp_async4(s_to + 4 * (lane + N), p.v_scale + from, row[0] >= 0);
+            }
+            return got & (N == 32 ? 0xffffffffu : (1u << (N & 31)) - 1);
+        }
     }
-}
+};
 
 // ---------------------------------------------------------------------------------------------------------------- few queries
 // All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
 // with a ring of its own, and are joined at the end.  Slices are equally long for every request; how many of them a request has follows
 // from its length on the device, so the same launch serves a captured step whatever the lengths become.
-// Queries in registers beside two groups of keys: up to 256 channels of queries (one block of eight of up to 256, two of up to 128).
-template <int NB> constexpr int FEW_KG = NB * HD <= 256 ? 2 : 1;
-constexpr int STAGES = 3;
+#ifndef Q8_KG
+#define Q8_KG 1
+#endif
+#ifndef Q8_STAGES
+#define Q8_STAGES 3
+#endif
+template <int NB> constexpr int FEW_KG = NB * HD <= 128 ? Q8_KG : 1;
+constexpr int STAGES = Q8_STAGES;
 template <int NB> constexpr int SMEM_RING = WARPS * STAGES * STAGE<FEW_KG<NB>>;
 constexpr int JOIN_LD = HD + 8;
 constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD) * 4;
 template <int NB> constexpr int SMEM_FEW = SMEM_RING<NB> > SMEM_JOIN ? SMEM_RING<NB> : SMEM_JOIN;
+// blocks an SM runs at once: by shared memory, and by registers (about 60 beside the queries and outputs)
+template <int NB> constexpr int BY_SMEM = (227 * 1024) / (SMEM_FEW<NB> + 1024);
+template <int NB> constexpr int BY_REGS = 512 / (((60 + NB * CHUNKS * 6) + 7) / 8 * 8);
+template <int NB> constexpr int FEW_BLOCKS = BY_SMEM<NB> < BY_REGS<NB> ? (BY_SMEM<NB> > 0 ? BY_SMEM<NB> : 1) : (BY_REGS<NB> > 0 ? BY_REGS<NB> : 1);
 
 struct Walk { int first, tiles, per, live; };   // in tiles of TILE keys: where it begins, how many, of a slice; slices that have any
 __device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last) {
@@ -308,8 +421,8 @@ __device__ __forceinline__ void write_row(const Params& p, size_t token, int hea
 }
 __device__ __forceinline__ float sink_term(const Params& p, int head, float M) { return p.sink ? exp2f(p.sink[head] * LOG2E - M) : 0.f; }
 
-template <int NB>
-__global__ void __launch_bounds__(THREADS)
+template <int NB, bool WHOLE>
+__global__ void __launch_bounds__(THREADS, FEW_BLOCKS<NB>)
 few_kernel(Params p) {
     BW_PDL_TRIGGER();
     extern __shared__ __align__(16) uint8_t smem[];
@@ -328,14 +441,13 @@ few_kernel(Params p) {
     uint8_t* ring = smem + warp * STAGES * STAGE<KG>;
     // a warp's steps: every fourth N keys of the slice
     const int first = t0 * TILE + warp * N, end = min(t1 * TILE, last + 1);
-    // the row of this lane's key of the next step that is fetched: looked up a step ahead of its use
-    int next = first < end ? key_row(p, bt, g, first + (lane & (N - 1)), kv_len) : -1;
+    Feed<KG, WHOLE> next;
+    next.find(p, bt, g, first, end, kv_len);
     unsigned there[STAGES];
     auto feed = [&](int key0, int st) {
         if (key0 < end) {
-            there[st] = __ballot_sync(0xffffffffu, next >= 0) & ALL;
-            fetch<KG>(p, ring + st * STAGE<KG>, next);
-            next = key0 + WARPS * N < end ? key_row(p, bt, g, key0 + WARPS * N + (lane & (N - 1)), kv_len) : -1;
+            there[st] = next.fetch(p, ring + st * STAGE<KG>);
+            next.find(p, bt, g, key0 + WARPS * N, end, kv_len);
         }
         cp_async_commit();
     };
@@ -355,7 +467,7 @@ few_kernel(Params p) {
             const uint32_t at = smem_u32(ring + st * STAGE<KG>);
             const float* sc = reinterpret_cast<const float*>(ring + st * STAGE<KG> + 2 * N * STRIDE);
             const bool need_mask = there[st] != ALL || key0 + N - 1 > q_pos0 || key0 < see_all;
-            some_keys<NB, KG>(s, at, at + N * STRIDE, sc, sc + N, key0, there[st], need_mask, p.scale_log2);
+            some_keys<NB, KG>(s, at, at + N * STRIDE, sc, sc + N, key0, there[st], need_mask);
             __syncwarp();
         }
     }
@@ -485,10 +597,10 @@ many_kernel(Params p, Portions work) {
     auto feed = [&](int t) {
         if (t < t1) {
             const int st = (t - t0) % RING;
-            const int row = key_row(p, bt, g, t * MANY_TILE + warp * KEYS + (lane & 15), kv_len);
-            const unsigned b = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            Feed<1, false> f;
+            f.find(p, bt, g, t * MANY_TILE + warp * KEYS, kv_len, kv_len);
+            const unsigned b = f.fetch(p, smem + (st * WARPS + warp) * STAGE<1>);
             if (lane == 0) there[st * WARPS + warp] = b;
-            fetch<1>(p, smem + (st * WARPS + warp) * STAGE<1>, row);
         }
         cp_async_commit();
     };
@@ -510,7 +622,7 @@ many_kernel(Params p, Portions work) {
                 const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
                 const unsigned ok = there[st * WARPS + w];
                 const bool need_mask = ok != 0xffffu || key0 + KEYS - 1 > my_first || key0 < see_all;
-                some_keys<2, 1>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask, p.scale_log2);
+                some_keys<2, 1>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask);
             }
         }
         __syncthreads();
@@ -565,8 +677,7 @@ BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int req
     }
     *per = 1;
     if (most == 0) return 0;
-    constexpr int at_once = (227 * 1024) / (SMEM_FEW<1> + 1024);
-    const long long room = (long long)(at_once < 4 ? at_once : 4) * bw::num_sms();          // blocks that run at once
+    const long long room = (long long)FEW_BLOCKS<1> * bw::num_sms();          // blocks that run at once
     long long lo = 1, hi = most;
     while (lo < hi) {
         const long long mid = (lo + hi) / 2;
@@ -576,6 +687,15 @@ BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int req
     }
     *per = (int)lo;
     return (int)((most + lo - 1) / lo);
+}
+
+template <int NB, bool WHOLE>
+static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
+    static bool done[bw::MAX_DEVICES];
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<NB, WHOLE>, SMEM_FEW<NB>, done); e != cudaSuccess) return (int)e;
+    bw::launch(few_kernel<NB, WHOLE>, grid, dim3(THREADS), SMEM_FEW<NB>, s, p);
+    BW_LAUNCH_CHECK();
+    return 0;
 }
 
 // q, out: bfloat16 [tokens][nh][HD]; lengths on the host (q_len, h_q_start) as in bw_attention_q8_plan, per and slices as it gave them; part_o,
@@ -591,9 +711,7 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, part_o, part_ml,
              max_blocks, nh, nkv, G, page_size, num_pages, window > 0 ? window : 0, chunk > 0 ? chunk : 0, requests, per, slices, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
-    static bool few1_done[bw::MAX_DEVICES], few2_done[bw::MAX_DEVICES], many_done[bw::MAX_DEVICES];
-    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<1>, SMEM_FEW<1>, few1_done); e != cudaSuccess) return (int)e;
-    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<2>, SMEM_FEW<2>, few2_done); e != cudaSuccess) return (int)e;
+    static bool many_done[bw::MAX_DEVICES];
     if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
     Portions work{};
     int most_rows = 0;
@@ -623,8 +741,9 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
     const dim3 grid((unsigned)slices, (unsigned)nkv, (unsigned)requests);
-    if (few1) { bw::launch(few_kernel<1>, grid, dim3(THREADS), SMEM_FEW<1>, s, p); BW_LAUNCH_CHECK(); }
-    if (few2) { bw::launch(few_kernel<2>, grid, dim3(THREADS), SMEM_FEW<2>, s, p); BW_LAUNCH_CHECK(); }
+    const bool whole = page_size % KEYS == 0;
+    if (few1) if (const int e = whole ? launch_few<1, true>(p, grid, s) : launch_few<1, false>(p, grid, s)) return e;
+    if (few2) if (const int e = whole ? launch_few<2, true>(p, grid, s) : launch_few<2, false>(p, grid, s)) return e;
     if (slices > 1) {
         bw::launch(join_kernel, dim3((unsigned)most_rows, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
         BW_LAUNCH_CHECK();

@@ -41,14 +41,15 @@ def row_index(positions, req, table, page_size):
 
 
 def attention(q, k, v, ks, vs, cu_q, q_start, kv_len, table, scale, window=0, chunk=0, sink=None):
-    """(out, sum of p |v|, sum over channels of |q k| of the largest key) of every (token, head, channel), float64.  q [T, nh, hd] and the
-    pages as the kernels get them, moved to the CPU."""
+    """(out, sum of p |v|, largest scale * sum of |q| * 1280 ks of a key, largest p vs of a key times the sum of its channel's numbers) of
+    every (token, head, channel), float64.  q [T, nh, hd] and the pages as the kernels get them, moved to the CPU."""
     T, nh, hd = q.shape
     num_pages, nkv, page, _ = k.shape
     G = nh // nkv
     out = torch.zeros(T, nh, hd, dtype=torch.float64)
     mass = torch.zeros_like(out)
     score_abs = torch.zeros(T, nh, 1, dtype=torch.float64)
+    least = torch.zeros_like(out)
     for r in range(len(q_start)):
         for t in range(int(cu_q[r]), int(cu_q[r + 1])):
             pos = int(q_start[r]) + t - int(cu_q[r])
@@ -76,15 +77,20 @@ def attention(q, k, v, ks, vs, cu_q, q_start, kv_len, table, scale, window=0, ch
                 p = e / total
                 out[t, g * G:(g + 1) * G] = p @ vv
                 mass[t, g * G:(g + 1) * G] = p @ vv.abs()
-                score_abs[t, g * G:(g + 1) * G, 0] = (qq.abs() @ kk.abs().t()).amax(-1) * scale
-    return out, mass, score_abs
+                score_abs[t, g * G:(g + 1) * G, 0] = qq.abs().sum(-1) * 1280 * ks[pid, g, slot].double().max() * scale
+                w = (p * vs[pid, g, slot].double()).amax(-1, keepdim=True)
+                least[t, g * G:(g + 1) * G] = w * v[pid, g, slot].double().abs().sum(0)
+    return out, mass, score_abs, least
 
 
-def attention_bound(out, mass, score_abs, hd):
-    """What the kernels may be off by: the result's rounding to bfloat16 (2^-8 of it), the weights' (2^-8 of sum p |v|, and of what that moves), and
-    the float32 arithmetic: a score is a sum of hd products (each partial sum off by at most 2^-23 of the sum of magnitudes, as the matrix
-    units may cut instead of round) times two factors, taken as an exponent in weights and denominator; the exponential 2^-21; sums of
-    weights and outputs in float32, 2^-16 for the longest lists tested here."""
+def attention_bound(out, mass, score_abs, least, hd):
+    """What the kernels may be off by:
+      the result's rounding to bfloat16, 2^-8 of it;
+      the weights', p vs in float16: 2^-11 of each, so of sum p |v|, and where that is less than its smallest step, 2^-25 of the largest weight;
+      a score's: hd / 16 products of sixteen terms added in the matrix units, where a key's numbers stand 1152 too high (below 1280), each
+      sum cut at 2^-23 of the magnitudes so far, and two steps for what comes off and the factors; as an exponent it is in weights
+      and denominator;
+      2^-16 for exponentials, and sums of the longest lists tested here in float32."""
     u = 2.0 ** -8
-    ds = (hd + 8) * 2.0 ** -23 * score_abs
-    return u * out.abs() + (u * (1 + u) + 2 * torch.expm1(2 * ds) + 2.0 ** -16) * mass + 1e-30
+    ds = (hd / 16 + 2) * 2.0 ** -23 * score_abs
+    return u * out.abs() + (1 + u) * ((2.0 ** -11 + 2 * torch.expm1(2 * ds) + 2.0 ** -16) * mass + 2.0 ** -25 * least) + 1e-30

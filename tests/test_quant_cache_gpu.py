@@ -78,9 +78,9 @@ class Case:
         b = self.batch(bound)
         got = ops.quant_attention(q.cuda(), pages or self.pages(), b, b.block_tables[0], nh, scale, window or None, chunk or None,
                                   None if sink is None else sink.cuda())
-        want, mass, score_abs = attention(q.view(self.T, nh, self.hd), self.k, self.v, self.k_scale, self.v_scale, self.cu, self.start, self.total,
+        want, mass, score_abs, least = attention(q.view(self.T, nh, self.hd), self.k, self.v, self.k_scale, self.v_scale, self.cu, self.start, self.total,
                                           self.table, scale, window, chunk, sink)
-        tol = attention_bound(want, mass, score_abs, self.hd)
+        tol = attention_bound(want, mass, score_abs, least, self.hd)
         got = got.cpu().double().view_as(want)
         assert torch.isfinite(got).all()
         over = ((got - want).abs() / tol).max().item()
@@ -276,8 +276,8 @@ def test_attention_in_a_graph_of_any_length():
         fresh = torch.randn(c.T, 8 * 128, generator=c.gen).to(torch.bfloat16)
         q.copy_(fresh)
         graph.replay()
-        want, mass, score_abs = attention(fresh.view(3, 8, 128), c.k, c.v, c.k_scale, c.v_scale, c.cu, starts, [s + 1 for s in starts], c.table, 0.088)
-        tol = attention_bound(want, mass, score_abs, 128)
+        want, mass, score_abs, least = attention(fresh.view(3, 8, 128), c.k, c.v, c.k_scale, c.v_scale, c.cu, starts, [s + 1 for s in starts], c.table, 0.088)
+        tol = attention_bound(want, mass, score_abs, least, 128)
         assert ((out.cpu().double().view_as(want) - want).abs() <= tol).all()
 
 
