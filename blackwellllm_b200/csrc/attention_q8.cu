@@ -388,7 +388,7 @@ struct Feed {
 #define Q8_KG 1
 #endif
 #ifndef Q8_STAGES
-#define Q8_STAGES 3
+#define Q8_STAGES 2
 #endif
 template <int NB> constexpr int FEW_KG = NB * HD <= 128 ? Q8_KG : 1;
 constexpr int STAGES = Q8_STAGES;
@@ -699,11 +699,11 @@ static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
 }
 
 // q, out: bfloat16 [tokens][nh][HD]; lengths on the host (q_len, h_q_start) as in bw_attention_q8_plan, per and slices as it gave them; part_o,
-// part_ml: room for requests * nkv * slices * 16 rows of HD and of 2 floats, where slices > 1.
+// part_ml: room for requests * nkv * slices * 16 rows of HD and of 2 floats, where slices > 1; few_only: requests with more rows are left out.
 BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
                               const int* cu_q, const int* q_start, const int* kv_len, const int* table, int max_blocks, const int* h_q_len,
                               int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, float scale,
-                              const float* sink, int per, int slices, float* part_o, float* part_ml, void* stream) {
+                              const float* sink, int per, int slices, float* part_o, float* part_ml, int few_only, void* stream) {
     if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || per <= 0) return BW_ERR_BAD_ARG;
     if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v) & 15) || (slices > 1 && (!part_o || !part_ml))) return BW_ERR_BAD_ARG;
     if ((long long)num_pages * nkv * page_size > 0x7fffffffll || nkv > 65535 || requests > 65535) return BW_ERR_UNSUPPORTED;
@@ -732,6 +732,7 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
             if (rows > most_rows) most_rows = (int)rows;
             continue;
         }
+        if (few_only) continue;
         if (rows > 0x7fffffffll / 2) return BW_ERR_UNSUPPORTED;
         work.request[work.n] = r;
         work.first[work.n + 1] = work.first[work.n] + (int)((rows + ROWS - 1) / ROWS);

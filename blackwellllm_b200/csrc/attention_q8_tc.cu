@@ -1,0 +1,699 @@
+// Attention over the 8-bit cache for portions of prompts, on the 5th-generation tensor cores (head size HEAD_DIM: a compile-time multiple
+// of 64 up to 256; what attention_q8.cu says of the formula holds here).
+//
+// A block works on 256 stacked rows (row = token * G + head of the group) of one (request, kv head) as two tiles of 128 (one, of head sizes
+// above 128: tensor memory holds no more) against tiles of 64 keys:
+//   * four warps widen: rows of whole numbers from the cache (16 bytes a load, straight into registers) become float16 times the row's scale
+//     over the largest scale of the 64 (a power of two, which goes back into the scores, and for the values into the exponent), and
+//     are written as the 128-byte-swizzled operands of the tensor cores.  Both tiles of rows use them: widening is a third of the
+//     block's instructions, and the reason why a block has 256 rows and is alone on its SM;
+//   * one warp issues the products: S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, O += P V with P from tensor memory;
+//   * eight warps, one thread a row, make P: maximum, exponentials, sums; P is written over the S it came from as float16 pairs.
+// Roundings: K and V to float16 (2^-11 of an element; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
+// beside the largest), and the result to bfloat16.  Scores, sums and outputs are float32; the queries are multiplied by a power of two a row
+// (attention_q8.cu) and exact.  The exponents' reference follows the largest t + log2 of the tile's value scale lazily (by steps of more than
+// 8), so O is seldom rescaled.
+// A key that is no number (its scale, or its value's, is NaN) has NaN as its score: rows that see it become NaN, masked rows do not.  Keys behind
+// the request's end or on a page that is not held are zeros, and masked.
+//
+// Work is the list of all (rows, tile of keys) steps of the launch, cut into equal stretches, one a block, so that the last wave is not mostly
+// empty and a few rows over many keys still fill the GPU.  A stretch that begins or ends inside a block of rows leaves its sums in
+// memory; join_kernel adds them in the order of the keys.  Every wait is bounded (status word).
+#include "tcgen05.cuh"
+#include <cuda_fp16.h>
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<multiple of 64>"
+#endif
+
+using bf16 = __nv_bfloat16;
+
+namespace {
+
+constexpr int HD = HEAD_DIM;
+static_assert(HD % 64 == 0 && HD >= 64 && HD <= 256, "head size must be a multiple of 64 in [64, 256]");
+constexpr int NS = HD / 64;                 // 128-byte slices of a widened row
+constexpr int BM = 128, BN = 64;
+constexpr int NQ = HD <= 128 ? 2 : 1;       // tiles of rows a block
+constexpr int ROWS = NQ * BM;
+constexpr int STAGES = 2;
+constexpr int Q_SLICE = BM * 128, KV_SLICE = BN * 128;
+constexpr int Q_BYTES = NS * Q_SLICE, KV_BYTES = NS * KV_SLICE;
+constexpr int RING = STAGES + 2;            // what the softmax reads of a tile of keys: a widening warp is at most that far ahead of it
+constexpr int WIDEN_WARPS = 4, MMA_WARP = 4 * NQ + WIDEN_WARPS;
+constexpr int THREADS = 32 * (MMA_WARP + 1);
+constexpr int SMEM_BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + RING * 32 + 32 * 8 + 16;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t idesc_f16(int N, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+constexpr uint32_t IDESC_QK = idesc_f16(BN, false), IDESC_PV = idesc_f16(HD, true);
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MOST_BLOCKS = 160;            // blocks of a launch
+constexpr int MOST_PORTIONS = 16;           // requests of a launch
+
+__device__ int g_status = 0;
+
+struct Params {
+    const bf16* q; bf16* out;
+    const int8_t* k; const int8_t* v; const float* k_scale; const float* v_scale;
+    const int* kv_len; const int* table; const float* sink;
+    float* part_o; float* part_ml;          // [2 x blocks][HD / 4][ROWS][4] and [2 x blocks][ROWS][2]
+    int max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, portions;
+    float scale_log2;
+};
+struct Portion { int request, tok, n_tok, q_pos0, first, n_blocks; };      // first: the first of its n_blocks * nkv items
+struct Work {
+    Portion portion[MOST_PORTIONS];
+    int item[MOST_BLOCKS], offset[MOST_BLOCKS], steps[MOST_BLOCKS];        // where a block's stretch begins, and its length
+};
+struct Splits { int n; int item[MOST_BLOCKS]; short from[MOST_BLOCKS], to[MOST_BLOCKS]; };   // items that several blocks share: from .. to
+
+// An item: 256 rows of one (request, kv head).
+struct Item {
+    int request, tok, g, row0, n_rows, q_pos0, t0, tiles;    // tok: its request's first token; t0, tiles: the tiles of keys that its rows see
+};
+__host__ __device__ __forceinline__ void tiles_of(int q_pos0, int row0, int n_rows, int G, int window, int chunk, int& t0, int& n) {
+    const int first = q_pos0 + row0 / G, last = q_pos0 + (row0 + n_rows - 1) / G;
+    t0 = bw::first_visible(first, window, chunk) / BN;
+    n = last / BN + 1 - t0;
+}
+__host__ __device__ __forceinline__ Item item_of(const Portion* portions, int count, int index, int nkv, int G, int window, int chunk) {
+    int i = 0;
+    while (i + 1 < count && index >= portions[i + 1].first) ++i;
+    const Portion& p = portions[i];
+    const int local = index - p.first, block = p.n_blocks - 1 - local / nkv;      // the latest rows first: they have the most keys
+    Item it;
+    it.request = p.request; it.tok = p.tok; it.g = local % nkv; it.row0 = block * ROWS; it.q_pos0 = p.q_pos0;
+    const int all = p.n_tok * G;
+    it.n_rows = all - it.row0 < ROWS ? all - it.row0 : ROWS;
+    tiles_of(it.q_pos0, it.row0, it.n_rows, G, window, chunk, it.t0, it.tiles);
+    return it;
+}
+
+// A block's walk over its stretch: tiles of one item after another.
+struct Walk {
+    int index, offset, left;     // the item, tiles of it that lie before, steps to go (with the current one)
+    Item it;
+    int tile, end;               // of the current item's part: the tile, and the first behind the part
+    bool opens, closes;          // the part begins, or ends, with the item
+    __device__ __forceinline__ void open(const Params& p, const Work& w) {
+        it = item_of(w.portion, p.portions, index, p.nkv, p.G, p.window, p.chunk);
+        const int n = min(left, it.tiles - offset);
+        tile = it.t0 + offset;
+        end = tile + n;
+        opens = offset == 0; closes = offset + n == it.tiles;
+    }
+    __device__ __forceinline__ void start(const Params& p, const Work& w) {
+        index = w.item[blockIdx.x]; offset = w.offset[blockIdx.x]; left = w.steps[blockIdx.x];
+        if (left > 0) open(p, w);
+    }
+    // to the next step; true if it is the first of another item
+    __device__ __forceinline__ bool step(const Params& p, const Work& w) {
+        --left; ++tile;
+        if (tile < end || left == 0) return false;
+        ++index; offset = 0;
+        open(p, w);
+        return true;
+    }
+    // past the whole part
+    __device__ __forceinline__ void pass(const Params& p, const Work& w) {
+        left -= end - tile;
+        if (left == 0) return;
+        ++index; offset = 0;
+        open(p, w);
+    }
+};
+__device__ __forceinline__ int q_tiles(const Item& it) { return NQ == 2 && it.n_rows > BM ? 2 : 1; }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ bw::f32x2 add2(bw::f32x2 a, bw::f32x2 b) {
+    bw::f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// A row's factor as two float16 numbers that add up to it, each twice.
+struct Factor { uint32_t hi, lo; };
+__device__ __forceinline__ Factor factor_of(float f) {
+    const float hi = __half2float(__float2half_rn(f));
+    return {pack_f16x2(f, f), pack_f16x2(f - hi, f - hi)};
+}
+// Two bytes of r (128 too large) times the factor, in float16: 0x6400 | byte is 1024 + byte, 1152 less is the whole number, exact; its product with
+// the factor is rounded once (the low part's product is 2^-11 of it and rounded by 2^-11 of that).
+template <int SEL>
+__device__ __forceinline__ uint32_t widen2(uint32_t r, const Factor& f) {
+    uint32_t n, d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(n) : "r"(__byte_perm(r, 0x64646464u, SEL)), "r"(0x64806480u));
+    asm("{\n.reg .b32 t;\nmul.rn.f16x2 t, %1, %2;\nfma.rn.f16x2 %0, %1, %3, t;\n}" : "=r"(d) : "r"(n), "r"(f.lo), "r"(f.hi));
+    return d;
+}
+// 16 channels (unit c) of key `key` into a tile of operands
+__device__ __forceinline__ void widen16(uint8_t* tile, int key, int c, uint4 x, const Factor& f) {
+    const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+    uint8_t* row = tile + (c >> 2) * KV_SLICE + key * 128;
+    const int u = 2 * (c & 3), k7 = key & 7;
+    *reinterpret_cast<uint4*>(row + ((u ^ k7) << 4)) =
+        make_uint4(widen2<0x4140>(w[0], f), widen2<0x4342>(w[0], f), widen2<0x4140>(w[1], f), widen2<0x4342>(w[1], f));
+    *reinterpret_cast<uint4*>(row + (((u + 1) ^ k7) << 4)) =
+        make_uint4(widen2<0x4140>(w[2], f), widen2<0x4342>(w[2], f), widen2<0x4140>(w[3], f), widen2<0x4342>(w[3], f));
+}
+// The smallest power of two that is not below any finite one of a warp's non-negative numbers (bits of the largest); at least 2^-100.
+__device__ __forceinline__ float power_above(unsigned bits) {
+    const unsigned up = (bits + 0x7fffffu) & 0x7f800000u;
+    return __uint_as_float(max(up, 27u << 23));
+}
+
+// What the softmax needs of a tile of keys.
+struct TileInfo { float k_ref, log2_v, inv_v, pad; unsigned there[2]; unsigned pad2[2]; };
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work) {
+    BW_PDL_TRIGGER();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* q_s = smem;                                // [NQ][Q_BYTES]
+    uint8_t* k_s = q_s + NQ * Q_BYTES;                  // [STAGES][KV_BYTES]
+    uint8_t* v_s = k_s + STAGES * KV_BYTES;
+    TileInfo* info = reinterpret_cast<TileInfo*>(v_s + STAGES * KV_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(info + RING);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+    const uint32_t bar0 = bw::smem_u32(bars);
+    const uint32_t q_full = bar0, k_full = bar0 + 8 * NQ, k_empty = k_full + 8 * STAGES, v_full = k_empty + 8 * STAGES, v_empty = v_full + 8 * STAGES;
+    const uint32_t s_full = v_empty + 8 * STAGES, p_full = s_full + 16 * NQ, pv_done = p_full + 16 * NQ;     // [tile of rows][buffer]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int q = 0; q < NQ; ++q) bw::mbar_init(q_full + 8 * q, 4);
+        for (int s = 0; s < STAGES; ++s) {
+            bw::mbar_init(k_full + 8 * s, WIDEN_WARPS); bw::mbar_init(v_full + 8 * s, WIDEN_WARPS);
+            bw::mbar_init(k_empty + 8 * s, 1); bw::mbar_init(v_empty + 8 * s, 1);
+        }
+        for (int s = 0; s < 2 * NQ; ++s) {
+            bw::mbar_init(s_full + 8 * s, 1); bw::mbar_init(p_full + 8 * s, 4); bw::mbar_init(pv_done + 8 * s, 1);
+        }
+        bw::fence_barrier_init();
+        tmem_slot[1] = (uint32_t)g_status;
+    }
+    if (warp == MMA_WARP) bw::tmem_alloc(bw::smem_u32(tmem_slot), TMEM_COLS);
+    bw::tc_fence_before();
+    __syncthreads();
+    bw::tc_fence_after();
+    BW_PDL_WAIT();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_O = tmem_base + 128 * NQ;        // S: [tile of rows][buffer] of 64 columns, then O: [tile of rows] of HD
+    auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+
+    Walk w;
+    w.start(p, work);
+    if (tmem_slot[1] != 0) w.left = 0;                   // an earlier launch gave up: nothing is done
+
+    if (warp == MMA_WARP) {
+        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem_base, 0), q0 = bw::smem_u32(q_s), k0 = bw::smem_u32(k_s), v0 = bw::smem_u32(v_s);
+        int n_q[2] = {0, 0}, loaded[2] = {0, 0};         // of each tile of rows: steps that S was issued for, times that its queries came
+        bool ok = true;
+        // S of step `it` of the walk
+        auto issue_qk = [&](int it, int tiles_q) {
+            const int s = it % STAGES;
+            if (!all(bw::mbar_wait(k_full + 8 * s, (it / STAGES) & 1, &g_status, 32))) return false;
+            for (int q = 0; q < tiles_q; ++q) {
+                const int b = n_q[q] & 1;
+                // the buffer holds P of the step before last, which the P V issued for it may still read
+                if (n_q[q] >= 2 && !all(bw::mbar_wait(pv_done + 8 * (2 * q + b), ((n_q[q] >> 1) - 1) & 1, &g_status, 33))) return false;
+                bw::tc_fence_after();
+                if (bw::elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        const uint64_t da = bw::umma_smem_desc_sw128(q0 + q * Q_BYTES + (ks >> 2) * Q_SLICE) + 2 * (ks & 3);
+                        const uint64_t db = bw::umma_smem_desc_sw128(k0 + s * KV_BYTES + (ks >> 2) * KV_SLICE) + 2 * (ks & 3);
+                        bw::umma_bf16(tmem0 + 128 * q + 64 * b, da, db, IDESC_QK, ks != 0);
+                    }
+                    bw::umma_commit(s_full + 8 * (2 * q + b));
+                    if (q == tiles_q - 1) bw::umma_commit(k_empty + 8 * s);
+                }
+                __syncwarp();
+                ++n_q[q];
+            }
+            return true;
+        };
+        // P V of step `it`, whose S has numbers c[] among the steps of its tiles of rows
+        auto issue_pv = [&](int it, int tiles_q, const int (&c)[2], bool first) {
+            const int s = it % STAGES;
+            if (!all(bw::mbar_wait(v_full + 8 * s, (it / STAGES) & 1, &g_status, 34))) return false;
+            for (int q = 0; q < tiles_q; ++q) {
+                const int b = c[q] & 1;
+                if (!all(bw::mbar_wait(p_full + 8 * (2 * q + b), (c[q] >> 1) & 1, &g_status, 35))) return false;
+                bw::tc_fence_after();
+                if (bw::elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < BN / 16; ++kk) {
+                        const uint64_t db = bw::umma_smem_desc_mn_sw128(v0 + s * KV_BYTES, KV_SLICE) + (uint64_t)kk * (2048 >> 4);
+                        bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, db, IDESC_PV, !(first && kk == 0));
+                    }
+                    bw::umma_commit(pv_done + 8 * (2 * q + b));
+                    if (q == tiles_q - 1) bw::umma_commit(v_empty + 8 * s);
+                }
+                __syncwarp();
+            }
+            return true;
+        };
+        auto begin_item = [&](int tiles_q) {
+            for (int q = 0; q < tiles_q; ++q) {
+                if (!all(bw::mbar_wait(q_full + 8 * q, loaded[q] & 1, &g_status, 36))) return false;
+                ++loaded[q];
+            }
+            return true;
+        };
+        int it = 0;
+        if (w.left > 0) {
+            int cur_q = q_tiles(w.it), c[2] = {0, 0};
+            bool first = true;
+            ok = begin_item(cur_q) && issue_qk(0, cur_q);
+            while (ok) {
+                const bool more = w.left > 1;
+                const bool another = w.step(p, work);
+                const int nq = more ? q_tiles(w.it) : 0;
+                const int at[2] = {n_q[0], n_q[1]};
+                if (more && !another) ok = issue_qk(it + 1, nq);            // S of the next step, while P of this one is made
+                if (ok) ok = issue_pv(it, cur_q, c, first);
+                if (!more) break;
+                // (the next item's queries take the place of this one's once its rows are done)
+                if (ok && another) ok = begin_item(nq) && issue_qk(it + 1, nq);
+                c[0] = at[0]; c[1] = at[1];
+                cur_q = nq; first = another;
+                ++it;
+            }
+        }
+    } else if (warp >= 4 * NQ) {
+        // ---------------------------------------------------------------- widening
+        const int ww = warp - 4 * NQ, mine = 8 * ww + (lane & 7);       // this lane's keys of a tile: mine and mine + 32
+        constexpr int PER = NS;                                          // units of 16 channels a key: (lane >> 3) + 4 j
+        struct Rows { int a, b; };                                       // of the keys lane and lane + 32; -1: none
+        auto look_up = [&](const Walk& x) {
+            const int* bt = p.table + (size_t)x.it.request * p.max_blocks;
+            const int len = p.kv_len[x.it.request];
+            int got[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = x.tile * BN + lane + 32 * i, blk = key / p.page_size;
+                int page = -1;
+                if (key < len && blk < p.max_blocks) page = bt[blk];
+                got[i] = page >= 0 && page < p.num_pages ? (page * p.nkv + x.it.g) * p.page_size + (key - blk * p.page_size) : -1;
+            }
+            return Rows{got[0], got[1]};
+        };
+        auto load = [&](const int8_t* from, const Rows& rows, uint4 (&x)[2][PER]) {
+            const int r[2] = {__shfl_sync(0xffffffffu, rows.a, mine), __shfl_sync(0xffffffffu, rows.b, mine)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < PER; ++j)
+                    x[i][j] = r[i] >= 0 ? *reinterpret_cast<const uint4*>(from + (size_t)r[i] * HD + 16 * ((lane >> 3) + 4 * j)) : make_uint4(0, 0, 0, 0);
+        };
+        auto scales = [&](const float* from, const Rows& rows, float (&x)[2]) {
+            x[0] = rows.a >= 0 ? from[rows.a] : 0.f;
+            x[1] = rows.b >= 0 ? from[rows.b] : 0.f;
+        };
+        if (w.left > 0) {
+            Walk ahead = w;
+            Rows cur = look_up(ahead), next{-1, -1};
+            int steps_ahead = ahead.left;
+            if (steps_ahead > 1) { ahead.step(p, work); next = look_up(ahead); }
+            uint4 kx[2][PER], vx[2][PER];
+            float ks[2], vs[2];
+            load(p.k, cur, kx);
+            scales(p.k_scale, cur, ks); scales(p.v_scale, cur, vs);
+            const int total = w.left;
+            for (int it = 0; it < total; ++it) {
+                const int s = it % STAGES;
+                load(p.v, cur, vx);
+                // references and factors
+                unsigned kb = 0, vb = 0;
+                bool bad[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const unsigned a = __float_as_uint(ks[i]), b = __float_as_uint(vs[i]);
+                    bad[i] = a >= 0x7f800000u || b >= 0x7f800000u;
+                    if (!bad[i]) { kb = max(kb, a); vb = max(vb, b); }
+                }
+                const float k_ref = power_above(__reduce_max_sync(0xffffffffu, kb)), v_ref = power_above(__reduce_max_sync(0xffffffffu, vb));
+                const float inv_k = 1.f / k_ref, inv_v = 1.f / v_ref;
+                const float nan = __uint_as_float(0x7fffffffu);
+                float fk[2], fv[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    fk[i] = __shfl_sync(0xffffffffu, bad[i] ? nan : ks[i] * inv_k, mine);
+                    fv[i] = __shfl_sync(0xffffffffu, bad[i] ? 0.f : vs[i] * inv_v, mine);
+                }
+                const unsigned there0 = __ballot_sync(0xffffffffu, cur.a >= 0), there1 = __ballot_sync(0xffffffffu, cur.b >= 0);
+                if (it >= STAGES && !all(bw::mbar_wait(k_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 37))) break;
+                if (ww == 0 && lane == 0) {
+                    TileInfo t;
+                    t.k_ref = k_ref; t.inv_v = inv_v;
+                    t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
+                    t.there[0] = there0; t.there[1] = there1;
+                    t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
+                    info[it % RING] = t;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const Factor f = factor_of(fk[i]);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) widen16(k_s + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, kx[i][j], f);
+                }
+                bw::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) bw::mbar_arrive(k_full + 8 * s);
+                if (it + 1 < total) {
+                    load(p.k, next, kx);
+                    scales(p.k_scale, next, ks); scales(p.v_scale, next, vs);
+                }
+                const Rows after = next;
+                if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
+                if (it >= STAGES && !all(bw::mbar_wait(v_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 38))) break;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const Factor f = factor_of(fv[i]);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) widen16(v_s + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, vx[i][j], f);
+                }
+                bw::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) bw::mbar_arrive(v_full + 8 * s);
+                cur = after;
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax: tile of rows `q`, one thread a row
+        const int q = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * HD + lanes;
+        int it = 0, c = 0;              // steps of the walk, and those of them that this tile of rows has
+        bool ok = true;
+        while (ok && w.left > 0) {
+            const Item item = w.it;
+            const bool mine = q < q_tiles(item);
+            const int gr = item.row0 + q * BM + row;                    // the row among the request's
+            const bool row_ok = q * BM + row < item.n_rows;
+            const int tok = gr / p.G, head = item.g * p.G + gr - tok * p.G, qpos = item.q_pos0 + tok;
+            const size_t at = ((size_t)(item.tok + tok) * p.nh + head) * HD;
+            float sc = 0.f;             // what turns a product into a power of two, but for the tile's reference
+            if (mine) {
+                // the row's queries as float16 times a power of two
+                const uint4* src = reinterpret_cast<const uint4*>(p.q + at);
+                unsigned most = 0;
+#pragma unroll 4
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint4 x = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
+                    most = max(max(max(most, max(x.x & 0x7fffu, x.x >> 16 & 0x7fffu)), max(x.y & 0x7fffu, x.y >> 16 & 0x7fffu)),
+                               max(max(x.z & 0x7fffu, x.z >> 16 & 0x7fffu), max(x.w & 0x7fffu, x.w >> 16 & 0x7fffu)));
+                }
+                unsigned ex = max(most >> 7, 15u);
+                if (ex == 255) ex = 141;                                // an infinity or NaN: as it is
+                const float up = __uint_as_float((268 - ex) << 23);
+                sc = __uint_as_float((ex - 14) << 23) * p.scale_log2;
+                uint8_t* dst = q_s + q * Q_BYTES + row * 128;
+#pragma unroll 4
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint4 x = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
+                    auto two = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up); };
+                    *reinterpret_cast<uint4*>(dst + (i >> 3) * Q_SLICE + (((i & 7) ^ (row & 7)) << 4)) = make_uint4(two(x.x), two(x.y), two(x.z), two(x.w));
+                }
+                bw::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) bw::mbar_arrive(q_full + 8 * q);
+            } else {
+                it += w.end - w.tile;
+                w.pass(p, work);
+                continue;
+            }
+
+            const int lo = bw::first_visible(qpos, p.window, p.chunk);
+            // the warp's rows that exist: positions of the first and the last
+            const int warp_row = item.row0 + q * BM + (warp & 3) * 32, end_row = item.row0 + item.n_rows - 1;
+            const int first_pos = item.q_pos0 + min(warp_row, end_row) / p.G, last_pos = item.q_pos0 + min(warp_row + 31, end_row) / p.G;
+            const int see_all = bw::first_visible(last_pos, p.window, p.chunk);
+            float m = -INFINITY, l = 0.f;
+            const int t_first = w.tile, t_end = w.end;
+            for (int t = t_first; t < t_end; ++t, ++it, ++c) {
+                const int b = c & 1;
+                if (!all(bw::mbar_wait(s_full + 8 * (2 * q + b), (c >> 1) & 1, &g_status, 39))) { ok = false; break; }
+                bw::tc_fence_after();
+                const TileInfo ti = info[it % RING];
+                const int key0 = t * BN;
+                uint32_t v[BN];
+                bw::tmem_ld_32x32(tmem_S + 64 * b, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                bw::tmem_ld_32x32(tmem_S + 64 * b + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+                bw::tmem_ld_wait();
+                const bool gone = (ti.there[0] & ti.there[1]) != 0xffffffffu;
+                if (gone || key0 + BN - 1 > first_pos || key0 < see_all) {      // one branch a tile
+                    // key j is seen for j <= qpos - key0 and j >= lo - key0, if it is there: a mask of 64 bits
+                    const int hi_j = qpos - key0, lo_j = lo - key0;
+                    unsigned long long seen = (unsigned long long)ti.there[1] << 32 | ti.there[0];
+                    if (hi_j < 0 || lo_j > 63) seen = 0;
+                    else {
+                        if (hi_j < 63) seen &= (2ull << hi_j) - 1;
+                        if (lo_j > 0) seen &= ~0ull << lo_j;
+                    }
+                    const unsigned seen0 = (unsigned)seen, seen1 = (unsigned)(seen >> 32);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (!(seen0 >> j & 1)) v[j] = 0xff800000u;
+                        if (!(seen1 >> j & 1)) v[32 + j] = 0xff800000u;
+                    }
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < BN; j += 2)
+                    mx4[(j >> 1) & 3] = fmaxf(mx4[(j >> 1) & 3], fmaxf(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+                const float f = fmaxf(sc * ti.k_ref, 1e-36f);     // (positive: the maximum commutes with it, and -infinity stays)
+                const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), f, ti.log2_v);
+                const bool grow = row_ok && mx > m + 8.f;
+                float shrink = 1.f;
+                if (grow) {
+                    shrink = m == -INFINITY ? 1.f : ex2(m - mx);
+                    l *= shrink;
+                    m = mx;
+                }
+                if (t > t_first && __any_sync(0xffffffffu, grow)) {
+                    // O may be read once the P V of the step before is done
+                    if (!all(bw::mbar_wait(pv_done + 8 * (2 * q + (b ^ 1)), ((c - 1) >> 1) & 1, &g_status, 40))) { ok = false; break; }
+                    bw::tc_fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        uint32_t o[16];
+                        bw::tmem_ld_32x16(tmem_Oq + c0, o);
+                        bw::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                        bw::tmem_st_32x16(tmem_Oq + c0, o);
+                    }
+                    bw::tmem_st_wait();
+                }
+                const float less = ti.log2_v - (m == -INFINITY ? 0.f : m);
+                const bw::f32x2 f2 = bw::pack2(f, f), less2 = bw::pack2(less, less);
+                bw::f32x2 sum2[2] = {0ull, 0ull};
+#pragma unroll
+                for (int j = 0; j < BN; j += 2) {
+                    float a, d;
+                    bw::unpack2(bw::fma2(bw::pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f2, less2), a, d);
+                    a = ex2(a);
+                    d = ex2(d);
+                    sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], bw::pack2(a, d));
+                    v[j >> 1] = pack_f16x2(a, d);
+                }
+                bw::tmem_st_32x32(tmem_S + 64 * b, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                l = fmaf(bw::sum2(add2(sum2[0], sum2[1])), ti.inv_v, l);
+                bw::tmem_st_wait();
+                bw::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bw::mbar_arrive(p_full + 8 * (2 * q + b));
+            }
+            if (!ok || !(ok = all(bw::mbar_wait(pv_done + 8 * (2 * q + ((c - 1) & 1)), ((c - 1) >> 1) & 1, &g_status, 41)))) break;
+            bw::tc_fence_after();
+            if (w.opens && w.closes) {
+                if (p.sink && row_ok) l += ex2(p.sink[head] * LOG2E - m);
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                bf16* dst = p.out + at;
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    uint32_t o[32];
+                    bw::tmem_ld_32x32(tmem_Oq + c0, o);
+                    bw::tmem_ld_wait();
+                    if (row_ok) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+                            auto two = [&](int i) { return bw::pack_bf16x2(__uint_as_float(o[j + i]) * inv, __uint_as_float(o[j + i + 1]) * inv); };
+                            *reinterpret_cast<uint4*>(dst + c0 + j) = make_uint4(two(0), two(2), two(4), two(6));
+                        }
+                    }
+                }
+            } else {
+                // a part of the item: the block's first part (1 if it begins with the item, so it is its last) leaves its sums
+                const size_t slot = 2 * (size_t)blockIdx.x + (w.opens ? 1 : 0);
+                const int r = q * BM + row;
+                float4* dst = reinterpret_cast<float4*>(p.part_o) + slot * (HD / 4) * ROWS + r;
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    uint32_t o[32];
+                    bw::tmem_ld_32x32(tmem_Oq + c0, o);
+                    bw::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        dst[(size_t)((c0 + j) >> 2) * ROWS] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+                }
+                reinterpret_cast<float2*>(p.part_ml)[slot * ROWS + r] = make_float2(m, l);
+            }
+            // (the queries' place is written again, and O: both are done with)
+            bw::tc_fence_before();
+            w.pass(p, work);
+        }
+    }
+    bw::tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) bw::tmem_dealloc(tmem_base, TMEM_COLS);
+}
+
+// The items that several blocks share: a thread a row, four channels a block.
+__global__ void __launch_bounds__(ROWS)
+join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work, const __grid_constant__ Splits splits) {
+    BW_PDL_TRIGGER();
+    BW_PDL_WAIT();
+    const int i = blockIdx.x, quad = blockIdx.y, r = threadIdx.x;
+    const Item it = item_of(work.portion, p.portions, splits.item[i], p.nkv, p.G, p.window, p.chunk);
+    if (r >= it.n_rows) return;
+    const int from = splits.from[i], to = splits.to[i];
+    // the first block's part begins with the item: its slot is the second
+    auto slot_of = [&](int b) { return (size_t)(2 * b + (b == from ? 1 : 0)); };
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;
+    const float4* part = reinterpret_cast<const float4*>(p.part_o) + (size_t)quad * ROWS + r;
+    float M = -INFINITY, L = 0.f;
+    for (int b = from; b <= to; ++b) M = fmaxf(M, ml[slot_of(b) * ROWS].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int b = from; b <= to; ++b) {
+        const float2 x = ml[slot_of(b) * ROWS];
+        const float4 o = part[slot_of(b) * (HD / 4) * ROWS];
+        const float f = x.x == -INFINITY ? 0.f : ex2(x.x - M);
+        acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y); acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
+        L = fmaf(x.y, f, L);
+    }
+    const int gr = it.row0 + r, tok = gr / p.G, head = it.g * p.G + gr - tok * p.G;
+    if (p.sink) L += ex2(p.sink[head] * LOG2E - M);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *reinterpret_cast<uint2*>(p.out + ((size_t)(it.tok + tok) * p.nh + head) * HD + 4 * quad) =
+        make_uint2(bw::pack_bf16x2(acc.x * inv, acc.y * inv), bw::pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining.
+constexpr int LEAST_STEPS = 4;
+int blocks_for(long long steps) {
+    const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;
+    const long long n = (steps + LEAST_STEPS - 1) / LEAST_STEPS;
+    return (int)(n < sms ? n : sms);
+}
+
+}  // namespace
+
+// The launches of a call, handed one after the other to `run(work, portions, items, steps)`, which returns 0 or an error: the requests whose segments
+// have more than `min_rows` stacked rows, sixteen at a time.
+template <typename Run>
+static int launches(const int* h_q_len, const int* h_q_start, int requests, int min_rows, int G, int nkv, int window, int chunk, Run run) {
+    Work work{};
+    int count = 0, items = 0, tok = 0;
+    auto flush = [&]() -> int {
+        if (!count) return 0;
+        long long steps = 0;
+        for (int i = 0; i < items; ++i) steps += item_of(work.portion, count, i, nkv, G, window, chunk).tiles;
+        const int e = run(work, count, items, steps);
+        count = items = 0;
+        return e;
+    };
+    for (int r = 0; r < requests; ++r) {
+        const int n = h_q_len[r];
+        if (n < 0) return BW_ERR_BAD_ARG;
+        const long long rows = (long long)n * G, blocks = (rows + ROWS - 1) / ROWS;
+        if (rows > min_rows) {
+            if (rows > 0x3fffffffll || items + blocks * nkv > 0x3fffffffll) return BW_ERR_UNSUPPORTED;
+            work.portion[count] = {r, tok, n, h_q_start[r], items, (int)blocks};
+            items += (int)blocks * nkv;
+            if (++count == MOST_PORTIONS) if (const int e = flush()) return e;
+        }
+        tok += n;
+    }
+    return flush();
+}
+
+// Room that a call needs for the sums of shared items, in floats (negative: an error).
+BW_EXPORT long long bw_attention_q8_tc_room(const int* h_q_len, const int* h_q_start, int requests, int min_rows, int G, int nkv, int window, int chunk) {
+    if (requests < 0 || G <= 0 || nkv <= 0) return BW_ERR_BAD_ARG;
+    long long most = 0;
+    const int e = launches(h_q_len, h_q_start, requests, min_rows, G, nkv, window > 0 ? window : 0, chunk > 0 ? chunk : 0,
+                           [&](Work&, int, int, long long steps) { const int n = blocks_for(steps); if (n > most) most = n; return 0; });
+    return e ? e : 2 * most * ROWS * (HD + 2);
+}
+
+// q, out: bfloat16 [tokens][nh][HD]; h_q_len, h_q_start: on the host; room: what bw_attention_q8_tc_room says (kept until the call's kernels are
+// done; the launches of one call follow one another and share it).
+BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
+                                 const int* kv_len, const int* table, int max_blocks, const int* h_q_len, const int* h_q_start, int requests,
+                                 int min_rows, int nh, int nkv, int page_size, int num_pages, int window, int chunk, float scale,
+                                 const float* sink, float* room, long long room_floats, void* stream) {
+    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || !room) return BW_ERR_BAD_ARG;
+    if (!(scale > 0.f)) return BW_ERR_UNSUPPORTED;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room) & 15) return BW_ERR_BAD_ARG;
+    if ((long long)num_pages * nkv * page_size > 0x7fffffffll) return BW_ERR_UNSUPPORTED;
+    static bool done[bw::MAX_DEVICES];
+    if (cudaError_t e = bw::allow_dynamic_smem(attn_q8_tc_kernel, SMEM_BYTES, done); e != cudaSuccess) return (int)e;
+    const int G = nh / nkv;
+    window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    return launches(h_q_len, h_q_start, requests, min_rows, G, nkv, window, chunk, [&](Work& work, int count, int items, long long steps) -> int {
+        const int blocks = blocks_for(steps);
+        if (room_floats < 2ll * blocks * ROWS * (HD + 2)) return BW_ERR_BAD_ARG;
+        const Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, kv_len, table, sink, room,
+                       room + 2ll * blocks * ROWS * HD, max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, count, scale * LOG2E};
+        // the stretches, and the items that they cut
+        Splits splits{};
+        int b = 0;
+        long long at = 0;                          // steps before the item
+        auto begin_of = [&](int x) { return steps * x / blocks; };
+        for (int i = 0; i < items; ++i) {
+            const int n = item_of(work.portion, count, i, nkv, G, window, chunk).tiles;
+            for (; b < blocks && begin_of(b) < at + n; ++b) {          // blocks that begin in this item
+                work.item[b] = i; work.offset[b] = (int)(begin_of(b) - at); work.steps[b] = (int)(begin_of(b + 1) - begin_of(b));
+            }
+            // block b - 1 has the item's last step; the one with its first:
+            int first = b - 1;
+            while (begin_of(first) > at) --first;
+            if (first != b - 1) {
+                splits.item[splits.n] = i; splits.from[splits.n] = (short)first; splits.to[splits.n] = (short)(b - 1);
+                ++splits.n;
+            }
+            at += n;
+        }
+        bw::launch(attn_q8_tc_kernel, dim3((unsigned)blocks), dim3(THREADS), SMEM_BYTES, s, p, work);
+        BW_LAUNCH_CHECK();
+        if (splits.n) {
+            bw::launch(join_kernel, dim3((unsigned)splits.n, HD / 4), dim3(ROWS), 0, s, p, work, splits);
+            BW_LAUNCH_CHECK();
+        }
+        return 0;
+    });
+}
+
+// 0 if no bounded wait ever gave up; clears the status (synchronises the device).
+BW_EXPORT int bw_attention_q8_tc_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+    return v;
+}

@@ -59,8 +59,8 @@ __device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
 // channels come as two vectors.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS)
-append_kernel(const T* __restrict__ qkv, int planes, long long plane_stride, const float* __restrict__ turns, int rd, int paired,
-              bf16* __restrict__ q_out, int nh, Rows p, int lanes, int append) {
+append_kernel(const T* qkv, int planes, long long plane_stride, const float* turns, int rd, int paired,
+              bf16* q_out, int nh, Rows p, int lanes, int append) {
     BW_PDL_TRIGGER();
     BW_PDL_WAIT();
     const int heads = nh + 2 * p.nkv, half = rd >> 1;
@@ -179,7 +179,7 @@ __device__ __forceinline__ void store8(float* dst, const float (&u)[4], const fl
 // Keys and values of the listed tokens, [tokens, kv heads, head size] each; zeros where the table names no page.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-read_kernel(Rows p, T* __restrict__ k_out, T* __restrict__ v_out) {
+read_kernel(Rows p, T* k_out, T* v_out) {
     BW_PDL_TRIGGER();
     BW_PDL_WAIT();
     const unsigned per = (unsigned)p.hd >> 3;

@@ -112,7 +112,7 @@ __device__ __forceinline__ u64 merge_warps(u64 k, u64 (*lists)[32]) {
 
 template <bool VEC>
 __device__ __forceinline__ float4 load4(const float* row, int c, int V) {
-    if (VEC && c + 4 <= V) return __ldg(reinterpret_cast<const float4*>(row + c));
+    if (VEC && c + 4 <= V) return *reinterpret_cast<const float4*>(row + c);
     float4 v;
     v.x = c < V ? row[c] : -INFINITY; v.y = c + 1 < V ? row[c + 1] : -INFINITY;
     v.z = c + 2 < V ? row[c + 2] : -INFINITY; v.w = c + 3 < V ? row[c + 3] : -INFINITY;

@@ -1537,7 +1537,9 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
 
 
 _ATTN_Q8_PLAN_ARGS = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]
-_ATTN_Q8_ARGS = [c_void_p] * 10 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]
+_ATTN_Q8_ARGS = [c_void_p] * 10 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]
+_ATTN_Q8_TC_ARGS = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, c_void_p]
+QUANT_FEW_ROWS = 16     # up to so many stacked rows (tokens times heads of a group) a request is the key-slice kernel's
 
 
 def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torch.Tensor, nh: int, scale: float, window: Optional[int] = None,
@@ -1563,6 +1565,24 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     window, chunk = int(window or 0), int(chunk or 0)
     h_len, h_start = (c_int * R)(*batch.h_q_len[:R]), (c_int * R)(*batch.h_q_start[:R])
     macros = attention_q8_macros(hd)
+    if hd % 64 == 0 and scale > 0 and max(batch.h_q_len[:R]) * G > QUANT_FEW_ROWS:
+        # portions of prompts: the tcgen05 kernel, where it is built for the head size (else the mma.sync kernel below takes them)
+        room_of = load_library("attention_q8_tc", macros).bw_attention_q8_tc_room
+        if not room_of.argtypes:
+            room_of.argtypes, room_of.restype = [c_void_p, c_void_p] + [c_int] * 6, c_ll
+        floats = room_of(h_len, h_start, R, QUANT_FEW_ROWS, G, nkv, window, chunk)
+        if floats < 0:
+            _check(int(floats), "quant_attention")
+        room = torch.empty(floats, dtype=torch.float32, device=q.device)
+        tc = _fn("attention_q8_tc", "bw_attention_q8_tc", _ATTN_Q8_TC_ARGS, macros=macros)
+        _check(tc(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(kv_len), _ptr(block_table),
+                  block_table.shape[1], h_len, h_start, R, QUANT_FEW_ROWS, nh, nkv, page_size, num_pages, window, chunk, float(scale), _ptr(sink),
+                  _ptr(room), floats, _stream()), "quant_attention")
+        if min(n for n in batch.h_q_len[:R]) * G > QUANT_FEW_ROWS:
+            return out
+        few = 1
+    else:
+        few = 0
     per = c_int(1)
     slices = _fn("attention_q8", "bw_attention_q8_plan", _ATTN_Q8_PLAN_ARGS, macros=macros)(
         h_len, h_start, R, G, nkv, window, chunk, int(batch.static_bound or 0), ctypes.byref(per))
@@ -1576,11 +1596,21 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     fn = _fn("attention_q8", "bw_attention_q8", _ATTN_Q8_ARGS, macros=macros)
     _check(fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start),
               _ptr(kv_len), _ptr(block_table), block_table.shape[1], h_len, R, nh, nkv, page_size, num_pages, window, chunk, float(scale),
-              _ptr(sink), per.value, slices, _ptr(part_o), _ptr(part_ml), _stream()), "quant_attention")
+              _ptr(sink), per.value, slices, _ptr(part_o), _ptr(part_ml), few, _stream()), "quant_attention")
     return out
 
 
 _ATTN_Q8_MACROS = {}
+
+
+def attention_q8_status() -> int:
+    """0 if no bounded wait in the tcgen05 attention over an 8-bit cache ever gave up (synchronises the device)."""
+    total = 0
+    for key, lib in list(_loaded_libs().items()):
+        if key.startswith("attention_q8_tc"):
+            lib.bw_attention_q8_tc_status.restype = c_int
+            total |= int(lib.bw_attention_q8_tc_status())
+    return total
 
 
 def attention_q8_macros(hd: int) -> dict:
