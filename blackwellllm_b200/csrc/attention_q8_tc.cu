@@ -325,16 +325,21 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         if (w.left > 0) {
             Walk ahead = w;
             Rows cur = look_up(ahead), next{-1, -1};
-            int steps_ahead = ahead.left;
-            if (steps_ahead > 1) { ahead.step(p, work); next = look_up(ahead); }
-            uint4 kx[2][PER], vx[2][PER];
-            float ks[2], vs[2];
+            if (ahead.left > 1) { ahead.step(p, work); next = look_up(ahead); }
+            // rows of a step are loaded a whole step before they are widened, and looked up one before that
+            uint4 kx[2][PER], vx[2][PER], k_next[2][PER], v_next[2][PER];
+            float ks[2], vs[2], ks_next[2], vs_next[2];
             load(p.k, cur, kx);
+            load(p.v, cur, vx);
             scales(p.k_scale, cur, ks); scales(p.v_scale, cur, vs);
             const int total = w.left;
             for (int it = 0; it < total; ++it) {
                 const int s = it % STAGES;
-                load(p.v, cur, vx);
+                scales(p.k_scale, next, ks_next); scales(p.v_scale, next, vs_next);       // (rows -1, and zeros, behind the last step)
+                load(p.k, next, k_next);
+                load(p.v, next, v_next);
+                Rows after{-1, -1};
+                if (it + 2 < total) { ahead.step(p, work); after = look_up(ahead); }
                 // references and factors
                 unsigned kb = 0, vb = 0;
                 bool bad[2];
@@ -372,12 +377,6 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(k_full + 8 * s);
-                if (it + 1 < total) {
-                    load(p.k, next, kx);
-                    scales(p.k_scale, next, ks); scales(p.v_scale, next, vs);
-                }
-                const Rows after = next;
-                if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
                 if (it >= STAGES && !all(bw::mbar_wait(v_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 38))) break;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -388,7 +387,13 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(v_full + 8 * s);
-                cur = after;
+                cur = next; next = after;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    ks[i] = ks_next[i]; vs[i] = vs_next[i];
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) { kx[i][j] = k_next[i][j]; vx[i][j] = v_next[i][j]; }
+                }
             }
         }
     } else {
@@ -409,23 +414,33 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             if (mine) {
                 // the row's queries as float16 times a power of two
                 const uint4* src = reinterpret_cast<const uint4*>(p.q + at);
+                uint8_t* dst = q_s + q * Q_BYTES + row * 128;
                 unsigned most = 0;
-#pragma unroll 4
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint4 x = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
-                    most = max(max(max(most, max(x.x & 0x7fffu, x.x >> 16 & 0x7fffu)), max(x.y & 0x7fffu, x.y >> 16 & 0x7fffu)),
-                               max(max(x.z & 0x7fffu, x.z >> 16 & 0x7fffu), max(x.w & 0x7fffu, x.w >> 16 & 0x7fffu)));
+                constexpr int PART = HD <= 128 ? HD / 8 : 16;       // loads in flight together (the row's in one pass up to head size 128)
+                uint4 x[PART];
+#pragma unroll 1
+                for (int i0 = 0; i0 < HD / 8; i0 += PART) {
+#pragma unroll
+                    for (int i = 0; i < PART; ++i) x[i] = row_ok && i0 + i < HD / 8 ? src[i0 + i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < PART; ++i)
+                        most = max(max(max(most, max(x[i].x & 0x7fffu, x[i].x >> 16 & 0x7fffu)), max(x[i].y & 0x7fffu, x[i].y >> 16 & 0x7fffu)),
+                                   max(max(x[i].z & 0x7fffu, x[i].z >> 16 & 0x7fffu), max(x[i].w & 0x7fffu, x[i].w >> 16 & 0x7fffu)));
                 }
                 unsigned ex = max(most >> 7, 15u);
                 if (ex == 255) ex = 141;                                // an infinity or NaN: as it is
                 const float up = __uint_as_float((268 - ex) << 23);
                 sc = __uint_as_float((ex - 14) << 23) * p.scale_log2;
-                uint8_t* dst = q_s + q * Q_BYTES + row * 128;
-#pragma unroll 4
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint4 x = row_ok ? src[i] : make_uint4(0, 0, 0, 0);
-                    auto two = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up); };
-                    *reinterpret_cast<uint4*>(dst + (i >> 3) * Q_SLICE + (((i & 7) ^ (row & 7)) << 4)) = make_uint4(two(x.x), two(x.y), two(x.z), two(x.w));
+                auto two = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up); };
+#pragma unroll 1
+                for (int i0 = 0; i0 < HD / 8; i0 += PART) {
+#pragma unroll
+                    for (int i = 0; i < PART; ++i) {
+                        if (HD > 128) x[i] = row_ok && i0 + i < HD / 8 ? src[i0 + i] : make_uint4(0, 0, 0, 0);
+                        const int u = i0 + i;
+                        if (u < HD / 8)
+                            *reinterpret_cast<uint4*>(dst + (u >> 3) * Q_SLICE + (((u & 7) ^ (row & 7)) << 4)) = make_uint4(two(x[i].x), two(x[i].y), two(x[i].z), two(x[i].w));
+                    }
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
@@ -595,15 +610,16 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
 
 // Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining.
 constexpr int LEAST_STEPS = 4;
-int blocks_for(long long steps) {
+constexpr int ITEM_COST = 3;         // what an item costs beside its steps (its queries, the first scores, its outputs), in steps
+int blocks_for(long long cost) {
     const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;
-    const long long n = (steps + LEAST_STEPS - 1) / LEAST_STEPS;
+    const long long n = (cost + LEAST_STEPS + ITEM_COST - 1) / (LEAST_STEPS + ITEM_COST);
     return (int)(n < sms ? n : sms);
 }
 
 }  // namespace
 
-// The launches of a call, handed one after the other to `run(work, portions, items, steps)`, which returns 0 or an error: the requests whose segments
+// The launches of a call, handed one after the other to `run(work, portions, items, cost)`, which returns 0 or an error: the requests whose segments
 // have more than `min_rows` stacked rows, sixteen at a time.
 template <typename Run>
 static int launches(const int* h_q_len, const int* h_q_start, int requests, int min_rows, int G, int nkv, int window, int chunk, Run run) {
@@ -611,9 +627,9 @@ static int launches(const int* h_q_len, const int* h_q_start, int requests, int 
     int count = 0, items = 0, tok = 0;
     auto flush = [&]() -> int {
         if (!count) return 0;
-        long long steps = 0;
-        for (int i = 0; i < items; ++i) steps += item_of(work.portion, count, i, nkv, G, window, chunk).tiles;
-        const int e = run(work, count, items, steps);
+        long long cost = 0;
+        for (int i = 0; i < items; ++i) cost += item_of(work.portion, count, i, nkv, G, window, chunk).tiles + ITEM_COST;
+        const int e = run(work, count, items, cost);
         count = items = 0;
         return e;
     };
@@ -637,7 +653,7 @@ BW_EXPORT long long bw_attention_q8_tc_room(const int* h_q_len, const int* h_q_s
     if (requests < 0 || G <= 0 || nkv <= 0) return BW_ERR_BAD_ARG;
     long long most = 0;
     const int e = launches(h_q_len, h_q_start, requests, min_rows, G, nkv, window > 0 ? window : 0, chunk > 0 ? chunk : 0,
-                           [&](Work&, int, int, long long steps) { const int n = blocks_for(steps); if (n > most) most = n; return 0; });
+                           [&](Work&, int, int, long long cost) { const int n = blocks_for(cost); if (n > most) most = n; return 0; });
     return e ? e : 2 * most * ROWS * (HD + 2);
 }
 
@@ -656,29 +672,34 @@ BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, co
     const int G = nh / nkv;
     window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
     cudaStream_t s = (cudaStream_t)stream;
-    return launches(h_q_len, h_q_start, requests, min_rows, G, nkv, window, chunk, [&](Work& work, int count, int items, long long steps) -> int {
-        const int blocks = blocks_for(steps);
+    return launches(h_q_len, h_q_start, requests, min_rows, G, nkv, window, chunk, [&](Work& work, int count, int items, long long cost) -> int {
+        const int blocks = blocks_for(cost);
         if (room_floats < 2ll * blocks * ROWS * (HD + 2)) return BW_ERR_BAD_ARG;
         const Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, kv_len, table, sink, room,
                        room + 2ll * blocks * ROWS * HD, max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, count, scale * LOG2E};
-        // the stretches, and the items that they cut
+        // Stretches of equal cost, and the items that they cut.  A cut that falls on what an item costs beside its steps falls before the item.
         Splits splits{};
         int b = 0;
-        long long at = 0;                          // steps before the item
-        auto begin_of = [&](int x) { return steps * x / blocks; };
+        long long at = 0;                          // cost of the items before
+        int open = -1, open_offset = 0;            // the block that has steps up to here, and the offset in this item where it began (if in it)
         for (int i = 0; i < items; ++i) {
             const int n = item_of(work.portion, count, i, nkv, G, window, chunk).tiles;
-            for (; b < blocks && begin_of(b) < at + n; ++b) {          // blocks that begin in this item
-                work.item[b] = i; work.offset[b] = (int)(begin_of(b) - at); work.steps[b] = (int)(begin_of(b + 1) - begin_of(b));
+            int from = b - 1;                      // the block that has the item's first step, unless one begins with it
+            open_offset = 0;
+            for (; b < blocks && cost * b / blocks < at + n + ITEM_COST; ++b) {
+                long long offset = cost * b / blocks - at - ITEM_COST;
+                if (offset < 0) offset = 0;
+                if (open >= 0) work.steps[open] += (int)offset - open_offset;
+                if (offset == 0) from = b;         // (a block whose cut falls here too begins where the next does: it has no steps)
+                work.item[b] = i; work.offset[b] = (int)offset; work.steps[b] = 0;
+                open = b; open_offset = (int)offset;
             }
-            // block b - 1 has the item's last step; the one with its first:
-            int first = b - 1;
-            while (begin_of(first) > at) --first;
-            if (first != b - 1) {
-                splits.item[splits.n] = i; splits.from[splits.n] = (short)first; splits.to[splits.n] = (short)(b - 1);
+            if (open >= 0) work.steps[open] += n - open_offset;
+            if (from != b - 1) {
+                splits.item[splits.n] = i; splits.from[splits.n] = (short)from; splits.to[splits.n] = (short)(b - 1);
                 ++splits.n;
             }
-            at += n;
+            at += n + ITEM_COST;
         }
         bw::launch(attn_q8_tc_kernel, dim3((unsigned)blocks), dim3(THREADS), SMEM_BYTES, s, p, work);
         BW_LAUNCH_CHECK();
