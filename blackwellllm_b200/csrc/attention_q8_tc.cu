@@ -9,7 +9,7 @@
 //     block's instructions, and the reason why a block has 256 rows and is alone on its SM;
 //   * one warp issues the products: S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, O += P V with P from tensor memory;
 //   * eight warps, one thread a row, make P: maximum, exponentials, sums; P is written over the S it came from as float16 pairs.
-// Roundings: K and V to float16 (2^-11 of an element; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
+// Roundings: K and V to float16 (2^-11 of an element, a value's scale by as much again; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
 // beside the largest), and the result to bfloat16.  Scores, sums and outputs are float32; the queries are multiplied by a power of two a row
 // (attention_q8.cu) and exact.  The exponents' reference follows the largest t + log2 of the tile's value scale lazily (by steps of more than
 // 8), so O is seldom rescaled.
@@ -61,6 +61,7 @@ struct Params {
     float* part_o; float* part_ml;          // [2 x blocks][HD / 4][ROWS][4] and [2 x blocks][ROWS][2]
     int max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, portions;
     float scale_log2;
+    unsigned per_page;                      // 2^32 / page_size, rounded down
 };
 struct Portion { int request, tok, n_tok, q_pos0, first, n_blocks; };      // first: the first of its n_blocks * nkv items
 struct Work {
@@ -157,7 +158,16 @@ __device__ __forceinline__ uint32_t widen2(uint32_t r, const Factor& f) {
     asm("{\n.reg .b32 t;\nmul.rn.f16x2 t, %1, %2;\nfma.rn.f16x2 %0, %1, %3, t;\n}" : "=r"(d) : "r"(n), "r"(f.lo), "r"(f.hi));
     return d;
 }
+// The same with the factor rounded to float16 (values: 2^-11 of a key's value; a score would be off by that much of itself).
+template <int SEL>
+__device__ __forceinline__ uint32_t widen2(uint32_t r, uint32_t f) {
+    uint32_t n, d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(n) : "r"(__byte_perm(r, 0x64646464u, SEL)), "r"(0x64806480u));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(n), "r"(f));
+    return d;
+}
 // 16 channels (unit c) of key `key` into a tile of operands
+template <typename Factor>
 __device__ __forceinline__ void widen16(uint8_t* tile, int key, int c, uint4 x, const Factor& f) {
     const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
     uint8_t* row = tile + (c >> 2) * KV_SLICE + key * 128;
@@ -217,25 +227,30 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     if (tmem_slot[1] != 0) w.left = 0;                   // an earlier launch gave up: nothing is done
 
     if (warp == MMA_WARP) {
-        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem_base, 0), q0 = bw::smem_u32(q_s), k0 = bw::smem_u32(k_s), v0 = bw::smem_u32(v_s);
-        int n_q[2] = {0, 0}, loaded[2] = {0, 0};         // of each tile of rows: steps that S was issued for, times that its queries came
+        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem_base, 0);
+        // descriptors of the first operands; others lie a multiple of 16 bytes behind (added to the low word: addresses stay below its field)
+        const uint64_t dq = bw::umma_smem_desc_sw128(bw::smem_u32(q_s)), dk = bw::umma_smem_desc_sw128(bw::smem_u32(k_s)),
+                       dv = bw::umma_smem_desc_mn_sw128(bw::smem_u32(v_s), KV_SLICE);
+        auto behind = [](uint64_t d, uint32_t units) { return (d & 0xffffffff00000000ull) | (uint32_t)((uint32_t)d + units); };
+        int n_q[NQ] = {}, loaded[NQ] = {};               // of each tile of rows: steps that S was issued for, times that its queries came
         bool ok = true;
         // S of step `it` of the walk
         auto issue_qk = [&](int it, int tiles_q) {
             const int s = it % STAGES;
             if (!all(bw::mbar_wait(k_full + 8 * s, (it / STAGES) & 1, &g_status, 32))) return false;
-            for (int q = 0; q < tiles_q; ++q) {
+            const uint64_t dks = behind(dk, s * (KV_BYTES >> 4));
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                if (q >= tiles_q) break;
                 const int b = n_q[q] & 1;
                 // the buffer holds P of the step before last, which the P V issued for it may still read
                 if (n_q[q] >= 2 && !all(bw::mbar_wait(pv_done + 8 * (2 * q + b), ((n_q[q] >> 1) - 1) & 1, &g_status, 33))) return false;
                 bw::tc_fence_after();
                 if (bw::elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        const uint64_t da = bw::umma_smem_desc_sw128(q0 + q * Q_BYTES + (ks >> 2) * Q_SLICE) + 2 * (ks & 3);
-                        const uint64_t db = bw::umma_smem_desc_sw128(k0 + s * KV_BYTES + (ks >> 2) * KV_SLICE) + 2 * (ks & 3);
-                        bw::umma_bf16(tmem0 + 128 * q + 64 * b, da, db, IDESC_QK, ks != 0);
-                    }
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        bw::umma_bf16(tmem0 + 128 * q + 64 * b, behind(dq, (q * Q_BYTES + (ks >> 2) * Q_SLICE) / 16 + 2 * (ks & 3)),
+                                      behind(dks, (ks >> 2) * (KV_SLICE / 16) + 2 * (ks & 3)), IDESC_QK, ks != 0);
                     bw::umma_commit(s_full + 8 * (2 * q + b));
                     if (q == tiles_q - 1) bw::umma_commit(k_empty + 8 * s);
                 }
@@ -245,19 +260,21 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             return true;
         };
         // P V of step `it`, whose S has numbers c[] among the steps of its tiles of rows
-        auto issue_pv = [&](int it, int tiles_q, const int (&c)[2], bool first) {
+        auto issue_pv = [&](int it, int tiles_q, const int (&c)[NQ], bool first) {
             const int s = it % STAGES;
             if (!all(bw::mbar_wait(v_full + 8 * s, (it / STAGES) & 1, &g_status, 34))) return false;
-            for (int q = 0; q < tiles_q; ++q) {
+            const uint64_t dvs = behind(dv, s * (KV_BYTES >> 4));
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                if (q >= tiles_q) break;
                 const int b = c[q] & 1;
                 if (!all(bw::mbar_wait(p_full + 8 * (2 * q + b), (c[q] >> 1) & 1, &g_status, 35))) return false;
                 bw::tc_fence_after();
                 if (bw::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < BN / 16; ++kk) {
-                        const uint64_t db = bw::umma_smem_desc_mn_sw128(v0 + s * KV_BYTES, KV_SLICE) + (uint64_t)kk * (2048 >> 4);
-                        bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, db, IDESC_PV, !(first && kk == 0));
-                    }
+                    for (int kk = 0; kk < BN / 16; ++kk)
+                        bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, behind(dvs, kk * (2048 / 16)), IDESC_PV,
+                                         !(first && kk == 0));
                     bw::umma_commit(pv_done + 8 * (2 * q + b));
                     if (q == tiles_q - 1) bw::umma_commit(v_empty + 8 * s);
                 }
@@ -266,7 +283,9 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             return true;
         };
         auto begin_item = [&](int tiles_q) {
-            for (int q = 0; q < tiles_q; ++q) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                if (q >= tiles_q) break;
                 if (!all(bw::mbar_wait(q_full + 8 * q, loaded[q] & 1, &g_status, 36))) return false;
                 ++loaded[q];
             }
@@ -274,20 +293,23 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         };
         int it = 0;
         if (w.left > 0) {
-            int cur_q = q_tiles(w.it), c[2] = {0, 0};
+            int cur_q = q_tiles(w.it), c[NQ] = {};
             bool first = true;
             ok = begin_item(cur_q) && issue_qk(0, cur_q);
             while (ok) {
                 const bool more = w.left > 1;
                 const bool another = w.step(p, work);
                 const int nq = more ? q_tiles(w.it) : 0;
-                const int at[2] = {n_q[0], n_q[1]};
+                int at[NQ];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) at[q] = n_q[q];
                 if (more && !another) ok = issue_qk(it + 1, nq);            // S of the next step, while P of this one is made
                 if (ok) ok = issue_pv(it, cur_q, c, first);
                 if (!more) break;
                 // (the next item's queries take the place of this one's once its rows are done)
                 if (ok && another) ok = begin_item(nq) && issue_qk(it + 1, nq);
-                c[0] = at[0]; c[1] = at[1];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) c[q] = at[q];
                 cur_q = nq; first = another;
                 ++it;
             }
@@ -297,17 +319,32 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         const int ww = warp - 4 * NQ, mine = 8 * ww + (lane & 7);       // this lane's keys of a tile: mine and mine + 32
         constexpr int PER = NS;                                          // units of 16 channels a key: (lane >> 3) + 4 j
         struct Rows { int a, b; };                                       // of the keys lane and lane + 32; -1: none
+        // the pages of the keys lane and lane + 32 as the table has them (-1: none); made into rows only a step later, so that nothing waits
+        struct Pages { int page[2], slot[2], g; };
+        int item_seen = -1, len = 0;
+        const int* bt = nullptr;
         auto look_up = [&](const Walk& x) {
-            const int* bt = p.table + (size_t)x.it.request * p.max_blocks;
-            const int len = p.kv_len[x.it.request];
-            int got[2];
+            if (x.index != item_seen) {
+                item_seen = x.index;
+                len = p.kv_len[x.it.request];
+                bt = p.table + (size_t)x.it.request * p.max_blocks;
+            }
+            Pages got{{-1, -1}, {0, 0}, x.it.g};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int key = x.tile * BN + lane + 32 * i, blk = key / p.page_size;
-                int page = -1;
-                if (key < len && blk < p.max_blocks) page = bt[blk];
-                got[i] = page >= 0 && page < p.num_pages ? (page * p.nkv + x.it.g) * p.page_size + (key - blk * p.page_size) : -1;
+                // the key's block: by a reciprocal that is at most one too low
+                const int key = x.tile * BN + lane + 32 * i;
+                int blk = (int)__umulhi((unsigned)key, p.per_page), slot = key - blk * p.page_size;
+                if (slot >= p.page_size) { slot -= p.page_size; ++blk; }
+                got.slot[i] = slot;
+                if (key < len && blk < p.max_blocks) got.page[i] = bt[blk];
             }
+            return got;
+        };
+        auto rows_of = [&](const Pages& x) {
+            int got[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) got[i] = (unsigned)x.page[i] < (unsigned)p.num_pages ? (x.page[i] * p.nkv + x.g) * p.page_size + x.slot[i] : -1;
             return Rows{got[0], got[1]};
         };
         auto load = [&](const int8_t* from, const Rows& rows, uint4 (&x)[2][PER]) {
@@ -324,7 +361,8 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         };
         if (w.left > 0) {
             Walk ahead = w;
-            Rows cur = look_up(ahead), next{-1, -1};
+            Rows cur = rows_of(look_up(ahead));
+            Pages next{{-1, -1}, {0, 0}, 0};
             if (ahead.left > 1) { ahead.step(p, work); next = look_up(ahead); }
             // rows of a step are loaded a whole step before they are widened, and looked up one before that
             uint4 kx[2][PER], vx[2][PER], k_next[2][PER], v_next[2][PER];
@@ -335,11 +373,12 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             const int total = w.left;
             for (int it = 0; it < total; ++it) {
                 const int s = it % STAGES;
-                scales(p.k_scale, next, ks_next); scales(p.v_scale, next, vs_next);       // (rows -1, and zeros, behind the last step)
-                load(p.k, next, k_next);
-                load(p.v, next, v_next);
-                Rows after{-1, -1};
-                if (it + 2 < total) { ahead.step(p, work); after = look_up(ahead); }
+                const Rows rows = rows_of(next);                                          // (behind the last step: none, and zeros)
+                scales(p.k_scale, rows, ks_next); scales(p.v_scale, rows, vs_next);
+                load(p.k, rows, k_next);
+                load(p.v, rows, v_next);
+                next = Pages{{-1, -1}, {0, 0}, 0};
+                if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
                 // references and factors
                 unsigned kb = 0, vb = 0;
                 bool bad[2];
@@ -350,7 +389,8 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                     if (!bad[i]) { kb = max(kb, a); vb = max(vb, b); }
                 }
                 const float k_ref = power_above(__reduce_max_sync(0xffffffffu, kb)), v_ref = power_above(__reduce_max_sync(0xffffffffu, vb));
-                const float inv_k = 1.f / k_ref, inv_v = 1.f / v_ref;
+                // (powers of two: the exponent turned around)
+                const float inv_k = __uint_as_float((254u << 23) - __float_as_uint(k_ref)), inv_v = __uint_as_float((254u << 23) - __float_as_uint(v_ref));
                 const float nan = __uint_as_float(0x7fffffffu);
                 float fk[2], fv[2];
 #pragma unroll
@@ -380,14 +420,14 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 if (it >= STAGES && !all(bw::mbar_wait(v_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 38))) break;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const Factor f = factor_of(fv[i]);
+                    const uint32_t f = pack_f16x2(fv[i], fv[i]);
 #pragma unroll
                     for (int j = 0; j < PER; ++j) widen16(v_s + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, vx[i][j], f);
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(v_full + 8 * s);
-                cur = next; next = after;
+                cur = rows;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     ks[i] = ks_next[i]; vs[i] = vs_next[i];
@@ -676,7 +716,8 @@ BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, co
         const int blocks = blocks_for(cost);
         if (room_floats < 2ll * blocks * ROWS * (HD + 2)) return BW_ERR_BAD_ARG;
         const Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, kv_len, table, sink, room,
-                       room + 2ll * blocks * ROWS * HD, max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, count, scale * LOG2E};
+                       room + 2ll * blocks * ROWS * HD, max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, blocks, count, scale * LOG2E,
+                       page_size == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned)page_size)};
         // Stretches of equal cost, and the items that they cut.  A cut that falls on what an item costs beside its steps falls before the item.
         Splits splits{};
         int b = 0;
