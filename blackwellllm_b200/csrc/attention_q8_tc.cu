@@ -3,11 +3,12 @@
 //
 // A block works on 256 stacked rows (row = token * G + head of the group) of one (request, kv head) as two tiles of 128 (one, of head sizes
 // above 128: tensor memory holds no more) against tiles of 64 keys:
-//   * four warps widen: rows of whole numbers from the cache (16 bytes a load, straight into registers) become float16 times the row's scale
+//   * eight warps widen, four keys and four values: rows of whole numbers from the cache (16 bytes a load, straight into registers) become float16 times the row's scale
 //     over the largest scale of the 64 (a power of two, which goes back into the scores, and for the values into the exponent), and
 //     are written as the 128-byte-swizzled operands of the tensor cores.  Both tiles of rows use them: widening is a third of the
 //     block's instructions, and the reason why a block has 256 rows and is alone on its SM;
-//   * one warp issues the products: S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, O += P V with P from tensor memory;
+//   * one warp issues S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, another O += P V with P from tensor memory (one warp for
+//     both spent two thirds of its time between its products);
 //   * eight warps, one thread a row, make P: maximum, exponentials, sums; P is written over the S it came from as float16 pairs.
 // Roundings: K and V to float16 (2^-11 of an element, a value's scale by as much again; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
 // beside the largest), and the result to bfloat16.  Scores, sums and outputs are float32; the queries are multiplied by a power of two a row
@@ -40,8 +41,14 @@ constexpr int STAGES = 2;
 constexpr int Q_SLICE = BM * 128, KV_SLICE = BN * 128;
 constexpr int Q_BYTES = NS * Q_SLICE, KV_BYTES = NS * KV_SLICE;
 constexpr int RING = STAGES + 2;            // what the softmax reads of a tile of keys: a widening warp is at most that far ahead of it
-constexpr int WIDEN_WARPS = 4, MMA_WARP = 4 * NQ + WIDEN_WARPS;
-constexpr int THREADS = 32 * (MMA_WARP + 1);
+// Groups of four warps: NQ of the softmax, one that widens keys, one that widens values, and one whose first two warps issue products.  A block is
+// launched with 96 registers a thread (128 with four groups) and the groups trade them: 256 * 136 + 256 * 80 + 128 * 48 = 61,440, all of them,
+// and 128 * 168 + 256 * 112 + 128 * 48 = 56,320 of 65,536.
+constexpr int KEY_WARP = 4 * NQ, VALUE_WARP = KEY_WARP + 4, QK_WARP = VALUE_WARP + 4, PV_WARP = QK_WARP + 1;
+constexpr int THREADS = 32 * (QK_WARP + 4);
+constexpr int SOFTMAX_REGS = NQ == 2 ? 136 : 168, WIDEN_REGS = NQ == 2 ? 80 : 112, ISSUE_REGS = 48;
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int SMEM_BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + RING * 32 + 32 * 8 + 16;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t idesc_f16(int N, bool b_mn_major) {
@@ -204,7 +211,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     if (threadIdx.x == 0) {
         for (int q = 0; q < NQ; ++q) bw::mbar_init(q_full + 8 * q, 4);
         for (int s = 0; s < STAGES; ++s) {
-            bw::mbar_init(k_full + 8 * s, WIDEN_WARPS); bw::mbar_init(v_full + 8 * s, WIDEN_WARPS);
+            bw::mbar_init(k_full + 8 * s, 4); bw::mbar_init(v_full + 8 * s, 4);
             bw::mbar_init(k_empty + 8 * s, 1); bw::mbar_init(v_empty + 8 * s, 1);
         }
         for (int s = 0; s < 2 * NQ; ++s) {
@@ -213,7 +220,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         bw::fence_barrier_init();
         tmem_slot[1] = (uint32_t)g_status;
     }
-    if (warp == MMA_WARP) bw::tmem_alloc(bw::smem_u32(tmem_slot), TMEM_COLS);
+    if (warp == QK_WARP) bw::tmem_alloc(bw::smem_u32(tmem_slot), TMEM_COLS);
     bw::tc_fence_before();
     __syncthreads();
     bw::tc_fence_after();
@@ -226,97 +233,90 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     w.start(p, work);
     if (tmem_slot[1] != 0) w.left = 0;                   // an earlier launch gave up: nothing is done
 
-    if (warp == MMA_WARP) {
+    if (warp >= QK_WARP) {
+        fewer_registers<ISSUE_REGS>();
         const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem_base, 0);
         // descriptors of the first operands; others lie a multiple of 16 bytes behind (added to the low word: addresses stay below its field)
-        const uint64_t dq = bw::umma_smem_desc_sw128(bw::smem_u32(q_s)), dk = bw::umma_smem_desc_sw128(bw::smem_u32(k_s)),
-                       dv = bw::umma_smem_desc_mn_sw128(bw::smem_u32(v_s), KV_SLICE);
         auto behind = [](uint64_t d, uint32_t units) { return (d & 0xffffffff00000000ull) | (uint32_t)((uint32_t)d + units); };
-        int n_q[NQ] = {}, loaded[NQ] = {};               // of each tile of rows: steps that S was issued for, times that its queries came
-        bool ok = true;
-        // S of step `it` of the walk
-        auto issue_qk = [&](int it, int tiles_q) {
-            const int s = it % STAGES;
-            if (!all(bw::mbar_wait(k_full + 8 * s, (it / STAGES) & 1, &g_status, 32))) return false;
-            const uint64_t dks = behind(dk, s * (KV_BYTES >> 4));
+        int n[NQ] = {};                                  // steps of each tile of rows so far
+        if (warp == QK_WARP) {
+            const uint64_t dq = bw::umma_smem_desc_sw128(bw::smem_u32(q_s)), dk = bw::umma_smem_desc_sw128(bw::smem_u32(k_s));
+            int loaded[NQ] = {};                         // times that a tile's queries came
+            bool begins = true, ok = true;
+            for (int it = 0; ok && w.left > 0; ++it) {
+                const int s = it % STAGES, tiles_q = q_tiles(w.it);
+                if (begins) {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                if (q >= tiles_q) break;
-                const int b = n_q[q] & 1;
-                // the buffer holds P of the step before last, which the P V issued for it may still read
-                if (n_q[q] >= 2 && !all(bw::mbar_wait(pv_done + 8 * (2 * q + b), ((n_q[q] >> 1) - 1) & 1, &g_status, 33))) return false;
-                bw::tc_fence_after();
-                if (bw::elect_one()) {
+                    for (int q = 0; q < NQ; ++q)
+                        if (ok && q < tiles_q) {
+                            ok = all(bw::mbar_wait(q_full + 8 * q, loaded[q] & 1, &g_status, 36));
+                            ++loaded[q];
+                        }
+                    // whoever was in the item before has read what it needs of its keys' tiles (`info` holds them a few steps long)
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        bw::umma_bf16(tmem0 + 128 * q + 64 * b, behind(dq, (q * Q_BYTES + (ks >> 2) * Q_SLICE) / 16 + 2 * (ks & 3)),
-                                      behind(dks, (ks >> 2) * (KV_SLICE / 16) + 2 * (ks & 3)), IDESC_QK, ks != 0);
-                    bw::umma_commit(s_full + 8 * (2 * q + b));
-                    if (q == tiles_q - 1) bw::umma_commit(k_empty + 8 * s);
+                    for (int q = 0; q < NQ; ++q)
+                        if (ok && n[q] > 0) ok = all(bw::mbar_wait(pv_done + 8 * (2 * q + ((n[q] - 1) & 1)), ((n[q] - 1) >> 1) & 1, &g_status, 42));
+                    if (!ok) break;
                 }
-                __syncwarp();
-                ++n_q[q];
-            }
-            return true;
-        };
-        // P V of step `it`, whose S has numbers c[] among the steps of its tiles of rows
-        auto issue_pv = [&](int it, int tiles_q, const int (&c)[NQ], bool first) {
-            const int s = it % STAGES;
-            if (!all(bw::mbar_wait(v_full + 8 * s, (it / STAGES) & 1, &g_status, 34))) return false;
-            const uint64_t dvs = behind(dv, s * (KV_BYTES >> 4));
+                if (!all(bw::mbar_wait(k_full + 8 * s, (it / STAGES) & 1, &g_status, 32))) break;
+                const uint64_t dks = behind(dk, s * (KV_BYTES >> 4));
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                if (q >= tiles_q) break;
-                const int b = c[q] & 1;
-                if (!all(bw::mbar_wait(p_full + 8 * (2 * q + b), (c[q] >> 1) & 1, &g_status, 35))) return false;
-                bw::tc_fence_after();
-                if (bw::elect_one()) {
+                for (int q = 0; q < NQ; ++q) {
+                    if (q >= tiles_q) break;
+                    const int b = n[q] & 1;
+                    // the buffer holds P of the step before last, which the P V issued for it may still read
+                    if (n[q] >= 2) ok = all(bw::mbar_wait(pv_done + 8 * (2 * q + b), ((n[q] >> 1) - 1) & 1, &g_status, 33));
+                    if (!ok) break;
+                    bw::tc_fence_after();
+                    if (bw::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < BN / 16; ++kk)
-                        bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, behind(dvs, kk * (2048 / 16)), IDESC_PV,
-                                         !(first && kk == 0));
-                    bw::umma_commit(pv_done + 8 * (2 * q + b));
-                    if (q == tiles_q - 1) bw::umma_commit(v_empty + 8 * s);
+                        for (int ks = 0; ks < HD / 16; ++ks)
+                            bw::umma_bf16(tmem0 + 128 * q + 64 * b, behind(dq, (q * Q_BYTES + (ks >> 2) * Q_SLICE) / 16 + 2 * (ks & 3)),
+                                          behind(dks, (ks >> 2) * (KV_SLICE / 16) + 2 * (ks & 3)), IDESC_QK, ks != 0);
+                        bw::umma_commit(s_full + 8 * (2 * q + b));
+                        if (q == tiles_q - 1) bw::umma_commit(k_empty + 8 * s);
+                    }
+                    __syncwarp();
+                    ++n[q];
                 }
-                __syncwarp();
+                begins = w.step(p, work);
             }
-            return true;
-        };
-        auto begin_item = [&](int tiles_q) {
+        } else if (warp == PV_WARP) {
+            const uint64_t dv = bw::umma_smem_desc_mn_sw128(bw::smem_u32(v_s), KV_SLICE);
+            bool begins = true, ok = true;
+            for (int it = 0; ok && w.left > 0; ++it) {
+                const int s = it % STAGES, tiles_q = q_tiles(w.it);
+                if (!all(bw::mbar_wait(v_full + 8 * s, (it / STAGES) & 1, &g_status, 34))) break;
+                const uint64_t dvs = behind(dv, s * (KV_BYTES >> 4));
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                if (q >= tiles_q) break;
-                if (!all(bw::mbar_wait(q_full + 8 * q, loaded[q] & 1, &g_status, 36))) return false;
-                ++loaded[q];
-            }
-            return true;
-        };
-        int it = 0;
-        if (w.left > 0) {
-            int cur_q = q_tiles(w.it), c[NQ] = {};
-            bool first = true;
-            ok = begin_item(cur_q) && issue_qk(0, cur_q);
-            while (ok) {
-                const bool more = w.left > 1;
-                const bool another = w.step(p, work);
-                const int nq = more ? q_tiles(w.it) : 0;
-                int at[NQ];
+                for (int q = 0; q < NQ; ++q) {
+                    if (q >= tiles_q) break;
+                    const int b = n[q] & 1;
+                    ok = all(bw::mbar_wait(p_full + 8 * (2 * q + b), (n[q] >> 1) & 1, &g_status, 35));
+                    if (!ok) break;
+                    bw::tc_fence_after();
+                    if (bw::elect_one()) {
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) at[q] = n_q[q];
-                if (more && !another) ok = issue_qk(it + 1, nq);            // S of the next step, while P of this one is made
-                if (ok) ok = issue_pv(it, cur_q, c, first);
-                if (!more) break;
-                // (the next item's queries take the place of this one's once its rows are done)
-                if (ok && another) ok = begin_item(nq) && issue_qk(it + 1, nq);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) c[q] = at[q];
-                cur_q = nq; first = another;
-                ++it;
+                        for (int kk = 0; kk < BN / 16; ++kk)
+                            bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, behind(dvs, kk * (2048 / 16)), IDESC_PV,
+                                             !(begins && kk == 0));
+                        bw::umma_commit(pv_done + 8 * (2 * q + b));
+                        if (q == tiles_q - 1) bw::umma_commit(v_empty + 8 * s);
+                    }
+                    __syncwarp();
+                    ++n[q];
+                }
+                begins = w.step(p, work);
             }
         }
-    } else if (warp >= 4 * NQ) {
+    } else if (warp >= KEY_WARP) {
         // ---------------------------------------------------------------- widening
-        const int ww = warp - 4 * NQ, mine = 8 * ww + (lane & 7);       // this lane's keys of a tile: mine and mine + 32
+        fewer_registers<WIDEN_REGS>();
+        const bool keys = warp < VALUE_WARP;
+        const int ww = (warp - KEY_WARP) & 3, mine = 8 * ww + (lane & 7);      // this lane's keys of a tile: mine and mine + 32
+        const int8_t* from = keys ? p.k : p.v;
+        uint8_t* tiles = keys ? k_s : v_s;
+        const uint32_t full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
         constexpr int PER = NS;                                          // units of 16 channels a key: (lane >> 3) + 4 j
         struct Rows { int a, b; };                                       // of the keys lane and lane + 32; -1: none
         // the pages of the keys lane and lane + 32 as the table has them (-1: none); made into rows only a step later, so that nothing waits
@@ -347,7 +347,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             for (int i = 0; i < 2; ++i) got[i] = (unsigned)x.page[i] < (unsigned)p.num_pages ? (x.page[i] * p.nkv + x.g) * p.page_size + x.slot[i] : -1;
             return Rows{got[0], got[1]};
         };
-        auto load = [&](const int8_t* from, const Rows& rows, uint4 (&x)[2][PER]) {
+        auto load = [&](const Rows& rows, uint4 (&x)[2][PER]) {
             const int r[2] = {__shfl_sync(0xffffffffu, rows.a, mine), __shfl_sync(0xffffffffu, rows.b, mine)};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -365,18 +365,16 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             Pages next{{-1, -1}, {0, 0}, 0};
             if (ahead.left > 1) { ahead.step(p, work); next = look_up(ahead); }
             // rows of a step are loaded a whole step before they are widened, and looked up one before that
-            uint4 kx[2][PER], vx[2][PER], k_next[2][PER], v_next[2][PER];
+            uint4 x[2][PER], x_next[2][PER];
             float ks[2], vs[2], ks_next[2], vs_next[2];
-            load(p.k, cur, kx);
-            load(p.v, cur, vx);
+            load(cur, x);
             scales(p.k_scale, cur, ks); scales(p.v_scale, cur, vs);
             const int total = w.left;
             for (int it = 0; it < total; ++it) {
                 const int s = it % STAGES;
                 const Rows rows = rows_of(next);                                          // (behind the last step: none, and zeros)
                 scales(p.k_scale, rows, ks_next); scales(p.v_scale, rows, vs_next);
-                load(p.k, rows, k_next);
-                load(p.v, rows, v_next);
+                load(rows, x_next);
                 next = Pages{{-1, -1}, {0, 0}, 0};
                 if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
                 // references and factors
@@ -392,52 +390,52 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 // (powers of two: the exponent turned around)
                 const float inv_k = __uint_as_float((254u << 23) - __float_as_uint(k_ref)), inv_v = __uint_as_float((254u << 23) - __float_as_uint(v_ref));
                 const float nan = __uint_as_float(0x7fffffffu);
-                float fk[2], fv[2];
+                float f[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    fk[i] = __shfl_sync(0xffffffffu, bad[i] ? nan : ks[i] * inv_k, mine);
-                    fv[i] = __shfl_sync(0xffffffffu, bad[i] ? 0.f : vs[i] * inv_v, mine);
+                    const float own = keys ? (bad[i] ? nan : ks[i] * inv_k) : (bad[i] ? 0.f : vs[i] * inv_v);
+                    f[i] = __shfl_sync(0xffffffffu, own, mine);
                 }
-                const unsigned there0 = __ballot_sync(0xffffffffu, cur.a >= 0), there1 = __ballot_sync(0xffffffffu, cur.b >= 0);
-                if (it >= STAGES && !all(bw::mbar_wait(k_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 37))) break;
-                if (ww == 0 && lane == 0) {
-                    TileInfo t;
-                    t.k_ref = k_ref; t.inv_v = inv_v;
-                    t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
-                    t.there[0] = there0; t.there[1] = there1;
-                    t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
-                    info[it % RING] = t;
-                }
+                if (it >= STAGES && !all(bw::mbar_wait(empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, keys ? 37 : 38))) break;
+                if (keys) {
+                    const unsigned there0 = __ballot_sync(0xffffffffu, cur.a >= 0), there1 = __ballot_sync(0xffffffffu, cur.b >= 0);
+                    if (ww == 0 && lane == 0) {
+                        TileInfo t;
+                        t.k_ref = k_ref; t.inv_v = inv_v;
+                        t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
+                        t.there[0] = there0; t.there[1] = there1;
+                        t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
+                        info[it % RING] = t;
+                    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const Factor f = factor_of(fk[i]);
+                    for (int i = 0; i < 2; ++i) {
+                        const Factor two = factor_of(f[i]);
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) widen16(k_s + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, kx[i][j], f);
+                        for (int j = 0; j < PER; ++j) widen16(tiles + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, x[i][j], two);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t one = pack_f16x2(f[i], f[i]);
+#pragma unroll
+                        for (int j = 0; j < PER; ++j) widen16(tiles + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, x[i][j], one);
+                    }
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) bw::mbar_arrive(k_full + 8 * s);
-                if (it >= STAGES && !all(bw::mbar_wait(v_empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, 38))) break;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t f = pack_f16x2(fv[i], fv[i]);
-#pragma unroll
-                    for (int j = 0; j < PER; ++j) widen16(v_s + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, vx[i][j], f);
-                }
-                bw::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) bw::mbar_arrive(v_full + 8 * s);
+                if (lane == 0) bw::mbar_arrive(full + 8 * s);
                 cur = rows;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     ks[i] = ks_next[i]; vs[i] = vs_next[i];
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) { kx[i][j] = k_next[i][j]; vx[i][j] = v_next[i][j]; }
+                    for (int j = 0; j < PER; ++j) x[i][j] = x_next[i][j];
                 }
             }
         }
     } else {
         // ---------------------------------------------------------------- softmax: tile of rows `q`, one thread a row
+        more_registers<SOFTMAX_REGS>();
         const int q = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * HD + lanes;
@@ -614,7 +612,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     }
     bw::tc_fence_before();
     __syncthreads();
-    if (warp == MMA_WARP) bw::tmem_dealloc(tmem_base, TMEM_COLS);
+    if (warp == QK_WARP) bw::tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
 // The items that several blocks share: a thread a row, four channels a block.
