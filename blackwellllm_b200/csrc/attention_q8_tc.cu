@@ -10,7 +10,7 @@
 //   * one warp issues S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, another O += P V with P from tensor memory (one warp for
 //     both spent two thirds of its time between its products);
 //   * eight warps, one thread a row, make P: maximum, exponentials, sums; P is written over the S it came from as float16 pairs.
-// Roundings: K and V to float16 (2^-11 of an element, a value's scale by as much again; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
+// Roundings: K and V to float16, twice (their scale, and the product: 2^-11 of an element each; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
 // beside the largest), and the result to bfloat16.  Scores, sums and outputs are float32; the queries are multiplied by a power of two a row
 // (attention_q8.cu) and exact.  The exponents' reference follows the largest t + log2 of the tile's value scale lazily (by steps of more than
 // 8), so O is seldom rescaled.
@@ -42,11 +42,11 @@ constexpr int Q_SLICE = BM * 128, KV_SLICE = BN * 128;
 constexpr int Q_BYTES = NS * Q_SLICE, KV_BYTES = NS * KV_SLICE;
 constexpr int RING = STAGES + 2;            // what the softmax reads of a tile of keys: a widening warp is at most that far ahead of it
 // Groups of four warps: NQ of the softmax, one that widens keys, one that widens values, and one whose first two warps issue products.  A block is
-// launched with 96 registers a thread (128 with four groups) and the groups trade them: 256 * 136 + 256 * 80 + 128 * 48 = 61,440, all of them,
+// launched with 96 registers a thread (128 with four groups) and the groups trade them: 256 * 144 + 256 * 72 + 128 * 48 = 61,440, all of them,
 // and 128 * 168 + 256 * 112 + 128 * 48 = 56,320 of 65,536.
 constexpr int KEY_WARP = 4 * NQ, VALUE_WARP = KEY_WARP + 4, QK_WARP = VALUE_WARP + 4, PV_WARP = QK_WARP + 1;
 constexpr int THREADS = 32 * (QK_WARP + 4);
-constexpr int SOFTMAX_REGS = NQ == 2 ? 136 : 168, WIDEN_REGS = NQ == 2 ? 80 : 112, ISSUE_REGS = 48;
+constexpr int SOFTMAX_REGS = NQ == 2 ? 144 : 168, WIDEN_REGS = NQ == 2 ? 72 : 112, ISSUE_REGS = 48;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int SMEM_BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + RING * 32 + 32 * 8 + 16;
@@ -150,22 +150,8 @@ __device__ __forceinline__ bw::f32x2 add2(bw::f32x2 a, bw::f32x2 b) {
     return d;
 }
 
-// A row's factor as two float16 numbers that add up to it, each twice.
-struct Factor { uint32_t hi, lo; };
-__device__ __forceinline__ Factor factor_of(float f) {
-    const float hi = __half2float(__float2half_rn(f));
-    return {pack_f16x2(f, f), pack_f16x2(f - hi, f - hi)};
-}
-// Two bytes of r (128 too large) times the factor, in float16: 0x6400 | byte is 1024 + byte, 1152 less is the whole number, exact; its product with
-// the factor is rounded once (the low part's product is 2^-11 of it and rounded by 2^-11 of that).
-template <int SEL>
-__device__ __forceinline__ uint32_t widen2(uint32_t r, const Factor& f) {
-    uint32_t n, d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(n) : "r"(__byte_perm(r, 0x64646464u, SEL)), "r"(0x64806480u));
-    asm("{\n.reg .b32 t;\nmul.rn.f16x2 t, %1, %2;\nfma.rn.f16x2 %0, %1, %3, t;\n}" : "=r"(d) : "r"(n), "r"(f.lo), "r"(f.hi));
-    return d;
-}
-// The same with the factor rounded to float16 (values: 2^-11 of a key's value; a score would be off by that much of itself).
+// Two bytes of r (128 too large) times a row's factor (a float16 number, twice): 0x6400 | byte is 1024 + byte, 1152 less is the whole number,
+// exact; the product is rounded.
 template <int SEL>
 __device__ __forceinline__ uint32_t widen2(uint32_t r, uint32_t f) {
     uint32_t n, d;
@@ -173,16 +159,11 @@ __device__ __forceinline__ uint32_t widen2(uint32_t r, uint32_t f) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(n), "r"(f));
     return d;
 }
-// 16 channels (unit c) of key `key` into a tile of operands
-template <typename Factor>
-__device__ __forceinline__ void widen16(uint8_t* tile, int key, int c, uint4 x, const Factor& f) {
+// 16 channels of a key, as the two units of its row of operands
+__device__ __forceinline__ void widen16(uint8_t* first, uint8_t* second, uint4 x, uint32_t f) {
     const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-    uint8_t* row = tile + (c >> 2) * KV_SLICE + key * 128;
-    const int u = 2 * (c & 3), k7 = key & 7;
-    *reinterpret_cast<uint4*>(row + ((u ^ k7) << 4)) =
-        make_uint4(widen2<0x4140>(w[0], f), widen2<0x4342>(w[0], f), widen2<0x4140>(w[1], f), widen2<0x4342>(w[1], f));
-    *reinterpret_cast<uint4*>(row + (((u + 1) ^ k7) << 4)) =
-        make_uint4(widen2<0x4140>(w[2], f), widen2<0x4342>(w[2], f), widen2<0x4140>(w[3], f), widen2<0x4342>(w[3], f));
+    *reinterpret_cast<uint4*>(first) = make_uint4(widen2<0x4140>(w[0], f), widen2<0x4342>(w[0], f), widen2<0x4140>(w[1], f), widen2<0x4342>(w[1], f));
+    *reinterpret_cast<uint4*>(second) = make_uint4(widen2<0x4140>(w[2], f), widen2<0x4342>(w[2], f), widen2<0x4140>(w[3], f), widen2<0x4342>(w[3], f));
 }
 // The smallest power of two that is not below any finite one of a warp's non-negative numbers (bits of the largest); at least 2^-100.
 __device__ __forceinline__ float power_above(unsigned bits) {
@@ -347,90 +328,90 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             for (int i = 0; i < 2; ++i) got[i] = (unsigned)x.page[i] < (unsigned)p.num_pages ? (x.page[i] * p.nkv + x.g) * p.page_size + x.slot[i] : -1;
             return Rows{got[0], got[1]};
         };
-        auto load = [&](const Rows& rows, uint4 (&x)[2][PER]) {
-            const int r[2] = {__shfl_sync(0xffffffffu, rows.a, mine), __shfl_sync(0xffffffffu, rows.b, mine)};
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < PER; ++j)
-                    x[i][j] = r[i] >= 0 ? *reinterpret_cast<const uint4*>(from + (size_t)r[i] * HD + 16 * ((lane >> 3) + 4 * j)) : make_uint4(0, 0, 0, 0);
-        };
-        auto scales = [&](const float* from, const Rows& rows, float (&x)[2]) {
-            x[0] = rows.a >= 0 ? from[rows.a] : 0.f;
-            x[1] = rows.b >= 0 ? from[rows.b] : 0.f;
-        };
+        auto prefetch = [](const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); };
+        auto scale = [&](const float* of, int row) { return row >= 0 ? of[row] : 0.f; };
         if (w.left > 0) {
             Walk ahead = w;
-            Rows cur = rows_of(look_up(ahead));
+            Rows rows = rows_of(look_up(ahead));
             Pages next{{-1, -1}, {0, 0}, 0};
             if (ahead.left > 1) { ahead.step(p, work); next = look_up(ahead); }
-            // rows of a step are loaded a whole step before they are widened, and looked up one before that
-            uint4 x[2][PER], x_next[2][PER];
-            float ks[2], vs[2], ks_next[2], vs_next[2];
-            load(cur, x);
-            scales(p.k_scale, cur, ks); scales(p.v_scale, cur, vs);
+            // A unit of the next step is loaded as soon as this step's is widened, into the same registers: it has a whole step to come.  Where no
+            // row is, the pool's first is read, and its factor is 0.
+            uint4 x[2][PER];
+            const int8_t* base = from + 16 * (lane >> 3);
+            auto unit_of = [&](const int8_t* row, int j) { return *reinterpret_cast<const uint4*>(row + 64 * j); };
+            {
+                const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) { x[0][j] = unit_of(a, j); x[1][j] = unit_of(b, j); }
+            }
+            float ks[2] = {scale(p.k_scale, rows.a), scale(p.k_scale, rows.b)}, vs[2] = {scale(p.v_scale, rows.a), scale(p.v_scale, rows.b)};
+            unsigned there0 = __ballot_sync(0xffffffffu, rows.a >= 0), there1 = __ballot_sync(0xffffffffu, rows.b >= 0);
+            // where this lane's units go: rows mine and mine + 32, units 2 (lane >> 3) and the next of every slice, permuted by the row
+            uint8_t* first = tiles + mine * 128 + (((2 * (lane >> 3)) ^ (lane & 7)) << 4);
+            uint8_t* second = tiles + mine * 128 + (((2 * (lane >> 3) + 1) ^ (lane & 7)) << 4);
             const int total = w.left;
             for (int it = 0; it < total; ++it) {
                 const int s = it % STAGES;
-                const Rows rows = rows_of(next);                                          // (behind the last step: none, and zeros)
-                scales(p.k_scale, rows, ks_next); scales(p.v_scale, rows, vs_next);
-                load(rows, x_next);
-                next = Pages{{-1, -1}, {0, 0}, 0};
-                if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
+                rows = rows_of(next);                                                     // of the next step (behind the last: none)
+                const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
+                // (into the first-level cache now; loaded only behind the fence below, which waits for loads under way)
+                if ((lane >> 3) == ww) {
+                    prefetch(from + (size_t)max(rows.a, 0) * HD);
+                    prefetch(from + (size_t)max(rows.b, 0) * HD);
+                    if (HD > 128) {
+                        prefetch(from + (size_t)max(rows.a, 0) * HD + 128);
+                        prefetch(from + (size_t)max(rows.b, 0) * HD + 128);
+                    }
+                }
+                prefetch(p.k_scale + max(rows.a, 0)); prefetch(p.k_scale + max(rows.b, 0));
+                prefetch(p.v_scale + max(rows.a, 0)); prefetch(p.v_scale + max(rows.b, 0));
                 // references and factors
                 unsigned kb = 0, vb = 0;
                 bool bad[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const unsigned a = __float_as_uint(ks[i]), b = __float_as_uint(vs[i]);
-                    bad[i] = a >= 0x7f800000u || b >= 0x7f800000u;
-                    if (!bad[i]) { kb = max(kb, a); vb = max(vb, b); }
+                    const unsigned y = __float_as_uint(ks[i]), z = __float_as_uint(vs[i]);
+                    bad[i] = max(y, z) >= 0x7f800000u;
+                    kb = max(kb, bad[i] ? 0u : y);
+                    vb = max(vb, bad[i] ? 0u : z);
                 }
                 const float k_ref = power_above(__reduce_max_sync(0xffffffffu, kb)), v_ref = power_above(__reduce_max_sync(0xffffffffu, vb));
                 // (powers of two: the exponent turned around)
-                const float inv_k = __uint_as_float((254u << 23) - __float_as_uint(k_ref)), inv_v = __uint_as_float((254u << 23) - __float_as_uint(v_ref));
-                const float nan = __uint_as_float(0x7fffffffu);
-                float f[2];
+                const float inv_v = __uint_as_float((254u << 23) - __float_as_uint(v_ref)),
+                            inv = keys ? __uint_as_float((254u << 23) - __float_as_uint(k_ref)) : inv_v;
+                uint32_t f[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float own = keys ? (bad[i] ? nan : ks[i] * inv_k) : (bad[i] ? 0.f : vs[i] * inv_v);
-                    f[i] = __shfl_sync(0xffffffffu, own, mine);
+                    const float own = bad[i] ? (keys ? __uint_as_float(0x7fffffffu) : 0.f) : (keys ? ks[i] : vs[i]) * inv;
+                    f[i] = __shfl_sync(0xffffffffu, pack_f16x2(own, own), mine);
                 }
                 if (it >= STAGES && !all(bw::mbar_wait(empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, keys ? 37 : 38))) break;
-                if (keys) {
-                    const unsigned there0 = __ballot_sync(0xffffffffu, cur.a >= 0), there1 = __ballot_sync(0xffffffffu, cur.b >= 0);
-                    if (ww == 0 && lane == 0) {
-                        TileInfo t;
-                        t.k_ref = k_ref; t.inv_v = inv_v;
-                        t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
-                        t.there[0] = there0; t.there[1] = there1;
-                        t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
-                        info[it % RING] = t;
-                    }
+                if (warp == KEY_WARP && lane == 0) {
+                    TileInfo t;
+                    t.k_ref = k_ref; t.inv_v = inv_v;
+                    t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
+                    t.there[0] = there0; t.there[1] = there1;
+                    t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
+                    info[it % RING] = t;
+                }
+                there0 = __ballot_sync(0xffffffffu, rows.a >= 0); there1 = __ballot_sync(0xffffffffu, rows.b >= 0);
+                // (one piece of code for keys and values: what an SM quarter's warps run over and over has to fit its instruction cache)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const Factor two = factor_of(f[i]);
-#pragma unroll
-                        for (int j = 0; j < PER; ++j) widen16(tiles + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, x[i][j], two);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t one = pack_f16x2(f[i], f[i]);
-#pragma unroll
-                        for (int j = 0; j < PER; ++j) widen16(tiles + s * KV_BYTES, mine + 32 * i, (lane >> 3) + 4 * j, x[i][j], one);
-                    }
+                for (int j = 0; j < PER; ++j) {
+                    const int to = s * KV_BYTES + j * KV_SLICE;
+                    widen16(first + to, second + to, x[0][j], f[0]);
+                    widen16(first + to + 32 * 128, second + to + 32 * 128, x[1][j], f[1]);
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(full + 8 * s);
-                cur = rows;
+                ks[0] = scale(p.k_scale, rows.a); ks[1] = scale(p.k_scale, rows.b);
+                vs[0] = scale(p.v_scale, rows.a); vs[1] = scale(p.v_scale, rows.b);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    ks[i] = ks_next[i]; vs[i] = vs_next[i];
-#pragma unroll
-                    for (int j = 0; j < PER; ++j) x[i][j] = x_next[i][j];
-                }
+                for (int j = 0; j < PER; ++j) { x[0][j] = unit_of(a, j); x[1][j] = unit_of(b, j); }
+                next = Pages{{-1, -1}, {0, 0}, 0};
+                if (it + 2 < total) { ahead.step(p, work); next = look_up(ahead); }
             }
         }
     } else {
@@ -441,44 +422,53 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * HD + lanes;
         int it = 0, c = 0;              // steps of the walk, and those of them that this tile of rows has
         bool ok = true;
+        constexpr int UNITS = HD / 8;   // of 16 bytes: a row of queries or outputs
+        uint8_t* rows32 = q_s + q * Q_BYTES + (warp & 3) * 32 * 128;        // the warp's rows of the queries' tile
+        auto unit_at = [&](int r, int u) { return reinterpret_cast<uint4*>(rows32 + (u >> 3) * Q_SLICE + r * 128 + (((u & 7) ^ (r & 7)) << 4)); };
+        // Every unit of the warp's rows once: f(row of the warp, unit, element of the queries or outputs, whether the row exists).  Rolled up, as
+        // everything that runs once an item, or nearly: code that is not in the instruction cache costs more than it does (a row's load,
+        // conversion and store, unrolled, took 13,000 cycles).
+        auto move_rows = [&](int own_row, bool row_ok, auto f) {
+#pragma unroll 4
+            for (int i = 0; i < UNITS; ++i) {
+                const int idx = lane + 32 * i, r = idx / UNITS, u = idx - r * UNITS;
+                const int at = __shfl_sync(0xffffffffu, row_ok ? own_row : -1, r);
+                f(r, u, (size_t)(at >= 0 ? at : 0) * HD + 8 * u, at >= 0);
+            }
+        };
         while (ok && w.left > 0) {
             const Item item = w.it;
             const bool mine = q < q_tiles(item);
             const int gr = item.row0 + q * BM + row;                    // the row among the request's
             const bool row_ok = q * BM + row < item.n_rows;
             const int tok = gr / p.G, head = item.g * p.G + gr - tok * p.G, qpos = item.q_pos0 + tok;
-            const size_t at = ((size_t)(item.tok + tok) * p.nh + head) * HD;
+            const int own_row = (item.tok + tok) * p.nh + head;         // of the queries and outputs
             float sc = 0.f;             // what turns a product into a power of two, but for the tile's reference
             if (mine) {
-                // the row's queries as float16 times a power of two
-                const uint4* src = reinterpret_cast<const uint4*>(p.q + at);
-                uint8_t* dst = q_s + q * Q_BYTES + row * 128;
+                // The warp's 32 rows come together (16 bytes a lane, neighbours of a row side by side: a row a lane would touch 32 lines with every
+                // load) and lie in their place in shared memory as they are; then every lane turns its row into float16 times a power of two.
+                move_rows(own_row, row_ok, [&](int r, int u, size_t from, bool live) {
+                    const int bytes = live ? 16 : 0;       // 0: zeros are written
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(bw::smem_u32(unit_at(r, u))), "l"(p.q + from), "r"(bytes) : "memory");
+                });
+                asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
                 unsigned most = 0;
-                constexpr int PART = HD <= 128 ? HD / 8 : 16;       // loads in flight together (the row's in one pass up to head size 128)
-                uint4 x[PART];
-#pragma unroll 1
-                for (int i0 = 0; i0 < HD / 8; i0 += PART) {
-#pragma unroll
-                    for (int i = 0; i < PART; ++i) x[i] = row_ok && i0 + i < HD / 8 ? src[i0 + i] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < PART; ++i)
-                        most = max(max(max(most, max(x[i].x & 0x7fffu, x[i].x >> 16 & 0x7fffu)), max(x[i].y & 0x7fffu, x[i].y >> 16 & 0x7fffu)),
-                                   max(max(x[i].z & 0x7fffu, x[i].z >> 16 & 0x7fffu), max(x[i].w & 0x7fffu, x[i].w >> 16 & 0x7fffu)));
+#pragma unroll 4
+                for (int u = 0; u < UNITS; ++u) {
+                    const uint4 x = *unit_at(lane, u);
+                    most = max(max(max(most, max(x.x & 0x7fffu, x.x >> 16 & 0x7fffu)), max(x.y & 0x7fffu, x.y >> 16 & 0x7fffu)),
+                               max(max(x.z & 0x7fffu, x.z >> 16 & 0x7fffu), max(x.w & 0x7fffu, x.w >> 16 & 0x7fffu)));
                 }
                 unsigned ex = max(most >> 7, 15u);
                 if (ex == 255) ex = 141;                                // an infinity or NaN: as it is
                 const float up = __uint_as_float((268 - ex) << 23);
                 sc = __uint_as_float((ex - 14) << 23) * p.scale_log2;
                 auto two = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up); };
-#pragma unroll 1
-                for (int i0 = 0; i0 < HD / 8; i0 += PART) {
-#pragma unroll
-                    for (int i = 0; i < PART; ++i) {
-                        if (HD > 128) x[i] = row_ok && i0 + i < HD / 8 ? src[i0 + i] : make_uint4(0, 0, 0, 0);
-                        const int u = i0 + i;
-                        if (u < HD / 8)
-                            *reinterpret_cast<uint4*>(dst + (u >> 3) * Q_SLICE + (((u & 7) ^ (row & 7)) << 4)) = make_uint4(two(x[i].x), two(x[i].y), two(x[i].z), two(x[i].w));
-                    }
+#pragma unroll 4
+                for (int u = 0; u < UNITS; ++u) {
+                    const uint4 x = *unit_at(lane, u);
+                    *unit_at(lane, u) = make_uint4(two(x.x), two(x.y), two(x.z), two(x.w));
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
@@ -575,20 +565,23 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             if (w.opens && w.closes) {
                 if (p.sink && row_ok) l += ex2(p.sink[head] * LOG2E - m);
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                bf16* dst = p.out + at;
+                // (the queries are done with: the warp's outputs take their place, and go out 16 bytes a lane, a row's side by side)
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
                     uint32_t o[32];
                     bw::tmem_ld_32x32(tmem_Oq + c0, o);
                     bw::tmem_ld_wait();
-                    if (row_ok) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            auto two = [&](int i) { return bw::pack_bf16x2(__uint_as_float(o[j + i]) * inv, __uint_as_float(o[j + i + 1]) * inv); };
-                            *reinterpret_cast<uint4*>(dst + c0 + j) = make_uint4(two(0), two(2), two(4), two(6));
-                        }
+                    for (int j = 0; j < 32; j += 8) {
+                        auto two = [&](int i) { return bw::pack_bf16x2(__uint_as_float(o[j + i]) * inv, __uint_as_float(o[j + i + 1]) * inv); };
+                        *unit_at(lane, (c0 + j) >> 3) = make_uint4(two(0), two(2), two(4), two(6));
                     }
                 }
+                __syncwarp();
+                move_rows(own_row, row_ok, [&](int r, int u, size_t to, bool live) {
+                    if (live) *reinterpret_cast<uint4*>(p.out + to) = *unit_at(r, u);
+                });
+                __syncwarp();
             } else {
                 // a part of the item: the block's first part (1 if it begins with the item, so it is its last) leaves its sums
                 const size_t slot = 2 * (size_t)blockIdx.x + (w.opens ? 1 : 0);

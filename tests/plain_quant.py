@@ -111,10 +111,10 @@ def attention_bound(e, hd, wide=None):
       sum cut at 2^-23 of the magnitudes so far, and two steps for what comes off and the factors; as an exponent it is in weights
       and denominator;
       2^-16 for exponentials, and sums of the longest lists tested here in float32.
-    ``wide`` [T]: rows of the tcgen05 kernel, where keys and values are rounded to float16 too, as multiples of a power of two that is less
-    than twice the largest scale of the 64 keys beside them: 2^-11 of sum |q k|, and where that is less than float16's smallest step, 2^-25
-    of twice that scale for every channel; of values 2^-10 of sum p |v| (their scale is rounded
-    too), and 2^-25 of twice theirs; the weights are multiples of p times it."""
+    ``wide`` [T]: rows of the tcgen05 kernel, where keys and values are rounded to float16 too (their scale, then the product), as multiples of
+    a power of two that is less than twice the largest scale of the 64 keys beside them: 2^-10 of sum |q k|, and where that is less than
+    float16's smallest step, 2^-25 of twice that scale for every channel, and of a number of 127 at most for the scale; of values 2^-10 of
+    sum p |v|, and as much of twice theirs; the weights are multiples of p times it."""
     u = 2.0 ** -8
 
     def bound(ds, rounding, small):
@@ -122,6 +122,7 @@ def attention_bound(e, hd, wide=None):
     sums = (hd / 16 + 2) * 2.0 ** -23
     tol = bound(sums * e.raised, 2.0 ** -11, 2.0 ** -25 * e.least)
     if wide is not None and wide.any():
-        more = bound((sums + 2.0 ** -11) * e.scores + 2.0 ** -24 * e.coarse, 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -20, 2.0 ** -24 * (e.least_v + e.most_v))
+        more = bound((sums + 2.0 ** -10) * e.scores + 128 * 2.0 ** -24 * e.coarse, 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -20,
+                     2.0 ** -24 * (e.least_v + 128 * e.most_v))
         tol = torch.where(wide[:, None, None], more, tol)
     return tol
