@@ -294,11 +294,16 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         // ---------------------------------------------------------------- widening
         fewer_registers<WIDEN_REGS>();
         const bool keys = warp < VALUE_WARP;
-        const int ww = (warp - KEY_WARP) & 3, mine = 8 * ww + (lane & 7);      // this lane's keys of a tile: mine and mine + 32
+        // This lane's keys of a tile are mine and mine + 32.  Eight lanes, whose 16 bytes move together, take units 0 to 3 of a slice of one key and
+        // of the other slice of the next (of the same slice, where rows are an odd number of slices long): in the cache that is 128 bytes from
+        // different banks, and among the operands, whose units are permuted by the key's number, too.  (Eight keys' units with the same
+        // number, as first written, took eight turns: two thirds of the data pipe's time.)
+        const int ww = (warp - KEY_WARP) & 3, odd = lane >> 2 & 1, mine = 8 * ww + 2 * (lane >> 3) + odd;
+        constexpr bool SWAP = NS % 2 == 0;
         const int8_t* from = keys ? p.k : p.v;
         uint8_t* tiles = keys ? k_s : v_s;
         const uint32_t full = keys ? k_full : v_full, empty = keys ? k_empty : v_empty;
-        constexpr int PER = NS;                                          // units of 16 channels a key: (lane >> 3) + 4 j
+        constexpr int PER = NS;                                          // units of 16 channels a key
         struct Rows { int a, b; };                                       // of the keys lane and lane + 32; -1: none
         // the pages of the keys lane and lane + 32 as the table has them (-1: none); made into rows only a step later, so that nothing waits
         struct Pages { int page[2], slot[2], g; };
@@ -338,8 +343,9 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             // A unit of the next step is loaded as soon as this step's is widened, into the same registers: it has a whole step to come.  Where no
             // row is, the pool's first is read, and its factor is 0.
             uint4 x[2][PER];
-            const int8_t* base = from + 16 * (lane >> 3);
-            auto unit_of = [&](const int8_t* row, int j) { return *reinterpret_cast<const uint4*>(row + 64 * j); };
+            const int8_t* base = from + 16 * (lane & 3);
+            const int swap = SWAP && odd ? 1 : 0;            // slice j of this lane is slice j ^ swap of the row
+            auto unit_of = [&](const int8_t* row, int j) { return *reinterpret_cast<const uint4*>(row + 64 * j + (j & 1 ? -64 : 64) * swap); };
             {
                 const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
 #pragma unroll
@@ -347,9 +353,9 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             }
             float ks[2] = {scale(p.k_scale, rows.a), scale(p.k_scale, rows.b)}, vs[2] = {scale(p.v_scale, rows.a), scale(p.v_scale, rows.b)};
             unsigned there0 = __ballot_sync(0xffffffffu, rows.a >= 0), there1 = __ballot_sync(0xffffffffu, rows.b >= 0);
-            // where this lane's units go: rows mine and mine + 32, units 2 (lane >> 3) and the next of every slice, permuted by the row
-            uint8_t* first = tiles + mine * 128 + (((2 * (lane >> 3)) ^ (lane & 7)) << 4);
-            uint8_t* second = tiles + mine * 128 + (((2 * (lane >> 3) + 1) ^ (lane & 7)) << 4);
+            // where this lane's units go: rows mine and mine + 32, units 2 (lane & 3) and the next of every slice, permuted by the row
+            uint8_t* first = tiles + mine * 128 + (((2 * (lane & 3)) ^ (mine & 7)) << 4);
+            uint8_t* second = tiles + mine * 128 + (((2 * (lane & 3) + 1) ^ (mine & 7)) << 4);
             const int total = w.left;
             for (int it = 0; it < total; ++it) {
                 const int s = it % STAGES;
@@ -399,7 +405,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 // (one piece of code for keys and values: what an SM quarter's warps run over and over has to fit its instruction cache)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    const int to = s * KV_BYTES + j * KV_SLICE;
+                    const int to = s * KV_BYTES + j * KV_SLICE + (j & 1 ? -KV_SLICE : KV_SLICE) * swap;
                     widen16(first + to, second + to, x[0][j], f[0]);
                     widen16(first + to + 32 * 128, second + to + 32 * 128, x[1][j], f[1]);
                 }
