@@ -459,13 +459,14 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 });
                 asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
                 __syncwarp();
-                unsigned most = 0;
+                unsigned most2 = 0;                       // of the even and of the odd channels, as 16-bit numbers
 #pragma unroll 4
                 for (int u = 0; u < UNITS; ++u) {
                     const uint4 x = *unit_at(lane, u);
-                    most = max(max(max(most, max(x.x & 0x7fffu, x.x >> 16 & 0x7fffu)), max(x.y & 0x7fffu, x.y >> 16 & 0x7fffu)),
-                               max(max(x.z & 0x7fffu, x.z >> 16 & 0x7fffu), max(x.w & 0x7fffu, x.w >> 16 & 0x7fffu)));
+                    most2 = __vmaxu2(__vmaxu2(most2, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+                    most2 = __vmaxu2(__vmaxu2(most2, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
                 }
+                const unsigned most = max(most2 & 0xffffu, most2 >> 16);
                 unsigned ex = max(most >> 7, 15u);
                 if (ex == 255) ex = 141;                                // an infinity or NaN: as it is
                 const float up = __uint_as_float((268 - ex) << 23);
@@ -646,8 +647,14 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
 }
 
 // Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining.
-constexpr int LEAST_STEPS = 4;
-constexpr int ITEM_COST = 3;         // what an item costs beside its steps (its queries, the first scores, its outputs), in steps
+#ifndef Q8_ITEM_COST
+#define Q8_ITEM_COST 5
+#endif
+#ifndef Q8_LEAST
+#define Q8_LEAST 4
+#endif
+constexpr int LEAST_STEPS = Q8_LEAST;
+constexpr int ITEM_COST = Q8_ITEM_COST;         // what an item costs beside its steps (its queries, the first scores, its outputs), in steps
 int blocks_for(long long cost) {
     const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;
     const long long n = (cost + LEAST_STEPS + ITEM_COST - 1) / (LEAST_STEPS + ITEM_COST);
