@@ -57,6 +57,7 @@ struct Params {
     float* part_o; float* part_ml;  // results of key slices: [request][kv head][slice][16][HD] and [..][2]
     int max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests;
     int per, slices;                // key slices: tiles of each, most of them that any request has
+    int cluster;                    // the slices of a (request, kv head) are one cluster of blocks and join there
     float scale_log2;
 };
 
@@ -394,12 +395,28 @@ template <int NB> constexpr int FEW_KG = NB * HD <= 128 ? Q8_KG : 1;
 constexpr int STAGES = Q8_STAGES;
 template <int NB> constexpr int SMEM_RING = WARPS * STAGES * STAGE<FEW_KG<NB>>;
 constexpr int JOIN_LD = HD + 8;
-constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD) * 4;
+constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD + 2 * 16) * 4;
 template <int NB> constexpr int SMEM_FEW = SMEM_RING<NB> > SMEM_JOIN ? SMEM_RING<NB> : SMEM_JOIN;
 // blocks an SM runs at once: by shared memory, and by registers (about 60 beside the queries and outputs)
 template <int NB> constexpr int BY_SMEM = (227 * 1024) / (SMEM_FEW<NB> + 1024);
 template <int NB> constexpr int BY_REGS = 512 / (((60 + NB * CHUNKS * 6) + 7) / 8 * 8);
 template <int NB> constexpr int FEW_BLOCKS = BY_SMEM<NB> < BY_REGS<NB> ? (BY_SMEM<NB> > 0 ? BY_SMEM<NB> : 1) : (BY_REGS<NB> > 0 ? BY_REGS<NB> : 1);
+
+constexpr int MOST_CLUSTER = 8;
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// from another block of the cluster, at the place where it is in this one's shared memory
+template <typename T> __device__ __forceinline__ T read_block(uint32_t at, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    T v;
+    if constexpr (sizeof(T) == 16)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    else
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
 
 struct Walk { int first, tiles, per, live; };   // in tiles of TILE keys: where it begins, how many, of a slice; slices that have any
 __device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last) {
@@ -433,7 +450,7 @@ few_kernel(Params p) {
     if (n_tok <= 0 || n_rows > 8 * NB || (NB == 2 && n_rows <= 8)) return;
     const int q_pos0 = p.q_start[r], last = q_pos0 + n_tok - 1, kv_len = p.kv_len[r];
     const Walk walk = walk_of(p, q_pos0, last);
-    if (slice >= walk.live) return;
+    if (slice >= walk.live) return;        // (a cluster's barrier waits for no block that has left)
     const int t0 = walk.first + slice * walk.per, t1 = min(walk.first + walk.tiles, t0 + walk.per);
     const int* bt = p.table + (size_t)r * p.max_blocks;
     constexpr int KG = FEW_KG<NB>, N = KG * KEYS;      // keys of a warp's step
@@ -477,6 +494,7 @@ few_kernel(Params p) {
     float* ms = reinterpret_cast<float*>(smem);
     float* ls = ms + WARPS * 16;
     float* os = ls + WARPS * 16;
+    float* ml = os + WARPS * 16 * JOIN_LD;      // [16][2]: the block's reference and sum of a row, for its cluster
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -509,12 +527,45 @@ few_kernel(Params p) {
         if (walk.live == 1) {
             const int t = row / p.G, head = g * p.G + row - t * p.G;
             write_row(p, (size_t)(tok + t), head, c, acc, L + sink_term(p, head, M));
+        } else if (p.cluster) {
+            // (in the place of the first warp's, which this thread alone reads)
+            *reinterpret_cast<float4*>(os + row * JOIN_LD + c) = acc;
+            if (c == 0) { ml[2 * row] = M; ml[2 * row + 1] = L; }
         } else {
             const size_t at = (((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
             *reinterpret_cast<float4*>(p.part_o + at * HD + c) = acc;
             if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
         }
     }
+    if (!p.cluster || walk.live == 1) return;
+    // every block takes its share of (row, four channels) from all the cluster's blocks, in the order of the keys
+    cluster_sync();
+    const uint32_t os_at = smem_u32(os), ml_at = smem_u32(ml);
+    for (int idx = slice * THREADS + threadIdx.x; idx < n_rows * (HD / 4); idx += walk.live * THREADS) {
+        const int row = idx / (HD / 4), c = (idx - row * (HD / 4)) * 4;
+        float4 v[MOST_CLUSTER];
+        float2 x[MOST_CLUSTER];
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < MOST_CLUSTER; ++i) {
+            if (i >= walk.live) break;
+            x[i] = read_block<float2>(ml_at + 8 * row, i);
+            v[i] = read_block<float4>(os_at + 4 * (row * JOIN_LD + c), i);
+        }
+#pragma unroll
+        for (int i = 0; i < MOST_CLUSTER; ++i) if (i < walk.live) M = fmaxf(M, x[i].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < MOST_CLUSTER; ++i) {
+            if (i >= walk.live) break;
+            const float f = x[i].x == -INFINITY ? 0.f : exp2f(x[i].x - M);
+            acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+            L += x[i].y * f;
+        }
+        const int t = row / p.G, head = g * p.G + row - t * p.G;
+        write_row(p, (size_t)(tok + t), head, c, acc, L + sink_term(p, head, M));
+    }
+    cluster_sync();      // a block's shared memory stays until it has been read
 }
 
 // Joins the slices of every request that has more than one: a block per (row, kv head, request), groups of HD / 4 threads that take every
@@ -533,18 +584,21 @@ join_kernel(Params p) {
     if (live <= 1) return;
     __shared__ float4 red[JOIN_GROUPS][QUADS];
     __shared__ float red_l[JOIN_GROUPS];
+    __shared__ float scratch[32];
     const size_t base = ((size_t)r * p.nkv + g) * p.slices * 16 + row;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
     float M = -INFINITY;
-    for (int i = 0; i < live; ++i) M = fmaxf(M, ml[base + (size_t)i * 16].x);
+    for (int i = threadIdx.x; i < live; i += 256) M = fmaxf(M, ml[base + (size_t)i * 16].x);
+    M = bw::block_max(M, scratch);
     const int group = threadIdx.x / QUADS, quad = threadIdx.x - group * QUADS;
     if (group < JOIN_GROUPS) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float L = 0.f;
+#pragma unroll 4
         for (int i = group; i < live; i += JOIN_GROUPS) {
             const float2 x = ml[base + (size_t)i * 16];
-            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
             const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + (size_t)i * 16) * HD)[quad];
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
             L += x.y * f;
         }
@@ -650,13 +704,36 @@ many_kernel(Params p, Portions work) {
 
 }  // namespace
 
-// Key slices of the requests with at most 16 rows: how many tiles of TILE keys a slice has (*per) so that the slices of all requests fill
-// the GPU about once, and the most slices of any request (the return value; 0: there is no such request).  Lengths are the host's: of the
-// step, or, for a step that is captured, the longest that may come (`bound` > 0: for every request).
-BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound,
-                                   int* per) {
-    if (requests < 0 || G <= 0 || nkv <= 0 || !per) return BW_ERR_BAD_ARG;
-    long long most = 0, total = 0;
+// Clusters of `size` blocks of the key-slice kernel that run at once on the current device (0: none, or not known), looked up once.
+template <int NB, bool WHOLE>
+static int clusters_at_once(int size) {
+    static int known[bw::MAX_DEVICES][MOST_CLUSTER + 1];      // one more than the number
+    int& n = known[bw::current_device()][size];
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)size); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW<NB>;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        int got = 0;
+        if (cudaFuncSetAttribute(few_kernel<NB, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_FEW<NB>) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&got, few_kernel<NB, WHOLE>, &cfg) != cudaSuccess) { cudaGetLastError(); got = 0; }
+        n = got + 1;
+    }
+    return n - 1;
+}
+
+// Key slices of the requests with at most 16 rows.  Lengths are the host's: of the step, or, for a step that is captured, the longest that may
+// come (`bound` > 0: for every request).  `per`: tiles of a slice, so that the slices of all requests fill the GPU about once; `slices`: the
+// most of any request (0: there is no such request).
+// Where requests are about equally long, up to eight slices that all run at once are a cluster and join there; a join of its own (a launch,
+// and a trip through memory: about two tiles' time) serves more slices, and requests of many lengths, whose clusters would be half empty:
+// us with clusters and without, a token at 701 keys 6.2 and 7.6, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
+// them 63.5 and 55.8, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 11.8.
+constexpr int CLUSTER_EXTRA = 2;
+struct Plan { int per, slices, cluster; };
+static Plan plan_slices(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound, bool whole) {
     auto tiles_of = [&](int r) -> long long {
         if (q_len[r] <= 0 || (long long)q_len[r] * G > 16) return 0;
         const long long first = bound > 0 ? 0 : bw::first_visible(q_start[r], window, chunk), end = bound > 0 ? bound : (long long)q_start[r] + q_len[r];
@@ -670,14 +747,18 @@ BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int req
         }
         return n;
     };
+    long long most = 0, least = 0x7fffffff, few = 0;
+    bool wide = false;                        // more than eight rows: the larger kernel, of which fewer run at once
     for (int r = 0; r < requests; ++r) {
         const long long n = tiles_of(r);
-        total += n;
+        if (n == 0) continue;
+        ++few;
+        wide |= q_len[r] * G > 8;
         if (n > most) most = n;
+        if (n < least) least = n;
     }
-    *per = 1;
-    if (most == 0) return 0;
-    const long long room = (long long)FEW_BLOCKS<1> * bw::num_sms();          // blocks that run at once
+    if (most == 0) return {1, 0, 0};
+    const long long room = (long long)(wide ? FEW_BLOCKS<2> : FEW_BLOCKS<1>) * bw::num_sms();          // blocks that run at once
     long long lo = 1, hi = most;
     while (lo < hi) {
         const long long mid = (lo + hi) / 2;
@@ -685,31 +766,63 @@ BW_EXPORT int bw_attention_q8_plan(const int* q_len, const int* q_start, int req
         for (int r = 0; r < requests; ++r) blocks += (tiles_of(r) + mid - 1) / mid;
         if (blocks * nkv <= room) hi = mid; else lo = mid + 1;
     }
-    *per = (int)lo;
-    return (int)((most + lo - 1) / lo);
+    const long long slices = (most + lo - 1) / lo;
+    if (slices > 1 && 4 * least >= 3 * most) {
+        for (int size = slices < MOST_CLUSTER ? (int)slices : MOST_CLUSTER; size > 1; --size) {
+            const long long per = (most + size - 1) / size;
+            if (per > lo + CLUSTER_EXTRA) break;
+            const int at_once = wide ? (whole ? clusters_at_once<2, true>(size) : clusters_at_once<2, false>(size))
+                                     : (whole ? clusters_at_once<1, true>(size) : clusters_at_once<1, false>(size));
+            if (few * nkv <= at_once) return {(int)per, (int)((most + per - 1) / per), 1};
+        }
+    }
+    return {(int)lo, (int)slices, 0};
 }
 
 template <int NB, bool WHOLE>
 static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
     static bool done[bw::MAX_DEVICES];
     if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<NB, WHOLE>, SMEM_FEW<NB>, done); e != cudaSuccess) return (int)e;
-    bw::launch(few_kernel<NB, WHOLE>, grid, dim3(THREADS), SMEM_FEW<NB>, s, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW<NB>; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (p.cluster) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = grid.x; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (bw::pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr; cfg.numAttrs = n;
+    if (const cudaError_t e = cudaLaunchKernelEx(&cfg, few_kernel<NB, WHOLE>, p); e != cudaSuccess) return (int)e;
     BW_LAUNCH_CHECK();
     return 0;
 }
 
-// q, out: bfloat16 [tokens][nh][HD]; lengths on the host (q_len, h_q_start) as in bw_attention_q8_plan, per and slices as it gave them; part_o,
-// part_ml: room for requests * nkv * slices * 16 rows of HD and of 2 floats, where slices > 1; few_only: requests with more rows are left out.
+// q, out: bfloat16 [tokens][nh][HD]; h_q_len, h_q_start: lengths on the host; bound: see plan_slices.  few_only: requests with more than 16 rows
+// are left out.  room: where the joining needs memory, for *need floats; with none given (null), or too little (room_floats), *need is set, the call
+// returns BW_ERR_ROOM and has launched nothing.
+#define BW_ERR_ROOM (-11)
 BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
                               const int* cu_q, const int* q_start, const int* kv_len, const int* table, int max_blocks, const int* h_q_len,
-                              int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, float scale,
-                              const float* sink, int per, int slices, float* part_o, float* part_ml, int few_only, void* stream) {
-    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || per <= 0) return BW_ERR_BAD_ARG;
-    if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v) & 15) || (slices > 1 && (!part_o || !part_ml))) return BW_ERR_BAD_ARG;
+                              const int* h_q_start, int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, int bound,
+                              float scale, const float* sink, float* room, long long room_floats, long long* need, int few_only, void* stream) {
+    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0) return BW_ERR_BAD_ARG;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room) & 15) return BW_ERR_BAD_ARG;
     if ((long long)num_pages * nkv * page_size > 0x7fffffffll || nkv > 65535 || requests > 65535) return BW_ERR_UNSUPPORTED;
     const int G = nh / nkv;
-    Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, part_o, part_ml,
-             max_blocks, nh, nkv, G, page_size, num_pages, window > 0 ? window : 0, chunk > 0 ? chunk : 0, requests, per, slices, scale * LOG2E};
+    window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
+    const bool whole = page_size % KEYS == 0;
+    const Plan plan = plan_slices(h_q_len, h_q_start, requests, G, nkv, window, chunk, bound, whole);
+    const long long rows = plan.slices > 1 && !plan.cluster ? (long long)requests * nkv * plan.slices * 16 : 0;
+    if (rows * (HD + 2) > room_floats) { *need = rows * (HD + 2); return BW_ERR_ROOM; }
+    const int slices = plan.slices;
+    Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, room, room + rows * HD,
+             max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
     static bool many_done[bw::MAX_DEVICES];
     if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
@@ -742,10 +855,9 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
     const dim3 grid((unsigned)slices, (unsigned)nkv, (unsigned)requests);
-    const bool whole = page_size % KEYS == 0;
     if (few1) if (const int e = whole ? launch_few<1, true>(p, grid, s) : launch_few<1, false>(p, grid, s)) return e;
     if (few2) if (const int e = whole ? launch_few<2, true>(p, grid, s) : launch_few<2, false>(p, grid, s)) return e;
-    if (slices > 1) {
+    if (slices > 1 && !plan.cluster) {
         bw::launch(join_kernel, dim3((unsigned)most_rows, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
         BW_LAUNCH_CHECK();
     }

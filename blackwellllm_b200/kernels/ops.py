@@ -864,16 +864,12 @@ def token_log_probs(logits: torch.Tensor, target: torch.Tensor, top: int = 0) ->
     if not 0 <= top <= min(TOKEN_LOG_PROBS_MAX_TOP, V):
         raise KernelError(f"token_log_probs: top must be 0 to {TOKEN_LOG_PROBS_MAX_TOP} and at most the row's {V} tokens, got {top}")
     _same_device("token_log_probs", logits, target)
-    # one allocation: three numbers and two lists a row
-    both = torch.empty(R * (3 + 2 * top), dtype=torch.float32, device=logits.device)
-    ints = both.view(torch.int32)
-    got = TokenLogProbs(both[:R], both[R:2 * R], ints[2 * R:3 * R], ints[3 * R:(3 + top) * R].view(R, top), both[(3 + top) * R:].view(R, top))
+    got = TokenLogProbs(logits.new_empty(R), logits.new_empty(R), target.new_empty(R), target.new_empty((R, top)), logits.new_empty((R, top)))
     if R == 0:
         return got
     fn = _fn("token_probs", "bw_token_probs", _TOKEN_PROBS_ARGS)
-    at = both.data_ptr()
-    _check(fn(logits.data_ptr(), target.data_ptr(), at, at + 4 * R, at + 8 * R, at + 12 * R, at + 4 * (3 + top) * R, R, V, top,
-              logits.stride(0) if R > 1 else V, _stream()), "token_log_probs")
+    _check(fn(logits.data_ptr(), target.data_ptr(), got[0].data_ptr(), got[1].data_ptr(), got[2].data_ptr(), got[3].data_ptr(), got[4].data_ptr(),
+              R, V, top, logits.stride(0) if R > 1 else V, _stream()), "token_log_probs")
     return got
 
 
@@ -1457,19 +1453,36 @@ def check_quant_supported(head_dim: int, group: int = 1) -> None:
         raise KernelError(f"8-bit cache: {group} query heads per kv head exceed the attention kernels' limit of {MAX_GROUP_BF16}")
 
 
-def _quant_pages(pages: QuantPages, block_table: torch.Tensor, what: str):
-    if pages.k.dim() != 4 or pages.v.shape != pages.k.shape:
-        raise KernelError(f"{what}: keys and values must be [num_pages, nkv, page_size, head_dim]")
-    num_pages, nkv, page_size, hd = pages.k.shape
-    if pages.k_scale.shape != (num_pages, nkv, page_size) or pages.v_scale.shape != pages.k_scale.shape:
-        raise KernelError(f"{what}: scales must be [num_pages, nkv, page_size]")
-    _dev(pages.k, "k", torch.int8); _dev(pages.v, "v", torch.int8)
-    _dev(pages.k_scale, "k_scale", torch.float32); _dev(pages.v_scale, "v_scale", torch.float32)
-    _dev(block_table, "block_table", torch.int32)
-    if block_table.dim() != 2:
-        raise KernelError(f"{what}: the block table must be [requests, blocks]")
-    check_quant_supported(hd)
-    return num_pages, nkv, page_size, hd
+def _quant_pages(pages: QuantPages, block_table: torch.Tensor, here: int, what: str):
+    k, v, ks, vs = pages.k, pages.v, pages.k_scale, pages.v_scale
+    shape = k.shape
+    # (one expression while all is well: a decode step calls this for every layer)
+    if not (k.dtype == v.dtype == torch.int8 and ks.dtype == vs.dtype == torch.float32 and block_table.dtype == torch.int32
+            and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == here
+            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and block_table.is_contiguous()
+            and len(shape) == 4 and v.shape == shape and ks.shape == vs.shape == shape[:3] and block_table.dim() == 2
+            and shape[3] % 16 == 0 and 0 < shape[3] <= QUANT_MAX_HEAD_DIM):
+        for name, t, dtype in (("k", k, torch.int8), ("v", v, torch.int8), ("k_scale", ks, torch.float32), ("v_scale", vs, torch.float32),
+                               ("block_table", block_table, torch.int32)):
+            _dev(t, f"{what}: {name}", dtype)
+        if len(shape) != 4 or v.shape != shape:
+            raise KernelError(f"{what}: keys and values must be [num_pages, nkv, page_size, head_dim]")
+        if ks.shape != shape[:3] or vs.shape != shape[:3]:
+            raise KernelError(f"{what}: scales must be [num_pages, nkv, page_size]")
+        if block_table.dim() != 2:
+            raise KernelError(f"{what}: the block table must be [requests, blocks]")
+        check_quant_supported(shape[3])
+        _same_device(what, k, v, ks, vs, block_table)
+        raise KernelError(f"{what}: the pages cannot be used")
+    return shape
+
+
+def _quant_tokens(positions: torch.Tensor, req_of_token: torch.Tensor, n: int, here: int, what: str) -> None:
+    if not (positions.dtype == req_of_token.dtype == torch.int32 and positions.get_device() == req_of_token.get_device() == here
+            and positions.is_contiguous() and req_of_token.is_contiguous() and positions.numel() == req_of_token.numel() == n):
+        _dev(positions, f"{what}: positions", torch.int32); _dev(req_of_token, f"{what}: req_of_token", torch.int32)
+        _same_device(what, positions, req_of_token)
+        raise KernelError(f"{what}: one position and one request per token")
 
 
 _QUANT_APPEND_ARGS = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_int, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_void_p]
@@ -1491,21 +1504,21 @@ def quant_append(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch
             raise KernelError("quant_append: planes are float32 [S, T, width]")
         n_planes, plane_stride = qkv.shape[0], qkv.stride(0)
         qkv = qkv[0]
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_append")
-    _dev(qkv, "qkv"); _dev(positions, "positions", torch.int32); _dev(req_of_token, "req_of_token", torch.int32)
+    here = torch._C._cuda_getDevice()
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_append")
+    _dev(qkv, "qkv")
     if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
         raise KernelError(f"quant_append: qkv must be [T, (nh + 2 nkv) * head_dim = {(nh + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
     T = qkv.shape[0]
-    if positions.numel() != T or req_of_token.numel() != T:
-        raise KernelError("quant_append: one position and one request per token")
+    _quant_tokens(positions, req_of_token, T, here, "quant_append")
     rd = 0
     if table is not None:
         _dev(table, "table", torch.float32)
         if table.dim() != 2 or table.shape[0] != T or table.shape[1] % 2 or table.shape[1] > hd:
             raise KernelError("quant_append: the cos/sin table must be [T, rotary_dim], rotary_dim even and at most the head size")
         rd = table.shape[1]
-    _same_device("quant_append", qkv, positions, req_of_token, block_table, table, pages.k, pages.v, pages.k_scale, pages.v_scale)
-    q = torch.empty((T, nh * hd), dtype=torch.bfloat16, device=qkv.device)
+    _same_device("quant_append", qkv, table)
+    q = qkv.new_empty((T, nh * hd), dtype=torch.bfloat16)
     if T == 0:
         return q
     fn = _fn("quant_cache", "bw_quant_append", _QUANT_APPEND_ARGS)
@@ -1519,13 +1532,11 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
                out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values that an 8-bit cache holds, [n, nkv, head_dim] each in ``out_dtype`` (bfloat16 or float32): row i is position
     ``positions[i]`` of request ``req_of_token[i]`` (a row of the block table).  Zeros where no page is held."""
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_read")
-    _dev(positions, "positions", torch.int32); _dev(req_of_token, "req_of_token", torch.int32)
+    here = torch._C._cuda_getDevice()
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_read")
     n = positions.numel()
-    if req_of_token.numel() != n:
-        raise KernelError("quant_read: one request per position")
-    _same_device("quant_read", positions, req_of_token, block_table, pages.k, pages.v, pages.k_scale, pages.v_scale)
-    k = torch.empty((n, nkv, hd), dtype=out_dtype, device=pages.k.device)
+    _quant_tokens(positions, req_of_token, n, here, "quant_read")
+    k = pages.k_scale.new_empty((n, nkv, hd), dtype=out_dtype)
     v = torch.empty_like(k)
     code = _code(k, "out")
     if n == 0:
@@ -1536,8 +1547,8 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
     return k, v
 
 
-_ATTN_Q8_PLAN_ARGS = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]
-_ATTN_Q8_ARGS = [c_void_p] * 10 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]
+_ATTN_Q8_ARGS = ([c_void_p] * 10 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, ctypes.POINTER(c_ll), c_int,
+                                                                            c_void_p])
 _ATTN_Q8_TC_ARGS = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, c_void_p]
 QUANT_FEW_ROWS = 16     # up to so many stacked rows (tokens times heads of a group) a request is the key-slice kernel's
 
@@ -1547,25 +1558,32 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     """:func:`paged_attention` over an 8-bit cache (which already holds this step's keys and values): bfloat16 queries [T, nh * head_dim],
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
     held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator."""
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, "quant_attention")
+    here = torch._C._cuda_getDevice()
+    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_attention")
     _dev(q, "q", torch.bfloat16)
     if nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
         raise KernelError("quant_attention: q must be [T, nh * head_dim] with nh a multiple of the kv heads")
     G, R = nh // nkv, batch.R
-    check_quant_supported(hd, G)
+    if G > MAX_GROUP_BF16:
+        check_quant_supported(hd, G)
     _check_sink(sink, nh)
-    cu_q, q_start, kv_len = (_dev(t, n, torch.int32) for t, n in ((batch.cu_q, "cu_q"), (batch.q_start, "q_start"), (batch.kv_len, "kv_len")))
+    cu_q, q_start, kv_len, lens, starts = batch.cu_q, batch.q_start, batch.kv_len, batch.h_q_len, batch.h_q_start
+    for t, name in ((cu_q, "cu_q"), (q_start, "q_start"), (kv_len, "kv_len")):
+        _dev(t, name, torch.int32)
+    if len(lens) != R:
+        lens = lens[:R]
     if q.shape[0] != batch.T or block_table.shape[0] < R or cu_q.numel() < R + 1 or q_start.numel() < R or kv_len.numel() < R \
-            or len(batch.h_q_len) < R or len(batch.h_q_start) < R or sum(batch.h_q_len[:R]) != batch.T:
+            or len(lens) != R or len(starts) < R or sum(lens) != batch.T:
         raise KernelError("quant_attention: the batch's segments, the queries and the block table do not fit together")
-    _same_device("quant_attention", q, cu_q, q_start, kv_len, block_table, sink, pages.k, pages.v, pages.k_scale, pages.v_scale)
+    _same_device("quant_attention", q, cu_q, q_start, kv_len, sink)
     out = torch.empty_like(q)
     if batch.T == 0:
         return out
     window, chunk = int(window or 0), int(chunk or 0)
-    h_len, h_start = (c_int * R)(*batch.h_q_len[:R]), (c_int * R)(*batch.h_q_start[:R])
+    ints = c_int * R
+    h_len, h_start = ints(*lens), ints(*starts[:R])
     macros = attention_q8_macros(hd)
-    if hd % 64 == 0 and scale > 0 and max(batch.h_q_len[:R]) * G > QUANT_FEW_ROWS:
+    if hd % 64 == 0 and scale > 0 and max(lens) * G > QUANT_FEW_ROWS:
         # portions of prompts: the tcgen05 kernel, where it is built for the head size (else the mma.sync kernel below takes them)
         room_of = load_library("attention_q8_tc", macros).bw_attention_q8_tc_room
         if not room_of.argtypes:
@@ -1578,28 +1596,27 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
         _check(tc(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(kv_len), _ptr(block_table),
                   block_table.shape[1], h_len, h_start, R, QUANT_FEW_ROWS, nh, nkv, page_size, num_pages, window, chunk, float(scale), _ptr(sink),
                   _ptr(room), floats, _stream()), "quant_attention")
-        if min(n for n in batch.h_q_len[:R]) * G > QUANT_FEW_ROWS:
+        if min(lens) * G > QUANT_FEW_ROWS:
             return out
         few = 1
     else:
         few = 0
-    per = c_int(1)
-    slices = _fn("attention_q8", "bw_attention_q8_plan", _ATTN_Q8_PLAN_ARGS, macros=macros)(
-        h_len, h_start, R, G, nkv, window, chunk, int(batch.static_bound or 0), ctypes.byref(per))
-    if slices < 0:
-        _check(slices, "quant_attention")
-    part_o = part_ml = None
-    if slices > 1:
-        rows = R * nkv * slices * 16
-        part_o = torch.empty((rows, hd), dtype=torch.float32, device=q.device)
-        part_ml = torch.empty((rows, 2), dtype=torch.float32, device=q.device)
     fn = _fn("attention_q8", "bw_attention_q8", _ATTN_Q8_ARGS, macros=macros)
-    _check(fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start),
-              _ptr(kv_len), _ptr(block_table), block_table.shape[1], h_len, R, nh, nkv, page_size, num_pages, window, chunk, float(scale),
-              _ptr(sink), per.value, slices, _ptr(part_o), _ptr(part_ml), few, _stream()), "quant_attention")
+    need = c_ll(0)
+    room, floats = None, 0
+    while True:
+        code = fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start), _ptr(kv_len),
+                  _ptr(block_table), block_table.shape[1], h_len, h_start, R, nh, nkv, page_size, num_pages, window, chunk,
+                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need), few, _stream())
+        if code != _ERR_ROOM or room is not None:
+            break
+        floats = need.value             # many slices of few requests join through memory
+        room = torch.empty(floats, dtype=torch.float32, device=q.device)
+    _check(code, "quant_attention")
     return out
 
 
+_ERR_ROOM = -11
 _ATTN_Q8_MACROS = {}
 
 

@@ -226,9 +226,10 @@ def test_attention_more_portions_than_one_launch_takes(count):
     Case([(18 + i % 3, i, 18 + i % 3 + i) for i in range(count)], 1, 64, 16, seed=count).fill().check_attention(2)
 
 
-def test_attention_slices_are_joined_in_order():
-    """One request, long: many slices; the same inputs give the same bits, also beside other requests of the same plan."""
-    c = Case([(1, 5000, 5001)], 1, 128, 16, seed=9).fill()
+@pytest.mark.parametrize("keys", [700, 5001, 30001])
+def test_attention_slices_are_joined_in_order(keys):
+    """One request, long: many slices, joined in a cluster or through memory; the same inputs give the same bits."""
+    c = Case([(1, keys - 1, keys)], 1, 128, 16, seed=keys).fill()
     b, pages = c.batch(), c.pages()
     q = torch.randn(1, 4 * 128, generator=c.gen).to(torch.bfloat16).cuda()
     outs = [ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.088) for _ in range(5)]
