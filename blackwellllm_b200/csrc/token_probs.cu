@@ -95,17 +95,19 @@ __device__ __forceinline__ u64 merge32(u64 a, u64 b) {
     }
     return k;
 }
-// the 32 best of the block's lists (one a warp), in warp 0
-__device__ __forceinline__ u64 merge_warps(u64 k, u64 (*lists)[32]) {
+// the 32 best of the first n warps' lists, in warp 0 (all threads of the block call it)
+__device__ __forceinline__ u64 merge_warps(u64 k, u64 (*lists)[32], int n) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    lists[warp][lane] = k;
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) {
+    int o = 1;
+    while (o < n) o <<= 1;
+    if (warp < n) lists[warp][lane] = k;
+    for (o >>= 1; o > 0; o >>= 1) {
         __syncthreads();
-        if (warp < o) {
+        if (warp < o && warp + o < n) {
             k = merge32(k, lists[warp + o][lane]);
             lists[warp][lane] = k;
         }
+        n = min(n, o);
     }
     return k;
 }
@@ -119,155 +121,204 @@ __device__ __forceinline__ float4 load4(const float* row, int c, int V) {
     return v;
 }
 
+__device__ __forceinline__ bw::f32x2 add2(bw::f32x2 a, bw::f32x2 b) {
+    bw::f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// What a block found in its share of a row.
+struct Found { Part part; int count, bad; };
+constexpr int MOST_BLOCKS = 8;
 struct Shared {
-    Part parts[WARPS];
-    int counts[WARPS];
-    int bad;
+    Found warps[WARPS];
     u64 lists[WARPS][32];
-    // the block's result, read by the cluster's first block
-    Part part; int count; u64 best[32];
+    u64 loose[WARPS][128];       // a warp's candidates before they are sorted
+    u64 best[32];                // the block's best thread keys
+    Found found[MOST_BLOCKS];    // in the cluster's first block: of every block
+    u64 found_best[MOST_BLOCKS][32];
 };
+template <typename T> __device__ __forceinline__ T* in_first_block(T* at) { return cg::this_cluster().map_shared_rank(at, 0); }
+
+// A thread's elements so far.  The best stays out of the sums: of four elements and the best before them, seven minima and maxima leave the best
+// and four others (min and max of a pair at a time), and those are added.  The sums' exponents stand against `ref`, a best of earlier, until the
+// best is more than SLACK above it: moving a reference with every new best is done by some lane of a warp nearly every time, and cost three
+// quarters of the instructions.
+constexpr float SLACK = 16.f;
+struct Running {
+    float best = -INFINITY, ref = -INFINITY;
+    int four, count = 0;                     // the four where the best first stood; elements that stand before the target
+    bw::f32x2 z = 0ull, w = 0ull;            // sums of e^(x - ref) and of (x - ref) e^(x - ref)
+};
+__device__ __forceinline__ void take4(Running& s, float4 x, int f, float xt, int target) {
+    // (the maxima keep what is no number, and the best with them: it is looked at in the end)
+    const float h0 = max_or_nan(x.x, x.y), l0 = fminf(x.x, x.y), h1 = max_or_nan(x.z, x.w), l1 = fminf(x.z, x.w);
+    const float most = max_or_nan(h0, h1), l2 = fminf(h0, h1), l3 = fminf(most, s.best);
+    if (!(most < xt)) {
+        const int c = 4 * f;
+        if (c > target) s.count += (x.x > xt) + (x.y > xt) + (x.z > xt) + (x.w > xt);
+        else if (c + 3 < target) s.count += (x.x >= xt) + (x.y >= xt) + (x.z >= xt) + (x.w >= xt);
+        else s.count += (x.x > xt || (x.x == xt && c < target)) + (x.y > xt || (x.y == xt && c + 1 < target)) +
+                        (x.z > xt || (x.z == xt && c + 2 < target)) + (x.w > xt || (x.w == xt && c + 3 < target));
+    }
+    if (most > s.best) s.four = f;
+    s.best = max_or_nan(s.best, most);
+    if (s.best > s.ref + SLACK) {
+        const float d = fmaxf(s.ref - s.best, LEAST), e = ex2(d * LOG2E);
+        const bw::f32x2 e2 = bw::pack2(e, e);
+        s.w = bw::mul2(e2, bw::fma2(bw::pack2(d, d), s.z, s.w));
+        s.z = bw::mul2(e2, s.z);
+        s.ref = s.best;
+    }
+    // (-infinity, here or as the reference so far, comes out as a term of 0)
+    const bw::f32x2 less = bw::pack2(-s.ref, -s.ref), l2e = bw::pack2(LOG2E, LOG2E);
+    auto add = [&](float u, float v) {
+        float d0, d1, a0, a1;
+        bw::unpack2(add2(bw::pack2(u, v), less), d0, d1);
+        const bw::f32x2 d = bw::pack2(fmaxf(d0, LEAST), fmaxf(d1, LEAST));
+        bw::unpack2(bw::mul2(d, l2e), a0, a1);
+        const bw::f32x2 t = bw::pack2(ex2(a0), ex2(a1));
+        s.z = add2(s.z, t);
+        s.w = bw::fma2(t, d, s.w);
+    };
+    add(l0, l1);
+    add(l2, l3);
+}
+// the same against the best
+__device__ __forceinline__ Part part_of(const Running& s) {
+    if (s.ref == -INFINITY) return {s.best, 0.f, 0.f};
+    const float d = fmaxf(s.ref - s.best, LEAST), e = ex2(d * LOG2E), z = bw::sum2(s.z);
+    return {s.best, e * z, e * fmaf(d, z, bw::sum2(s.w))};
+}
+
+__device__ __forceinline__ Found shuffled(const Found& a, int o) {
+    return {{__shfl_xor_sync(0xffffffffu, a.part.m, o), __shfl_xor_sync(0xffffffffu, a.part.z, o), __shfl_xor_sync(0xffffffffu, a.part.w, o)},
+            __shfl_xor_sync(0xffffffffu, a.count, o), __shfl_xor_sync(0xffffffffu, a.bad, o)};
+}
+// joined over groups of n neighbouring lanes (a power of two), both lanes of a pair in the same order
+__device__ __forceinline__ Found join_lanes(Found a, int n) {
+    for (int o = n >> 1; o > 0; o >>= 1) {
+        const Found b = shuffled(a, o);
+        a.part = (threadIdx.x & o) ? join(b.part, a.part) : join(a.part, b.part);
+        a.count += b.count;
+        a.bad |= b.bad;
+    }
+    return a;
+}
 
 // grid: rows * blocks; a row's `blocks` blocks are one cluster.
 template <bool VEC>
 __global__ void __launch_bounds__(THREADS, 2)
 token_probs_kernel(Args p, int blocks) {
     BW_PDL_TRIGGER();
-    BW_PDL_WAIT();
     __shared__ Shared sh;
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // (the cluster's blocks have begun: waited for below)
     const int r = blockIdx.x / blocks, part = blockIdx.x - r * blocks;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* row = p.logits + (size_t)r * p.ld;
-    const int target = p.target[r];
-    const bool given = target >= 0 && target < p.V;
-    const float xt = given ? row[target] : INFINITY;
     // the block's share: whole fours
     const int fours = (p.V + 3) / 4, each = (fours + blocks - 1) / blocks;
     const int f0 = min(fours, part * each), f1 = min(fours, f0 + each);
-    if (threadIdx.x == 0) sh.bad = 0;
-
-    Part me{-INFINITY, 0.f, 0.f};
-    int id = 4 * (f0 + (int)threadIdx.x), count = 0;
-    const bool any = f0 + (int)threadIdx.x < f1;
-    bool bad = false;
-    for (int f = f0 + threadIdx.x; f < f1; f += UNROLL * THREADS) {
-        float x[UNROLL][4];
+    BW_PDL_WAIT();
+    // four fours of a thread are on their way while it works on the four before
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float4 x[UNROLL];
+    const int own = f0 + (int)threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) x[u] = own + u * THREADS < f1 ? load4<VEC>(row, 4 * (own + u * THREADS), p.V) : none;
+    const int target = p.target[r];
+    const bool given = target >= 0 && target < p.V;
+    const float xt = given ? row[target] : INFINITY;
+    Running s;
+    s.four = own;
+    for (int f = own; f < f1; f += UNROLL * THREADS) {
+        float4 next[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int c = 4 * (f + u * THREADS);
-            const float4 v = f + u * THREADS < f1 ? load4<VEC>(row, c, p.V) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+            const int g = f + (UNROLL + u) * THREADS;
+            next[u] = g < f1 ? load4<VEC>(row, 4 * g, p.V) : none;
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int c = 4 * (f + u * THREADS);
-            if (c >= 4 * f1) continue;
-            const float cm = max_or_nan(max_or_nan(x[u][0], x[u][1]), max_or_nan(x[u][2], x[u][3]));
-            int skip = -1;
-            if (!(cm <= me.m)) {
-                bad |= !(cm < INFINITY);
-                skip = x[u][0] == cm ? 0 : x[u][1] == cm ? 1 : x[u][2] == cm ? 2 : 3;
-                const float d = fmaxf(me.m - cm, LEAST), f2 = ex2(d * LOG2E);
-                if (me.m == -INFINITY) me.z = me.w = 0.f;
-                else { me.w = f2 * (me.w + d * (1.f + me.z)); me.z = f2 * (1.f + me.z); }
-                me.m = cm; id = c + skip;
-            }
-            float z = 0.f;
+        for (int u = 0; u < UNROLL; ++u)
+            if (f + u * THREADS < f1) take4(s, x[u], f + u * THREADS, xt, target);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // (-infinity, here or as the maximum so far, comes out as a term of 0)
-                const float d = fmaxf(x[u][e] - me.m, LEAST);
-                const float t = e == skip ? 0.f : ex2(d * LOG2E);
-                z += t;
-                me.w = fmaf(t, d, me.w);
-            }
-            me.z += z;
-            if (c > target) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) count += x[u][e] > xt;
-            } else if (c + 3 < target) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) count += x[u][e] >= xt;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) count += x[u][e] > xt || (x[u][e] == xt && c + e < target);
-            }
-        }
+        for (int u = 0; u < UNROLL; ++u) x[u] = next[u];
     }
-    const u64 mine = any ? key_of(me.m, id) : 0;
-    __syncthreads();
-    if (bad) sh.bad = 1;
-    // the block's triple and count
-    Part all = me;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Part other{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.z, o), __shfl_xor_sync(0xffffffffu, all.w, o)};
-        // (both lanes of a pair join the same two in the same order)
-        all = (lane & o) ? join(other, all) : join(all, other);
-        count += __shfl_xor_sync(0xffffffffu, count, o);
-    }
-    if (lane == 0) { sh.parts[warp] = all; sh.counts[warp] = count; }
+    Found all{part_of(s), s.count, !(s.best < INFINITY)};
+    all = join_lanes(all, 32);
+    if (lane == 0) sh.warps[warp] = all;
     u64 list = 0;
     if (p.top > 0) {
-        list = merge_warps(sort32(mine), sh.lists);        // (its first barrier also stands before the reads below)
+        u64 mine = 0;
+        if (own < f1) {
+            const float4 v = load4<VEC>(row, 4 * s.four, p.V);          // again, for which of the four it was
+            mine = key_of(s.best, 4 * s.four + (v.x == s.best ? 0 : v.y == s.best ? 1 : v.z == s.best ? 2 : 3));
+        }
+        list = merge_warps(sort32(mine), sh.lists, WARPS);
         if (p.top > 1) {
             // warp 0 has the best thread keys; the owners of the first `top` read their elements again
             if (warp == 0) sh.best[lane] = lane < p.top ? list : 0;
             __syncthreads();
             const u64 bound = sh.best[p.top - 1];
-            const int rounds = (f1 - f0 + THREADS - 1) / THREADS;
+            const int rounds = (f1 - f0 + THREADS - 1) / THREADS, items = p.top * rounds;
             list = 0;
-            for (int i0 = 0; i0 < p.top * rounds; i0 += THREADS) {       // (uniform)
+            for (int i0 = 0; i0 < items; i0 += THREADS) {                // (uniform)
+                if (i0 + 32 * warp >= items) continue;
                 const int i = i0 + (int)threadIdx.x, who = i / rounds, it = i - who * rounds;
-                const u64 owner = who < p.top ? sh.best[who] : 0;
+                const u64 owner = i < items ? sh.best[who] : 0;
                 const int f = owner ? f0 + it * THREADS + (id_of(owner) / 4 - f0) % THREADS : f1;
-                const float4 v = f < f1 ? load4<VEC>(row, 4 * f, p.V) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float x[4] = {v.x, v.y, v.z, v.w};
+                const float4 v = f < f1 ? load4<VEC>(row, 4 * f, p.V) : none;
+                const float y[4] = {v.x, v.y, v.z, v.w};
+                // the warp's candidates side by side, then 32 of them at a time: mostly a few in all
+                int n = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    u64 k = f < f1 && 4 * f + e < p.V ? key_of(x[e], 4 * f + e) : 0;
-                    if (k < bound) k = 0;
-                    if (__any_sync(0xffffffffu, k != 0)) list = merge32(list, sort32(k));
+                    const u64 k = f < f1 && 4 * f + e < p.V ? key_of(y[e], 4 * f + e) : 0;
+                    const bool is = k != 0 && k >= bound;
+                    const unsigned b = __ballot_sync(0xffffffffu, is);
+                    if (is) sh.loose[warp][n + __popc(b & ((1u << lane) - 1))] = k;
+                    n += __popc(b);
                 }
+                __syncwarp();
+                for (int j = 0; j < n; j += 32) list = merge32(list, sort32(j + lane < n ? sh.loose[warp][j + lane] : 0));
+                __syncwarp();
             }
             __syncthreads();
-            list = merge_warps(list, sh.lists);
+            list = merge_warps(list, sh.lists, min(WARPS, (items + 31) / 32));
         }
-        if (warp == 0) sh.best[lane] = list;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Part s = sh.parts[0];
-        int n = sh.counts[0];
-        for (int w = 1; w < WARPS; ++w) { s = join(s, sh.parts[w]); n += sh.counts[w]; }
-        sh.part = s; sh.count = n;
+    if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (warp == 0) {
+        all = join_lanes(lane < WARPS ? sh.warps[lane] : Found{{-INFINITY, 0.f, 0.f}, 0, 0}, WARPS);
+        // into the cluster's first block
+        if (lane == 0) *(blocks > 1 ? in_first_block(&sh.found[part]) : &sh.found[0]) = all;
+        if (p.top > 0) *(blocks > 1 ? in_first_block(&sh.found_best[part][lane]) : &sh.found_best[0][lane]) = list;
     }
-    if (blocks > 1) cg::this_cluster().sync();
-    else __syncthreads();
-    if (part == 0 && warp == 0) {
-        Part s = sh.part;
-        int n = sh.count, wrong = sh.bad;
-        u64 best = p.top > 0 ? sh.best[lane] : 0;
-        for (int b = 1; b < blocks; ++b) {
-            const Shared* other = cg::this_cluster().map_shared_rank(&sh, b);
-            s = join(s, other->part);
-            n += other->count;
-            wrong |= other->bad;
-            if (p.top > 0) best = merge32(best, other->best[lane]);
-        }
-        const bool none = wrong || !(s.m > -INFINITY);       // no distribution: NaN, an infinite logit, or nothing but -infinity
-        const float log_z = log1pf(s.z), nan = __uint_as_float(0x7fffffffu);
-        if (lane == 0) {
-            p.log_prob[r] = none || !given ? nan : (xt - s.m) - log_z;
-            p.entropy[r] = none ? nan : log_z - s.w / (1.f + s.z);
-            p.rank[r] = none || !given ? -1 : n;
-        }
-        if (lane < p.top) {
-            p.top_ids[(size_t)r * p.top + lane] = none ? -1 : id_of(best);
-            p.top_log_probs[(size_t)r * p.top + lane] = none ? nan : (value_of(best) - s.m) - log_z;
-        }
+    if (blocks > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (part != 0) return;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncwarp();
     }
-    if (blocks > 1) cg::this_cluster().sync();      // a block's shared memory stays until it has been read
+    if (p.top > 0) list = blocks > 1 ? merge_warps(warp < blocks ? sh.found_best[warp][lane] : 0, sh.lists, blocks) : list;
+    if (warp != 0) return;
+    all = join_lanes(lane < blocks ? sh.found[lane] : Found{{-INFINITY, 0.f, 0.f}, 0, 0}, MOST_BLOCKS);
+    all = Found{{__shfl_sync(0xffffffffu, all.part.m, 0), __shfl_sync(0xffffffffu, all.part.z, 0), __shfl_sync(0xffffffffu, all.part.w, 0)},
+                __shfl_sync(0xffffffffu, all.count, 0), __shfl_sync(0xffffffffu, all.bad, 0)};
+    const Part& q = all.part;
+    const bool nothing = all.bad || !(q.m > -INFINITY);       // no distribution: NaN, an infinite logit, or nothing but -infinity
+    const float log_z = log1pf(q.z), nan = __uint_as_float(0x7fffffffu);
+    if (lane == 0) {
+        p.log_prob[r] = nothing || !given ? nan : (xt - q.m) - log_z;
+        p.entropy[r] = nothing ? nan : log_z - q.w / (1.f + q.z);
+        p.rank[r] = nothing || !given ? -1 : all.count;
+    }
+    if (lane < p.top) {
+        p.top_ids[(size_t)r * p.top + lane] = nothing ? -1 : id_of(list);
+        p.top_log_probs[(size_t)r * p.top + lane] = nothing ? nan : (value_of(list) - q.m) - log_z;
+    }
 }
 
 }  // namespace
