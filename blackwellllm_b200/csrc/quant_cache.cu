@@ -24,17 +24,25 @@ struct Rows {
     int8_t* k; int8_t* v; float* k_scale; float* v_scale;
     const int* positions; const int* req; const int* table;
     int tokens, requests, max_blocks, page_size, num_pages, nkv, hd;
+    unsigned per_page;           // the page size's reciprocal (divide)
 };
 
-// Where the row of (token t, kv head g) lies, in rows; -1: the table names no page for its position.
-__device__ __forceinline__ long long row_of(const Rows& p, int t, int g) {
+// n / d for d whose reciprocal `inv` is 2^32 / d rounded down (2^32 - 1 for 1): that is at most one too low.
+__device__ __forceinline__ unsigned divide(unsigned n, unsigned d, unsigned inv) {
+    const unsigned q = __umulhi(n, inv);
+    return q + (n - q * d >= d ? 1u : 0u);
+}
+inline unsigned reciprocal_of(unsigned d) { return d == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / d); }
+
+// Where the row of (token t, kv head 0) lies, in rows (head g's: g pages' length behind); -1: the table names no page for its position.
+__device__ __forceinline__ long long row_of(const Rows& p, int t) {
     const int pos = p.positions[t], r = p.req[t];
     if (pos < 0 || r < 0 || r >= p.requests) return -1;
-    const int blk = pos / p.page_size;
+    const int blk = (int)divide((unsigned)pos, (unsigned)p.page_size, p.per_page);
     if (blk >= p.max_blocks) return -1;
     const int page = p.table[(size_t)r * p.max_blocks + blk];
     if (page < 0 || page >= p.num_pages) return -1;
-    return ((long long)page * p.nkv + g) * p.page_size + (pos - blk * p.page_size);
+    return (long long)page * p.nkv * p.page_size + (pos - blk * p.page_size);
 }
 
 template <typename T> __device__ __forceinline__ void load4(const T* src, float (&v)[4]);
@@ -57,18 +65,20 @@ __device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
 // that turn together, (u, u + rd / 2) for u < rd / 2, or the two channels 2 u, 2 u + 1 that do not turn.  `paired`: the two of a rotated
 // pair stand side by side in the source.  VEC: rd is a multiple of 8 and the rows are aligned, so a lane's units are of one kind and their
 // channels come as two vectors.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int LANES>
 __global__ void __launch_bounds__(THREADS)
 append_kernel(const T* qkv, int planes, long long plane_stride, const float* turns, int rd, int paired,
-              bf16* q_out, int nh, Rows p, int lanes, int append) {
+              bf16* q_out, int nh, Rows p, unsigned per_heads, int append) {
     BW_PDL_TRIGGER();
     BW_PDL_WAIT();
     const int heads = nh + 2 * p.nkv, half = rd >> 1;
-    const unsigned group = (blockIdx.x * (unsigned)THREADS + threadIdx.x) / (unsigned)lanes;
-    const int l = threadIdx.x & (lanes - 1);
-    const int t = (int)(group / (unsigned)heads), head = (int)(group - (unsigned)t * heads);
+    const unsigned group = (blockIdx.x * (unsigned)THREADS + threadIdx.x) / LANES;
+    const int l = threadIdx.x & (LANES - 1);
+    const int t = (int)divide(group, (unsigned)heads, per_heads), head = (int)(group - (unsigned)t * heads);
     const bool live = t < p.tokens && 8 * l < p.hd;
     const bool is_q = head < nh, is_v = head >= nh + p.nkv;
+    // (where the row goes is looked up while the row itself is on its way)
+    long long row = append && live && !is_q ? row_of(p, t) : -1;
     float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
     bool turned[4];
 #pragma unroll
@@ -98,13 +108,21 @@ append_kernel(const T* qkv, int planes, long long plane_stride, const float* tur
 #pragma unroll
             for (int i = 0; i < 4; ++i) { a[i] += u[i]; b[i] += w[i]; }
         }
+        float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (VEC && turned[0]) {
+            load4(turns + (size_t)t * rd + 4 * l, c);
+            load4(turns + (size_t)t * rd + half + 4 * l, s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (turned[i]) { c[i] = turns[(size_t)t * rd + 4 * l + i]; s[i] = turns[(size_t)t * rd + half + 4 * l + i]; }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!turned[i]) continue;
-            const float c = turns[(size_t)t * rd + 4 * l + i], s = turns[(size_t)t * rd + half + 4 * l + i];
             const float x = a[i], y = b[i];
-            a[i] = x * c - y * s;
-            b[i] = y * c + x * s;
+            a[i] = x * c[i] - y * s[i];
+            b[i] = y * c[i] + x * s[i];
         }
     }
     // a lane's channels: 4 l + i and 4 l + i + rd / 2 where they turn, else 8 l + 2 i and the next
@@ -130,11 +148,10 @@ append_kernel(const T* qkv, int planes, long long plane_stride, const float* tur
     unsigned most = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) most = max(most, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
-    for (int o = lanes >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (!live || is_q) return;
-    const int g = is_v ? head - nh - p.nkv : head - nh;
-    const long long row = row_of(p, t, g);
+#pragma unroll
+    for (int o = LANES >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (row < 0) return;
+    row += (long long)(is_v ? head - nh - p.nkv : head - nh) * p.page_size;
     const float big = __uint_as_float(most);
     const bool fine = most < 0x7f800000u, some = big >= LEAST;
     const float inv = fine && some ? 127.f / big : 0.f;
@@ -163,9 +180,14 @@ append_kernel(const T* qkv, int planes, long long plane_stride, const float* tur
     if (l == 0) (is_v ? p.v_scale : p.k_scale)[row] = !fine ? __uint_as_float(0x7fffffffu) : (some ? big / 127.f : 0.f);
 }
 
+// Four whole numbers times s.  A byte with its top bit turned over, in the lowest place of 2^23, is 2^23 + 128 more than the number (the
+// converting instruction runs at an eighth of this).
 __device__ __forceinline__ void widen(uint32_t c, float s, float (&v)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(c >> (8 * i)) * s;
+    c ^= 0x80808080u;
+    v[0] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7650)) - 8388736.f) * s;
+    v[1] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7651)) - 8388736.f) * s;
+    v[2] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7652)) - 8388736.f) * s;
+    v[3] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7653)) - 8388736.f) * s;
 }
 __device__ __forceinline__ void store8(bf16* dst, const float (&u)[4], const float (&w)[4]) {
     *reinterpret_cast<uint4*>(dst) = make_uint4(bw::pack_bf16x2(u[0], u[1]), bw::pack_bf16x2(u[2], u[3]),
@@ -176,32 +198,38 @@ __device__ __forceinline__ void store8(float* dst, const float (&u)[4], const fl
     reinterpret_cast<float4*>(dst)[1] = make_float4(w[0], w[1], w[2], w[3]);
 }
 
-// Keys and values of the listed tokens, [tokens, kv heads, head size] each; zeros where the table names no page.
+// Keys and values of the listed tokens, [tokens, kv heads, head size] each; zeros where the table names no page.  A block takes `each` tokens:
+// their places are looked up once, by a thread a token, and then eight channels a thread are read and written (with a look-up and three
+// divisions of its own for every thread, arithmetic was what the kernel took its time for).
+constexpr int MOST_EACH = 32;
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-read_kernel(Rows p, T* k_out, T* v_out) {
+read_kernel(Rows p, T* k_out, T* v_out, int each, unsigned per_token, unsigned per_units) {
     BW_PDL_TRIGGER();
     BW_PDL_WAIT();
-    const unsigned per = (unsigned)p.hd >> 3;
-    const unsigned idx = blockIdx.x * (unsigned)THREADS + threadIdx.x;
-    const unsigned tg = idx / per, l = idx - tg * per;
-    const int t = (int)(tg / (unsigned)p.nkv), g = (int)(tg - (unsigned)t * p.nkv);
-    if (t >= p.tokens) return;
-    const long long row = row_of(p, t, g);
-    uint2 kc = make_uint2(0, 0), vc = make_uint2(0, 0);
-    float ks = 0.f, vs = 0.f;
-    if (row >= 0) {
-        const size_t at = (size_t)row * p.hd + 8 * l;
-        kc = *reinterpret_cast<const uint2*>(p.k + at);
-        vc = *reinterpret_cast<const uint2*>(p.v + at);
-        ks = p.k_scale[row]; vs = p.v_scale[row];
+    __shared__ long long place[MOST_EACH];
+    const int t0 = blockIdx.x * each, n = min(each, p.tokens - t0);
+    if ((int)threadIdx.x < n) place[threadIdx.x] = row_of(p, t0 + threadIdx.x);
+    __syncthreads();
+    const unsigned units = (unsigned)p.hd >> 3, items = units * p.nkv;
+    for (unsigned i = threadIdx.x; i < items * n; i += THREADS) {
+        const unsigned j = divide(i, items, per_token), rest = i - j * items, g = divide(rest, units, per_units), l = rest - g * units;
+        const long long at = place[j];
+        uint2 kc = make_uint2(0, 0), vc = make_uint2(0, 0);
+        float ks = 0.f, vs = 0.f;
+        if (at >= 0) {
+            const size_t row = (size_t)at + (size_t)g * p.page_size, from = row * p.hd + 8 * l;
+            kc = *reinterpret_cast<const uint2*>(p.k + from);
+            vc = *reinterpret_cast<const uint2*>(p.v + from);
+            ks = p.k_scale[row]; vs = p.v_scale[row];
+        }
+        float u[4], w[4];
+        const size_t to = (size_t)t0 * items * 8 + (size_t)i * 8;
+        widen(kc.x, ks, u); widen(kc.y, ks, w);
+        store8(k_out + to, u, w);
+        widen(vc.x, vs, u); widen(vc.y, vs, w);
+        store8(v_out + to, u, w);
     }
-    float u[4], w[4];
-    const size_t to = (size_t)tg * p.hd + 8 * l;
-    widen(kc.x, ks, u); widen(kc.y, ks, w);
-    store8(k_out + to, u, w);
-    widen(vc.x, vs, u); widen(vc.y, vs, w);
-    store8(v_out + to, u, w);
 }
 
 bool sizes_ok(const Rows& p) {
@@ -217,23 +245,28 @@ BW_EXPORT int bw_quant_append(const void* qkv, int type, int planes, long long p
                               void* q_out, int nh, void* k, void* v, float* k_scale, float* v_scale, const int* positions,
                               const int* req, const int* table, int tokens, int requests, int max_blocks, int page_size, int num_pages,
                               int nkv, int hd, int append, void* stream) {
-    Rows p{(int8_t*)k, (int8_t*)v, k_scale, v_scale, positions, req, table, tokens, requests, max_blocks, page_size, num_pages, nkv, hd};
+    Rows p{(int8_t*)k, (int8_t*)v, k_scale, v_scale, positions, req, table, tokens, requests, max_blocks, page_size, num_pages, nkv, hd, 0};
     if (!sizes_ok(p) || nh < 0 || planes < 1 || rd < 0 || rd > hd || (rd & 1) || (rd && !turns)) return BW_ERR_BAD_ARG;
     if (tokens == 0) return 0;
     int lanes = 2;
     while (8 * lanes < hd) lanes *= 2;
-    const long long threads = (long long)tokens * (nh + 2 * nkv) * lanes;
+    const int heads = nh + 2 * nkv;
+    const long long threads = (long long)tokens * heads * lanes;
     if (threads + THREADS > 0xffffffffll) return BW_ERR_UNSUPPORTED;
+    p.per_page = reciprocal_of((unsigned)page_size);
     const int es = type == BW_F32 ? 4 : 2;
-    const bool vec = rd % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)(plane_stride * es)) & (4 * es - 1)) == 0 &&
+    const bool vec = rd % 8 == 0 && ((uintptr_t)turns & 15) == 0 && (((uintptr_t)qkv | (uintptr_t)(plane_stride * es)) & (4 * es - 1)) == 0 &&
                      (((uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
     const dim3 grid((unsigned)((threads + THREADS - 1) / THREADS)), block(THREADS);
     cudaStream_t s = (cudaStream_t)stream;
-#define BW_APPEND(T, VEC) bw::launch(append_kernel<T, VEC>, grid, block, 0, s, (const T*)qkv, planes, plane_stride, turns, rd, paired, \
-                                     (bf16*)q_out, nh, p, lanes, append)
-    if (type == BW_F32) { if (vec) BW_APPEND(float, true); else BW_APPEND(float, false); }
-    else if (type == BW_BF16) { if (vec) BW_APPEND(bf16, true); else BW_APPEND(bf16, false); }
+#define BW_APPEND(T, VEC, LANES) bw::launch(append_kernel<T, VEC, LANES>, grid, block, 0, s, (const T*)qkv, planes, plane_stride, turns, rd, paired, \
+                                            (bf16*)q_out, nh, p, reciprocal_of((unsigned)heads), append)
+#define BW_APPEND_LANES(T, VEC) switch (lanes) { case 2: BW_APPEND(T, VEC, 2); break; case 4: BW_APPEND(T, VEC, 4); break; case 8: BW_APPEND(T, VEC, 8); break; \
+                                                 case 16: BW_APPEND(T, VEC, 16); break; default: BW_APPEND(T, VEC, 32); }
+    if (type == BW_F32) { if (vec) BW_APPEND_LANES(float, true) else BW_APPEND_LANES(float, false) }
+    else if (type == BW_BF16) { if (vec) BW_APPEND_LANES(bf16, true) else BW_APPEND_LANES(bf16, false) }
     else return BW_ERR_UNSUPPORTED;
+#undef BW_APPEND_LANES
 #undef BW_APPEND
     BW_LAUNCH_CHECK();
     return 0;
@@ -243,15 +276,21 @@ BW_EXPORT int bw_quant_read(const void* k, const void* v, const float* k_scale, 
                             const int* table, void* k_out, void* v_out, int type, int tokens, int requests, int max_blocks,
                             int page_size, int num_pages, int nkv, int hd, void* stream) {
     Rows p{(int8_t*)k, (int8_t*)v, (float*)k_scale, (float*)v_scale, positions, req, table, tokens, requests, max_blocks, page_size,
-           num_pages, nkv, hd};
+           num_pages, nkv, hd, 0};
     if (!sizes_ok(p) || (((uintptr_t)k | (uintptr_t)v) & 7) || (((uintptr_t)k_out | (uintptr_t)v_out) & 15)) return BW_ERR_BAD_ARG;
     if (tokens == 0) return 0;
-    const long long threads = (long long)tokens * nkv * (hd / 8);
-    if (threads + THREADS > 0xffffffffll) return BW_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((threads + THREADS - 1) / THREADS)), block(THREADS);
+    p.per_page = reciprocal_of((unsigned)page_size);
+    // a block's tokens: about four rounds of its threads (65,536 tokens of 8 kv heads of 128: one round 88 us, two 76, four and eight 72), fewer where the blocks would not fill the GPU
+    const int items = nkv * (hd / 8);
+    if ((long long)items * MOST_EACH > 0x7fffffffll) return BW_ERR_UNSUPPORTED;
+    int each = (4 * THREADS + items - 1) / items;
+    if (each > MOST_EACH) each = MOST_EACH;
+    while (each > 1 && tokens < (long long)each * 4 * bw::num_sms()) each = (each + 1) / 2;
+    const dim3 grid((unsigned)((tokens + each - 1) / each)), block(THREADS);
+    const unsigned per_token = reciprocal_of((unsigned)items), per_units = reciprocal_of((unsigned)hd / 8);
     cudaStream_t s = (cudaStream_t)stream;
-    if (type == BW_F32) bw::launch(read_kernel<float>, grid, block, 0, s, p, (float*)k_out, (float*)v_out);
-    else if (type == BW_BF16) bw::launch(read_kernel<bf16>, grid, block, 0, s, p, (bf16*)k_out, (bf16*)v_out);
+    if (type == BW_F32) bw::launch(read_kernel<float>, grid, block, 0, s, p, (float*)k_out, (float*)v_out, each, per_token, per_units);
+    else if (type == BW_BF16) bw::launch(read_kernel<bf16>, grid, block, 0, s, p, (bf16*)k_out, (bf16*)v_out, each, per_token, per_units);
     else return BW_ERR_UNSUPPORTED;
     BW_LAUNCH_CHECK();
     return 0;

@@ -121,12 +121,6 @@ __device__ __forceinline__ float4 load4(const float* row, int c, int V) {
     return v;
 }
 
-__device__ __forceinline__ bw::f32x2 add2(bw::f32x2 a, bw::f32x2 b) {
-    bw::f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // What a block found in its share of a row.
 struct Found { Part part; int count, bad; };
 constexpr int MOST_BLOCKS = 8;
@@ -148,7 +142,7 @@ constexpr float SLACK = 16.f;
 struct Running {
     float best = -INFINITY, ref = -INFINITY;
     int four, count = 0;                     // the four where the best first stood; elements that stand before the target
-    bw::f32x2 z = 0ull, w = 0ull;            // sums of e^(x - ref) and of (x - ref) e^(x - ref)
+    float z[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};      // sums of e^(x - ref) and of (x - ref) e^(x - ref), of every other element
 };
 __device__ __forceinline__ void take4(Running& s, float4 x, int f, float xt, int target) {
     // (the maxima keep what is no number, and the best with them: it is looked at in the end)
@@ -165,30 +159,27 @@ __device__ __forceinline__ void take4(Running& s, float4 x, int f, float xt, int
     s.best = max_or_nan(s.best, most);
     if (s.best > s.ref + SLACK) {
         const float d = fmaxf(s.ref - s.best, LEAST), e = ex2(d * LOG2E);
-        const bw::f32x2 e2 = bw::pack2(e, e);
-        s.w = bw::mul2(e2, bw::fma2(bw::pack2(d, d), s.z, s.w));
-        s.z = bw::mul2(e2, s.z);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { s.w[i] = e * fmaf(d, s.z[i], s.w[i]); s.z[i] *= e; }
         s.ref = s.best;
     }
-    // (-infinity, here or as the reference so far, comes out as a term of 0)
-    const bw::f32x2 less = bw::pack2(-s.ref, -s.ref), l2e = bw::pack2(LOG2E, LOG2E);
-    auto add = [&](float u, float v) {
-        float d0, d1, a0, a1;
-        bw::unpack2(add2(bw::pack2(u, v), less), d0, d1);
-        const bw::f32x2 d = bw::pack2(fmaxf(d0, LEAST), fmaxf(d1, LEAST));
-        bw::unpack2(bw::mul2(d, l2e), a0, a1);
-        const bw::f32x2 t = bw::pack2(ex2(a0), ex2(a1));
-        s.z = add2(s.z, t);
-        s.w = bw::fma2(t, d, s.w);
+    // (-infinity, here or as the reference so far, comes out as a term of 0.  One element an instruction: packed pairs, which would have to be put
+    // together from what the minima leave, took twice the instructions)
+    auto add = [&](float x, int i) {
+        const float d = fmaxf(x - s.ref, LEAST), t = ex2(d * LOG2E);
+        s.z[i] += t;
+        s.w[i] = fmaf(t, d, s.w[i]);
     };
-    add(l0, l1);
-    add(l2, l3);
+    add(l0, 0);
+    add(l1, 1);
+    add(l2, 0);
+    add(l3, 1);
 }
 // the same against the best
 __device__ __forceinline__ Part part_of(const Running& s) {
     if (s.ref == -INFINITY) return {s.best, 0.f, 0.f};
-    const float d = fmaxf(s.ref - s.best, LEAST), e = ex2(d * LOG2E), z = bw::sum2(s.z);
-    return {s.best, e * z, e * fmaf(d, z, bw::sum2(s.w))};
+    const float d = fmaxf(s.ref - s.best, LEAST), e = ex2(d * LOG2E), z = s.z[0] + s.z[1];
+    return {s.best, e * z, e * fmaf(d, z, s.w[0] + s.w[1])};
 }
 
 __device__ __forceinline__ Found shuffled(const Found& a, int o) {
@@ -206,9 +197,10 @@ __device__ __forceinline__ Found join_lanes(Found a, int n) {
     return a;
 }
 
-// grid: rows * blocks; a row's `blocks` blocks are one cluster.
-template <bool VEC>
-__global__ void __launch_bounds__(THREADS, 2)
+// grid: rows * blocks; a row's `blocks` blocks are one cluster.  AT_ONCE: blocks on an SM (three while all SMs have work for long; where few blocks are
+// launched at all they would gather on some of them).
+template <bool VEC, int AT_ONCE>
+__global__ void __launch_bounds__(THREADS, AT_ONCE)
 token_probs_kernel(Args p, int blocks) {
     BW_PDL_TRIGGER();
     __shared__ Shared sh;
@@ -220,30 +212,25 @@ token_probs_kernel(Args p, int blocks) {
     const int fours = (p.V + 3) / 4, each = (fours + blocks - 1) / blocks;
     const int f0 = min(fours, part * each), f1 = min(fours, f0 + each);
     BW_PDL_WAIT();
-    // four fours of a thread are on their way while it works on the four before
-    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    float4 x[UNROLL];
-    const int own = f0 + (int)threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) x[u] = own + u * THREADS < f1 ? load4<VEC>(row, 4 * (own + u * THREADS), p.V) : none;
-    const int target = p.target[r];
+    const int own = f0 + (int)threadIdx.x, target = p.target[r];
     const bool given = target >= 0 && target < p.V;
     const float xt = given ? row[target] : INFINITY;
     Running s;
     s.four = own;
-    for (int f = own; f < f1; f += UNROLL * THREADS) {
-        float4 next[UNROLL];
+    // four whole fours at a time without a look at the row's end, then what is left
+    int f = own;
+    const int whole = min(f1, p.V / 4);
+    for (; f + (UNROLL - 1) * THREADS < whole; f += UNROLL * THREADS) {
+        float4 x[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int g = f + (UNROLL + u) * THREADS;
-            next[u] = g < f1 ? load4<VEC>(row, 4 * g, p.V) : none;
+            const float* at = row + 4 * (f + u * THREADS);
+            x[u] = VEC ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (f + u * THREADS < f1) take4(s, x[u], f + u * THREADS, xt, target);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) x[u] = next[u];
+        for (int u = 0; u < UNROLL; ++u) take4(s, x[u], f + u * THREADS, xt, target);
     }
+    for (; f < f1; f += THREADS) take4(s, load4<VEC>(row, 4 * f, p.V), f, xt, target);
     Found all{part_of(s), s.count, !(s.best < INFINITY)};
     all = join_lanes(all, 32);
     if (lane == 0) sh.warps[warp] = all;
@@ -267,7 +254,7 @@ token_probs_kernel(Args p, int blocks) {
                 const int i = i0 + (int)threadIdx.x, who = i / rounds, it = i - who * rounds;
                 const u64 owner = i < items ? sh.best[who] : 0;
                 const int f = owner ? f0 + it * THREADS + (id_of(owner) / 4 - f0) % THREADS : f1;
-                const float4 v = f < f1 ? load4<VEC>(row, 4 * f, p.V) : none;
+                const float4 v = f < f1 ? load4<VEC>(row, 4 * f, p.V) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float y[4] = {v.x, v.y, v.z, v.w};
                 // the warp's candidates side by side, then 32 of them at a time: mostly a few in all
                 int n = 0;
@@ -332,10 +319,12 @@ BW_EXPORT int bw_token_probs(const float* logits, const int* target, float* log_
     if (top < 0 || top > MAX_TOP || top > V || (top && (!top_ids || !top_log_probs))) return BW_ERR_BAD_ARG;
     const Args p{logits, target, log_prob, entropy, rank, top_ids, top_log_probs, V, top, (size_t)ld};
     const bool vec = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
-    // as many blocks a row as run at once (two an SM), while each has a few thousand elements
-    const long long room = 2LL * bw::num_sms();
+    // Few rows: as many blocks a row as run at once (two an SM), while each has a few thousand elements.  Many: a block a row; shared rows cost more in
+    // sorting than they even out (1,024 rows of 128,256 with one alternative: 106 us, as two blocks each 112, as four 154).
+    const long long sms = bw::num_sms();
+    const bool few = R <= 2 * sms;
     int blocks = 1;
-    while (blocks < 8 && R * 2LL * blocks <= room && V >= 8192 * blocks) blocks *= 2;
+    while (few && blocks < 8 && R * 2LL * blocks <= 2 * sms && V >= 8192 * blocks) blocks *= 2;
     if ((long long)R * blocks > 0x7fffffffll) return BW_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(R * blocks)); cfg.blockDim = dim3(THREADS); cfg.stream = (cudaStream_t)stream;
@@ -345,8 +334,9 @@ BW_EXPORT int bw_token_probs(const float* logits, const int* target, float* log_
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = bw::pdl_enabled() ? 2 : 1;
-    const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, token_probs_kernel<true>, p, blocks)
-                              : cudaLaunchKernelEx(&cfg, token_probs_kernel<false>, p, blocks);
+    const auto kernel = few ? (vec ? token_probs_kernel<true, 2> : token_probs_kernel<false, 2>)
+                            : (vec ? token_probs_kernel<true, 3> : token_probs_kernel<false, 3>);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, blocks);
     if (e != cudaSuccess) return (int)e;
     BW_LAUNCH_CHECK();
     return 0;
