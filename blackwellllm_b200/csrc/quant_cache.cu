@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
 // pair stand side by side in the source.  VEC: rd is a multiple of 8 and the rows are aligned, so a lane's units are of one kind and their
 // channels come as two vectors.
 template <typename T, bool VEC, int LANES>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 8)
 append_kernel(const T* qkv, int planes, long long plane_stride, const float* turns, int rd, int paired,
               bf16* q_out, int nh, Rows p, unsigned per_heads, int append) {
     BW_PDL_TRIGGER();
@@ -85,6 +85,7 @@ append_kernel(const T* qkv, int planes, long long plane_stride, const float* tur
     for (int i = 0; i < 4; ++i) turned[i] = !is_v && 4 * l + i < half;
     if (live) {
         const T* src = qkv + ((size_t)t * heads + head) * p.hd;
+#pragma unroll 1
         for (int pl = 0; pl < planes; ++pl, src += plane_stride) {
             float u[4], w[4];
             if constexpr (VEC) {
@@ -143,7 +144,7 @@ append_kernel(const T* qkv, int planes, long long plane_stride, const float* tur
             }
         }
     }
-    if (!append) return;          // (uniform)
+    if (!__any_sync(0xffffffffu, row >= 0)) return;          // nothing of this warp's is written to the cache
     // the largest magnitude as an ordered whole number: what is no number stands above infinity and stays
     unsigned most = 0;
 #pragma unroll
