@@ -7,7 +7,8 @@ its own block table; a page id indexes the same page in every layer of its group
 (as one page id does across all layers in the reference,
 src/core/paging/paged_kv_cache.h:74-78,96-107).  A pool is one tensor
 ``[entries, 2, num_pages, num_kv_heads, page_size, head_dim]`` (2: keys, values; 1 where a mixer's values are
-part of its key rows).  A schedule entry may ask for several things at once (a tuple of requests: pages for its
+part of its key rows); of a group that asks for 8 bits it is int8, with the rows' scales in a second tensor
+``[entries, 2, num_pages, num_kv_heads, page_size]``.  A schedule entry may ask for several things at once (a tuple of requests: pages for its
 mixer, a state for the block around it); its view is then a tuple in the same order.
 
 A request gets pages when it grows (:meth:`CacheManager.append`, all or nothing
@@ -76,6 +77,7 @@ class PagedKVView:
     k_pages: Optional[torch.Tensor]  # [num_pages, num_kv_heads, page_size, head_dim]
     v_pages: Optional[torch.Tensor]
     page_size: int
+    quant: Optional[object] = None   # ops.QuantPages where the group is kept in 8 bits (k_pages, v_pages: its numbers)
 
 
 @dataclass
@@ -90,6 +92,7 @@ class _Group:
     entries: List[int]              # the schedule entries whose pages lie in this pool, in pool order
     num_pages: int
     pool: Optional[torch.Tensor] = None
+    scales: Optional[torch.Tensor] = None   # of a group in 8 bits
 
 
 class _Slots:
@@ -148,11 +151,19 @@ class CacheManager:
             r = grp.request
             planes = 1 if r.single_plane else 2
             if device is not None:
-                grp.pool = torch.zeros((len(grp.entries), planes, n, r.num_kv_heads, page_size, r.head_dim),
-                                       dtype=dtype, device=device)
+                shape = (len(grp.entries), planes, n, r.num_kv_heads, page_size, r.head_dim)
+                grp.pool = torch.zeros(shape, dtype=torch.int8 if r.quantized else dtype, device=device)
+                if r.quantized:
+                    grp.scales = torch.zeros(shape[:-1], dtype=torch.float32, device=device)
             for i, key in enumerate(keys_of[g]):
-                made[key] = PagedKVView(g, None if grp.pool is None else grp.pool[i, 0],
-                                        None if grp.pool is None else grp.pool[i, planes - 1], page_size)
+                if grp.pool is None:
+                    made[key] = PagedKVView(g, None, None, page_size)
+                    continue
+                k, v, quant = grp.pool[i, 0], grp.pool[i, planes - 1], None
+                if r.quantized:
+                    from ..kernels.ops import QuantPages
+                    quant = QuantPages(k, v, grp.scales[i, 0], grp.scales[i, planes - 1])
+                made[key] = PagedKVView(g, k, v, page_size, quant)
         for pos, k, rq in flat:
             if isinstance(rq, FixedStateRequest):
                 st = None if device is None else torch.zeros((max_requests, *rq.shape), dtype=rq.dtype,

@@ -47,6 +47,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--random-weights", action="store_true", help="random weights from --config and --seed")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--kv-dtype", choices=["model", "int8"], default="model",
+                    help="keys and values in the cache: as the model, or int8 with a scale per token and kv head")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--num-pages", type=int, default=None)
     ap.add_argument("--max-batch-tokens", type=int, default=2048)
@@ -99,6 +101,8 @@ def make_engine(args):
                           temperature=args.temperature, top_p=args.top_p)
     kw = dict(dtype=args.dtype, page_size=args.page_size, num_pages=args.num_pages,
               max_batch_tokens=args.max_batch_tokens, seed=args.seed)
+    if args.kv_dtype != "model":
+        kw["kv_dtype"] = args.kv_dtype
     if args.random_weights:
         if not args.config:
             raise SystemExit("--random-weights needs --config JSON")

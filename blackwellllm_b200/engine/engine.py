@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from ..cache.manager import (ERR_BAD_TOKEN, ERR_BAD_WANT, ERR_NO_SLOT, ERR_OUT_OF_PAGES, ERR_TOO_MANY_TOKENS,
-                             ERR_TOO_SMALL, CacheManager, native)
+                             ERR_TOO_SMALL, CacheManager, PagedKVView, native)
 from ..cache.pages import OutOfPages
 from ..config.registry import load_config, parse_config
 from ..config.specs import ModelConfig
@@ -44,6 +44,8 @@ class EngineError(RuntimeError):
 @dataclass
 class EngineOptions:
     dtype: object = "bfloat16"      # "bfloat16" | "float32"
+    kv_dtype: Optional[str] = None  # keys and values in the cache: None (as the model) | "int8" (a scale per token and kv head;
+                                    # bfloat16 models whose attention layers all take it)
     page_size: int = 16
     num_pages: Optional[int] = None  # pages per cache group; None: from max_tokens or kv_fraction
     max_tokens: Optional[int] = None  # tokens the cache holds (each request rounded up to a page)
@@ -111,11 +113,23 @@ class Engine:
     def _build(cls, config: ModelConfig, options: EngineOptions):
         if options.dtype not in _DTYPES:
             raise EngineError(f"dtype must be 'bfloat16' or 'float32', got {options.dtype!r}")
+        if options.kv_dtype not in (None, "int8"):
+            raise EngineError(f"kv_dtype must be None (as the model) or 'int8', got {options.kv_dtype!r}")
+        if options.kv_dtype == "int8" and _DTYPES[options.dtype] != torch.bfloat16:
+            raise EngineError(f"kv_dtype='int8' goes with dtype 'bfloat16', not {options.dtype!r}")
         device = torch.device(options.device)
         require_cuda(device)
         torch.cuda.set_device(device)
-        ctx = BuildContext(device, _DTYPES[options.dtype])
-        return DecoderModel(config, ctx), ctx
+        return cls._model(config, BuildContext(device, _DTYPES[options.dtype], quant_cache=options.kv_dtype == "int8"))
+
+    @staticmethod
+    def _model(config: ModelConfig, ctx: BuildContext):
+        model = DecoderModel(config, ctx)
+        if ctx.quant_cache:
+            pages = [r for entry in model.cache_requests() for r in flatten_cache_requests(entry) if isinstance(r, PagedKVRequest)]
+            if not pages or not all(r.quantized for r in pages):
+                raise EngineError("kv_dtype='int8': the model has layers that keep their keys and values in the model's dtype only, or none")
+        return model, ctx
 
     @classmethod
     def from_folder(cls, model_dir: str, **opts) -> "Engine":
@@ -161,7 +175,7 @@ class Engine:
         if not groups:
             return 1
         esize = 4 if self.dtype == torch.float32 else 2
-        per_page = sum(n * (1 if r.single_plane else 2) * r.num_kv_heads * o.page_size * r.head_dim * esize for r, n in groups.items())
+        per_page = sum(n * r.page_bytes(o.page_size, esize) for r, n in groups.items())
         free, _ = torch.cuda.mem_get_info(self.device)
         return max(1, int(free * o.kv_fraction) // per_page)
 
@@ -175,6 +189,29 @@ class Engine:
 
     def has_request(self, rid) -> bool:
         return self.cache.has(rid)
+
+    def cached_kv(self, rid, layer: int, start: int = 0, stop: Optional[int] = None):
+        """The keys (as attention reads them: rotated) and values that the request's cache holds for positions ``start`` to
+        ``stop`` (None: all) of a layer that owns pages: two tensors [positions, kv heads, head size] in the model's dtype; of a cache in 8
+        bits the numbers times their scales.  Zeros at positions whose pages a window has given back."""
+        from ..kernels import ops
+        if not self.cache.has(rid):
+            raise EngineError(f"request {rid!r} is not live")
+        view = self.cache.views[layer] if 0 <= layer < len(self.cache.views) else None
+        if not isinstance(view, PagedKVView):
+            raise EngineError(f"layer {layer} owns no pages of keys and values")
+        n = self.cache.length(rid)
+        stop = n if stop is None else stop
+        if not 0 <= start <= stop <= n:
+            raise EngineError(f"positions {start} to {stop} are not within the request's {n} cached ones")
+        with torch.cuda.device(self.device):
+            table = torch.from_numpy(self.cache.block_row(rid, view.group)).to(self.device)[None]
+            pos = torch.arange(start, stop, dtype=torch.int32, device=self.device)
+            if view.quant is not None:
+                return ops.quant_read(view.quant, pos, torch.zeros_like(pos), table, self.dtype)
+            page, inside = table[0][(pos // view.page_size).long()].long(), (pos % view.page_size).long()
+            gone = (page < 0)[:, None, None]
+            return tuple(p[page.clamp(min=0), :, inside].masked_fill(gone, 0) for p in (view.k_pages, view.v_pages))
 
     # ------------------------------------------------------------------ the step
     def prepare(self, entries: Sequence[StepEntry], min_blocks: int = 0, into=None,

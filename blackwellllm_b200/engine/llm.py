@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Dict, List, Mapping, Optional, Sequence, Union
+from typing import Dict, List, Mapping, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -54,10 +54,30 @@ class GenerationResult:
     token_ids: List[int]
     finish_reason: str
     preemptions: int = 0
+    logprobs: Optional[List["TokenLogProb"]] = None   # one per generated token, where SamplingParams.logprobs asked for them
+
+
+@dataclass
+class TokenLogProb:
+    """A token under the model's own distribution (before temperature, nucleus and repetition penalty)."""
+    token_id: int
+    log_prob: float
+    rank: int                               # how many tokens stand before it (equally probable ones by their ids)
+    entropy: float                          # of the distribution, in nats
+    top: List[Tuple[int, float]]            # the most probable tokens and their log probabilities
 
 
 _GREEDY = SamplingParams(temperature=0.0, top_p=1.0)
 FROM_LAST = -1   # DecodeRequest.token_id: the token that the previous forward_batch sampled for the sequence
+
+
+_SCORE_PORTION = 512   # tokens of a scored text in a step: a row of float32 logits each
+
+
+def _listed(told: "ops.TokenLogProbs", tokens: Sequence[int], rows: Sequence[int]) -> List[TokenLogProb]:
+    """Rows of what :func:`ops.token_log_probs` found, on the host (waits for it)."""
+    log_prob, entropy, rank, ids, log_probs = (t.cpu().tolist() for t in told)
+    return [TokenLogProb(tokens[i], log_prob[i], rank[i], entropy[i], list(zip(ids[i], log_probs[i]))) for i in rows]
 
 
 class PendingTokens:
@@ -101,13 +121,15 @@ class BlackwellEngine:
                  config: Optional[Mapping[str, object]] = None, random_seed: int = 0, random_std: float = 0.02,
                  dtype: str = "bfloat16", page_size: int = 16, num_pages: Optional[int] = None,
                  max_batch_tokens: int = 2048, chunk: Optional[int] = None, kv_fraction: Optional[float] = None,
-                 seed: int = 0, device: str = "cuda:0", cuda_graphs: bool = True, ignore_unexpected: bool = False):
+                 seed: int = 0, device: str = "cuda:0", cuda_graphs: bool = True, ignore_unexpected: bool = False,
+                 kv_dtype: Optional[str] = None):
         """``model``: a folder with config.json and model.safetensors.  Or ``config``
         (the config.json object) for random weights from ``random_seed``.  The cache
         holds ``max_batch_size`` sequences of ``max_context_length`` tokens unless
         ``num_pages`` or ``kv_fraction`` (of free device memory) says otherwise.
         ``ignore_unexpected``: tensors of the checkpoint that the model does not use are
-        passed over with a note instead of being an error."""
+        passed over with a note instead of being an error.  ``kv_dtype="int8"``: keys and values are cached in 8 bits
+        with a scale per token and kv head, about half the bytes (bfloat16 models)."""
         self.request = request or InferenceConfig()
         rq = self.request
         if rq.max_context_length <= 0 or rq.max_batch_size < 1:
@@ -118,7 +140,7 @@ class BlackwellEngine:
                              kv_fraction=kv_fraction or 0.6, max_requests=max(rq.max_batch_size, 1),
                              max_batch_tokens=max(max_batch_tokens, rq.max_batch_size), device=device,
                              max_context=rq.max_context_length, cuda_graphs=cuda_graphs,
-                             ignore_unexpected=ignore_unexpected)
+                             ignore_unexpected=ignore_unexpected, kv_dtype=kv_dtype)
         if (model is None) == (config is None):
             raise EngineError("give either a model folder or a config for random weights")
         # the context is checked against the model before any weight is read
@@ -226,6 +248,32 @@ class BlackwellEngine:
         if row is None or not 0 <= token_id < self.vocab_size:
             return 0.0
         return min(1.0, max(0.0, math.exp(self._log_prob(row[None, :], token_id))))
+
+    def score(self, token_ids: Sequence[int], top: int = 0) -> List[TokenLogProb]:
+        """Every token of a text but its first under the model: log probability, rank, entropy and the ``top`` most probable
+        tokens in its place (at most ops.TOKEN_LOG_PROBS_MAX_TOP).  The text takes a request slot and pages while it is scored."""
+        ids = [int(t) for t in token_ids]
+        for t in ids:
+            self._check_token(t)
+        if not 0 <= top <= ops.TOKEN_LOG_PROBS_MAX_TOP:
+            raise EngineError(f"top must be 0 to {ops.TOKEN_LOG_PROBS_MAX_TOP}, got {top}")
+        if len(ids) > self.request.max_context_length:
+            raise EngineError("the tokens do not fit max_context_length")
+        self._drop_ahead()
+        self._last_logits = {}
+        rid, out, at = ("score",), [], 0
+        try:
+            while at + 1 < len(ids):
+                n = min(len(ids) - 1 - at, self.max_batch_tokens, _SCORE_PORTION)
+                logits = self.engine.step([StepEntry(rid, ids[at:at + n], list(range(n)))])
+                given = ids[at + 1:at + 1 + n]
+                target = torch.tensor(given, dtype=torch.int32, device=logits.device)
+                out += _listed(ops.token_log_probs(logits, target, min(top, self.vocab_size)), given, range(n))
+                at += n
+        finally:
+            if self.engine.cache.has(rid):
+                self.engine.cache.free_request(rid)
+        return out
 
     def _check_token(self, token_id: int) -> None:
         if not 0 <= token_id < self.vocab_size:
@@ -342,10 +390,16 @@ class BlackwellEngine:
         self._last_logits = {}
         samplers = [e.request for e in plan.entries if e.samples]
         sampled: Dict[int, int] = {}
-        picked = None
+        picked = told = None
         if samplers:
+            asking = [i for i, r in enumerate(samplers) if r.params.logprobs is not None]
+            # (the repetition penalty changes the logits in place: what is asked about is the model's own distribution)
+            own = logits.clone() if asking and any(samplers[i].params.penalized(samplers[i].generated) for i in asking) else logits
             picked = self.sampler.sample_async(logits, [r.params for r in samplers], [r.seed for r in samplers],
                                                [len(r.generated) for r in samplers], [r.generated for r in samplers])
+            if asking:
+                top = min(max(samplers[i].params.logprobs for i in asking), self.vocab_size)
+                told = ops.token_log_probs(own, picked, top)
         nxt = self._prepare_ahead(plan)        # host work while the GPU runs this step
         if picked is not None:
             sampled = {r.rid: t for r, t in zip(samplers, picked.tolist())}     # waits for the step
@@ -362,9 +416,15 @@ class BlackwellEngine:
                 for e in nxt[0].entries:    # the tokens that were being sampled while the step was prepared
                     e.tokens = [sampled[e.request.rid]]
                 self._ahead = nxt
+        if told is not None:
+            for i, entry in zip(asking, _listed(told, [sampled[r.rid] for r in samplers], asking)):
+                r = samplers[i]
+                entry.top = entry.top[:r.params.logprobs]
+                r.logprobs.append(entry)
         for r in done:   # handed to the caller here: a long-lived engine keeps no finished request
             self.scheduler.finished.pop(r.rid, None)
-        return [GenerationResult(r.rid, r.prompt, r.generated, r.finish_reason, r.preemptions) for r in done]
+        return [GenerationResult(r.rid, r.prompt, r.generated, r.finish_reason, r.preemptions,
+                                 r.logprobs if r.params.logprobs is not None else None) for r in done]
 
     def _prepare_ahead(self, plan):
         """The next step, prepared while this one runs, if it is certain to be "one token for each

@@ -49,6 +49,7 @@ class Request:
     finish_reason: Optional[str] = None
     preemptions: int = 0
     admitted_at: int = -1          # admission counter: larger = more recent
+    logprobs: List[object] = field(default_factory=list)   # of the generated tokens, where params.logprobs asks for them
 
     @property
     def tokens(self) -> List[int]:

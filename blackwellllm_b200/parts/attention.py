@@ -46,6 +46,9 @@ keeps a head's sum of squares, so the kernel divides before it rotates, which is
 value projection: the key projection is cached twice, normed and rotated as the key, as it is as the value),
 ``head_temperature`` (a learned number per query head on its scores: the queries are multiplied by it) and
 ``output_scale`` (a constant on the mixer's output: the values are multiplied by it in float32 before they are cached).
+
+With ``BuildContext.quant_cache`` keys and values are cached in 8 bits: the plain route (projection, rotation, attention; with a window, blocks
+of positions or a sink) through ``ops.quant_append`` and ``ops.quant_attention``.  A mixer with any other option refuses it.
 """
 from __future__ import annotations
 
@@ -155,13 +158,26 @@ class GQAAttention(Mixer):
         # (the general route hands ops.paged_attention finished queries: beyond the query heads per kv head that the
         # tensor-core kernels stack, it takes the CUDA-core kernel; the fused route goes to the tensor-core kernels only)
         ops.check_attention_supported(ctx.dtype, self.dpad, 1 if self.general else self.nh // self.nkv)
+        self.quant = bool(getattr(ctx, "quant_cache", False))
+        if self.quant:
+            other = [name for name, on in (("head norms, temperatures, gates or mixed, shared, scaled or padded values", self.general),
+                                           ("a distance bias", self.has_dist), ("a table of biases by distance", self.rel_far is not None),
+                                           ("a soft cap", self.softcap is not None), ("kept first keys", bool(self.window and self.keep_first)))
+                     if on]
+            if ctx.dtype != torch.bfloat16:
+                other.append("float32")
+            if getattr(self.position, "interleaved", False) or getattr(self.position, "magnitude", 1.0) != 1.0:
+                other.append("paired or scaled rotation")
+            if other:
+                raise ops.KernelError("8-bit cache: attention with " + ", ".join(other) + " keeps its keys and values in the model's dtype only")
+            ops.check_quant_supported(self.dpad, self.nh // self.nkv)
         self.qkv: Linear = None
         self.project = None
         self.o: Linear = None
 
     def cache_request(self):
         # (a run with ``shares_kv`` is never asked: its schedule entry names the run whose cache it reads)
-        return PagedKVRequest(self.nkv, self.dpad, self.window, self.keep_first if self.window else 0)
+        return PagedKVRequest(self.nkv, self.dpad, self.window, self.keep_first if self.window else 0, quantized=self.quant)
 
     def param_specs(self) -> List[ParamSpec]:
         H, q, k, v = self.hidden_size, self.nh * self.hd, self.nkv * self.hd, self.nkv * self.dv
@@ -299,6 +315,9 @@ class GQAAttention(Mixer):
         return self._attend(q, qkv, x, batch, cache)
 
     def _attend(self, q, qkv, x, batch, cache):
+        if cache.quant is not None:
+            return ops.quant_attention(q, cache.quant, batch, batch.block_tables[cache.group], self.nh, self.scale, self.window, self.chunk,
+                                       self.sink)
         gate = None
         if self.gated:   # the attention kernels multiply by the gate's sigmoid as they write a row
             if self.gate_per_head:

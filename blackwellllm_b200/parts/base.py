@@ -58,6 +58,7 @@ class ParamSpec:
 class BuildContext:
     device: torch.device
     dtype: torch.dtype  # torch.float32 (true 32-bit path) or torch.bfloat16
+    quant_cache: bool = False   # paged keys and values in 8 bits (mixers that cannot refuse it where they are built)
     _side: Optional[torch.cuda.Stream] = field(default=None, repr=False, compare=False)
 
     def side_stream(self) -> "torch.cuda.Stream":
@@ -72,12 +73,19 @@ class PagedKVRequest:
     """A mixer's need for paged keys and values: per token ``2 * num_kv_heads *
     head_dim`` elements; ``window``: only that many latest tokens stay needed, and with ``keep_first`` the
     first so many tokens of a request as well.  ``single_plane``: keys and values are the same rows (a mixer
-    whose values are a part of its key rows): one plane is kept and both views show it."""
+    whose values are a part of its key rows): one plane is kept and both views show it.  ``quantized``: int8 with a
+    float32 scale per (token, kv head) instead of the cache's dtype (``ops.QuantPages``)."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     keep_first: int = 0
     single_plane: bool = False
+    quantized: bool = False
+
+    def page_bytes(self, page_size: int, element_bytes: int) -> int:
+        """Bytes of one page, keys and values, in a cache of elements of so many bytes."""
+        rows = (1 if self.single_plane else 2) * self.num_kv_heads * page_size
+        return rows * (self.head_dim + 4 if self.quantized else self.head_dim * element_bytes)
 
 
 @dataclass(frozen=True)

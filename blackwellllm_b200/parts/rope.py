@@ -16,7 +16,8 @@ queries that grows with the logarithm of the position (``q_temp``), for heads wh
 from their key size; ``has_kv=False``: the rows hold queries only (a run that reads another run's cache).
 
 :class:`NoPosition` rotates nothing.  Both append rotated keys and raw values to
-the cache pages in the same kernel.
+the cache pages in the same kernel; to pages in 8 bits (``cache.quant``) through ``ops.quant_append``, from the
+projection's float32 rows whatever their number.
 """
 from __future__ import annotations
 
@@ -101,6 +102,9 @@ class RotaryEncoding(PositionEncoding):
         if self.interleaved or self.magnitude != 1.0:
             return self.norm_rotate_append(qkv, batch, cache, nh, nkv, hd, hd, None, None, 0.0, append)
         table = self._table(batch)
+        if cache.quant is not None:
+            return ops.quant_append(qkv, batch.positions, batch.req_of_token, batch.block_tables[cache.group], cache.quant, nh,
+                                    table=table, append=append)
         return ops.rope_append(qkv, batch.positions, batch.req_of_token, batch.block_tables[cache.group],
                                self.inv_freq, self.rotary_dim, cache.k_pages, cache.v_pages, nh, nkv, hd,
                                append=append, table=table)
@@ -117,6 +121,11 @@ class RotaryEncoding(PositionEncoding):
         b = bias.index_select(0, order).contiguous() if bias is not None else None
 
         def project(x, batch, cache, append=True):
+            if cache.quant is not None:
+                few = batch.T <= ops.GEMM_FUSED_REDUCE_MAX_TOKENS and ops.DEFER_SUMS
+                qkv = ops.gemm_tc_planes(x, w, b) if few else ops.gemm_tc(x, w, b, out_dtype=torch.float32)
+                return ops.quant_append(qkv, batch.positions, batch.req_of_token, batch.block_tables[cache.group], cache.quant, nh,
+                                        table=self._table(batch), paired=True, append=append)
             if batch.T <= ops.GEMM_FUSED_REDUCE_MAX_TOKENS:
                 # few tokens: the product leaves its K splits as planes, which the rotation's kernel
                 # adds while it reads them (the rotation in the product's own epilogue, after a sum
@@ -151,6 +160,8 @@ class NoPosition(PositionEncoding):
         pass
 
     def rotate_append(self, qkv, batch, cache, nh, nkv, hd, append=True):
+        if cache.quant is not None:
+            return ops.quant_append(qkv, batch.positions, batch.req_of_token, batch.block_tables[cache.group], cache.quant, nh, append=append)
         return ops.rope_append(qkv, batch.positions, batch.req_of_token, batch.block_tables[cache.group],
                                None, 0, cache.k_pages, cache.v_pages, nh, nkv, hd, append=append)
 

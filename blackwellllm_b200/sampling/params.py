@@ -71,7 +71,9 @@ class SamplingParams:
     most probable tokens whose mass reaches it.  ``seed`` None: derived from the
     engine's seed and the request's number.  ``repetition_penalty`` > 1 makes the
     request's last ``repetition_window`` generated tokens (0: all of them) less
-    likely; <= 1 is off."""
+    likely; <= 1 is off.  ``logprobs`` (0 to 32; None: off): every generated token
+    comes with its log probability, rank and entropy under the model, and with
+    so many of the most probable tokens."""
     temperature: float = 0.6
     top_p: float = 0.9
     max_new_tokens: int = 1024
@@ -80,6 +82,7 @@ class SamplingParams:
     ignore_eos: bool = False
     repetition_penalty: float = 1.0
     repetition_window: int = 64
+    logprobs: Optional[int] = None
 
     def __post_init__(self):
         if self.temperature < 0:
@@ -92,6 +95,8 @@ class SamplingParams:
             raise ValueError("repetition_penalty must be > 0 (<= 1 switches it off)")
         if self.repetition_window < 0:
             raise ValueError("repetition_window must be >= 0")
+        if self.logprobs is not None and not 0 <= operator.index(self.logprobs) <= 32:
+            raise ValueError("logprobs must be None (off) or 0 to 32")
 
     def penalized(self, generated: Sequence[int]) -> Sequence[int]:
         """The ids that the repetition penalty acts on, given what the request has generated."""

@@ -1,0 +1,151 @@
+"""The 8-bit cache and the log probabilities of generated tokens without a GPU: what options, models and the cache manager make of them."""
+import contextlib
+
+import pytest
+import torch
+
+import tiny
+import tiny_fuvevik
+import tiny_gafulix
+import tiny_vubotar
+import tiny_zanivik
+import tiny_zigipel
+import tiny_zogulorn
+from blackwellllm_b200 import cli
+from blackwellllm_b200.cache.manager import CacheManager
+from blackwellllm_b200.config.registry import parse_config
+from blackwellllm_b200.engine.engine import Engine, EngineError, EngineOptions, StepEntry
+from blackwellllm_b200.kernels import ops
+from blackwellllm_b200.models.decoder import DecoderModel
+from blackwellllm_b200.parts.base import BuildContext, PagedKVRequest
+from blackwellllm_b200.sampling.params import SamplingParams
+
+CPU = torch.device("cpu")
+
+
+@pytest.mark.parametrize("name", list(tiny.CONFIGS))
+def test_the_dense_models_keep_their_keys_and_values_in_8_bits(name):
+    cfg = parse_config(tiny.CONFIGS[name][0])
+    plain = DecoderModel(cfg, BuildContext(CPU, torch.bfloat16)).cache_requests()
+    model, _ = Engine._model(cfg, BuildContext(CPU, torch.bfloat16, quant_cache=True))
+    quant = model.cache_requests()
+    assert len(quant) == len(plain) > 0 and all(r.quantized for r in quant) and not any(r.quantized for r in plain)
+    for a, b in zip(quant, plain):
+        assert (a.num_kv_heads, a.head_dim, a.window) == (b.num_kv_heads, b.head_dim, b.window)
+        assert a.page_bytes(16, 2) == 2 * 16 * a.num_kv_heads * (a.head_dim + 4)
+        assert b.page_bytes(16, 2) == 2 * 16 * b.num_kv_heads * b.head_dim * 2
+
+
+@pytest.mark.parametrize("module", [tiny_fuvevik, tiny_gafulix, tiny_vubotar, tiny_zanivik, tiny_zigipel, tiny_zogulorn])
+def test_a_design_whose_layers_keep_something_else_is_refused_where_it_is_built(module):
+    """Head norms, latent keys, gates, soft caps and the like have no form over 8 bits: an error, never a cache in the wrong type."""
+    refused = 0
+    for raw, _ in module.CONFIGS.values():
+        cfg = parse_config(raw)
+        try:
+            model, _ = Engine._model(cfg, BuildContext(CPU, torch.bfloat16, quant_cache=True))
+        except (EngineError, ops.KernelError) as e:
+            refused += 1
+            assert "8-bit cache" in str(e) or "kv_dtype" in str(e)
+        else:
+            assert all(r.quantized for e in model.cache_requests() for r in (e if isinstance(e, tuple) else (e,)) if isinstance(r, PagedKVRequest))
+    assert refused
+
+
+def test_options():
+    cfg = parse_config(tiny.TINY_LLAMA)
+    with pytest.raises(EngineError, match="kv_dtype must be"):
+        Engine._build(cfg, EngineOptions(kv_dtype="int4"))
+    with pytest.raises(EngineError, match="bfloat16"):
+        Engine._build(cfg, EngineOptions(kv_dtype="int8", dtype="float32"))
+    with pytest.raises(ops.KernelError, match="float32"):
+        DecoderModel(cfg, BuildContext(CPU, torch.float32, quant_cache=True))
+    ap = cli.build_parser()
+    assert ap.parse_args([]).kv_dtype == "model" and ap.parse_args(["--kv-dtype", "int8"]).kv_dtype == "int8"
+    with pytest.raises(SystemExit):
+        ap.parse_args(["--kv-dtype", "int4"])
+
+
+def test_head_sizes_and_groups_that_the_kernels_do_not_take():
+    for hd, group in ((24, 1), (272, 1), (0, 1), (64, 17)):
+        with pytest.raises(ops.KernelError, match="8-bit cache"):
+            ops.check_quant_supported(hd, group)
+    raw = dict(tiny.TINY_LLAMA, num_attention_heads=34, num_key_value_heads=2)
+    with pytest.raises(ops.KernelError):
+        DecoderModel(parse_config(raw), BuildContext(CPU, torch.bfloat16, quant_cache=True))
+
+
+def test_pools():
+    """Numbers and scales of a group lie in two tensors, each layer has its own part of both, and another group keeps its type."""
+    a, b = PagedKVRequest(2, 16, None, quantized=True), PagedKVRequest(2, 16, None)
+    cache = CacheManager([a, b, a], 8, 5, 2, dtype=torch.bfloat16, device=CPU)
+    assert len(cache.groups) == 2 and [v.group for v in cache.views] == [0, 1, 0]
+    one, plain, two = cache.views
+    assert plain.quant is None and plain.k_pages.dtype == torch.bfloat16 and cache.groups[1].scales is None
+    for v in (one, two):
+        assert v.quant.k is v.k_pages and v.quant.v is v.v_pages
+        for t in (v.quant.k, v.quant.v):
+            assert t.dtype == torch.int8 and t.shape == (5, 2, 8, 16) and t.is_contiguous()
+        for t in (v.quant.k_scale, v.quant.v_scale):
+            assert t.dtype == torch.float32 and t.shape == (5, 2, 8) and t.is_contiguous()
+    parts = [t for v in (one, two) for t in (v.quant.k, v.quant.v, v.quant.k_scale, v.quant.v_scale)]
+    for i, t in enumerate(parts):
+        t.fill_(i + 1)
+    assert all(bool((t == i + 1).all()) for i, t in enumerate(parts))
+    kept = CacheManager([a], 8, 5, 2, device=None)
+    assert kept.views[0].quant is None and kept.views[0].k_pages is None
+
+
+def test_how_many_log_probabilities_may_be_asked_for():
+    assert SamplingParams().logprobs is None
+    for n in (0, 1, 32):
+        assert SamplingParams(logprobs=n).logprobs == n
+    for n in (-1, 33):
+        with pytest.raises(ValueError, match="logprobs"):
+            SamplingParams(logprobs=n)
+    with pytest.raises(TypeError):
+        SamplingParams(logprobs=2.5)
+
+
+class PagesOnly:
+    """A stand-in model that owns pages and computes nothing."""
+
+    def __init__(self, vocab):
+        self.vocab, self.blocks = vocab, []
+
+    def cache_requests(self):
+        return [PagedKVRequest(2, 16, None), PagedKVRequest(2, 16, 16), None]
+
+    def forward(self, batch, views):
+        return torch.zeros((len(batch.logit_rows), self.vocab), dtype=torch.float32)
+
+
+def test_cached_rows_are_read_by_position(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    cfg = parse_config(tiny.TINY_LLAMA)
+    eng = Engine(cfg, PagesOnly(cfg.vocab_size), EngineOptions(dtype="float32", page_size=8, num_pages=12, max_requests=3,
+                                                               cuda_graphs=False, device="cpu"))
+    eng.step([StepEntry("b", [1] * 3, []), StepEntry("a", [1] * 29, [])])
+    for v in eng.cache.views[:2]:
+        v.k_pages.copy_(torch.randn(v.k_pages.shape))
+        v.v_pages.copy_(torch.randn(v.v_pages.shape))
+    for layer in (0, 1):
+        v, table = eng.cache.views[layer], eng.cache.block_table("a", layer)
+        k, val = eng.cached_kv("a", layer)
+        assert k.shape == val.shape == (29, 2, 16)
+        for p in range(29):
+            page = table[p // 8]
+            assert torch.equal(k[p], v.k_pages[page, :, p % 8] if page >= 0 else torch.zeros(2, 16))
+            assert torch.equal(val[p], v.v_pages[page, :, p % 8] if page >= 0 else torch.zeros(2, 16))
+        some = eng.cached_kv("a", layer, 7, 18)
+        assert torch.equal(some[0], k[7:18]) and torch.equal(some[1], val[7:18])
+    assert -1 in eng.cache.block_table("a", 1)
+    assert eng.cached_kv("b", 0, 3)[0].shape == (0, 2, 16)
+    with pytest.raises(EngineError, match="not live"):
+        eng.cached_kv("c", 0)
+    for layer in (-1, 2, 3):
+        with pytest.raises(EngineError, match="owns no pages"):
+            eng.cached_kv("a", layer)
+    for start, stop in ((-1, 2), (5, 4), (0, 30)):
+        with pytest.raises(EngineError, match="positions"):
+            eng.cached_kv("a", 0, start, stop)
