@@ -54,10 +54,12 @@ struct Params {
     const int8_t* k; const int8_t* v; const float* k_scale; const float* v_scale;
     const int* cu_q; const int* q_start; const int* kv_len; const int* table;
     const float* sink;              // float32 [nh] or null: one more term exp(sink) of a row's denominator
-    float* part_o; float* part_ml;  // results of key slices: [request][kv head][slice][16][HD] and [..][2]
+    float* part_o; float* part_ml;  // results of key slices: [request][kv head][slice][16][HD] and [..][2]; with `shared` [slice][kv head][16][HD]
     int max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests;
     int per, slices;                // key slices: tiles of each, most of them that any request has
     int cluster;                    // the slices of a (request, kv head) are one cluster of blocks and join there
+    int shared;                     // > 0: the requests share `slices` slices by their lengths (see deal_kernel), none counted longer than this
+    int* dealt;                     // then: which slice is whose
     float scale_log2;
 };
 
@@ -186,67 +188,57 @@ __device__ __forceinline__ void load_queries(const Params& p, Queries<NB>& s, in
     }
 }
 
-// 16 KG keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page (what lies in the rows
-// of the others is left over: whole numbers, and scales of any kind).  KG groups of sixteen keys go side by side: a group's products
-// are a chain, and a warp has little else to do meanwhile.
+// Sixteen keys from key0 on, in shared memory: rows of K and V, their scales; bit i of `there` is set if key i has a page (what lies in the rows
+// of the others is left over: whole numbers, and scales of any kind).  (Two groups of sixteen side by side in a warp's step hide each other's
+// chains of products, but their registers and rings cost blocks: 64 requests at 2,048 keys 65 us where one group took 48, 8 at 8,192 34 and 32.)
 // The reference follows its largest lazily: as long as nothing is more than 8 above it (a factor of 256) it stays, so most steps need one
 // vote instead of a maximum over the lanes and a pass over the outputs.
-template <int NB, int KG>
+template <int NB>
 __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint32_t v_rows, const float* ks, const float* vs, int key0,
                                           unsigned there, bool need_mask) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
     // matrices of an ldmatrix: keys 0-7 and 8-15 of one 16-byte unit, then of the next
     const int row = (lane & 7) + 8 * (lane >> 3 & 1), more = lane >> 4;
     const uint32_t at = (uint32_t)(row * STRIDE);
-    float sc[KG][NB][4];
+    float sc[NB][4];
 #pragma unroll
-    for (int h = 0; h < KG; ++h)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) sc[h][nb][0] = sc[h][nb][1] = sc[h][nb][2] = sc[h][nb][3] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c += 2) {
         // (an odd last unit: its second pair of matrices reads the first's again)
         const uint32_t col = at + 16 * unit(row, c + 1 < CHUNKS ? c + more : c);
-#pragma unroll
-        for (int h = 0; h < KG; ++h) {
-            uint32_t f[4];
-            ldsm4(k_rows + h * KEYS * STRIDE + col, f);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (c + i >= CHUNKS) break;
-                const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
-                const uint32_t a[4] = {raised2<0x4140>(x), raised2<0x4140>(y), raised2<0x4342>(x), raised2<0x4342>(y)};
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma(sc[h][nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
-            }
-        }
-    }
-    float most[NB][2], per_v[KG][2];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) most[nb][0] = most[nb][1] = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < KG; ++h) {
-        float kk[2], lv[2];
+        uint32_t f[4];
+        ldsm4(k_rows + col, f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            kk[i] = ks[16 * h + r + 8 * i];
-            const float v = vs[16 * h + r + 8 * i], v1 = v < LEAST_SCALE ? LEAST_SCALE : v;      // (NaN stays)
-            lv[i] = lg2(v1);
-            per_v[h][i] = reciprocal(v1);
+            if (c + i >= CHUNKS) break;
+            const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
+            const uint32_t a[4] = {raised2<0x4140>(x), raised2<0x4140>(y), raised2<0x4342>(x), raised2<0x4342>(y)};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma(sc[nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
         }
+    }
+    float most[NB][2], per_v[2], kk[2], lv[2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
+    for (int i = 0; i < 2; ++i) {
+        kk[i] = ks[r + 8 * i];
+        const float v = vs[r + 8 * i], v1 = v < LEAST_SCALE ? LEAST_SCALE : v;      // (NaN stays)
+        lv[i] = lg2(v1);
+        per_v[i] = reciprocal(v1);
+    }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = i & 1;
-                float t = fmaf((sc[h][nb][i] + s.off[nb][e]) * s.mul[nb][e], kk[i >> 1], lv[i >> 1]);
-                if (need_mask) {
-                    const int j = 16 * h + r + 8 * (i >> 1), kp = key0 + j;
-                    if (!(kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> j & 1))) t = -INFINITY;
-                }
-                sc[h][nb][i] = t;
-                most[nb][e] = fmaxf(most[nb][e], t);
+    for (int nb = 0; nb < NB; ++nb) {
+        most[nb][0] = most[nb][1] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = i & 1;
+            float t = fmaf((sc[nb][i] + s.off[nb][e]) * s.mul[nb][e], kk[i >> 1], lv[i >> 1]);
+            if (need_mask) {
+                const int j = r + 8 * (i >> 1), kp = key0 + j;
+                if (!(kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> j & 1))) t = -INFINITY;
             }
+            sc[nb][i] = t;
+            most[nb][e] = fmaxf(most[nb][e], t);
         }
     }
     bool grown = false;
@@ -273,38 +265,32 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
             }
         }
     }
-    uint32_t wf[KG][NB][2];
+    uint32_t wf[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const float ref[2] = {s.m[nb][0] == -INFINITY ? 0.f : s.m[nb][0], s.m[nb][1] == -INFINITY ? 0.f : s.m[nb][1]};
+        float w[4];
 #pragma unroll
-        for (int h = 0; h < KG; ++h) {
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = ex2(sc[h][nb][i] - ref[i & 1]);
-                // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
-                s.l[nb][i & 1] += need_mask && sc[h][nb][i] == -INFINITY ? 0.f : w[i] * per_v[h][i >> 1];
-            }
-            wf[h][nb][0] = turn8x8(pack_f16x2(w[0], w[1]));
-            wf[h][nb][1] = turn8x8(pack_f16x2(w[2], w[3]));
+        for (int i = 0; i < 4; ++i) {
+            w[i] = ex2(sc[nb][i] - ref[i & 1]);
+            // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
+            s.l[nb][i & 1] += need_mask && sc[nb][i] == -INFINITY ? 0.f : w[i] * per_v[i >> 1];
         }
+        wf[nb][0] = turn8x8(pack_f16x2(w[0], w[1]));
+        wf[nb][1] = turn8x8(pack_f16x2(w[2], w[3]));
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; c += 2) {
         const uint32_t col = at + 16 * unit(row, c + 1 < CHUNKS ? c + more : c);
+        uint32_t f[4];
+        ldsm4_t(v_rows + col, f);
 #pragma unroll
-        for (int h = 0; h < KG; ++h) {
-            uint32_t f[4];
-            ldsm4_t(v_rows + h * KEYS * STRIDE + col, f);
+        for (int i = 0; i < 2; ++i) {
+            if (c + i >= CHUNKS) break;
+            const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
+            const uint32_t a[4] = {widen2<0x4240>(x), widen2<0x4341>(x), widen2<0x4240>(y), widen2<0x4341>(y)};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (c + i >= CHUNKS) break;
-                const uint32_t x = f[2 * i] ^ TOP_BITS, y = f[2 * i + 1] ^ TOP_BITS;
-                const uint32_t a[4] = {widen2<0x4240>(x), widen2<0x4341>(x), widen2<0x4240>(y), widen2<0x4341>(y)};
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, wf[h][nb][0], wf[h][nb][1]);
-            }
+            for (int nb = 0; nb < NB; ++nb) mma(s.o[c + i][nb], a, wf[nb][0], wf[nb][1]);
         }
     }
 }
@@ -318,89 +304,69 @@ __device__ __forceinline__ int key_row(const Params& p, const int* bt, int g, in
     return page >= 0 && page < p.num_pages ? (page * p.nkv + g) * p.page_size + (key - blk * p.page_size) : -1;
 }
 
-// 16 KG keys into a stage (rows of K, of V, their scales), by one warp.  What is held is looked up a step ahead of its use (`find`).
+// Sixteen keys into a stage (rows of K, of V, their scales), by one warp.  What is held is looked up a step ahead of its use (`find`).
 // WHOLE: pages are a multiple of sixteen keys long, so sixteen keys are one stretch of memory and need one look-up; places behind the
 // request's last token are read with the others (and masked).  Otherwise every lane looks up a key of its own.
-template <int KG> constexpr int STAGE = 2 * KG * KEYS * (STRIDE + 4);
-template <int KG, bool WHOLE>
+constexpr int STAGE = 2 * KEYS * (STRIDE + 4);
+constexpr unsigned ALL = (1u << KEYS) - 1;         // all of them are held
+template <bool WHOLE>
 struct Feed {
-    static constexpr int N = KG * KEYS;
-    int row[WHOLE ? KG : 1];
+    int row;
     __device__ __forceinline__ void find(const Params& p, const int* bt, int g, int key0, int end, int kv_len) {
-        if constexpr (WHOLE) {
-#pragma unroll
-            for (int h = 0; h < KG; ++h) row[h] = key0 + 16 * h < end ? key_row(p, bt, g, key0 + 16 * h, kv_len) : -1;
-        } else {
-            row[0] = key0 < end ? key_row(p, bt, g, key0 + (threadIdx.x & (N - 1)), kv_len) : -1;
-        }
+        row = key0 < end ? key_row(p, bt, g, key0 + (WHOLE ? 0 : threadIdx.x & (KEYS - 1)), kv_len) : -1;
     }
     // which keys are held, as bits
     __device__ __forceinline__ unsigned fetch(const Params& p, uint8_t* stage) const {
         const int lane = threadIdx.x & 31;
-        const uint32_t k_to = smem_u32(stage), v_to = k_to + N * STRIDE, s_to = v_to + N * STRIDE;
+        const uint32_t k_to = smem_u32(stage), v_to = k_to + KEYS * STRIDE, s_to = v_to + KEYS * STRIDE;
+        const float* scales = lane < KEYS ? p.k_scale : p.v_scale;
         if constexpr (WHOLE) {
-            unsigned got = 0;
+            if (row < 0) return 0;        // (uniform)
+            const int8_t* k_from = p.k + (size_t)row * HD + 16 * lane;
+            const int8_t* v_from = p.v + (size_t)row * HD + 16 * lane;
 #pragma unroll
-            for (int h = 0; h < KG; ++h) {
-                if (row[h] < 0) continue;        // (uniform)
-                got |= 0xffffu << (16 * h);
-                const int8_t* k_from = p.k + (size_t)row[h] * HD + 16 * lane;
-                const int8_t* v_from = p.v + (size_t)row[h] * HD + 16 * lane;
-#pragma unroll
-                for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
-                    const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
-                    if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
-                    const uint32_t to = (16 * h + key) * STRIDE + 16 * unit(key, c);
-                    cp_async16(k_to + to, k_from + 512 * i, true);
-                    cp_async16(v_to + to, v_from + 512 * i, true);
-                }
-                cp_async4(s_to + 4 * ((lane < 16 ? 0 : N - 16) + 16 * h + lane), (lane < 16 ? p.k_scale : p.v_scale) + row[h] + (lane & 15), true);
-            }
-            return got;
-        } else {
-            const unsigned got = __ballot_sync(0xffffffffu, row[0] >= 0);
-#pragma unroll
-            for (int i = 0; i < (N * CHUNKS + 31) / 32; ++i) {
+            for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
                 const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
-                const int rw = __shfl_sync(0xffffffffu, row[0], key & (N - 1));
-                if ((N * CHUNKS) % 32 && key >= N) break;
+                if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
+                const uint32_t to = key * STRIDE + 16 * unit(key, c);
+                cp_async16(k_to + to, k_from + 512 * i, true);
+                cp_async16(v_to + to, v_from + 512 * i, true);
+            }
+            cp_async4(s_to + 4 * lane, scales + row + (lane & (KEYS - 1)), true);
+            return ALL;
+        } else {
+            const unsigned got = __ballot_sync(0xffffffffu, row >= 0);
+#pragma unroll
+            for (int i = 0; i < (KEYS * CHUNKS + 31) / 32; ++i) {
+                const int idx = lane + 32 * i, key = idx / CHUNKS, c = idx - key * CHUNKS;
+                const int rw = __shfl_sync(0xffffffffu, row, key & (KEYS - 1));
+                if ((KEYS * CHUNKS) % 32 && key >= KEYS) break;
                 const size_t off = rw >= 0 ? (size_t)rw * HD + 16 * c : 0;
                 const uint32_t to = key * STRIDE + 16 * unit(key, c);
                 cp_async16(k_to + to, p.k + off, rw >= 0);
                 cp_async16(v_to + to, p.v + off, rw >= 0);
             }
-            const int from = row[0] >= 0 ? row[0] : 0;
-            if constexpr (KG == 1) {
-                cp_async4(s_to + 4 * lane, (lane < 16 ? p.k_scale : p.v_scale) + from, row[0] >= 0);
-            } else {
-                cp_async4(s_to + 4 * lane, p.k_scale + from, row[0] >= 0);
-                cp_async4(s_to + 4 * (lane + N), p.v_scale + from, row[0] >= 0);
-            }
-            return got & (N == 32 ? 0xffffffffu : (1u << (N & 31)) - 1);
+            cp_async4(s_to + 4 * lane, scales + (row >= 0 ? row : 0), row >= 0);
+            return got & ALL;
         }
     }
 };
 
 // ---------------------------------------------------------------------------------------------------------------- few queries
 // All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
-// with a ring of its own, and are joined at the end.  Slices are equally long for every request; how many of them a request has follows
-// from its length on the device, so the same launch serves a captured step whatever the lengths become.
-#ifndef Q8_KG
-#define Q8_KG 1
-#endif
-#ifndef Q8_STAGES
-#define Q8_STAGES 2
-#endif
-template <int NB> constexpr int FEW_KG = NB * HD <= 128 ? Q8_KG : 1;
-constexpr int STAGES = Q8_STAGES;
-template <int NB> constexpr int SMEM_RING = WARPS * STAGES * STAGE<FEW_KG<NB>>;
+// with a ring of its own, and are joined at the end.  How many slices a request has follows from its length on the device, so the same launch
+// serves a captured step whatever the lengths become.
+// (Two stages: other blocks' warps hide what a longer ring would, and there are more of them.  64 requests at 2,048 keys 48 us, with three
+// stages 50, with four 68.)
+constexpr int STAGES = 2;
+constexpr int SMEM_RING = WARPS * STAGES * STAGE;
 constexpr int JOIN_LD = HD + 8;
 constexpr int SMEM_JOIN = (2 * WARPS * 16 + WARPS * 16 * JOIN_LD + 2 * 16) * 4;
-template <int NB> constexpr int SMEM_FEW = SMEM_RING<NB> > SMEM_JOIN ? SMEM_RING<NB> : SMEM_JOIN;
+constexpr int SMEM_FEW = SMEM_RING > SMEM_JOIN ? SMEM_RING : SMEM_JOIN;
 // blocks an SM runs at once: by shared memory, and by registers (about 60 beside the queries and outputs)
-template <int NB> constexpr int BY_SMEM = (227 * 1024) / (SMEM_FEW<NB> + 1024);
+constexpr int BY_SMEM = (227 * 1024) / (SMEM_FEW + 1024);
 template <int NB> constexpr int BY_REGS = 512 / (((60 + NB * CHUNKS * 6) + 7) / 8 * 8);
-template <int NB> constexpr int FEW_BLOCKS = BY_SMEM<NB> < BY_REGS<NB> ? (BY_SMEM<NB> > 0 ? BY_SMEM<NB> : 1) : (BY_REGS<NB> > 0 ? BY_REGS<NB> : 1);
+template <int NB> constexpr int FEW_BLOCKS = BY_SMEM < BY_REGS<NB> ? (BY_SMEM > 0 ? BY_SMEM : 1) : (BY_REGS<NB> > 0 ? BY_REGS<NB> : 1);
 
 constexpr int MOST_CLUSTER = 8;
 __device__ __forceinline__ void cluster_sync() {
@@ -418,13 +384,57 @@ template <typename T> __device__ __forceinline__ T read_block(uint32_t at, int r
     return v;
 }
 
+// Where only the device knows the lengths of a step (it was captured), `slices` blocks a kv head are dealt out by it: slices of one length for
+// all requests, the shortest of which there are not too many.  item: of which request a slice is, which one, how many the request has and where
+// they begin (x -1: there are fewer slices); first: where a request's slices begin, and how many.  One warp, 32 requests at a time.
+struct Dealt { int4* item; int2* first; };
+__host__ __device__ __forceinline__ Dealt dealt_at(int* at, int slices) { return {(int4*)at, (int2*)(at + 4 * (size_t)slices)}; }
+__global__ void __launch_bounds__(32)
+deal_kernel(Params p) {
+    BW_PDL_TRIGGER();
+    const int lane = threadIdx.x;
+    const Dealt to = dealt_at(p.dealt, p.slices);
+    BW_PDL_WAIT();
+    auto tiles_of = [&](int r) {
+        if (r >= p.requests) return 0;
+        const int n_tok = p.cu_q[r + 1] - p.cu_q[r], pos = p.q_start[r];
+        if (n_tok <= 0 || n_tok * p.G > 16) return 0;
+        // (one that is longer than was planned for gets longer slices, not more)
+        return min((pos + n_tok - 1) / TILE + 1 - bw::first_visible(pos, p.window, p.chunk) / TILE, p.shared);
+    };
+    const int mine = tiles_of(lane);
+    int all = mine;
+    for (int r = lane + 32; r < p.requests; r += 32) all += tiles_of(r);
+    all = __reduce_add_sync(0xffffffffu, all);
+    // between the length that fills all slices and the one with which one slice more a request fits, too (the host: slices > requests)
+    int per = max((all - 1) / p.slices + 1, 1);
+    for (int hi = max((all - 1) / (p.slices - p.requests) + 1, 1); per < hi;) {
+        const int mid = (per + hi) >> 1;
+        int n = (mine + mid - 1) / mid;
+        for (int r = lane + 32; r < p.requests; r += 32) n += (tiles_of(r) + mid - 1) / mid;
+        if (__reduce_add_sync(0xffffffffu, n) <= p.slices) hi = mid; else per = mid + 1;
+    }
+    int before = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += 32) {
+        const int n = ((r0 ? tiles_of(r0 + lane) : mine) + per - 1) / per;
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += x; }
+        const int at = before + upto - n;
+        if (r0 + lane < p.requests) to.first[r0 + lane] = make_int2(at, n);
+        for (int i = 0; i < n; ++i) to.item[at + i] = make_int4(r0 + lane, i, n, at);
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    for (int i = before + lane; i < p.slices; i += 32) to.item[i] = make_int4(-1, 0, 1, 0);
+}
+
 struct Walk { int first, tiles, per, live; };   // in tiles of TILE keys: where it begins, how many, of a slice; slices that have any
-__device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last) {
+__device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last, int of) {
     Walk w;
     w.first = bw::first_visible(q_pos0, p.window, p.chunk) / TILE;
     w.tiles = last / TILE + 1 - w.first;
     // (a request that is longer than the plan was made for gets longer slices, not more of them)
-    w.per = max(p.per, (w.tiles + p.slices - 1) / p.slices);
+    w.per = max(p.cluster || p.shared ? 1 : p.per, (w.tiles + of - 1) / of);
     w.live = (w.tiles + w.per - 1) / w.per;
     return w;
 }
@@ -443,48 +453,49 @@ __global__ void __launch_bounds__(THREADS, FEW_BLOCKS<NB>)
 few_kernel(Params p) {
     BW_PDL_TRIGGER();
     extern __shared__ __align__(16) uint8_t smem[];
-    const int slice = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+    const int g = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     BW_PDL_WAIT();
+    const int4 item = p.shared ? dealt_at(p.dealt, p.slices).item[blockIdx.x] : make_int4(blockIdx.z, blockIdx.x, p.slices, 0);
+    const int r = item.x, slice = item.y;
+    if (r < 0) return;
     const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
     if (n_tok <= 0 || n_rows > 8 * NB || (NB == 2 && n_rows <= 8)) return;
     const int q_pos0 = p.q_start[r], last = q_pos0 + n_tok - 1, kv_len = p.kv_len[r];
-    const Walk walk = walk_of(p, q_pos0, last);
+    const Walk walk = walk_of(p, q_pos0, last, item.z);
     if (slice >= walk.live) return;        // (a cluster's barrier waits for no block that has left)
     const int t0 = walk.first + slice * walk.per, t1 = min(walk.first + walk.tiles, t0 + walk.per);
     const int* bt = p.table + (size_t)r * p.max_blocks;
-    constexpr int KG = FEW_KG<NB>, N = KG * KEYS;      // keys of a warp's step
-    constexpr unsigned ALL = N == 32 ? 0xffffffffu : (1u << (N & 31)) - 1;
-    uint8_t* ring = smem + warp * STAGES * STAGE<KG>;
-    // a warp's steps: every fourth N keys of the slice
-    const int first = t0 * TILE + warp * N, end = min(t1 * TILE, last + 1);
-    Feed<KG, WHOLE> next;
+    uint8_t* ring = smem + warp * STAGES * STAGE;
+    // a warp's steps: every fourth sixteen keys of the slice
+    const int first = t0 * TILE + warp * KEYS, end = min(t1 * TILE, last + 1);
+    Feed<WHOLE> next;
     next.find(p, bt, g, first, end, kv_len);
     unsigned there[STAGES];
     auto feed = [&](int key0, int st) {
         if (key0 < end) {
-            there[st] = next.fetch(p, ring + st * STAGE<KG>);
-            next.find(p, bt, g, key0 + WARPS * N, end, kv_len);
+            there[st] = next.fetch(p, ring + st * STAGE);
+            next.find(p, bt, g, key0 + WARPS * KEYS, end, kv_len);
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) feed(first + st * WARPS * N, st);
+    for (int st = 0; st < STAGES - 1; ++st) feed(first + st * WARPS * KEYS, st);
     Queries<NB> s;
     load_queries<NB>(p, s, tok, g, 0, n_rows, q_pos0);
     const int see_all = bw::first_visible(last, p.window, p.chunk);      // from here on every query of the segment sees keys up to q_pos0
-    for (int base = first; base < end; base += STAGES * WARPS * N) {
+    for (int base = first; base < end; base += STAGES * WARPS * KEYS) {
 #pragma unroll
         for (int st = 0; st < STAGES; ++st) {
-            const int key0 = base + st * WARPS * N;
+            const int key0 = base + st * WARPS * KEYS;
             if (key0 >= end) break;
             cp_async_wait<STAGES - 2>();
             __syncwarp();
-            feed(key0 + (STAGES - 1) * WARPS * N, (st + STAGES - 1) % STAGES);
-            const uint32_t at = smem_u32(ring + st * STAGE<KG>);
-            const float* sc = reinterpret_cast<const float*>(ring + st * STAGE<KG> + 2 * N * STRIDE);
-            const bool need_mask = there[st] != ALL || key0 + N - 1 > q_pos0 || key0 < see_all;
-            some_keys<NB, KG>(s, at, at + N * STRIDE, sc, sc + N, key0, there[st], need_mask);
+            feed(key0 + (STAGES - 1) * WARPS * KEYS, (st + STAGES - 1) % STAGES);
+            const uint32_t at = smem_u32(ring + st * STAGE);
+            const float* sc = reinterpret_cast<const float*>(ring + st * STAGE + 2 * KEYS * STRIDE);
+            const bool need_mask = there[st] != ALL || key0 + KEYS - 1 > q_pos0 || key0 < see_all;
+            some_keys<NB>(s, at, at + KEYS * STRIDE, sc, sc + KEYS, key0, there[st], need_mask);
             __syncwarp();
         }
     }
@@ -532,7 +543,7 @@ few_kernel(Params p) {
             *reinterpret_cast<float4*>(os + row * JOIN_LD + c) = acc;
             if (c == 0) { ml[2 * row] = M; ml[2 * row + 1] = L; }
         } else {
-            const size_t at = (((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
+            const size_t at = (p.shared ? (size_t)blockIdx.x * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
             *reinterpret_cast<float4*>(p.part_o + at * HD + c) = acc;
             if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
         }
@@ -580,15 +591,18 @@ join_kernel(Params p) {
     const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
     if (n_tok <= 0 || n_rows > 16 || row >= n_rows) return;
     const int q_pos0 = p.q_start[r];
-    const int live = walk_of(p, q_pos0, q_pos0 + n_tok - 1).live;
+    const int2 mine = p.shared ? dealt_at(p.dealt, p.slices).first[r] : make_int2(0, p.slices);
+    const int live = walk_of(p, q_pos0, q_pos0 + n_tok - 1, mine.y).live;
     if (live <= 1) return;
     __shared__ float4 red[JOIN_GROUPS][QUADS];
     __shared__ float red_l[JOIN_GROUPS];
     __shared__ float scratch[32];
-    const size_t base = ((size_t)r * p.nkv + g) * p.slices * 16 + row;
+    // from one slice's row to the next one's
+    const size_t step = p.shared ? (size_t)p.nkv * 16 : 16;
+    const size_t base = (p.shared ? (size_t)mine.x * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices) * 16 + row;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
     float M = -INFINITY;
-    for (int i = threadIdx.x; i < live; i += 256) M = fmaxf(M, ml[base + (size_t)i * 16].x);
+    for (int i = threadIdx.x; i < live; i += 256) M = fmaxf(M, ml[base + i * step].x);
     M = bw::block_max(M, scratch);
     const int group = threadIdx.x / QUADS, quad = threadIdx.x - group * QUADS;
     if (group < JOIN_GROUPS) {
@@ -596,8 +610,8 @@ join_kernel(Params p) {
         float L = 0.f;
 #pragma unroll 4
         for (int i = group; i < live; i += JOIN_GROUPS) {
-            const float2 x = ml[base + (size_t)i * 16];
-            const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + (size_t)i * 16) * HD)[quad];
+            const float2 x = ml[base + i * step];
+            const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + i * step) * HD)[quad];
             const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
             L += x.y * f;
@@ -627,13 +641,13 @@ struct Portions { int n; int request[MANY]; int first[MANY + 1]; };   // first: 
 constexpr int ROWS = 16 * WARPS;
 constexpr int RING = 2;
 constexpr int MANY_TILE = WARPS * KEYS;                    // keys of a block's step
-constexpr int SMEM_MANY = RING * WARPS * STAGE<1> + 64;
+constexpr int SMEM_MANY = RING * WARPS * STAGE + 64;
 
 __global__ void __launch_bounds__(THREADS)
 many_kernel(Params p, Portions work) {
     BW_PDL_TRIGGER();
     extern __shared__ __align__(16) uint8_t smem[];
-    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE<1>);
+    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.x;
     int i = 0;
     while (i + 1 < work.n && (int)blockIdx.y >= work.first[i + 1]) ++i;
@@ -651,9 +665,9 @@ many_kernel(Params p, Portions work) {
     auto feed = [&](int t) {
         if (t < t1) {
             const int st = (t - t0) % RING;
-            Feed<1, false> f;
+            Feed<false> f;
             f.find(p, bt, g, t * MANY_TILE + warp * KEYS, kv_len, kv_len);
-            const unsigned b = f.fetch(p, smem + (st * WARPS + warp) * STAGE<1>);
+            const unsigned b = f.fetch(p, smem + (st * WARPS + warp) * STAGE);
             if (lane == 0) there[st * WARPS + warp] = b;
         }
         cp_async_commit();
@@ -672,11 +686,11 @@ many_kernel(Params p, Portions work) {
             for (int w = 0; w < WARPS; ++w) {
                 const int key0 = t * MANY_TILE + w * KEYS;
                 if (key0 > my_last) break;
-                const uint8_t* at = smem + (st * WARPS + w) * STAGE<1>;
+                const uint8_t* at = smem + (st * WARPS + w) * STAGE;
                 const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
                 const unsigned ok = there[st * WARPS + w];
-                const bool need_mask = ok != 0xffffu || key0 + KEYS - 1 > my_first || key0 < see_all;
-                some_keys<2, 1>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask);
+                const bool need_mask = ok != ALL || key0 + KEYS - 1 > my_first || key0 < see_all;
+                some_keys<2>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask);
             }
         }
         __syncthreads();
@@ -711,13 +725,13 @@ static int clusters_at_once(int size) {
     int& n = known[bw::current_device()][size];
     if (n == 0) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)size); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW<NB>;
+        cfg.gridDim = dim3((unsigned)size); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned)size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr; cfg.numAttrs = 1;
         int got = 0;
-        if (cudaFuncSetAttribute(few_kernel<NB, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_FEW<NB>) != cudaSuccess ||
+        if (cudaFuncSetAttribute(few_kernel<NB, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_FEW) != cudaSuccess ||
             cudaOccupancyMaxActiveClusters(&got, few_kernel<NB, WHOLE>, &cfg) != cudaSuccess) { cudaGetLastError(); got = 0; }
         n = got + 1;
     }
@@ -731,8 +745,9 @@ static int clusters_at_once(int size) {
 // and a trip through memory: about two tiles' time) serves more slices, and requests of many lengths, whose clusters would be half empty:
 // us with clusters and without, a token at 701 keys 6.2 and 7.6, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
 // them 63.5 and 55.8, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 11.8.
+// A step whose lengths only the device will know, and may be long, gets the slices that run at once, to share by what the lengths are then.
 constexpr int CLUSTER_EXTRA = 2;
-struct Plan { int per, slices, cluster; };
+struct Plan { int per, slices, cluster, shared; };
 static Plan plan_slices(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound, bool whole) {
     auto tiles_of = [&](int r) -> long long {
         if (q_len[r] <= 0 || (long long)q_len[r] * G > 16) return 0;
@@ -757,7 +772,7 @@ static Plan plan_slices(const int* q_len, const int* q_start, int requests, int 
         if (n > most) most = n;
         if (n < least) least = n;
     }
-    if (most == 0) return {1, 0, 0};
+    if (most == 0) return {1, 0, 0, 0};
     const long long room = (long long)(wide ? FEW_BLOCKS<2> : FEW_BLOCKS<1>) * bw::num_sms();          // blocks that run at once
     long long lo = 1, hi = most;
     while (lo < hi) {
@@ -767,24 +782,26 @@ static Plan plan_slices(const int* q_len, const int* q_start, int requests, int 
         if (blocks * nkv <= room) hi = mid; else lo = mid + 1;
     }
     const long long slices = (most + lo - 1) / lo;
-    if (slices > 1 && 4 * least >= 3 * most) {
+    if (slices > 1 && 4 * least >= 3 * most && (bound <= 0 || few == 1 || most <= MOST_CLUSTER)) {
         for (int size = slices < MOST_CLUSTER ? (int)slices : MOST_CLUSTER; size > 1; --size) {
             const long long per = (most + size - 1) / size;
             if (per > lo + CLUSTER_EXTRA) break;
             const int at_once = wide ? (whole ? clusters_at_once<2, true>(size) : clusters_at_once<2, false>(size))
                                      : (whole ? clusters_at_once<1, true>(size) : clusters_at_once<1, false>(size));
-            if (few * nkv <= at_once) return {(int)per, (int)((most + per - 1) / per), 1};
+            if (few * nkv <= at_once) return {(int)per, (int)((most + per - 1) / per), 1, 0};
         }
     }
-    return {(int)lo, (int)slices, 0};
+    if (bound > 0 && slices > 1 && room / nkv > requests && most * requests <= 0x7fffffffll)
+        return {1, (int)(room / nkv), 0, requests > 1 ? (int)most : 0};
+    return {(int)lo, (int)slices, 0, 0};
 }
 
 template <int NB, bool WHOLE>
 static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
     static bool done[bw::MAX_DEVICES];
-    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<NB, WHOLE>, SMEM_FEW<NB>, done); e != cudaSuccess) return (int)e;
+    if (cudaError_t e = bw::allow_dynamic_smem(few_kernel<NB, WHOLE>, SMEM_FEW, done); e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW<NB>; cfg.stream = s;
+    cfg.gridDim = grid; cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_FEW; cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int n = 0;
     if (p.cluster) {
@@ -803,26 +820,50 @@ static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
     return 0;
 }
 
+static void deal(const Params& p, cudaStream_t s) { bw::launch(deal_kernel, dim3(1), dim3(32), 0, s, p); }
+
+// For a step that is captured: which slice is whose, for any number of bw_attention_q8 calls on the same lengths, in *need ints of `dealt`.  With
+// none given (null) *need is set alone (0: the step needs none); it depends on what lies on the host only.
+BW_EXPORT int bw_attention_q8_deal(const int* cu_q, const int* q_start, const int* h_q_len, const int* h_q_start, int requests, int nh, int nkv,
+                                   int page_size, int window, int chunk, int bound, int* dealt, long long* need, void* stream) {
+    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0) return BW_ERR_BAD_ARG;
+    window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
+    const Plan plan = plan_slices(h_q_len, h_q_start, requests, nh / nkv, nkv, window, chunk, bound, page_size % KEYS == 0);
+    *need = plan.shared ? 4ll * plan.slices + 2ll * requests : 0;
+    if (!dealt || !plan.shared) return 0;
+    if ((uintptr_t)dealt & 15) return BW_ERR_BAD_ARG;
+    Params p{};
+    p.cu_q = cu_q; p.q_start = q_start; p.window = window; p.chunk = chunk; p.requests = requests; p.G = nh / nkv;
+    p.slices = plan.slices; p.shared = plan.shared; p.dealt = dealt;
+    deal(p, (cudaStream_t)stream);
+    BW_LAUNCH_CHECK();
+    return 0;
+}
+
 // q, out: bfloat16 [tokens][nh][HD]; h_q_len, h_q_start: lengths on the host; bound: see plan_slices.  few_only: requests with more than 16 rows
 // are left out.  room: where the joining needs memory, for *need floats; with none given (null), or too little (room_floats), *need is set, the call
-// returns BW_ERR_ROOM and has launched nothing.
+// returns BW_ERR_ROOM and has launched nothing.  dealt: what bw_attention_q8_deal left for these lengths, or null (then it is done here).
 #define BW_ERR_ROOM (-11)
 BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
                               const int* cu_q, const int* q_start, const int* kv_len, const int* table, int max_blocks, const int* h_q_len,
                               const int* h_q_start, int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, int bound,
-                              float scale, const float* sink, float* room, long long room_floats, long long* need, int few_only, void* stream) {
+                              float scale, const float* sink, float* room, long long room_floats, long long* need, int few_only, int* dealt,
+                              void* stream) {
     if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0) return BW_ERR_BAD_ARG;
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room) & 15) return BW_ERR_BAD_ARG;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room | (uintptr_t)dealt) & 15) return BW_ERR_BAD_ARG;
     if ((long long)num_pages * nkv * page_size > 0x7fffffffll || nkv > 65535 || requests > 65535) return BW_ERR_UNSUPPORTED;
     const int G = nh / nkv;
     window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
     const bool whole = page_size % KEYS == 0;
     const Plan plan = plan_slices(h_q_len, h_q_start, requests, G, nkv, window, chunk, bound, whole);
-    const long long rows = plan.slices > 1 && !plan.cluster ? (long long)requests * nkv * plan.slices * 16 : 0;
-    if (rows * (HD + 2) > room_floats) { *need = rows * (HD + 2); return BW_ERR_ROOM; }
+    const long long rows = plan.slices > 1 && !plan.cluster ? (long long)(plan.shared ? 1 : requests) * nkv * plan.slices * 16 : 0;
+    const long long wanted = rows * (HD + 2) + (plan.shared && !dealt ? 4ll * plan.slices + 2ll * requests : 0);
+    if (wanted > room_floats) { *need = wanted; return BW_ERR_ROOM; }
+    const bool deal_here = plan.shared && !dealt;
+    if (deal_here) dealt = reinterpret_cast<int*>(room + rows * (HD + 2));       // (rows is a multiple of 16)
     const int slices = plan.slices;
     Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, room, room + rows * HD,
-             max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, scale * LOG2E};
+             max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, plan.shared, dealt, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
     static bool many_done[bw::MAX_DEVICES];
     if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
@@ -854,7 +895,11 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (const int e = flush()) return e;
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
-    const dim3 grid((unsigned)slices, (unsigned)nkv, (unsigned)requests);
+    const dim3 grid((unsigned)slices, (unsigned)nkv, plan.shared ? 1u : (unsigned)requests);
+    if (deal_here) {
+        deal(p, s);
+        BW_LAUNCH_CHECK();
+    }
     if (few1) if (const int e = whole ? launch_few<1, true>(p, grid, s) : launch_few<1, false>(p, grid, s)) return e;
     if (few2) if (const int e = whole ? launch_few<2, true>(p, grid, s) : launch_few<2, false>(p, grid, s)) return e;
     if (slices > 1 && !plan.cluster) {

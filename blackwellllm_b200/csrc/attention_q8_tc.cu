@@ -646,15 +646,11 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
         make_uint2(bw::pack_bf16x2(acc.x * inv, acc.y * inv), bw::pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
-// Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining.
-#ifndef Q8_ITEM_COST
-#define Q8_ITEM_COST 5
-#endif
-#ifndef Q8_LEAST
-#define Q8_LEAST 4
-#endif
-constexpr int LEAST_STEPS = Q8_LEAST;
-constexpr int ITEM_COST = Q8_ITEM_COST;         // what an item costs beside its steps (its queries, the first scores, its outputs), in steps
+// Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining (100
+// tokens alone 21 us; with eight steps at least, and so fewer blocks, 28; two steps make no difference).
+constexpr int LEAST_STEPS = 4;
+// what an item costs beside its steps (its queries, the first scores, its outputs), in steps: 2,048 tokens 74 us counted as five, 76 as four, 77 as eight
+constexpr int ITEM_COST = 5;
 int blocks_for(long long cost) {
     const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;
     const long long n = (cost + LEAST_STEPS + ITEM_COST - 1) / (LEAST_STEPS + ITEM_COST);

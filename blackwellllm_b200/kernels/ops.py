@@ -1548,16 +1548,56 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
 
 
 _ATTN_Q8_ARGS = ([c_void_p] * 10 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, ctypes.POINTER(c_ll), c_int,
-                                                                            c_void_p])
+                                                                            c_void_p, c_void_p])
+_ATTN_Q8_DEAL_ARGS = [c_void_p] * 4 + [c_int] * 7 + [c_void_p, ctypes.POINTER(c_ll), c_void_p]
 _ATTN_Q8_TC_ARGS = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, c_void_p]
 QUANT_FEW_ROWS = 16     # up to so many stacked rows (tokens times heads of a group) a request is the key-slice kernel's
 
 
+class QuantDealt(NamedTuple):
+    """How :func:`quant_attention` divides the keys of a captured step among blocks; see :func:`quant_attention_deal`."""
+    key: tuple
+    ints: torch.Tensor
+
+
+def _dealt_key(batch, nh, nkv, hd, page_size, window, chunk):
+    return (batch.cu_q.data_ptr(), batch.q_start.data_ptr(), tuple(batch.h_q_len[:batch.R]), batch.static_bound, nh, nkv, hd, page_size, window, chunk)
+
+
+def quant_attention_deal(batch, nh: int, nkv: int, head_dim: int, page_size: int, window: Optional[int] = None,
+                         chunk: Optional[int] = None) -> Optional[QuantDealt]:
+    """For the layers of a step with ``static_bound``, whose lengths only the device will know: divides the keys once, by the lengths of
+    ``batch.q_start`` at that point of the stream, for every :func:`quant_attention` call of the step with these sizes (which else does it for
+    itself).  None where a step needs no such division."""
+    check_quant_supported(head_dim, nh // nkv)
+    if not batch.static_bound or batch.T == 0:
+        return None
+    for t, name in ((batch.cu_q, "cu_q"), (batch.q_start, "q_start")):
+        _dev(t, name, torch.int32)
+    R, window, chunk = batch.R, int(window or 0), int(chunk or 0)
+    if nh % nkv or len(batch.h_q_len) < R or len(batch.h_q_start) < R or batch.cu_q.numel() < R + 1 or batch.q_start.numel() < R:
+        raise KernelError("quant_attention_deal: the batch's segments and the heads do not fit together")
+    _same_device("quant_attention_deal", batch.cu_q, batch.q_start)
+    ints = c_int * R
+    h_len, h_start = ints(*batch.h_q_len[:R]), ints(*batch.h_q_start[:R])
+    fn = _fn("attention_q8", "bw_attention_q8_deal", _ATTN_Q8_DEAL_ARGS, macros=attention_q8_macros(head_dim))
+    need, at = c_ll(0), None
+    for _ in range(2):      # how much it is, then the work
+        _check(fn(_ptr(batch.cu_q), _ptr(batch.q_start), h_len, h_start, R, nh, nkv, page_size, window, chunk, int(batch.static_bound),
+                  _ptr(at), ctypes.byref(need), _stream()), "quant_attention_deal")
+        if not need.value:
+            return None
+        if at is None:
+            at = torch.empty(need.value, dtype=torch.int32, device=batch.cu_q.device)
+    return QuantDealt(_dealt_key(batch, nh, nkv, head_dim, page_size, window, chunk), at)
+
+
 def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torch.Tensor, nh: int, scale: float, window: Optional[int] = None,
-                    chunk: Optional[int] = None, sink: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    chunk: Optional[int] = None, sink: Optional[torch.Tensor] = None, dealt: Optional[QuantDealt] = None) -> torch.Tensor:
     """:func:`paged_attention` over an 8-bit cache (which already holds this step's keys and values): bfloat16 queries [T, nh * head_dim],
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
-    held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator."""
+    held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator.  ``dealt``: what
+    :func:`quant_attention_deal` made of the step."""
     here = torch._C._cuda_getDevice()
     num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_attention")
     _dev(q, "q", torch.bfloat16)
@@ -1582,6 +1622,8 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     window, chunk = int(window or 0), int(chunk or 0)
     ints = c_int * R
     h_len, h_start = ints(*lens), ints(*starts[:R])
+    if dealt is not None and dealt.key != _dealt_key(batch, nh, nkv, hd, page_size, window, chunk):
+        raise KernelError("quant_attention: `dealt` was made for another step or other sizes")
     macros = attention_q8_macros(hd)
     if hd % 64 == 0 and scale > 0 and max(lens) * G > QUANT_FEW_ROWS:
         # portions of prompts: the tcgen05 kernel, where it is built for the head size (else the mma.sync kernel below takes them)
@@ -1607,10 +1649,11 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     while True:
         code = fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start), _ptr(kv_len),
                   _ptr(block_table), block_table.shape[1], h_len, h_start, R, nh, nkv, page_size, num_pages, window, chunk,
-                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need), few, _stream())
+                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need), few,
+                  None if dealt is None else dealt.ints.data_ptr(), _stream())
         if code != _ERR_ROOM or room is not None:
             break
-        floats = need.value             # many slices of few requests join through memory
+        floats = need.value             # many slices of few requests join through memory; a captured step's are divided there
         room = torch.empty(floats, dtype=torch.float32, device=q.device)
     _check(code, "quant_attention")
     return out

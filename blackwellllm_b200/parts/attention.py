@@ -316,8 +316,14 @@ class GQAAttention(Mixer):
 
     def _attend(self, q, qkv, x, batch, cache):
         if cache.quant is not None:
+            dealt = None
+            if batch.static_bound:   # a step whose lengths only the device knows: its keys are divided once, for all layers of these sizes
+                key = ("quant_dealt", self.nh, self.nkv, self.dpad, cache.page_size, self.window, self.chunk)
+                if key not in batch.extras:
+                    batch.extras[key] = ops.quant_attention_deal(batch, self.nh, self.nkv, self.dpad, cache.page_size, self.window, self.chunk)
+                dealt = batch.extras[key]
             return ops.quant_attention(q, cache.quant, batch, batch.block_tables[cache.group], self.nh, self.scale, self.window, self.chunk,
-                                       self.sink)
+                                       self.sink, dealt)
         gate = None
         if self.gated:   # the attention kernels multiply by the gate's sigmoid as they write a row
             if self.gate_per_head:

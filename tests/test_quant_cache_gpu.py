@@ -289,6 +289,62 @@ def test_attention_in_a_graph_of_any_length():
         assert ((out.cpu().double().view_as(e.out) - e.out).abs() <= attention_bound(e, 128)).all()
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("count,nkv,group,window,bound", [(70, 1, 4, 0, 2048), (33, 2, 6, 300, 2048), (9, 2, 16, 0, 2048), (40, 1, 8, 0, 256)])
+def test_attention_in_a_graph_of_many_lengths(count, nkv, group, window, bound, shared):
+    """A captured step deals its blocks out by the lengths of the replay: many requests, one or two tokens or none each, short and long ones
+    (longer than the bound, too: such a request gets longer slices)."""
+    longest = 1500
+    g = torch.Generator().manual_seed(count)
+    lens = torch.randint(0, 3 if 2 * group <= 16 else 2, (count,), generator=g)
+    lens[:3] = 1
+    c = Case([(int(n), longest - int(n), longest) for n in lens], nkv, 64, 16, seed=count).fill()
+    b, pages, nh = c.batch(bound), c.pages(), nkv * group
+    q = torch.zeros(c.T, nh * 64, dtype=torch.bfloat16, device="cuda")
+    ops.quant_attention(q, pages, b, b.block_tables[0], nh, 0.125, window or None)
+    ops.quant_attention_deal(b, nh, nkv, 64, 16, window or None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dealt = ops.quant_attention_deal(b, nh, nkv, 64, 16, window or None) if shared else None
+        out, again = (ops.quant_attention(q, pages, b, b.block_tables[0], nh, 0.125, window or None, dealt=dealt) for _ in range(2))
+    for step in range(4):
+        ends = torch.randint(2, 60, (count,), generator=g)
+        if step == 1:
+            ends[1], ends[-1] = longest, 1100
+        elif step == 2:
+            ends[:] = 900
+        elif step == 3:
+            ends[:] = 2
+        starts = ends - lens
+        b.q_start.copy_(starts); b.kv_len.copy_(ends)
+        fresh = torch.randn(c.T, nh * 64, generator=c.gen).to(torch.bfloat16)
+        q.copy_(fresh)
+        out.fill_(float("nan")); again.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, again)
+        e = attention(fresh.view(-1, nh, 64), c.k, c.v, c.k_scale, c.v_scale, c.cu, starts.tolist(), ends.tolist(), c.table, 0.125, window)
+        assert ((out.cpu().double().view_as(e.out) - e.out).abs() <= attention_bound(e, 64)).all()
+
+
+def test_a_division_goes_with_its_step():
+    """How keys are divided is not taken from another step or for other sizes; a step whose lengths the host knows has none."""
+    c = Case([(1, 700, 701)] * 3, 2, 64, 16, seed=1).fill()
+    b, other, pages = c.batch(4096), c.batch(4096), c.pages()
+    q = torch.zeros(3, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    assert ops.quant_attention_deal(c.batch(), 8, 2, 64, 16) is None
+    dealt = ops.quant_attention_deal(b, 8, 2, 64, 16)
+    assert dealt is not None
+    ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125, dealt=dealt)
+    for batch, nh, window in ((other, 8, None), (b, 4, None), (b, 8, 128)):
+        with pytest.raises(ops.KernelError, match="another step"):
+            ops.quant_attention(q[:, :nh * 64].contiguous(), pages, batch, batch.block_tables[0], nh, 0.125, window, dealt=dealt)
+    b.h_q_len = [1, 1, 0]
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125, dealt=dealt)
+    with pytest.raises(ops.KernelError):
+        ops.quant_attention_deal(other, 7, 2, 64, 16)
+
+
 def test_refusals():
     c = Case([(1, 3, 4)], 2, 64, 16, seed=1).fill()
     pages, b = c.pages(), c.batch()
