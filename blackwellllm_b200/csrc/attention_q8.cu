@@ -352,7 +352,6 @@ struct Feed {
     }
 };
 
-// ---------------------------------------------------------------------------------------------------------------- few queries
 // All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
 // with a ring of its own, and are joined at the end.  How many slices a request has follows from its length on the device, so the same launch
 // serves a captured step whatever the lengths become.
@@ -633,89 +632,6 @@ join_kernel(Params p) {
     }
 }
 
-// ---------------------------------------------------------------------------------------------------------------- many queries
-// Portions of prompts: 64 rows of one (request, kv head) a block, sixteen a warp; the warps share the keys that the block fetches, 64 at a time
-// in a ring, and walk them up to the causal diagonal.
-constexpr int MANY = 16;                                   // requests with many rows that one launch takes
-struct Portions { int n; int request[MANY]; int first[MANY + 1]; };   // first: the block index of each one's first 64 rows
-constexpr int ROWS = 16 * WARPS;
-constexpr int RING = 2;
-constexpr int MANY_TILE = WARPS * KEYS;                    // keys of a block's step
-constexpr int SMEM_MANY = RING * WARPS * STAGE + 64;
-
-__global__ void __launch_bounds__(THREADS)
-many_kernel(Params p, Portions work) {
-    BW_PDL_TRIGGER();
-    extern __shared__ __align__(16) uint8_t smem[];
-    unsigned* there = reinterpret_cast<unsigned*>(smem + RING * WARPS * STAGE);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.x;
-    int i = 0;
-    while (i + 1 < work.n && (int)blockIdx.y >= work.first[i + 1]) ++i;
-    BW_PDL_WAIT();
-    const int r = work.request[i];
-    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, all_rows = n_tok * p.G;
-    // the latest rows first: they have the most keys
-    const int row0 = (work.first[i + 1] - 1 - (int)blockIdx.y) * ROWS;
-    if (row0 >= all_rows) return;
-    const int q_pos0 = p.q_start[r], kv_len = p.kv_len[r];
-    const int* bt = p.table + (size_t)r * p.max_blocks;
-    const int mine = row0 + 16 * warp, last_row = min(all_rows, row0 + ROWS) - 1;
-    const int first_pos = q_pos0 + row0 / p.G, last_pos = q_pos0 + last_row / p.G;
-    const int t0 = bw::first_visible(first_pos, p.window, p.chunk) / MANY_TILE, t1 = last_pos / MANY_TILE + 1;
-    auto feed = [&](int t) {
-        if (t < t1) {
-            const int st = (t - t0) % RING;
-            Feed<false> f;
-            f.find(p, bt, g, t * MANY_TILE + warp * KEYS, kv_len, kv_len);
-            const unsigned b = f.fetch(p, smem + (st * WARPS + warp) * STAGE);
-            if (lane == 0) there[st * WARPS + warp] = b;
-        }
-        cp_async_commit();
-    };
-    feed(t0);
-    Queries<2> s;
-    load_queries<2>(p, s, tok, g, mine, all_rows, q_pos0);
-    const int my_first = q_pos0 + mine / p.G, my_last = q_pos0 + min(last_row, mine + 15) / p.G;
-    const int see_all = bw::first_visible(my_last, p.window, p.chunk);
-    for (int t = t0; t < t1; ++t) {
-        feed(t + 1);
-        cp_async_wait<1>();
-        __syncthreads();
-        const int st = (t - t0) % RING;
-        if (mine <= last_row) {
-            for (int w = 0; w < WARPS; ++w) {
-                const int key0 = t * MANY_TILE + w * KEYS;
-                if (key0 > my_last) break;
-                const uint8_t* at = smem + (st * WARPS + w) * STAGE;
-                const float* sc = reinterpret_cast<const float*>(at + 2 * KEYS * STRIDE);
-                const unsigned ok = there[st * WARPS + w];
-                const bool need_mask = ok != ALL || key0 + KEYS - 1 > my_first || key0 < see_all;
-                some_keys<2>(s, smem_u32(at), smem_u32(at) + KEYS * STRIDE, sc, sc + KEYS, key0, ok, need_mask);
-            }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float l = s.l[nb][e];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            const int row = mine + 8 * nb + 2 * (lane & 3) + e;
-            if (row > last_row) continue;
-            const int t = row / p.G, head = g * p.G + row - t * p.G;
-            l += sink_term(p, head, s.m[nb][e]);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            bf16* dst = p.out + ((size_t)(tok + t) * p.nh + head) * HD + 2 * (lane >> 2);
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c)
-                *reinterpret_cast<uint32_t*>(dst + 16 * c) = bw::pack_bf16x2(s.o[c][nb][e] * inv, s.o[c][nb][2 + e] * inv);
-        }
-    }
-}
-
 }  // namespace
 
 // Clusters of `size` blocks of the key-slice kernel that run at once on the current device (0: none, or not known), looked up once.
@@ -840,14 +756,14 @@ BW_EXPORT int bw_attention_q8_deal(const int* cu_q, const int* q_start, const in
     return 0;
 }
 
-// q, out: bfloat16 [tokens][nh][HD]; h_q_len, h_q_start: lengths on the host; bound: see plan_slices.  few_only: requests with more than 16 rows
-// are left out.  room: where the joining needs memory, for *need floats; with none given (null), or too little (room_floats), *need is set, the call
+// q, out: bfloat16 [tokens][nh][HD]; h_q_len, h_q_start: lengths on the host; bound: see plan_slices.  Requests with more than 16 rows
+// are left out (attention_q8_tc.cu has them).  room: where the joining needs memory, for *need floats; with none given (null), or too little (room_floats), *need is set, the call
 // returns BW_ERR_ROOM and has launched nothing.  dealt: what bw_attention_q8_deal left for these lengths, or null (then it is done here).
 #define BW_ERR_ROOM (-11)
 BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, void* out,
                               const int* cu_q, const int* q_start, const int* kv_len, const int* table, int max_blocks, const int* h_q_len,
                               const int* h_q_start, int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, int bound,
-                              float scale, const float* sink, float* room, long long room_floats, long long* need, int few_only, int* dealt,
+                              float scale, const float* sink, float* room, long long room_floats, long long* need, int* dealt,
                               void* stream) {
     if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0) return BW_ERR_BAD_ARG;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room | (uintptr_t)dealt) & 15) return BW_ERR_BAD_ARG;
@@ -865,34 +781,14 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, room, room + rows * HD,
              max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, plan.shared, dealt, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
-    static bool many_done[bw::MAX_DEVICES];
-    if (cudaError_t e = bw::allow_dynamic_smem(many_kernel, SMEM_MANY, many_done); e != cudaSuccess) return (int)e;
-    Portions work{};
     int most_rows = 0;
     bool few1 = false, few2 = false;
-    auto flush = [&]() -> int {
-        if (!work.n) return 0;
-        if (work.first[work.n] > 65535) return BW_ERR_UNSUPPORTED;
-        bw::launch(many_kernel, dim3((unsigned)nkv, (unsigned)work.first[work.n]), dim3(THREADS), SMEM_MANY, s, p, work);
-        BW_LAUNCH_CHECK();
-        work = Portions{};
-        return 0;
-    };
     for (int r = 0; r < requests; ++r) {
         const long long rows = (long long)h_q_len[r] * G;
-        if (rows <= 0) continue;
-        if (rows <= 16) {
-            (rows <= 8 ? few1 : few2) = true;
-            if (rows > most_rows) most_rows = (int)rows;
-            continue;
-        }
-        if (few_only) continue;
-        if (rows > 0x7fffffffll / 2) return BW_ERR_UNSUPPORTED;
-        work.request[work.n] = r;
-        work.first[work.n + 1] = work.first[work.n] + (int)((rows + ROWS - 1) / ROWS);
-        if (++work.n == MANY) if (const int e = flush()) return e;
+        if (rows <= 0 || rows > 16) continue;
+        (rows <= 8 ? few1 : few2) = true;
+        if (rows > most_rows) most_rows = (int)rows;
     }
-    if (const int e = flush()) return e;
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
     const dim3 grid((unsigned)slices, (unsigned)nkv, plan.shared ? 1u : (unsigned)requests);

@@ -1,5 +1,5 @@
 // Attention over the 8-bit cache for portions of prompts, on the 5th-generation tensor cores (head size HEAD_DIM: a compile-time multiple
-// of 64 up to 256; what attention_q8.cu says of the formula holds here).
+// of 16 up to 256; what attention_q8.cu says of the formula holds here).
 //
 // A block works on 256 stacked rows (row = token * G + head of the group) of one (request, kv head) as two tiles of 128 (one, of head sizes
 // above 128: tensor memory holds no more) against tiles of 64 keys:
@@ -24,7 +24,7 @@
 #include <cuda_fp16.h>
 
 #ifndef HEAD_DIM
-#error "compile with -DHEAD_DIM=<multiple of 64>"
+#error "compile with -DHEAD_DIM=<multiple of 16>"
 #endif
 
 using bf16 = __nv_bfloat16;
@@ -32,8 +32,11 @@ using bf16 = __nv_bfloat16;
 namespace {
 
 constexpr int HD = HEAD_DIM;
-static_assert(HD % 64 == 0 && HD >= 64 && HD <= 256, "head size must be a multiple of 64 in [64, 256]");
-constexpr int NS = HD / 64;                 // 128-byte slices of a widened row
+static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16 in [16, 256]");
+constexpr int CHUNKS = HD / 16;             // 16-byte units of a row of the cache
+constexpr int NS = (HD + 63) / 64;          // 128-byte slices of a widened row, of which the last may be filled in part (no product reads the rest)
+constexpr int O_COLS = NS * 64;             // columns of tensor memory between the tiles' outputs
+constexpr int O_STEP = HD % 32 ? 16 : 32;   // columns of outputs that a thread reads at a time
 constexpr int BM = 128, BN = 64;
 constexpr int NQ = HD <= 128 ? 2 : 1;       // tiles of rows a block
 constexpr int ROWS = NQ * BM;
@@ -171,6 +174,12 @@ __device__ __forceinline__ float power_above(unsigned bits) {
     return __uint_as_float(max(up, 27u << 23));
 }
 
+template <int N>
+__device__ __forceinline__ void outputs_at(uint32_t at, uint32_t (&o)[N]) {
+    if constexpr (N == 32) bw::tmem_ld_32x32(at, o);
+    else bw::tmem_ld_32x16(at, o);
+}
+
 // What the softmax needs of a tile of keys.
 struct TileInfo { float k_ref, log2_v, inv_v, pad; unsigned there[2]; unsigned pad2[2]; };
 
@@ -207,7 +216,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     bw::tc_fence_after();
     BW_PDL_WAIT();
     const uint32_t tmem_base = *tmem_slot;
-    const uint32_t tmem_O = tmem_base + 128 * NQ;        // S: [tile of rows][buffer] of 64 columns, then O: [tile of rows] of HD
+    const uint32_t tmem_O = tmem_base + 128 * NQ;        // S: [tile of rows][buffer] of 64 columns, then O: [tile of rows] of O_COLS
     auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
     Walk w;
@@ -279,7 +288,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                     if (bw::elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < BN / 16; ++kk)
-                            bw::umma_bf16_ts(tmem0 + 128 * NQ + q * HD, tmem0 + 128 * q + 64 * b + 8 * kk, behind(dvs, kk * (2048 / 16)), IDESC_PV,
+                            bw::umma_bf16_ts(tmem0 + 128 * NQ + q * O_COLS, tmem0 + 128 * q + 64 * b + 8 * kk, behind(dvs, kk * (2048 / 16)), IDESC_PV,
                                              !(begins && kk == 0));
                         bw::umma_commit(pv_done + 8 * (2 * q + b));
                         if (q == tiles_q - 1) bw::umma_commit(v_empty + 8 * s);
@@ -345,7 +354,10 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             uint4 x[2][PER];
             const int8_t* base = from + 16 * (lane & 3);
             const int swap = SWAP && odd ? 1 : 0;            // slice j of this lane is slice j ^ swap of the row
-            auto unit_of = [&](const int8_t* row, int j) { return *reinterpret_cast<const uint4*>(row + 64 * j + (j & 1 ? -64 : 64) * swap); };
+            auto has = [&](int j) { return HD % 64 == 0 || 4 * (j ^ swap) + (lane & 3) < CHUNKS; };
+            auto unit_of = [&](const int8_t* row, int j) {
+                return has(j) ? *reinterpret_cast<const uint4*>(row + 64 * j + (j & 1 ? -64 : 64) * swap) : make_uint4(0, 0, 0, 0);
+            };
             {
                 const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
 #pragma unroll
@@ -405,6 +417,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 // (one piece of code for keys and values: what an SM quarter's warps run over and over has to fit its instruction cache)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
+                    if (!has(j)) continue;
                     const int to = s * KV_BYTES + j * KV_SLICE + (j & 1 ? -KV_SLICE : KV_SLICE) * swap;
                     widen16(first + to, second + to, x[0][j], f[0]);
                     widen16(first + to + 32 * 128, second + to + 32 * 128, x[1][j], f[1]);
@@ -425,7 +438,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         more_registers<SOFTMAX_REGS>();
         const int q = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * HD + lanes;
+        const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * O_COLS + lanes;
         int it = 0, c = 0;              // steps of the walk, and those of them that this tile of rows has
         bool ok = true;
         constexpr int UNITS = HD / 8;   // of 16 bytes: a row of queries or outputs
@@ -574,12 +587,12 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 // (the queries are done with: the warp's outputs take their place, and go out 16 bytes a lane, a row's side by side)
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    uint32_t o[32];
-                    bw::tmem_ld_32x32(tmem_Oq + c0, o);
+                for (int c0 = 0; c0 < HD; c0 += O_STEP) {
+                    uint32_t o[O_STEP];
+                    outputs_at(tmem_Oq + c0, o);
                     bw::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
+                    for (int j = 0; j < O_STEP; j += 8) {
                         auto two = [&](int i) { return bw::pack_bf16x2(__uint_as_float(o[j + i]) * inv, __uint_as_float(o[j + i + 1]) * inv); };
                         *unit_at(lane, (c0 + j) >> 3) = make_uint4(two(0), two(2), two(4), two(6));
                     }
@@ -595,12 +608,12 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 const int r = q * BM + row;
                 float4* dst = reinterpret_cast<float4*>(p.part_o) + slot * (HD / 4) * ROWS + r;
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    uint32_t o[32];
-                    bw::tmem_ld_32x32(tmem_Oq + c0, o);
+                for (int c0 = 0; c0 < HD; c0 += O_STEP) {
+                    uint32_t o[O_STEP];
+                    outputs_at(tmem_Oq + c0, o);
                     bw::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
+                    for (int j = 0; j < O_STEP; j += 4)
                         dst[(size_t)((c0 + j) >> 2) * ROWS] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
                 }
                 reinterpret_cast<float2*>(p.part_ml)[slot * ROWS + r] = make_float2(m, l);

@@ -1547,7 +1547,7 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
     return k, v
 
 
-_ATTN_Q8_ARGS = ([c_void_p] * 10 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, ctypes.POINTER(c_ll), c_int,
+_ATTN_Q8_ARGS = ([c_void_p] * 10 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, ctypes.POINTER(c_ll),
                                                                             c_void_p, c_void_p])
 _ATTN_Q8_DEAL_ARGS = [c_void_p] * 4 + [c_int] * 7 + [c_void_p, ctypes.POINTER(c_ll), c_void_p]
 _ATTN_Q8_TC_ARGS = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, c_void_p]
@@ -1606,6 +1606,8 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     G, R = nh // nkv, batch.R
     if G > MAX_GROUP_BF16:
         check_quant_supported(hd, G)
+    if not scale > 0:
+        raise KernelError(f"quant_attention: scale must be positive, got {scale}")
     _check_sink(sink, nh)
     cu_q, q_start, kv_len, lens, starts = batch.cu_q, batch.q_start, batch.kv_len, batch.h_q_len, batch.h_q_start
     for t, name in ((cu_q, "cu_q"), (q_start, "q_start"), (kv_len, "kv_len")):
@@ -1625,8 +1627,7 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     if dealt is not None and dealt.key != _dealt_key(batch, nh, nkv, hd, page_size, window, chunk):
         raise KernelError("quant_attention: `dealt` was made for another step or other sizes")
     macros = attention_q8_macros(hd)
-    if hd % 64 == 0 and scale > 0 and max(lens) * G > QUANT_FEW_ROWS:
-        # portions of prompts: the tcgen05 kernel, where it is built for the head size (else the mma.sync kernel below takes them)
+    if max(lens) * G > QUANT_FEW_ROWS:      # portions of prompts: the tcgen05 kernel
         room_of = load_library("attention_q8_tc", macros).bw_attention_q8_tc_room
         if not room_of.argtypes:
             room_of.argtypes, room_of.restype = [c_void_p, c_void_p] + [c_int] * 6, c_ll
@@ -1640,16 +1641,13 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
                   _ptr(room), floats, _stream()), "quant_attention")
         if min(lens) * G > QUANT_FEW_ROWS:
             return out
-        few = 1
-    else:
-        few = 0
     fn = _fn("attention_q8", "bw_attention_q8", _ATTN_Q8_ARGS, macros=macros)
     need = c_ll(0)
     room, floats = None, 0
     while True:
         code = fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start), _ptr(kv_len),
                   _ptr(block_table), block_table.shape[1], h_len, h_start, R, nh, nkv, page_size, num_pages, window, chunk,
-                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need), few,
+                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need),
                   None if dealt is None else dealt.ints.data_ptr(), _stream())
         if code != _ERR_ROOM or room is not None:
             break

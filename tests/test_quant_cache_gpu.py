@@ -82,7 +82,7 @@ class Case:
                       window, chunk, sink)
         want = e.out
         lens = torch.tensor([n for n, _, _ in self.segments])
-        wide = (lens * (nh // self.nkv) > ops.QUANT_FEW_ROWS)[self.req] & (self.hd % 64 == 0)
+        wide = (lens * (nh // self.nkv) > ops.QUANT_FEW_ROWS)[self.req]
         tol = attention_bound(e, self.hd, wide)
         got = got.cpu().double().view_as(want)
         assert ops.attention_q8_status() == 0
@@ -201,7 +201,7 @@ def test_attention_few_queries(hd, nh, nkv, page):
     Case(segs, nkv, hd, page, seed=hd + nh + page).fill().check_attention(nh)
 
 
-@pytest.mark.parametrize("hd", [128, 64, 80, 256, 192])
+@pytest.mark.parametrize("hd", [128, 64, 80, 256, 192, 16, 48, 96, 144, 208])
 @pytest.mark.parametrize("nh,nkv,page", [(8, 2, 16), (7, 1, 8), (16, 1, 24), (4, 4, 64)])
 def test_attention_portions(hd, nh, nkv, page):
     segs = [(37, 0, 37), (1, 70, 71), (19, 111, 130), (130, 5, 135), (3, 200, 203)]
@@ -343,6 +343,15 @@ def test_a_division_goes_with_its_step():
         ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125, dealt=dealt)
     with pytest.raises(ops.KernelError):
         ops.quant_attention_deal(other, 7, 2, 64, 16)
+
+
+def test_a_scale_that_is_not_positive():
+    c = Case([(1, 3, 4), (20, 0, 20)], 2, 64, 16, seed=1).fill()
+    b, pages = c.batch(), c.pages()
+    q = torch.zeros(21, 4 * 64, dtype=torch.bfloat16, device="cuda")
+    for scale in (0.0, -0.125, math.nan):
+        with pytest.raises(ops.KernelError, match="positive"):
+            ops.quant_attention(q, pages, b, b.block_tables[0], 4, scale)
 
 
 def test_refusals():
