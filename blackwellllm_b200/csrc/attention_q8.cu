@@ -736,13 +736,19 @@ static int launch_few(const Params& p, dim3 grid, cudaStream_t s) {
     return 0;
 }
 
+// Segments as the kernels may take them: positions that stay clear of 2^31 by more than a tile.
+static bool segments_ok(const int* h_q_len, const int* h_q_start, int requests) {
+    for (int r = 0; r < requests; ++r)
+        if (h_q_len[r] < 0 || h_q_start[r] < 0 || (long long)h_q_start[r] + h_q_len[r] > 0x7fffff00ll) return false;
+    return true;
+}
 static void deal(const Params& p, cudaStream_t s) { bw::launch(deal_kernel, dim3(1), dim3(32), 0, s, p); }
 
 // For a step that is captured: which slice is whose, for any number of bw_attention_q8 calls on the same lengths, in *need ints of `dealt`.  With
 // none given (null) *need is set alone (0: the step needs none); it depends on what lies on the host only.
 BW_EXPORT int bw_attention_q8_deal(const int* cu_q, const int* q_start, const int* h_q_len, const int* h_q_start, int requests, int nh, int nkv,
                                    int page_size, int window, int chunk, int bound, int* dealt, long long* need, void* stream) {
-    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0) return BW_ERR_BAD_ARG;
+    if (requests < 0 || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || !segments_ok(h_q_len, h_q_start, requests)) return BW_ERR_BAD_ARG;
     window = window > 0 ? window : 0; chunk = chunk > 0 ? chunk : 0;
     const Plan plan = plan_slices(h_q_len, h_q_start, requests, nh / nkv, nkv, window, chunk, bound, page_size % KEYS == 0);
     *need = plan.shared ? 4ll * plan.slices + 2ll * requests : 0;
@@ -765,7 +771,8 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
                               const int* h_q_start, int requests, int nh, int nkv, int page_size, int num_pages, int window, int chunk, int bound,
                               float scale, const float* sink, float* room, long long room_floats, long long* need, int* dealt,
                               void* stream) {
-    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0) return BW_ERR_BAD_ARG;
+    if (requests < 0 || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0) return BW_ERR_BAD_ARG;
+    if (!segments_ok(h_q_len, h_q_start, requests)) return BW_ERR_BAD_ARG;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room | (uintptr_t)dealt) & 15) return BW_ERR_BAD_ARG;
     if ((long long)num_pages * nkv * page_size > 0x7fffffffll || nkv > 65535 || requests > 65535) return BW_ERR_UNSUPPORTED;
     const int G = nh / nkv;

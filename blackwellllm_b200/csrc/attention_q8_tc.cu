@@ -688,7 +688,8 @@ static int launches(const int* h_q_len, const int* h_q_start, int requests, int 
     };
     for (int r = 0; r < requests; ++r) {
         const int n = h_q_len[r];
-        if (n < 0) return BW_ERR_BAD_ARG;
+        // (positions stay clear of 2^31 by more than a tile)
+        if (n < 0 || h_q_start[r] < 0 || (long long)h_q_start[r] + n > 0x7fffff00ll) return BW_ERR_BAD_ARG;
         const long long rows = (long long)n * G, blocks = (rows + ROWS - 1) / ROWS;
         if (rows > min_rows) {
             if (rows > 0x3fffffffll || items + blocks * nkv > 0x3fffffffll) return BW_ERR_UNSUPPORTED;
@@ -716,7 +717,7 @@ BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, co
                                  const int* kv_len, const int* table, int max_blocks, const int* h_q_len, const int* h_q_start, int requests,
                                  int min_rows, int nh, int nkv, int page_size, int num_pages, int window, int chunk, float scale,
                                  const float* sink, float* room, long long room_floats, void* stream) {
-    if (requests < 0 || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || !room) return BW_ERR_BAD_ARG;
+    if (requests < 0 || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || !room) return BW_ERR_BAD_ARG;
     if (!(scale > 0.f)) return BW_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)room) & 15) return BW_ERR_BAD_ARG;
     if ((long long)num_pages * nkv * page_size > 0x7fffffffll) return BW_ERR_UNSUPPORTED;

@@ -1453,12 +1453,13 @@ def check_quant_supported(head_dim: int, group: int = 1) -> None:
         raise KernelError(f"8-bit cache: {group} query heads per kv head exceed the attention kernels' limit of {MAX_GROUP_BF16}")
 
 
-def _quant_pages(pages: QuantPages, block_table: torch.Tensor, here: int, what: str):
+def _quant_pages(pages: QuantPages, block_table: torch.Tensor, what: str):
+    # the pages' shape, and the device, which is the current one
     k, v, ks, vs = pages.k, pages.v, pages.k_scale, pages.v_scale
-    shape = k.shape
+    shape, here = k.shape, k.get_device()
     # (one expression while all is well: a decode step calls this for every layer)
     if not (k.dtype == v.dtype == torch.int8 and ks.dtype == vs.dtype == torch.float32 and block_table.dtype == torch.int32
-            and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == here
+            and 0 <= here == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == torch._C._cuda_getDevice()
             and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and block_table.is_contiguous()
             and len(shape) == 4 and v.shape == shape and ks.shape == vs.shape == shape[:3] and block_table.dim() == 2
             and shape[3] % 16 == 0 and 0 < shape[3] <= QUANT_MAX_HEAD_DIM):
@@ -1474,7 +1475,7 @@ def _quant_pages(pages: QuantPages, block_table: torch.Tensor, here: int, what: 
         check_quant_supported(shape[3])
         _same_device(what, k, v, ks, vs, block_table)
         raise KernelError(f"{what}: the pages cannot be used")
-    return shape
+    return shape, here
 
 
 def _quant_tokens(positions: torch.Tensor, req_of_token: torch.Tensor, n: int, here: int, what: str) -> None:
@@ -1504,8 +1505,7 @@ def quant_append(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch
             raise KernelError("quant_append: planes are float32 [S, T, width]")
         n_planes, plane_stride = qkv.shape[0], qkv.stride(0)
         qkv = qkv[0]
-    here = torch._C._cuda_getDevice()
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_append")
+    (num_pages, nkv, page_size, hd), here = _quant_pages(pages, block_table, "quant_append")
     _dev(qkv, "qkv")
     if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
         raise KernelError(f"quant_append: qkv must be [T, (nh + 2 nkv) * head_dim = {(nh + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
@@ -1532,8 +1532,7 @@ def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.T
                out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values that an 8-bit cache holds, [n, nkv, head_dim] each in ``out_dtype`` (bfloat16 or float32): row i is position
     ``positions[i]`` of request ``req_of_token[i]`` (a row of the block table).  Zeros where no page is held."""
-    here = torch._C._cuda_getDevice()
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_read")
+    (num_pages, nkv, page_size, hd), here = _quant_pages(pages, block_table, "quant_read")
     n = positions.numel()
     _quant_tokens(positions, req_of_token, n, here, "quant_read")
     k = pages.k_scale.new_empty((n, nkv, hd), dtype=out_dtype)
@@ -1598,8 +1597,7 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
     held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator.  ``dealt``: what
     :func:`quant_attention_deal` made of the step."""
-    here = torch._C._cuda_getDevice()
-    num_pages, nkv, page_size, hd = _quant_pages(pages, block_table, here, "quant_attention")
+    (num_pages, nkv, page_size, hd), _ = _quant_pages(pages, block_table, "quant_attention")
     _dev(q, "q", torch.bfloat16)
     if nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
         raise KernelError("quant_attention: q must be [T, nh * head_dim] with nh a multiple of the kv heads")

@@ -1,5 +1,6 @@
 """The 8-bit cache and the log probabilities of generated tokens without a GPU: what options, models and the cache manager make of them."""
 import contextlib
+import ctypes
 
 import pytest
 import torch
@@ -16,6 +17,7 @@ from blackwellllm_b200.cache.manager import CacheManager
 from blackwellllm_b200.config.registry import parse_config
 from blackwellllm_b200.engine.engine import Engine, EngineError, EngineOptions, StepEntry
 from blackwellllm_b200.kernels import ops
+from blackwellllm_b200.kernels.build import load_library
 from blackwellllm_b200.models.decoder import DecoderModel
 from blackwellllm_b200.parts.base import BuildContext, PagedKVRequest
 from blackwellllm_b200.sampling.params import SamplingParams
@@ -73,6 +75,65 @@ def test_head_sizes_and_groups_that_the_kernels_do_not_take():
     raw = dict(tiny.TINY_LLAMA, num_attention_heads=34, num_key_value_heads=2)
     with pytest.raises(ops.KernelError):
         DecoderModel(parse_config(raw), BuildContext(CPU, torch.bfloat16, quant_cache=True))
+
+
+def test_operands_on_the_host_are_refused():
+    """There is no CPU path: an error, and nothing is written."""
+    pages = ops.QuantPages(torch.zeros(3, 2, 8, 16, dtype=torch.int8), torch.zeros(3, 2, 8, 16, dtype=torch.int8), torch.zeros(3, 2, 8), torch.zeros(3, 2, 8))
+    table, one = torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ops.KernelError):
+        ops.quant_append(torch.ones(1, 6 * 16), one, one, table, pages, 2)
+    with pytest.raises(ops.KernelError):
+        ops.quant_read(pages, one, one, table)
+    with pytest.raises(ops.KernelError):
+        ops.token_log_probs(torch.zeros(1, 9), one)
+    assert not pages.k.any() and not pages.v_scale.any()
+
+
+def entry(lib, name, res=ctypes.c_int):
+    fn = getattr(load_library(lib, {"HEAD_DIM": 64} if "attention" in lib else None), name)
+    fn.restype = res
+    return fn
+
+
+def ints(*values):
+    return (ctypes.c_int * len(values))(*values)
+
+
+def test_what_the_entry_points_refuse_before_they_touch_the_device():
+    """Sizes and segments that no kernel takes come back as error codes (-1: bad argument, -2: not supported)."""
+    p, ll, f = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float
+    at = [p(1 << 20)] * 9       # never followed
+    need = ll(0)
+    deal = entry("attention_q8", "bw_attention_q8_deal")
+    for lens, starts, nh, nkv, page in (((-1,), (0,), 4, 2, 16), ((1,), (-1,), 4, 2, 16), ((1,), (0x7fffffff,), 4, 2, 16), ((1,), (0,), 5, 2, 16),
+                                        ((1,), (0,), 0, 2, 16), ((1,), (0,), 4, 0, 16), ((1,), (0,), 4, 2, 0)):
+        assert deal(at[0], at[0], ints(*lens), ints(*starts), 1, nh, nkv, page, 0, 0, 4096, None, ctypes.byref(need), None) == -1
+    room = entry("attention_q8_tc", "bw_attention_q8_tc_room", ll)
+    for lens, starts, G, nkv in (((-1,), (0,), 4, 2), ((40,), (-1,), 4, 2), ((40,), (0x7fffffe0,), 4, 2), ((40,), (0,), 0, 2), ((40,), (0,), 4, 0)):
+        assert room(ints(*lens), ints(*starts), 1, 16, G, nkv, 0, 0) == -1
+    assert room(ints(0x7ffffff), ints(0), 1, 16, 16, 2, 0, 0) == -2
+    attend = entry("attention_q8", "bw_attention_q8")
+    for lens, starts, nh, nkv, page, pages, blocks in (((1,), (-5,), 4, 2, 16, 9, 9), ((-1,), (5,), 4, 2, 16, 9, 9), ((1,), (5,), 3, 2, 16, 9, 9),
+                                                       ((1,), (5,), 4, 2, 0, 9, 9), ((1,), (5,), 4, 2, 16, 0, 9), ((1,), (5,), 4, 2, 16, 9, 0)):
+        assert attend(*at, p(1 << 20), blocks, ints(*lens), ints(*starts), 1, nh, nkv, page, pages, 0, 0, 0, f(0.1), None, None, ll(0),
+                      ctypes.byref(need), None, None) == -1
+    assert attend(*at, p(1 << 20), 9, ints(1), ints(5), 1, 4, 2, 1 << 16, 1 << 16, 0, 0, 0, f(0.1), None, None, ll(0), ctypes.byref(need), None, None) == -2
+    append = entry("quant_cache", "bw_quant_append")
+    good = dict(planes=1, rd=0, nh=2, tokens=1, requests=1, blocks=1, page=16, pages=4, nkv=2, hd=64, type=0)
+    for name, value, code in (("planes", 0, -1), ("rd", 3, -1), ("rd", 66, -1), ("rd", 8, -1), ("nh", -1, -1), ("tokens", -1, -1), ("requests", 0, -1),
+                              ("blocks", 0, -1), ("page", 0, -1), ("pages", 0, -1), ("nkv", 0, -1), ("hd", 24, -1), ("hd", 272, -1),
+                              ("tokens", 0x7fffffff, -2), ("type", 7, -2)):
+        a = dict(good, **{name: value})
+        assert append(at[0], a["type"], a["planes"], ll(0), None, a["rd"], 0, at[0], a["nh"], *at[:7], a["tokens"], a["requests"], a["blocks"], a["page"],
+                      a["pages"], a["nkv"], a["hd"], 1, None) == code, (name, value)
+    read = entry("quant_cache", "bw_quant_read")
+    assert read(*at, 7, 1, 1, 1, 16, 4, 2, 64, None) == -2 and read(*at, 0, 1, 1, 1, 16, 4, 2, 40, None) == -1
+    assert read(*at[:7], p((1 << 20) + 8), at[0], 0, 1, 1, 1, 16, 4, 2, 64, None) == -1
+    probs = entry("token_probs", "bw_token_probs")
+    for V, top, ld in ((0, 0, 8), (8, 9, 8), (8, 33, 8), (8, -1, 8), (8, 0, 7), ((1 << 30) + 1, 0, 1 << 31)):
+        assert probs(*at[:7], 1, V, top, ll(ld), None) == -1
+    assert probs(None, *at[:6], 1, 8, 0, ll(8), None) == -1 and probs(*at[:5], None, None, 1, 8, 1, ll(8), None) == -1
 
 
 def test_pools():

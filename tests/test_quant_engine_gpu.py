@@ -174,6 +174,26 @@ def test_a_sequence_goes_back_and_on(folders):
     check(llm._last_logits[0], want[-1], bound)
 
 
+def test_a_batch_decoded_step_by_step(folders):
+    """forward_batch, with the tokens given and taken from the step before: every token is the oracle's best within the bound."""
+    from blackwellllm_b200 import DecodeRequest, FROM_LAST
+    raw, _, page = tiny.CONFIGS["llama"]
+    folder = folders[("llama", "bfloat16")]
+    llm = make(folder, page_size=page, kv_dtype="int8")
+    texts = {s: tiny.prompt(n, raw["vocab_size"], 90 + n) for s, n in ((3, 19), (1, 40))}
+    for s, t in texts.items():
+        t.append(llm.prefill(t, 0, 0.0, 1.0, seq_id=s))
+    for step in range(12):
+        last = {s: t[-1] for s, t in texts.items()}
+        got = llm.forward_batch([DecodeRequest(seq_id=s, token_id=last[s] if step < 6 else FROM_LAST, pos=len(t) - 1) for s, t in texts.items()])
+        for s, tok in zip(texts, got):
+            texts[s].append(tok)
+    for s, t in texts.items():
+        want, bound = oracle(raw, folder, t)
+        for i in range(len(t) - 13, len(t) - 1):
+            assert float(want[i].max() - want[i, t[i + 1]]) <= 2 * bound
+
+
 def test_generation_under_preemption_with_log_probabilities(folders):
     """Few pages: requests are sent back and recomputed.  Every generated token has its log probability, and what score() says of the same
     text agrees: both differ from the plain implementation's logits by the bound, a log probability from logits by twice their difference."""
