@@ -180,16 +180,16 @@ def find_cxx() -> str:
                      "blackwellllm_b200 cannot be built")
 
 
-def compile_host_library(name: str, verbose: bool = True) -> str:
-    """Builds (if needed) ``csrc/<name>.cpp`` with the host compiler; returns the library's path."""
+def compile_host_library(name: str, verbose: bool = True, flags=(), libs=(), key=None) -> str:
+    """Builds (if needed) ``csrc/<name>.cpp`` with the host compiler; returns the library's path.  ``key``: what else the result depends on."""
     src = os.path.join(CSRC, name + ".cpp")
     if not os.path.isfile(src):
         raise BuildError(f"no such source: {src}")
-    out = os.path.join(build_dir(), f"{name}-{_source_hash(src, HOST_FLAGS, {})}.so")
+    out = os.path.join(build_dir(), f"{name}-{_source_hash(src, HOST_FLAGS, key or {})}.so")
     if os.path.isfile(out):
         return out
     tmp = f"{out}.{os.getpid()}.tmp"
-    cmd = [find_cxx()] + HOST_FLAGS + ["-I", CSRC, "-o", tmp, src]
+    cmd = [find_cxx()] + HOST_FLAGS + list(flags) + ["-I", CSRC, "-o", tmp, src] + list(libs)
     t0 = time.time()
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if proc.returncode != 0:
@@ -214,3 +214,31 @@ def load_host_library(name: str) -> ctypes.CDLL:
             lib = ctypes.CDLL(compile_host_library(name))
             _loaded[key] = lib
         return lib
+
+
+# ------------------------------------------------------------------ Python modules over torch's C++ interface
+def compile_extension(name: str, verbose: bool = True) -> str:
+    """Builds (if needed) ``csrc/<name>.cpp`` as a Python module against the installed torch; returns its path."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(find_nvcc()))
+    flags = [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
+    flags.append(f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}")
+    libs = ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    return compile_host_library(name, verbose, flags, libs, {"python": sys.version, "torch": torch.__version__})
+
+
+def load_extension(name: str):
+    import importlib.machinery
+    import importlib.util
+    key = "module|" + name
+    with _lock:
+        module = _loaded.get(key)
+        if module is None:
+            loader = importlib.machinery.ExtensionFileLoader(name, compile_extension(name))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+            loader.exec_module(module)
+            _loaded[key] = module
+        return module

@@ -15,7 +15,7 @@ from typing import List, NamedTuple, Optional, Tuple
 import numpy as np
 import torch
 
-from .build import load_library
+from .build import load_extension, load_library
 
 F32, BF16 = 0, 1
 _TYPE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -126,6 +126,35 @@ def _fn(lib_name: str, fn_name: str, argtypes, macros=None, extra_flags=(), tag=
         rec[1] += s.elapsed_time(e)
         return rc
     return timed
+
+
+_op_calls = None
+_entries = {}      # (name of an entry point, key of its build) -> address
+
+
+def _entry(lib: str, name: str, hd: Optional[int] = None) -> int:
+    at = _entries.get((name, hd))
+    if at is None:
+        at = _entries[(name, hd)] = ctypes.cast(getattr(load_library(lib, {"HEAD_DIM": hd} if hd else None), name), c_void_p).value
+    return at
+
+
+def _call(name: str, *args):
+    """``name`` of csrc/op_calls.cpp: outputs, or an entry point's error code, or None where the operands do not fit."""
+    global _op_calls
+    if _op_calls is None:
+        _op_calls = load_extension("op_calls")
+    if _timings is None:
+        return getattr(_op_calls, name)(*args)
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    got = getattr(_op_calls, name)(*args)
+    end.record()
+    end.synchronize()
+    rec = _timings.setdefault("bw_" + name, [0, 0.0])
+    rec[0] += 1
+    rec[1] += begin.elapsed_time(end)
+    return got
 
 
 # ------------------------------------------------------------------ elementwise
@@ -847,13 +876,20 @@ class TokenLogProbs(NamedTuple):
 
 
 TOKEN_LOG_PROBS_MAX_TOP = 32
-_TOKEN_PROBS_ARGS = [c_void_p] * 7 + [c_int, c_int, c_int, c_ll, c_void_p]
 
 
 def token_log_probs(logits: torch.Tensor, target: torch.Tensor, top: int = 0) -> TokenLogProbs:
     """Log probability, rank, entropy and the ``top`` (at most 32) most probable tokens of every row of float32 ``logits`` [R, V] (rows may be
     apart), in one pass over them.  ``target`` int32 [R]; one outside [0, V) stands for none: log probability NaN, rank -1.  A row without a
     distribution (a NaN or +infinity among its logits, or nothing but -infinity) gets NaN, and -1 for rank and ids."""
+    if _pending is not None:
+        _dev(logits, "logits", contiguous=False)
+    got = _call("token_log_probs", _entry("token_probs", "bw_token_probs"), logits, target, top, TOKEN_LOG_PROBS_MAX_TOP) if logits.is_cuda else None
+    if type(got) is tuple:
+        _check(0, "token_log_probs")
+        return TokenLogProbs(*got)
+    if got is not None:
+        _check(got, "token_log_probs")
     _dev(logits, "logits", torch.float32, contiguous=False)
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
         raise KernelError("token_log_probs: logits must be [R, V] with contiguous rows that do not overlap")
@@ -864,13 +900,7 @@ def token_log_probs(logits: torch.Tensor, target: torch.Tensor, top: int = 0) ->
     if not 0 <= top <= min(TOKEN_LOG_PROBS_MAX_TOP, V):
         raise KernelError(f"token_log_probs: top must be 0 to {TOKEN_LOG_PROBS_MAX_TOP} and at most the row's {V} tokens, got {top}")
     _same_device("token_log_probs", logits, target)
-    got = TokenLogProbs(logits.new_empty(R), logits.new_empty(R), target.new_empty(R), target.new_empty((R, top)), logits.new_empty((R, top)))
-    if R == 0:
-        return got
-    fn = _fn("token_probs", "bw_token_probs", _TOKEN_PROBS_ARGS)
-    _check(fn(logits.data_ptr(), target.data_ptr(), got[0].data_ptr(), got[1].data_ptr(), got[2].data_ptr(), got[3].data_ptr(), got[4].data_ptr(),
-              R, V, top, logits.stride(0) if R > 1 else V, _stream()), "token_log_probs")
-    return got
+    raise KernelError("token_log_probs: the operands cannot be used")
 
 
 # ------------------------------------------------------------------ dispatch
@@ -1453,41 +1483,28 @@ def check_quant_supported(head_dim: int, group: int = 1) -> None:
         raise KernelError(f"8-bit cache: {group} query heads per kv head exceed the attention kernels' limit of {MAX_GROUP_BF16}")
 
 
-def _quant_pages(pages: QuantPages, block_table: torch.Tensor, what: str):
-    # the pages' shape, and the device, which is the current one
+def _explain_quant(pages: QuantPages, block_table: torch.Tensor, what: str):
+    # what csrc/op_calls.cpp asks of the pages; their sizes where nothing is wrong with them
     k, v, ks, vs = pages.k, pages.v, pages.k_scale, pages.v_scale
-    shape, here = k.shape, k.get_device()
-    # (one expression while all is well: a decode step calls this for every layer)
-    if not (k.dtype == v.dtype == torch.int8 and ks.dtype == vs.dtype == torch.float32 and block_table.dtype == torch.int32
-            and 0 <= here == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == torch._C._cuda_getDevice()
-            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and block_table.is_contiguous()
-            and len(shape) == 4 and v.shape == shape and ks.shape == vs.shape == shape[:3] and block_table.dim() == 2
-            and shape[3] % 16 == 0 and 0 < shape[3] <= QUANT_MAX_HEAD_DIM):
-        for name, t, dtype in (("k", k, torch.int8), ("v", v, torch.int8), ("k_scale", ks, torch.float32), ("v_scale", vs, torch.float32),
-                               ("block_table", block_table, torch.int32)):
-            _dev(t, f"{what}: {name}", dtype)
-        if len(shape) != 4 or v.shape != shape:
-            raise KernelError(f"{what}: keys and values must be [num_pages, nkv, page_size, head_dim]")
-        if ks.shape != shape[:3] or vs.shape != shape[:3]:
-            raise KernelError(f"{what}: scales must be [num_pages, nkv, page_size]")
-        if block_table.dim() != 2:
-            raise KernelError(f"{what}: the block table must be [requests, blocks]")
-        check_quant_supported(shape[3])
-        _same_device(what, k, v, ks, vs, block_table)
-        raise KernelError(f"{what}: the pages cannot be used")
-    return shape, here
+    for name, t, dtype in (("k", k, torch.int8), ("v", v, torch.int8), ("k_scale", ks, torch.float32), ("v_scale", vs, torch.float32),
+                           ("block_table", block_table, torch.int32)):
+        _dev(t, f"{what}: {name}", dtype)
+    if k.dim() != 4 or v.shape != k.shape:
+        raise KernelError(f"{what}: keys and values must be [num_pages, nkv, page_size, head_dim]")
+    if ks.shape != k.shape[:3] or vs.shape != k.shape[:3]:
+        raise KernelError(f"{what}: scales must be [num_pages, nkv, page_size]")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be [requests, blocks]")
+    check_quant_supported(k.shape[3])
+    _same_device(what, k, v, ks, vs, block_table)
+    return k.shape
 
 
-def _quant_tokens(positions: torch.Tensor, req_of_token: torch.Tensor, n: int, here: int, what: str) -> None:
-    if not (positions.dtype == req_of_token.dtype == torch.int32 and positions.get_device() == req_of_token.get_device() == here
-            and positions.is_contiguous() and req_of_token.is_contiguous() and positions.numel() == req_of_token.numel() == n):
-        _dev(positions, f"{what}: positions", torch.int32); _dev(req_of_token, f"{what}: req_of_token", torch.int32)
-        _same_device(what, positions, req_of_token)
+def _explain_tokens(positions: torch.Tensor, req_of_token: torch.Tensor, n: int, what: str) -> None:
+    _dev(positions, f"{what}: positions", torch.int32); _dev(req_of_token, f"{what}: req_of_token", torch.int32)
+    _same_device(what, positions, req_of_token)
+    if positions.numel() != n or req_of_token.numel() != n:
         raise KernelError(f"{what}: one position and one request per token")
-
-
-_QUANT_APPEND_ARGS = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_int, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 8 + [c_void_p]
-_QUANT_READ_ARGS = [c_void_p] * 9 + [c_int] * 8 + [c_void_p]
 
 
 def quant_append(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch.Tensor, block_table: torch.Tensor, pages: QuantPages,
@@ -1499,57 +1516,53 @@ def quant_append(qkv: torch.Tensor, positions: torch.Tensor, req_of_token: torch
     x * (127 / a), rounded to nearest; one with a below 2^-110 becomes zeros; one that holds an infinity or NaN reads back as NaN.  A token
     whose position has no page (-1 in the block table, or beyond it) is not written.  Two tokens of one call must not have the
     same request and position.  ``paired``: the q and k heads are in the order of :func:`rotary_row_order`."""
-    n_planes, plane_stride = 1, 0
+    if _pending is not None:
+        _dev(qkv, "qkv", contiguous=False)
+    q = _call("quant_append", _entry("quant_cache", "bw_quant_append"), pages.k, pages.v, pages.k_scale, pages.v_scale, block_table, qkv, positions,
+              req_of_token, nh, table, paired, append) if qkv.is_cuda else None
+    if q is not None:
+        if type(q) is int:
+            _check(q, "quant_append")
+        _check(0, "quant_append")
+        return q
+    _, nkv, _, hd = _explain_quant(pages, block_table, "quant_append")
     if qkv.dim() == 3:
         if qkv.dtype != torch.float32 or not qkv.shape[0]:
             raise KernelError("quant_append: planes are float32 [S, T, width]")
-        n_planes, plane_stride = qkv.shape[0], qkv.stride(0)
         qkv = qkv[0]
-    (num_pages, nkv, page_size, hd), here = _quant_pages(pages, block_table, "quant_append")
     _dev(qkv, "qkv")
+    _code(qkv, "qkv")
     if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
         raise KernelError(f"quant_append: qkv must be [T, (nh + 2 nkv) * head_dim = {(nh + 2 * nkv) * hd}], got {tuple(qkv.shape)}")
     T = qkv.shape[0]
-    _quant_tokens(positions, req_of_token, T, here, "quant_append")
-    rd = 0
+    _explain_tokens(positions, req_of_token, T, "quant_append")
     if table is not None:
         _dev(table, "table", torch.float32)
         if table.dim() != 2 or table.shape[0] != T or table.shape[1] % 2 or table.shape[1] > hd:
             raise KernelError("quant_append: the cos/sin table must be [T, rotary_dim], rotary_dim even and at most the head size")
-        rd = table.shape[1]
     _same_device("quant_append", qkv, table)
-    q = qkv.new_empty((T, nh * hd), dtype=torch.bfloat16)
-    if T == 0:
-        return q
-    fn = _fn("quant_cache", "bw_quant_append", _QUANT_APPEND_ARGS)
-    _check(fn(_ptr(qkv), _code(qkv, "qkv"), n_planes, plane_stride, _ptr(table) if rd else None, rd, int(paired), _ptr(q), nh, _ptr(pages.k),
-              _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(positions), _ptr(req_of_token), _ptr(block_table), T,
-              block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, hd, int(append), _stream()), "quant_append")
-    return q
+    raise KernelError("quant_append: the operands cannot be used")
 
 
 def quant_read(pages: QuantPages, positions: torch.Tensor, req_of_token: torch.Tensor, block_table: torch.Tensor,
                out_dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values that an 8-bit cache holds, [n, nkv, head_dim] each in ``out_dtype`` (bfloat16 or float32): row i is position
     ``positions[i]`` of request ``req_of_token[i]`` (a row of the block table).  Zeros where no page is held."""
-    (num_pages, nkv, page_size, hd), here = _quant_pages(pages, block_table, "quant_read")
-    n = positions.numel()
-    _quant_tokens(positions, req_of_token, n, here, "quant_read")
-    k = pages.k_scale.new_empty((n, nkv, hd), dtype=out_dtype)
-    v = torch.empty_like(k)
-    code = _code(k, "out")
-    if n == 0:
-        return k, v
-    fn = _fn("quant_cache", "bw_quant_read", _QUANT_READ_ARGS)
-    _check(fn(_ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(positions), _ptr(req_of_token), _ptr(block_table),
-              _ptr(k), _ptr(v), code, n, block_table.shape[0], block_table.shape[1], page_size, num_pages, nkv, hd, _stream()), "quant_read")
-    return k, v
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise KernelError(f"quant_read: bfloat16 or float32, not {out_dtype}")
+    got = _call("quant_read", _entry("quant_cache", "bw_quant_read"), pages.k, pages.v, pages.k_scale, pages.v_scale, block_table, positions, req_of_token,
+                out_dtype is torch.float32) if block_table.is_cuda else None
+    if got is not None:
+        if type(got) is int:
+            _check(got, "quant_read")
+        _check(0, "quant_read")
+        return got
+    _explain_quant(pages, block_table, "quant_read")
+    _explain_tokens(positions, req_of_token, positions.numel(), "quant_read")
+    raise KernelError("quant_read: the operands cannot be used")
 
 
-_ATTN_Q8_ARGS = ([c_void_p] * 10 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, ctypes.POINTER(c_ll),
-                                                                            c_void_p, c_void_p])
 _ATTN_Q8_DEAL_ARGS = [c_void_p] * 4 + [c_int] * 7 + [c_void_p, ctypes.POINTER(c_ll), c_void_p]
-_ATTN_Q8_TC_ARGS = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_void_p, c_void_p, c_ll, c_void_p]
 QUANT_FEW_ROWS = 16     # up to so many stacked rows (tokens times heads of a group) a request is the key-slice kernel's
 
 
@@ -1579,7 +1592,7 @@ def quant_attention_deal(batch, nh: int, nkv: int, head_dim: int, page_size: int
     _same_device("quant_attention_deal", batch.cu_q, batch.q_start)
     ints = c_int * R
     h_len, h_start = ints(*batch.h_q_len[:R]), ints(*batch.h_q_start[:R])
-    fn = _fn("attention_q8", "bw_attention_q8_deal", _ATTN_Q8_DEAL_ARGS, macros=attention_q8_macros(head_dim))
+    fn = _fn("attention_q8", "bw_attention_q8_deal", _ATTN_Q8_DEAL_ARGS, macros={"HEAD_DIM": head_dim})
     need, at = c_ll(0), None
     for _ in range(2):      # how much it is, then the work
         _check(fn(_ptr(batch.cu_q), _ptr(batch.q_start), h_len, h_start, R, nh, nkv, page_size, window, chunk, int(batch.static_bound),
@@ -1597,66 +1610,36 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
     held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator.  ``dealt``: what
     :func:`quant_attention_deal` made of the step."""
-    (num_pages, nkv, page_size, hd), _ = _quant_pages(pages, block_table, "quant_attention")
+    k = pages.k
+    window, chunk = int(window or 0), int(chunk or 0)
+    got = None
+    if block_table.is_cuda and k.dim() == 4:
+        _, nkv, page_size, hd = k.shape
+        if dealt is not None and dealt.key != _dealt_key(batch, nh, nkv, hd, page_size, window, chunk):
+            raise KernelError("quant_attention: `dealt` was made for another step or other sizes")
+        if 0 < hd <= QUANT_MAX_HEAD_DIM and hd % 16 == 0:
+            got = _call("quant_attention", _entry("attention_q8", "bw_attention_q8", hd), _entry("attention_q8_tc", "bw_attention_q8_tc_room", hd),
+                        _entry("attention_q8_tc", "bw_attention_q8_tc", hd), k, pages.v, pages.k_scale, pages.v_scale, block_table, q, batch.cu_q,
+                        batch.q_start, batch.kv_len, batch.h_q_len, batch.h_q_start, batch.T, batch.R, nh, MAX_GROUP_BF16, QUANT_FEW_ROWS, scale, window,
+                        chunk, int(batch.static_bound or 0), sink, None if dealt is None else dealt.ints)
+    if type(got) is tuple:
+        global launches
+        launches += got[1]
+        return got[0]
+    if got is not None:
+        _check(got, "quant_attention")
+    num_pages, nkv, page_size, hd = _explain_quant(pages, block_table, "quant_attention")
     _dev(q, "q", torch.bfloat16)
-    if nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
+    if nh < 1 or nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
         raise KernelError("quant_attention: q must be [T, nh * head_dim] with nh a multiple of the kv heads")
-    G, R = nh // nkv, batch.R
-    if G > MAX_GROUP_BF16:
-        check_quant_supported(hd, G)
+    check_quant_supported(hd, nh // nkv)
     if not scale > 0:
         raise KernelError(f"quant_attention: scale must be positive, got {scale}")
     _check_sink(sink, nh)
-    cu_q, q_start, kv_len, lens, starts = batch.cu_q, batch.q_start, batch.kv_len, batch.h_q_len, batch.h_q_start
-    for t, name in ((cu_q, "cu_q"), (q_start, "q_start"), (kv_len, "kv_len")):
+    for t, name in ((batch.cu_q, "cu_q"), (batch.q_start, "q_start"), (batch.kv_len, "kv_len")):
         _dev(t, name, torch.int32)
-    if len(lens) != R:
-        lens = lens[:R]
-    if q.shape[0] != batch.T or block_table.shape[0] < R or cu_q.numel() < R + 1 or q_start.numel() < R or kv_len.numel() < R \
-            or len(lens) != R or len(starts) < R or sum(lens) != batch.T:
-        raise KernelError("quant_attention: the batch's segments, the queries and the block table do not fit together")
-    _same_device("quant_attention", q, cu_q, q_start, kv_len, sink)
-    out = torch.empty_like(q)
-    if batch.T == 0:
-        return out
-    window, chunk = int(window or 0), int(chunk or 0)
-    ints = c_int * R
-    h_len, h_start = ints(*lens), ints(*starts[:R])
-    if dealt is not None and dealt.key != _dealt_key(batch, nh, nkv, hd, page_size, window, chunk):
-        raise KernelError("quant_attention: `dealt` was made for another step or other sizes")
-    macros = attention_q8_macros(hd)
-    if max(lens) * G > QUANT_FEW_ROWS:      # portions of prompts: the tcgen05 kernel
-        room_of = load_library("attention_q8_tc", macros).bw_attention_q8_tc_room
-        if not room_of.argtypes:
-            room_of.argtypes, room_of.restype = [c_void_p, c_void_p] + [c_int] * 6, c_ll
-        floats = room_of(h_len, h_start, R, QUANT_FEW_ROWS, G, nkv, window, chunk)
-        if floats < 0:
-            _check(int(floats), "quant_attention")
-        room = torch.empty(floats, dtype=torch.float32, device=q.device)
-        tc = _fn("attention_q8_tc", "bw_attention_q8_tc", _ATTN_Q8_TC_ARGS, macros=macros)
-        _check(tc(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(kv_len), _ptr(block_table),
-                  block_table.shape[1], h_len, h_start, R, QUANT_FEW_ROWS, nh, nkv, page_size, num_pages, window, chunk, float(scale), _ptr(sink),
-                  _ptr(room), floats, _stream()), "quant_attention")
-        if min(lens) * G > QUANT_FEW_ROWS:
-            return out
-    fn = _fn("attention_q8", "bw_attention_q8", _ATTN_Q8_ARGS, macros=macros)
-    need = c_ll(0)
-    room, floats = None, 0
-    while True:
-        code = fn(_ptr(q), _ptr(pages.k), _ptr(pages.v), _ptr(pages.k_scale), _ptr(pages.v_scale), _ptr(out), _ptr(cu_q), _ptr(q_start), _ptr(kv_len),
-                  _ptr(block_table), block_table.shape[1], h_len, h_start, R, nh, nkv, page_size, num_pages, window, chunk,
-                  int(batch.static_bound or 0), float(scale), _ptr(sink), _ptr(room), floats, ctypes.byref(need),
-                  None if dealt is None else dealt.ints.data_ptr(), _stream())
-        if code != _ERR_ROOM or room is not None:
-            break
-        floats = need.value             # many slices of few requests join through memory; a captured step's are divided there
-        room = torch.empty(floats, dtype=torch.float32, device=q.device)
-    _check(code, "quant_attention")
-    return out
-
-
-_ERR_ROOM = -11
-_ATTN_Q8_MACROS = {}
+    _same_device("quant_attention", q, batch.cu_q, batch.q_start, batch.kv_len, sink)
+    raise KernelError("quant_attention: the batch's segments, the queries and the block table do not fit together")
 
 
 def attention_q8_status() -> int:
@@ -1667,14 +1650,6 @@ def attention_q8_status() -> int:
             lib.bw_attention_q8_tc_status.restype = c_int
             total |= int(lib.bw_attention_q8_tc_status())
     return total
-
-
-def attention_q8_macros(hd: int) -> dict:
-    """The build of the attention over an 8-bit cache for this head size."""
-    macros = _ATTN_Q8_MACROS.get(hd)
-    if macros is None:
-        macros = _ATTN_Q8_MACROS[hd] = {"HEAD_DIM": hd}
-    return macros
 
 
 def rmsnorm_add(x: torch.Tensor, w: torch.Tensor, eps: float, stream: torch.Tensor) -> torch.Tensor:
