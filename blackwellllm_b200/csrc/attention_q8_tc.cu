@@ -214,13 +214,13 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     bw::tc_fence_before();
     __syncthreads();
     bw::tc_fence_after();
-    BW_PDL_WAIT();
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_O = tmem_base + 128 * NQ;        // S: [tile of rows][buffer] of 64 columns, then O: [tile of rows] of O_COLS
     auto all = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
     Walk w;
-    w.start(p, work);
+    w.start(p, work);                                    // (of the launch's own numbers, while the kernel before is still at work)
+    BW_PDL_WAIT();
     if (tmem_slot[1] != 0) w.left = 0;                   // an earlier launch gave up: nothing is done
 
     if (warp >= QK_WARP) {
@@ -342,7 +342,6 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             for (int i = 0; i < 2; ++i) got[i] = (unsigned)x.page[i] < (unsigned)p.num_pages ? (x.page[i] * p.nkv + x.g) * p.page_size + x.slot[i] : -1;
             return Rows{got[0], got[1]};
         };
-        auto prefetch = [](const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); };
         auto scale = [&](const float* of, int row) { return row >= 0 ? of[row] : 0.f; };
         if (w.left > 0) {
             Walk ahead = w;
@@ -374,16 +373,6 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 rows = rows_of(next);                                                     // of the next step (behind the last: none)
                 const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
                 // (into the first-level cache now; loaded only behind the fence below, which waits for loads under way)
-                if ((lane >> 3) == ww) {
-                    prefetch(from + (size_t)max(rows.a, 0) * HD);
-                    prefetch(from + (size_t)max(rows.b, 0) * HD);
-                    if (HD > 128) {
-                        prefetch(from + (size_t)max(rows.a, 0) * HD + 128);
-                        prefetch(from + (size_t)max(rows.b, 0) * HD + 128);
-                    }
-                }
-                prefetch(p.k_scale + max(rows.a, 0)); prefetch(p.k_scale + max(rows.b, 0));
-                prefetch(p.v_scale + max(rows.a, 0)); prefetch(p.v_scale + max(rows.b, 0));
                 // references and factors
                 unsigned kb = 0, vb = 0;
                 bool bad[2];
@@ -628,13 +617,17 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     if (warp == QK_WARP) bw::tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
-// The items that several blocks share: a thread a row, four channels a block.
-__global__ void __launch_bounds__(ROWS)
+// The items that several blocks share: a thread for four channels of a row.  A warp has eight rows of sixteen channels, so it reads whole lines of
+// the parts and writes whole sectors (a row a lane, four channels a block, wrote a quarter of each).  Four parts are read at a time, sums and
+// outputs together: mostly that is all of them, and the kernel is one trip to memory long.
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = JOIN_THREADS / 4;
+__global__ void __launch_bounds__(JOIN_THREADS)
 join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work, const __grid_constant__ Splits splits) {
     BW_PDL_TRIGGER();
-    BW_PDL_WAIT();
-    const int i = blockIdx.x, quad = blockIdx.y, r = threadIdx.x;
+    const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int quad = 4 * blockIdx.y + (lane >> 3), r = blockIdx.z * JOIN_ROWS + 8 * warp + (lane & 7);
     const Item it = item_of(work.portion, p.portions, splits.item[i], p.nkv, p.G, p.window, p.chunk);
+    BW_PDL_WAIT();
     if (r >= it.n_rows) return;
     const int from = splits.from[i], to = splits.to[i];
     // the first block's part begins with the item: its slot is the second
@@ -642,15 +635,28 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;
     const float4* part = reinterpret_cast<const float4*>(p.part_o) + (size_t)quad * ROWS + r;
     float M = -INFINITY, L = 0.f;
-    for (int b = from; b <= to; ++b) M = fmaxf(M, ml[slot_of(b) * ROWS].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int b = from; b <= to; ++b) {
-        const float2 x = ml[slot_of(b) * ROWS];
-        const float4 o = part[slot_of(b) * (HD / 4) * ROWS];
-        const float f = x.x == -INFINITY ? 0.f : ex2(x.x - M);
-        acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y); acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
-        L = fmaf(x.y, f, L);
+    for (int b = from; b <= to; b += 4) {
+        float2 x[4];
+        float4 o[4];
+        float most = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const size_t at = slot_of(min(b + j, to));
+            x[j] = ml[at * ROWS];
+            o[j] = part[at * (HD / 4) * ROWS];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (b + j <= to) most = fmaxf(most, x[j].x);
+        const float less = M == -INFINITY ? 0.f : ex2(M - most);
+        M = most;
+        acc.x *= less; acc.y *= less; acc.z *= less; acc.w *= less; L *= less;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = b + j > to || x[j].x == -INFINITY ? 0.f : ex2(x[j].x - M);
+            acc.x = fmaf(o[j].x, f, acc.x); acc.y = fmaf(o[j].y, f, acc.y); acc.z = fmaf(o[j].z, f, acc.z); acc.w = fmaf(o[j].w, f, acc.w);
+            L = fmaf(x[j].y, f, L);
+        }
     }
     const int gr = it.row0 + r, tok = gr / p.G, head = it.g * p.G + gr - tok * p.G;
     if (p.sink) L += ex2(p.sink[head] * LOG2E - M);
@@ -759,7 +765,7 @@ BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, co
         bw::launch(attn_q8_tc_kernel, dim3((unsigned)blocks), dim3(THREADS), SMEM_BYTES, s, p, work);
         BW_LAUNCH_CHECK();
         if (splits.n) {
-            bw::launch(join_kernel, dim3((unsigned)splits.n, HD / 4), dim3(ROWS), 0, s, p, work, splits);
+            bw::launch(join_kernel, dim3((unsigned)splits.n, HD / 16, ROWS / JOIN_ROWS), dim3(JOIN_THREADS), 0, s, p, work, splits);
             BW_LAUNCH_CHECK();
         }
         return 0;
