@@ -8,13 +8,17 @@
 // in an order that depends on V alone (threads take every so many-th four elements; then trees).
 //
 // The `top` (at most 32) most probable tokens, ties to the lowest id: a token is a 64-bit key, the logit's bits made ordered above, the
-// inverted id below; no two are equal.  Every thread knows the best key of its own elements from the pass; the top-th best of those is a
-// lower bound of the top-th best of all, and only the `top` threads at or above it can own a token of the list.  Their elements are read
-// again (a few percent of the row, from L2) and go, where they are above the bound, through lists of 32 sorted keys, one per warp, kept by
-// bitonic sorts and merges.
+// inverted id below; no two are equal.  Every thread knows the best key of its own elements from the pass.  The top-th best of the warps' best one,
+// two or four thread keys is a lower bound of the top-th best of all, and only the threads at or above it (`top` of them, or a few more)
+// can own a token of the list.  Their elements are read again (a few percent of the row, from L2), those above the bound are gathered, and
+// each finds its place by counting the larger ones.
+// (Sorting every warp's thread keys and merging the lists, twice, as first written: 130 us for 1,024 rows of 128,256 with 20 alternatives, now
+// 119; one row with five 9.7, now 7.7.)
 //
-// Bound by memory: 4 bytes an element.  A row is one block's, or, where there are few rows, shared by a cluster of 2, 4 or 8 blocks that join
-// through distributed shared memory.
+// Bound by memory: 4 bytes an element (1,024 rows of 128,256 without alternatives: 96 us, 5.5 TB/s).  A row is one block's, or, where there are few
+// rows, shared by a cluster of 2, 4 or 8 blocks that join through distributed shared memory; then what follows the pass over the row counts, a
+// chain of short steps between barriers.  What runs once a row is kept small (not inlined, not unrolled): its instructions come from L2 first
+// (one row 8.4 us with all of it in line, 7.7 so).
 #include "common.cuh"
 #include <cooperative_groups.h>
 
@@ -58,30 +62,29 @@ __device__ __forceinline__ float value_of(u64 key) {
 __device__ __forceinline__ int id_of(u64 key) { return (int)(0xffffffffu - (unsigned)key); }
 
 struct Part { float m, z, w; };
-// (-infinity: a part without an element that counts)
+// (m -infinity: a part without an element that counts, and its factor is 0; a difference of two of them, no number, becomes LEAST)
 __device__ __forceinline__ Part join(Part a, Part b) {
-    if (b.m > a.m) { const Part t = a; a = b; b = t; }
-    if (b.m == -INFINITY) return a;
-    const float d = fmaxf(b.m - a.m, LEAST), f = ex2(d * LOG2E);
-    a.z += f * (1.f + b.z);
-    a.w += f * (b.w + d * (1.f + b.z));
-    return a;
+    const bool swap = b.m > a.m;
+    const Part x = {swap ? b.m : a.m, swap ? b.z : a.z, swap ? b.w : a.w}, y = {swap ? a.m : b.m, swap ? a.z : b.z, swap ? a.w : b.w};
+    const float d = fmaxf(y.m - x.m, LEAST), f = ex2(d * LOG2E), n = 1.f + y.z;
+    return {x.m, x.z + f * n, x.w + f * (y.w + d * n)};
 }
 
-__device__ __forceinline__ u64 shfl_xor_key(u64 k, int o) { return __shfl_xor_sync(0xffffffffu, k, o); }
-// a warp's 32 keys in falling order (lane 0: the best)
-__device__ __forceinline__ u64 sort32(u64 k) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const u64 other = shfl_xor_key(k, o);
-            const bool falling = (lane & size) == 0 || size == 32;
-            const bool take_max = ((lane & o) == 0) == falling;
-            k = take_max ? (k > other ? k : other) : (k < other ? k : other);
-        }
-    return k;
+// a warp's largest key
+__device__ __forceinline__ u64 warp_max(u64 k) {
+    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32));
+    return (u64)hi << 32 | __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32) == hi ? (unsigned)k : 0u);
+}
+// The n keys, no two alike, put in falling order as far as the first `top`: a thread counts what is above its key.
+__device__ __noinline__ void place_keys(const u64* keys, int n, u64* sorted, int top) {
+    for (int a = threadIdx.x; a < n; a += THREADS) {
+        const u64 k = keys[a];
+        int above = 0;
+#pragma unroll 4
+        for (int b = 0; b < n; ++b) above += keys[b] > k;
+        if (k != 0 && above < top) sorted[above] = k;
+    }
+    __syncwarp();
 }
 // the 32 best of two lists in falling order, in falling order
 __device__ __forceinline__ u64 merge32(u64 a, u64 b) {
@@ -90,24 +93,8 @@ __device__ __forceinline__ u64 merge32(u64 a, u64 b) {
     u64 k = a > r ? a : r;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const u64 other = shfl_xor_key(k, o);
-        k = (lane & o) == 0 ? (k > other ? k : other) : (k < other ? k : other);
-    }
-    return k;
-}
-// the 32 best of the first n warps' lists, in warp 0 (all threads of the block call it)
-__device__ __forceinline__ u64 merge_warps(u64 k, u64 (*lists)[32], int n) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int o = 1;
-    while (o < n) o <<= 1;
-    if (warp < n) lists[warp][lane] = k;
-    for (o >>= 1; o > 0; o >>= 1) {
-        __syncthreads();
-        if (warp < o && warp + o < n) {
-            k = merge32(k, lists[warp + o][lane]);
-            lists[warp][lane] = k;
-        }
-        n = min(n, o);
+        const u64 other = __shfl_xor_sync(0xffffffffu, k, o);
+        k = ((lane & o) == 0) == (k > other) ? k : other;
     }
     return k;
 }
@@ -124,13 +111,17 @@ __device__ __forceinline__ float4 load4(const float* row, int c, int V) {
 // What a block found in its share of a row.
 struct Found { Part part; int count, bad; };
 constexpr int MOST_BLOCKS = 8;
+constexpr int ROOM = 256;
 struct Shared {
     Found warps[WARPS];
-    u64 lists[WARPS][32];
-    u64 loose[WARPS][128];       // a warp's candidates before they are sorted
-    u64 best[32];                // the block's best thread keys
+    u64 some[4 * WARPS];         // of every warp's thread keys the best few
+    u64 bound;
+    int owners, gathered;        // how many
+    int owner[THREADS];          // threads that can own a token of the list
+    u64 keys[ROOM + 4 * THREADS];     // tokens gathered, and room for a round's
+    u64 sorted[MAX_TOP];
     Found found[MOST_BLOCKS];    // in the cluster's first block: of every block
-    u64 found_best[MOST_BLOCKS][32];
+    u64 found_best[MOST_BLOCKS][MAX_TOP];
 };
 template <typename T> __device__ __forceinline__ T* in_first_block(T* at) { return cg::this_cluster().map_shared_rank(at, 0); }
 
@@ -186,11 +177,12 @@ __device__ __forceinline__ Found shuffled(const Found& a, int o) {
     return {{__shfl_xor_sync(0xffffffffu, a.part.m, o), __shfl_xor_sync(0xffffffffu, a.part.z, o), __shfl_xor_sync(0xffffffffu, a.part.w, o)},
             __shfl_xor_sync(0xffffffffu, a.count, o), __shfl_xor_sync(0xffffffffu, a.bad, o)};
 }
-// joined over groups of n neighbouring lanes (a power of two), both lanes of a pair in the same order
-__device__ __forceinline__ Found join_lanes(Found a, int n) {
+// joined over groups of n neighbouring lanes (a power of two); the first lane's is the result (others' may differ in a last bit)
+__device__ __noinline__ Found join_lanes(Found a, int n) {
+#pragma unroll 1
     for (int o = n >> 1; o > 0; o >>= 1) {
         const Found b = shuffled(a, o);
-        a.part = (threadIdx.x & o) ? join(b.part, a.part) : join(a.part, b.part);
+        a.part = join(a.part, b.part);
         a.count += b.count;
         a.bad |= b.bad;
     }
@@ -234,44 +226,82 @@ token_probs_kernel(Args p, int blocks) {
     Found all{part_of(s), s.count, !(s.best < INFINITY)};
     all = join_lanes(all, 32);
     if (lane == 0) sh.warps[warp] = all;
-    u64 list = 0;
+    __syncwarp();
     if (p.top > 0) {
+        if (threadIdx.x < MAX_TOP) sh.sorted[threadIdx.x] = 0;
+        if (threadIdx.x == 0) { sh.owners = sh.gathered = 0; sh.bound = 1; }        // (a short row has fewer keys: any may be in the list)
         u64 mine = 0;
         if (own < f1) {
             const float4 v = load4<VEC>(row, 4 * s.four, p.V);          // again, for which of the four it was
             mine = key_of(s.best, 4 * s.four + (v.x == s.best ? 0 : v.y == s.best ? 1 : v.z == s.best ? 2 : 3));
         }
-        list = merge_warps(sort32(mine), sh.lists, WARPS);
-        if (p.top > 1) {
-            // warp 0 has the best thread keys; the owners of the first `top` read their elements again
-            if (warp == 0) sh.best[lane] = lane < p.top ? list : 0;
+        const int few = p.top == 1 ? 1 : p.top <= 8 ? 2 : 4;             // of a warp
+        u64 left = mine;
+        for (int i = 0; i < few; ++i) {
+            const u64 k = warp_max(left);
+            if (left == k) left = 0;
+            if (lane == 0) sh.some[warp * few + i] = k;
+            __syncwarp();
+        }
+        __syncthreads();
+        const u64 a = lane < WARPS * few ? sh.some[lane] : 0, b = lane + 32 < WARPS * few ? sh.some[lane + 32] : 0;
+        for (int i = 0; i < few; ++i) {
+            const u64 k = sh.some[warp * few + i];
+            const int above = __popc(__ballot_sync(0xffffffffu, a > k)) + __popc(__ballot_sync(0xffffffffu, b > k));
+            if (lane == 0 && k != 0 && above == p.top - 1) sh.bound = k;
+            __syncwarp();
+        }
+        __syncthreads();
+        u64 bound = sh.bound;
+        if (p.top == 1) {
+            if (mine == bound) sh.sorted[0] = mine;
+        } else {
+            const bool is_owner = mine >= bound;
+            const unsigned vote = __ballot_sync(0xffffffffu, is_owner);
+            int to = 0;
+            if (lane == 0 && vote) to = atomicAdd(&sh.owners, __popc(vote));
+            __syncwarp();
+            to = __shfl_sync(0xffffffffu, to, 0);
+            if (is_owner) sh.owner[to + __popc(vote & ((1u << lane) - 1))] = (int)threadIdx.x;
             __syncthreads();
-            const u64 bound = sh.best[p.top - 1];
-            const int rounds = (f1 - f0 + THREADS - 1) / THREADS, items = p.top * rounds;
-            list = 0;
+            const int rounds = (f1 - f0 + THREADS - 1) / THREADS, items = sh.owners * rounds;
             for (int i0 = 0; i0 < items; i0 += THREADS) {                // (uniform)
-                if (i0 + 32 * warp >= items) continue;
-                const int i = i0 + (int)threadIdx.x, who = i / rounds, it = i - who * rounds;
-                const u64 owner = i < items ? sh.best[who] : 0;
-                const int f = owner ? f0 + it * THREADS + (id_of(owner) / 4 - f0) % THREADS : f1;
-                const float4 v = f < f1 ? load4<VEC>(row, 4 * f, p.V) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float y[4] = {v.x, v.y, v.z, v.w};
-                // the warp's candidates side by side, then 32 of them at a time: mostly a few in all
-                int n = 0;
+                const int i = i0 + (int)threadIdx.x, who = i / rounds, f = i < items ? f0 + (i - who * rounds) * THREADS + sh.owner[who] : f1;
+                u64 k[4] = {0, 0, 0, 0};
+                if (f < f1) {
+                    const float4 v = load4<VEC>(row, 4 * f, p.V);
+                    const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const u64 key = 4 * f + e < p.V ? key_of(y[e], 4 * f + e) : 0;
+                        k[e] = key >= bound ? key : 0;
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const u64 k = f < f1 && 4 * f + e < p.V ? key_of(y[e], 4 * f + e) : 0;
-                    const bool is = k != 0 && k >= bound;
-                    const unsigned b = __ballot_sync(0xffffffffu, is);
-                    if (is) sh.loose[warp][n + __popc(b & ((1u << lane) - 1))] = k;
-                    n += __popc(b);
+                    const unsigned b = __ballot_sync(0xffffffffu, k[e] != 0);
+                    if (!b) continue;
+                    int to = 0;
+                    if (lane == 0) to = atomicAdd(&sh.gathered, __popc(b));
+                    __syncwarp();
+                    to = __shfl_sync(0xffffffffu, to, 0);
+                    if (k[e]) sh.keys[to + __popc(b & ((1u << lane) - 1))] = k[e];
+                    __syncwarp();
                 }
-                __syncwarp();
-                for (int j = 0; j < n; j += 32) list = merge32(list, sort32(j + lane < n ? sh.loose[warp][j + lane] : 0));
-                __syncwarp();
+                __syncthreads();
+                const int have = sh.gathered;
+                const bool last = i0 + THREADS >= items;
+                if (last || have > ROOM) {
+                    place_keys(sh.keys, have, sh.sorted, p.top);
+                    if (last) break;
+                    // (a row that is made for it) the best stay, and the last of them is the bound from here on: no element comes twice
+                    __syncthreads();
+                    if ((int)threadIdx.x < p.top) sh.keys[threadIdx.x] = sh.sorted[threadIdx.x];
+                    if (threadIdx.x == 0) sh.gathered = p.top;
+                    bound = sh.sorted[p.top - 1];
+                }
+                __syncthreads();
             }
-            __syncthreads();
-            list = merge_warps(list, sh.lists, min(WARPS, (items + 31) / 32));
         }
     }
     __syncthreads();
@@ -280,17 +310,30 @@ token_probs_kernel(Args p, int blocks) {
         all = join_lanes(lane < WARPS ? sh.warps[lane] : Found{{-INFINITY, 0.f, 0.f}, 0, 0}, WARPS);
         // into the cluster's first block
         if (lane == 0) *(blocks > 1 ? in_first_block(&sh.found[part]) : &sh.found[0]) = all;
-        if (p.top > 0) *(blocks > 1 ? in_first_block(&sh.found_best[part][lane]) : &sh.found_best[0][lane]) = list;
+        if (blocks > 1 && p.top > 0) *in_first_block(&sh.found_best[part][lane]) = sh.sorted[lane];
     }
     if (blocks > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         if (part != 0) return;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (p.top > 0) {
+            // the blocks' lists, two by two
+            u64 list = warp < blocks ? sh.found_best[warp][lane] : 0;
+            for (int o = blocks >> 1; o > 0; o >>= 1) {
+                if (warp < o) {
+                    list = merge32(list, sh.found_best[warp + o][lane]);
+                    sh.found_best[warp][lane] = list;
+                }
+                __syncthreads();
+            }
+            if (warp == 0) sh.sorted[lane] = list;
+        }
+        __syncwarp();
     } else {
         __syncwarp();
     }
-    if (p.top > 0) list = blocks > 1 ? merge_warps(warp < blocks ? sh.found_best[warp][lane] : 0, sh.lists, blocks) : list;
     if (warp != 0) return;
+    const u64 list = lane < p.top ? sh.sorted[lane] : 0;
     all = join_lanes(lane < blocks ? sh.found[lane] : Found{{-INFINITY, 0.f, 0.f}, 0, 0}, MOST_BLOCKS);
     all = Found{{__shfl_sync(0xffffffffu, all.part.m, 0), __shfl_sync(0xffffffffu, all.part.z, 0), __shfl_sync(0xffffffffu, all.part.w, 0)},
                 __shfl_sync(0xffffffffu, all.count, 0), __shfl_sync(0xffffffffu, all.bad, 0)};

@@ -88,6 +88,30 @@ def test_ties_go_to_the_lowest_id(V):
     check(x.cuda(), [V // 2, 7, V - 1, 8, V - 3, 5], 32)
 
 
+@pytest.mark.parametrize("rows", [6, 301])
+@pytest.mark.parametrize("V", [152064, 9001])
+def test_alternatives_wherever_the_best_stand(rows, V):
+    """Rows in order, of one value, of few values, and with all the large ones in the elements of a few threads: lists of many candidates."""
+    g = torch.Generator().manual_seed(rows + V)
+    x = torch.randn(rows, V, generator=g)
+    x[0] = torch.linspace(-3, 3, V)
+    x[1] = torch.linspace(3, -3, V)
+    x[2] = 0.25
+    x[3] = torch.randint(0, 3, (V,), generator=g).float()
+    four = torch.arange(V) // 4
+    x[4] = torch.where(four % 512 < 224, x[4] + 50, x[4])       # seven warps of a block, where a block has the row
+    x[5] = torch.where(four % 512 == 77, x[5] + 50, x[5])
+    for top in (2, 7, 8, 9, 20, 32):
+        target = torch.arange(rows, dtype=torch.int32) % V
+        got = ops.token_log_probs(x.cuda(), target.cuda(), top)
+        again = ops.token_log_probs(x.cuda(), target.cuda(), top)
+        for r in range(6):
+            order = torch.sort(x[r].double(), descending=True, stable=True).indices
+            assert got.top_ids[r].tolist() == order[:top].tolist(), r
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    check(x[:6].cuda(), [0, 1, 2, 3, 4, 5], 32)
+
+
 def test_masked_and_broken_rows():
     V = 5003
     g = torch.Generator().manual_seed(1)
