@@ -414,6 +414,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(full + 8 * s);
+                __syncwarp();
                 ks[0] = scale(p.k_scale, rows.a); ks[1] = scale(p.k_scale, rows.b);
                 vs[0] = scale(p.v_scale, rows.a); vs[1] = scale(p.v_scale, rows.b);
 #pragma unroll
@@ -482,6 +483,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(q_full + 8 * q);
+                __syncwarp();
             } else {
                 it += w.end - w.tile;
                 w.pass(p, work);
@@ -568,6 +570,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 bw::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(p_full + 8 * (2 * q + b));
+                __syncwarp();
             }
             if (!ok || !(ok = all(bw::mbar_wait(pv_done + 8 * (2 * q + ((c - 1) & 1)), ((c - 1) >> 1) & 1, &g_status, 41)))) break;
             bw::tc_fence_after();
