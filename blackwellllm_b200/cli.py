@@ -14,7 +14,7 @@ where it has them.
 * ``--prefill``       ``fast``: the prompt in portions; ``loop``: one ``forward`` per token
 
 Added: ``--config JSON --random-weights`` (a model from a configuration and
-``--seed``), ``--dtype``, ``--page-size``, ``--num-pages``, ``--max-batch-tokens``,
+``--seed``), ``--dtype``, ``--kv-dtype`` (``int8``: keys and values cached in 8 bits), ``--page-size``, ``--num-pages``, ``--max-batch-tokens``,
 ``--temperature`` (0.6), ``--top-p`` (0.9), ``--max-new-tokens`` (1024),
 ``--prompt-ids 1,2,3`` (one shot, no loop), ``--stats``.
 
