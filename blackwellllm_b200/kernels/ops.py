@@ -1609,7 +1609,8 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
     """:func:`paged_attention` over an 8-bit cache (which already holds this step's keys and values): bfloat16 queries [T, nh * head_dim],
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
     held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator.  ``dealt``: what
-    :func:`quant_attention_deal` made of the step."""
+    :func:`quant_attention_deal` made of the step.  In a graph that is replayed with other lengths (``static_bound``) every request has at most
+    QUANT_FEW_ROWS tokens times heads of a group: longer portions stand where the host's positions were when they were recorded."""
     k = pages.k
     window, chunk = int(window or 0), int(chunk or 0)
     got = None
