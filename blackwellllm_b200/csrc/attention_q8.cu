@@ -661,11 +661,11 @@ static int clusters_at_once(int size) {
 // come (`bound` > 0: for every request).  `per`: tiles of a slice, so that the slices of all requests fill the GPU about once; `slices`: the
 // most of any request (0: there is no such request).
 // Where requests are about equally long, up to eight slices that all run at once are a cluster and join there; a join of its own (a launch,
-// and a trip through memory: about two tiles' time) serves more slices, and requests of many lengths, whose clusters would be half empty:
-// us with clusters and without, a token at 701 keys 6.2 and 7.6, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
+// and a trip through memory: about a tile's time) serves more slices, and requests of many lengths, whose clusters would be half empty:
+// us with clusters and without, a token at 701 keys 6.2 and 7.6, 2 at 2,000 8.9 and 9.5, 4 at 4,000 15.9 and 14.0, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
 // them 63.5 and 55.8, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 11.8.
 // A step whose lengths only the device will know, and may be long, gets the slices that run at once, to share by what the lengths are then.
-constexpr int CLUSTER_EXTRA = 2;
+constexpr int CLUSTER_EXTRA = 1;
 struct Plan { int per, slices, cluster, shared; };
 static Plan plan_slices(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound, bool whole) {
     auto tiles_of = [&](int r) -> long long {

@@ -677,7 +677,7 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
 // Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining (100
 // tokens alone 21 us; with eight steps at least, and so fewer blocks, 28; two steps make no difference).
 constexpr int LEAST_STEPS = 4;
-// what an item costs beside its steps (its queries, the first scores, its outputs), in steps: 2,048 tokens 74 us counted as five, 76 as four, 77 as eight
+// what an item costs beside its steps (its queries, the first scores, its outputs), in steps: 2,048 tokens 71 us counted as five, 73 as four, 72 as seven
 constexpr int ITEM_COST = 5;
 int blocks_for(long long cost) {
     const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;
