@@ -223,7 +223,10 @@ def compile_extension(name: str, verbose: bool = True) -> str:
 
     import torch
     root = os.path.dirname(torch.__file__)
-    cuda = os.path.dirname(os.path.dirname(find_nvcc()))
+    try:
+        cuda = os.path.dirname(os.path.dirname(find_nvcc()))
+    except BuildError:
+        cuda = "/usr/local/cuda"       # (a module that is built already needs no compiler)
     flags = [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
     flags.append(f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}")
     libs = ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]

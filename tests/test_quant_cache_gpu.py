@@ -384,3 +384,68 @@ def test_refusals():
         ops.quant_read(pages, b.positions, b.req_of_token[:0], table)
     with pytest.raises(ops.KernelError):
         ops.quant_read(pages, b.positions, b.req_of_token, table, torch.float16)
+
+
+def test_operands_that_do_not_fit_are_named_and_nothing_is_written():
+    """Every operand by itself wrong in type, place, shape, order or length: an error that is ours, and pages as they were."""
+    c = Case([(1, 3, 4), (20, 0, 20)], 2, 64, 16, seed=1).fill()
+    pages, b = c.pages(), c.batch()
+    table, nh = b.block_tables[0], 4
+    before = [t.clone() for t in (pages.k, pages.v, pages.k_scale, pages.v_scale)]
+    q = torch.zeros(21, nh * 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.ones(21, 8 * 64, device="cuda")
+    turns = torch.zeros(21, 64, device="cuda")
+
+    def wrong(t):
+        out = [t.double() if t.dtype == torch.float32 else t.float(), t.cpu(), t.flatten()]
+        if t.dim() > 1 and t.shape[-1] > 1:
+            out.append(t.transpose(-1, -2).contiguous().transpose(-1, -2))      # the same numbers in another order
+        return out
+
+    parts = [pages.k, pages.v, pages.k_scale, pages.v_scale]
+    tries = []
+    for i, t in enumerate(parts):
+        for w in wrong(t) + [t[:, :1].contiguous(), t[:-1]]:
+            bad = ops.QuantPages(*[w if j == i else p for j, p in enumerate(parts)])
+            tries += [lambda bad=bad: ops.quant_append(x, b.positions, b.req_of_token, table, bad, nh),
+                      lambda bad=bad: ops.quant_read(bad, b.positions, b.req_of_token, table),
+                      lambda bad=bad: ops.quant_attention(q, bad, b, table, nh, 0.1)]
+    for w in wrong(table):
+        tries += [lambda w=w: ops.quant_append(x, b.positions, b.req_of_token, w, pages, nh), lambda w=w: ops.quant_read(pages, b.positions, b.req_of_token, w),
+                  lambda w=w: ops.quant_attention(q, pages, b, w, nh, 0.1)]
+    tries.append(lambda: ops.quant_attention(q, pages, b, table[:1], nh, 0.1))
+    for w in (b.positions.long(), b.positions.cpu(), b.positions[:-1], b.positions.repeat_interleave(2)[::2]):
+        tries += [lambda w=w: ops.quant_append(x, w, b.req_of_token, table, pages, nh), lambda w=w: ops.quant_append(x, b.positions, w, table, pages, nh),
+                  lambda w=w: ops.quant_read(pages, w, b.req_of_token, table), lambda w=w: ops.quant_read(pages, b.positions, w, table)]
+    for w in wrong(x)[:2] + [x.flatten(), x.t().contiguous().t(), x[:, :-64].contiguous(), x[None, None], x[None].to(torch.bfloat16), x[None][:0],
+                             torch.ones(2, 21, 8 * 64 + 8, device="cuda")[:, :, :8 * 64]]:
+        tries.append(lambda w=w: ops.quant_append(w, b.positions, b.req_of_token, table, pages, nh))
+    for w in (turns.double(), turns.cpu(), turns[:-1], turns[:, :-1].contiguous(), torch.zeros(21, 66, device="cuda"), turns.t().contiguous().t()):
+        tries.append(lambda w=w: ops.quant_append(x, b.positions, b.req_of_token, table, pages, nh, table=w))
+    for w in wrong(q) + [q[:-1], q[:, :-64].contiguous()]:
+        tries.append(lambda w=w: ops.quant_attention(w, pages, b, table, nh, 0.1))
+    for name in ("cu_q", "q_start", "kv_len"):
+        for w in (getattr(b, name).long(), getattr(b, name).cpu(), getattr(b, name)[:1]):
+            other = c.batch()
+            setattr(other, name, w)
+            tries.append(lambda other=other: ops.quant_attention(q, pages, other, table, nh, 0.1))
+    for name, w in (("h_q_len", [1]), ("h_q_len", [1, 19]), ("h_q_len", [-1, 22]), ("h_q_len", [1, 2 ** 40]), ("h_q_start", [3]), ("h_q_start", [-3, 0]),
+                    ("h_q_start", [3, 2 ** 31 - 30]), ("T", 20), ("R", 3)):
+        other = c.batch()
+        setattr(other, name, w)
+        tries.append(lambda other=other: ops.quant_attention(q, pages, other, table, nh, 0.1))
+    for sink in (torch.zeros(nh, device="cuda").double(), torch.zeros(nh), torch.zeros(nh + 1, device="cuda"), torch.zeros(2 * nh, device="cuda")[::2]):
+        tries.append(lambda sink=sink: ops.quant_attention(q, pages, b, table, nh, 0.1, sink=sink))
+    for i, t in enumerate(tries):
+        with pytest.raises(ops.KernelError):
+            t()
+            pytest.fail(f"call {i} was taken")
+    assert all(torch.equal(a, t) for a, t in zip(before, parts))
+    # lengths as a tuple are as good as a list, and a batch without tokens has no rows
+    b.h_q_len, b.h_q_start = tuple(b.h_q_len), tuple(b.h_q_start)
+    assert ops.quant_attention(q, pages, b, table, nh, 0.1).shape == q.shape
+    none = Case([(0, 5, 5)], 2, 64, 16, seed=2).fill()
+    nb, np_ = none.batch(), none.pages()
+    assert ops.quant_attention(q[:0], np_, nb, nb.block_tables[0], nh, 0.1).shape == (0, nh * 64)
+    assert ops.quant_append(x[:0], nb.positions, nb.req_of_token, nb.block_tables[0], np_, nh).shape == (0, nh * 64)
+    assert ops.quant_read(np_, nb.positions, nb.req_of_token, nb.block_tables[0])[0].shape == (0, 2, 64)
