@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -34,6 +35,10 @@ bool whole(PyObject* o, int& n) {
     return true;
 }
 template <typename F> F entry(PyObject* address) { return reinterpret_cast<F>(PyLong_AsVoidPtr(address)); }
+// (past the dispatcher, which takes as long as the allocation)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, int device) {
+    return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
+}
 void* stream() { return (void*)c10::cuda::getCurrentCUDAStream().stream(); }
 const float* floats(const at::Tensor* t) { return t ? (const float*)t->const_data_ptr() : nullptr; }
 const int* ints(const at::Tensor* t) { return (const int*)t->const_data_ptr(); }
@@ -79,7 +84,7 @@ PyObject* quant_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int paired = PyObject_IsTrue(a[11]), append = PyObject_IsTrue(a[12]);
     if (paired < 0 || append < 0) return nullptr;
-    at::Tensor q = at::empty({T, (int64_t)nh * p.hd}, qkv->options().dtype(at::kBFloat16));
+    at::Tensor q = fresh({T, (int64_t)nh * p.hd}, at::kBFloat16, p.device);
     if (T > 0) {
         const int code = entry<AppendFn>(a[0])(qkv->const_data_ptr(), wide ? 0 : 1, (int)planes, d == 3 ? qkv->stride(0) : 0, rd ? floats(turns) : nullptr, (int)rd,
                                                paired, q.mutable_data_ptr(), nh, p.k->data_ptr(), p.v->data_ptr(), (float*)p.ks->data_ptr(),
@@ -109,8 +114,8 @@ PyObject* quant_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!is(pos, at::kInt, p.device) || !is(req, at::kInt, p.device) || pos->numel() != req->numel() || !small(pos->numel())) Py_RETURN_NONE;
     const bool wide = a[8] == Py_True;
     const int64_t T = pos->numel();
-    const auto options = p.ks->options().dtype(wide ? at::kFloat : at::kBFloat16);
-    at::Tensor k = at::empty({T, p.nkv, p.hd}, options), v = at::empty({T, p.nkv, p.hd}, options);
+    const at::ScalarType type = wide ? at::kFloat : at::kBFloat16;
+    at::Tensor k = fresh({T, p.nkv, p.hd}, type, p.device), v = fresh({T, p.nkv, p.hd}, type, p.device);
     if (T > 0) {
         const int code = entry<ReadFn>(a[0])(p.k->const_data_ptr(), p.v->const_data_ptr(), floats(p.ks), floats(p.vs), ints(pos), ints(req), ints(p.table),
                                              k.mutable_data_ptr(), v.mutable_data_ptr(), wide ? 0 : 1, (int)T, (int)p.table->size(0), (int)p.table->size(1),
@@ -159,14 +164,13 @@ PyObject* quant_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i : lens) { sum += i; most = i > most ? i : most; least = i < least ? i : least; }
     if (sum != T) Py_RETURN_NONE;
     const int G = nh / p.nkv, blocks = (int)p.table->size(1);
-    at::Tensor out = at::empty(q->sizes(), q->options());
+    at::Tensor out = fresh(q->sizes(), at::kBFloat16, p.device);
     long calls = 0;
     if (T > 0) {
-        const auto scratch = q->options().dtype(at::kFloat);
         if (most * G > few_rows) {
             const ll need = entry<RoomFn>(a[1])(lens.data(), starts.data(), R, few_rows, G, p.nkv, window, chunk);
             if (need < 0) return PyLong_FromLongLong(need);
-            at::Tensor room = at::empty({(int64_t)need}, scratch);
+            at::Tensor room = fresh({(int64_t)need}, at::kFloat, p.device);
             const int code = entry<ManyFn>(a[2])(q->const_data_ptr(), p.k->const_data_ptr(), p.v->const_data_ptr(), floats(p.ks), floats(p.vs),
                                                  out.mutable_data_ptr(), ints(len), ints(p.table), blocks, lens.data(), starts.data(), R, few_rows, nh, p.nkv,
                                                  p.page_size, p.num_pages, window, chunk, (float)scale, floats(sink), (float*)room.mutable_data_ptr(), need,
@@ -180,7 +184,7 @@ PyObject* quant_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             ll have = 0, need = 0;
             int code;
             do {
-                if (need) { room = at::empty({(int64_t)need}, scratch); have = need; }
+                if (need) { room = fresh({(int64_t)need}, at::kFloat, p.device); have = need; }
                 code = entry<FewFn>(a[0])(q->const_data_ptr(), p.k->const_data_ptr(), p.v->const_data_ptr(), floats(p.ks), floats(p.vs), out.mutable_data_ptr(),
                                           ints(cu), ints(start), ints(len), ints(p.table), blocks, lens.data(), starts.data(), R, nh, p.nkv, p.page_size,
                                           p.num_pages, window, chunk, bound, (float)scale, floats(sink), have ? (float*)room.mutable_data_ptr() : nullptr, have,
@@ -210,8 +214,8 @@ PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t R = x->size(0), V = x->size(1);
     if (V < 1 || !small(R) || !small(V) || x->stride(1) != 1 || (R > 1 && x->stride(0) < V) || target->numel() != R || top < 0 || top > most || top > V)
         Py_RETURN_NONE;
-    const auto f = x->options(), i = target->options();
-    at::Tensor got[5] = {at::empty({R}, f), at::empty({R}, f), at::empty({R}, i), at::empty({R, top}, i), at::empty({R, top}, f)};
+    at::Tensor got[5] = {fresh({R}, at::kFloat, device), fresh({R}, at::kFloat, device), fresh({R}, at::kInt, device), fresh({R, top}, at::kInt, device),
+                         fresh({R, top}, at::kFloat, device)};
     if (R > 0) {
         const int code = entry<ProbsFn>(a[0])(floats(x), ints(target), (float*)got[0].mutable_data_ptr(), (float*)got[1].mutable_data_ptr(),
                                               (int*)got[2].mutable_data_ptr(), (int*)got[3].mutable_data_ptr(), (float*)got[4].mutable_data_ptr(), (int)R, (int)V,

@@ -229,7 +229,7 @@ def compile_extension(name: str, verbose: bool = True) -> str:
         cuda = "/usr/local/cuda"       # (a module that is built already needs no compiler)
     flags = [f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
     flags.append(f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}")
-    libs = ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    libs = ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     return compile_host_library(name, verbose, flags, libs, {"python": sys.version, "torch": torch.__version__})
 
 
