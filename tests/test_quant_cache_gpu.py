@@ -449,3 +449,49 @@ def test_operands_that_do_not_fit_are_named_and_nothing_is_written():
     assert ops.quant_attention(q[:0], np_, nb, nb.block_tables[0], nh, 0.1).shape == (0, nh * 64)
     assert ops.quant_append(x[:0], nb.positions, nb.req_of_token, nb.block_tables[0], np_, nh).shape == (0, nh * 64)
     assert ops.quant_read(np_, nb.positions, nb.req_of_token, nb.block_tables[0])[0].shape == (0, 2, 64)
+
+
+def test_calls_on_two_streams_at_once_and_two_recorded_steps():
+    """Scratch is a call's own: decoding requests whose slices join through memory and portions of prompts, side by side on two streams, and
+    two graphs replayed in turn and side by side, give what each gives by itself."""
+    cases = [Case([(1, 9000, 9001), (1, 40, 41), (70, 300, 370)], 2, 64, 16, seed=s).fill() for s in (1, 2)]
+    work = []
+    for c in cases:
+        b = c.batch()
+        q = torch.randn(c.T, 8 * 64, generator=c.gen).to(torch.bfloat16).cuda()
+        work.append((q, c.pages(), b, b.block_tables[0]))
+
+    def run(i):
+        q, pages, b, table = work[i]
+        return ops.quant_attention(q, pages, b, table, 8, 0.125)
+
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+    # recorded: the same steps with their lengths left to the device
+    steps = []
+    for c in cases:
+        d = Case([(1, 9000, 9001), (1, 40, 41), (1, 700, 701)], 2, 64, 16, seed=c.T).fill()
+        b = d.batch(bound=16384)
+        q = torch.randn(d.T, 8 * 64, generator=d.gen).to(torch.bfloat16).cuda()
+        pages = d.pages()
+        alone = ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125)
+        steps.append((graph, out, alone, (q, pages, b)))
+    for _ in range(10):
+        for s, (graph, out, _, _) in zip(streams, steps):
+            with torch.cuda.stream(s):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, alone) for _, out, alone, _ in steps)
+    assert ops.attention_q8_status() == 0
