@@ -187,6 +187,7 @@ class CacheManager:
             if g.request.keep_first:
                 native().bwh_set_keep_first(self._h, gi, int(g.request.keep_first))
         self._handles: Dict[object, int] = {}
+        self._reserved: Dict[object, int] = {}      # tokens at a request's end that no launched step computes yet
         self._scratch = (ctypes.c_int * max(G, 1))()
         self.slots = _Slots(self)
 
@@ -205,6 +206,19 @@ class CacheManager:
 
     def length(self, rid) -> int:
         return int(native().bwh_length(self._h, self._handles[rid]))
+
+    def written(self, rid) -> int:
+        """The request's length without the tokens that are only reserved (:meth:`reserved`)."""
+        return self.length(rid) - self._reserved.get(rid, 0)
+
+    def reserved(self, rids, n: int) -> None:
+        """Records that the last ``n`` tokens of each request have their pages and that the step which computes them has not
+        been launched (0: it has).  Rolled back or freed, a request loses them first."""
+        for rid in rids:
+            if n and rid in self._handles:
+                self._reserved[rid] = n
+            else:
+                self._reserved.pop(rid, None)
 
     def slot(self, rid) -> int:
         return native().bwh_slot(self._h, self._handles[rid])
@@ -297,11 +311,14 @@ class CacheManager:
                              f"by the window and cannot be restored")
         if rc != 0:
             raise AssertionError(f"truncate({rid!r}, {new_length}): code {rc}: {_INVARIANTS.get(rc, 'bad argument')}")
+        if rid in self._reserved:
+            self.reserved([rid], max(0, self._reserved[rid] - (length - new_length)))
         if self._states and new_length == 0:
             self.zero_state(native().bwh_slot(self._h, h))
 
     def free_request(self, rid) -> None:
         h = self._handles.pop(rid)
+        self._reserved.pop(rid, None)
         rc = native().bwh_free_request(self._h, h)
         if rc < 0:
             raise AssertionError(f"free_request({rid!r}): code {rc}: {_INVARIANTS.get(rc, 'bad request')}")

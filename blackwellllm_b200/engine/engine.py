@@ -193,14 +193,15 @@ class Engine:
     def cached_kv(self, rid, layer: int, start: int = 0, stop: Optional[int] = None):
         """The keys (as attention reads them: rotated) and values that the request's cache holds for positions ``start`` to
         ``stop`` (None: all) of a layer that owns pages: two tensors [positions, kv heads, head size] in the model's dtype; of a cache in 8
-        bits the numbers times their scales.  Zeros at positions whose pages a window has given back."""
+        bits the numbers times their scales.  Zeros at positions whose pages a window has given back.  A token that a step
+        prepared ahead has reserved counts from that step's launch on."""
         from ..kernels import ops
         if not self.cache.has(rid):
             raise EngineError(f"request {rid!r} is not live")
         view = self.cache.views[layer] if 0 <= layer < len(self.cache.views) else None
         if not isinstance(view, PagedKVView):
             raise EngineError(f"layer {layer} owns no pages of keys and values")
-        n = self.cache.length(rid)
+        n = self.cache.written(rid)
         stop = n if stop is None else stop
         if not 0 <= start <= stop <= n:
             raise EngineError(f"positions {start} to {stop} are not within the request's {n} cached ones")
@@ -423,6 +424,7 @@ class Engine:
                                        replay_width=self._graph_width, defer_send=True)
         except (OutOfPages, EngineError):
             return None
+        self.cache.reserved(rids, 1)
         return PreparedDecode(list(rids), host, total, slot, self._builder.last_ring_slot)
 
     def launch_prepared(self, prep: "PreparedDecode", tokens: Sequence[int]) -> torch.Tensor:
@@ -440,6 +442,7 @@ class Engine:
             self.cancel_prepared(prep)
             raise
         prep.rids_done = True
+        self.cache.reserved(prep.rids, 0)
         self.cache.release_passed_many(prep.rids)
         self.steps_run += 1
         self.tokens_run += len(prep.rids)

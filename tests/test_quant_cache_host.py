@@ -210,3 +210,42 @@ def test_cached_rows_are_read_by_position(monkeypatch):
     for start, stop in ((-1, 2), (5, 4), (0, 30)):
         with pytest.raises(EngineError, match="positions"):
             eng.cached_kv("a", 0, start, stop)
+
+
+def test_cached_rows_end_before_a_token_that_is_only_reserved(monkeypatch):
+    """A step prepared ahead makes its requests longer by a token that nobody has computed: no row of it is read until the step is
+    launched, and none once it is cancelled, rolled back or its request is freed."""
+    class Graph:
+        def replay(self):
+            pass
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a, **k: None)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+    monkeypatch.setattr(torch.cuda, "graph", lambda graph: contextlib.nullcontext())
+    cfg = parse_config(tiny.TINY_LLAMA)
+    eng = Engine(cfg, PagesOnly(cfg.vocab_size), EngineOptions(dtype="float32", page_size=8, num_pages=12, max_requests=3, device="cpu", graph_after=1))
+
+    def rows():
+        return [eng.cached_kv(r, layer)[0].shape[0] for r in ("a", "b") for layer in (0, 1)]
+
+    eng.step([StepEntry("a", [1] * 5, []), StepEntry("b", [1] * 8, [])])
+    eng.step([StepEntry("a", [1], [0]), StepEntry("b", [1], [0])])       # recorded: from here on steps are prepared ahead
+    assert rows() == [6, 6, 9, 9]
+    prep = eng.prepare_decode_ahead(["a", "b"])
+    assert prep is not None and [eng.cache.length(r) for r in ("a", "b")] == [7, 10]
+    assert rows() == [6, 6, 9, 9]
+    with pytest.raises(EngineError, match="positions"):
+        eng.cached_kv("a", 0, 0, 7)
+    eng.launch_prepared(prep, [1, 2])
+    assert rows() == [7, 7, 10, 10]
+    prep = eng.prepare_decode_ahead(["a", "b"])
+    assert rows() == [7, 7, 10, 10]
+    eng.cancel_prepared(prep)
+    assert rows() == [7, 7, 10, 10] and [eng.cache.length(r) for r in ("a", "b")] == [7, 10]
+    # rolled back to a position before it, or freed and begun again, while the step is still prepared
+    eng.prepare_decode_ahead(["a", "b"])
+    eng.cache.truncate("a", 4)
+    eng.end_request("b")
+    eng.step([StepEntry("b", [1] * 3, [])])
+    assert rows() == [4, 4, 3, 3]
