@@ -9,10 +9,11 @@
 // (which is then off by at most a few 2^-24 of 1152 sum |q|, a few 1e-7 of the largest score that such a key can have).
 //   Queries: a row is multiplied by a power of two that brings its largest channel to 2^14 up to 2^15, so that bfloat16's eight bits
 //      fit float16's eleven whatever the row's size (channels below 2^-31 of the largest lose bits); the power comes off the score.
-//   Weights: with the value's scale inside the exponent, w_ij = 2^(t_ij + log2 vs_j - m_i), t the score in powers of two.  The reference m follows
-//      the largest t + log2 vs, so what counts most is near 1 and float16 rounds each weight by at most 2^-11 of itself, or of 2^-14: never
-//      more than 2^-25 of the largest.  The denominator is the sum of w / vs in float32.  A value's scale of 0 counts as 2^-100 (its
-//      whole numbers are zeros).
+//   Weights: w_ij = e_ij vs_j with e_ij = 2^(t_ij - m_i), t the score in powers of two.  The reference m follows the largest t + log2 vs, so what
+//      counts most is near 1 and float16 rounds each weight by at most 2^-11 of itself, or of 2^-14: never more than 2^-25 of the largest.
+//      The denominator is the sum of e in float32.  For the reference a scale counts as 2^-102 at least (rows of zeros have 0), so e stays
+//      below 2^110 and 2^18 keys below infinity; the smallest scale that is written, 2^-117, then still has weights of 2^-15.  Where m moves far
+//      (rows of zeros, then values that are large) sums are multiplied by the root of the factor twice, which never vanishes by itself.
 // Everything else is float32: scores, references, sums, outputs.
 //
 // The products are turned around: S^T = K Q^T and O^T = V^T W^T, keys and channels in the 16 rows of an instruction, queries in its 8
@@ -47,7 +48,7 @@ constexpr int KEYS = 16;                           // keys that a warp works on 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int TILE = 128;                          // keys that slices are counted in: a step of a block's warps, or two
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LEAST_SCALE = 7.888609052210118e-31f;   // 2^-100
+constexpr float LEAST_LOG = -102.f;                // a value's scale, in powers of two, as the reference sees it
 
 struct Params {
     const bf16* q; bf16* out;
@@ -103,11 +104,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float reciprocal(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -218,13 +214,15 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
             for (int nb = 0; nb < NB; ++nb) mma(sc[nb], a, s.qf[c + i][nb][0], s.qf[c + i][nb][1]);
         }
     }
-    float most[NB][2], per_v[2], kk[2], lv[2];
+    float most[NB][2], kk[2], vv[2], lv[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        kk[i] = ks[r + 8 * i];
-        const float v = vs[r + 8 * i], v1 = v < LEAST_SCALE ? LEAST_SCALE : v;      // (NaN stays)
-        lv[i] = lg2(v1);
-        per_v[i] = reciprocal(v1);
+        // (a key that is no number, or whose value is none, has NaN as its score, and nothing else of it reaches who does not see it)
+        const float k = ks[r + 8 * i], v = vs[r + 8 * i];
+        const bool fine = k < INFINITY && v < INFINITY;
+        kk[i] = fine ? k : __uint_as_float(0x7fffffffu);
+        vv[i] = fine ? v : 0.f;
+        lv[i] = fmaxf(lg2(vv[i]), LEAST_LOG);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -232,13 +230,13 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int e = i & 1;
-            float t = fmaf((sc[nb][i] + s.off[nb][e]) * s.mul[nb][e], kk[i >> 1], lv[i >> 1]);
+            float t = (sc[nb][i] + s.off[nb][e]) * s.mul[nb][e] * kk[i >> 1];
             if (need_mask) {
                 const int j = r + 8 * (i >> 1), kp = key0 + j;
                 if (!(kp <= s.pos[nb][e] && kp >= s.lo[nb][e] && (there >> j & 1))) t = -INFINITY;
             }
             sc[nb][i] = t;
-            most[nb][e] = fmaxf(most[nb][e], t);
+            most[nb][e] = fmaxf(most[nb][e], t + lv[i >> 1]);
         }
     }
     bool grown = false;
@@ -255,9 +253,10 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                 const float m_new = fmaxf(s.m[nb][e], mx);
-                corr[e] = m_new == -INFINITY ? 0.f : ex2(s.m[nb][e] - m_new);     // nothing seen so far: 0
+                const float root = m_new == -INFINITY ? 0.f : ex2(0.5f * (s.m[nb][e] - m_new));     // nothing seen so far: 0
+                corr[e] = root * root;
                 s.m[nb][e] = m_new;
-                s.l[nb][e] *= corr[e];
+                s.l[nb][e] = s.l[nb][e] * root * root;
             }
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
@@ -272,9 +271,9 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = ex2(sc[nb][i] - ref[i & 1]);
-            // (a key that is not seen counts nothing whatever its scale is: a later token's value may be no number)
-            s.l[nb][i & 1] += need_mask && sc[nb][i] == -INFINITY ? 0.f : w[i] * per_v[i >> 1];
+            const float x = ex2(sc[nb][i] - ref[i & 1]);
+            s.l[nb][i & 1] += x;
+            w[i] = x * vv[i >> 1];
         }
         wf[nb][0] = turn8x8(pack_f16x2(w[0], w[1]));
         wf[nb][1] = turn8x8(pack_f16x2(w[2], w[3]));
@@ -441,6 +440,12 @@ __device__ __forceinline__ Walk walk_of(const Params& p, int q_pos0, int last, i
     return w;
 }
 
+// Outputs and a sum that stand against the reference m, added to others against M >= m.
+__device__ __forceinline__ void add_part(float4& acc, float& L, float4 v, float m, float l, float M) {
+    const float root = m == -INFINITY ? 0.f : ex2(0.5f * (m - M)), f = root * root;
+    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    L += l * root * root;
+}
 __device__ __forceinline__ void write_row(const Params& p, size_t token, int head, int c, float4 v, float L) {
     // (a row that sees nothing is zeros; a sum that is no number stays one)
     const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -532,10 +537,8 @@ few_kernel(Params p) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float mw = ms[w * 16 + row], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
             const float4 v = *reinterpret_cast<const float4*>(os + (w * 16 + row) * JOIN_LD + c);
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-            L += ls[w * 16 + row] * f;
+            add_part(acc, L, v, ms[w * 16 + row], ls[w * 16 + row], M);
         }
         if (walk.live == 1) {
             const int t = row / p.G, head = g * p.G + row - t * p.G;
@@ -571,9 +574,7 @@ few_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < MOST_CLUSTER; ++i) {
             if (i >= walk.live) break;
-            const float f = x[i].x == -INFINITY ? 0.f : exp2f(x[i].x - M);
-            acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
-            L += x[i].y * f;
+            add_part(acc, L, v[i], x[i].x, x[i].y, M);
         }
         const int t = row / p.G, head = g * p.G + row - t * p.G;
         write_row(p, (size_t)(tok + t), head, c, acc, L + sink_term(p, head, M));
@@ -614,9 +615,7 @@ join_kernel(Params p) {
         for (int i = group; i < live; i += JOIN_GROUPS) {
             const float2 x = ml[base + i * step];
             const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + i * step) * HD)[quad];
-            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-            L += x.y * f;
+            add_part(acc, L, v, x.x, x.y, M);
         }
         red[group][quad] = acc;
         if (quad == 0) red_l[group] = L;

@@ -1460,6 +1460,7 @@ def _loaded_libs():
 class QuantPages:
     """Pages of keys and values held in 8 bits: ``k`` and ``v`` int8 [num_pages, nkv, page_size, head_dim], whole numbers of -127 to 127, and
     ``k_scale``, ``v_scale`` float32 [num_pages, nkv, page_size], one scale per (token, kv head): a channel's value is number * scale.
+    Attention takes value scales of 0 (with numbers of 0 alone) and of 2^-117, the smallest that is written, to 2^100.
     Views of a pool are fine as long as each is contiguous."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale")

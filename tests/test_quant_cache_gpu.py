@@ -495,3 +495,43 @@ def test_calls_on_two_streams_at_once_and_two_recorded_steps():
         torch.cuda.synchronize()
         assert all(torch.equal(out, alone) for _, out, alone, _ in steps)
     assert ops.attention_q8_status() == 0
+
+
+def scales_far_apart(c, kind):
+    """The case's value rows again: ``tiny`` from what is barely written on, ``zeros`` rows of nothing beside loud ones, ``wide`` everything."""
+    lo, hi = {"tiny": (-117, -95), "zeros": (29, 31), "wide": (-117, 95)}[kind]
+    draws = torch.rand(c.v_scale.shape, generator=c.gen)
+    c.v_scale = torch.exp2(lo + 0.02 + (hi - lo) * draws).float()
+    if kind == "zeros":
+        empty = torch.rand(c.v_scale.shape, generator=c.gen) < 0.7
+        c.v_scale[empty], c.v[empty] = 0.0, 0
+        # a request's first keys as well, so that a slice begins with them
+        for r in range(len(c.segments)):
+            first = int(c.table[r, 0])
+            c.v_scale[first], c.v[first] = 0.0, 0
+    return c
+
+
+def check_scales(c, nh):
+    """As ``check_attention``, with the bound for the scales that the reference counts as 2^-102 and nothing absolute in it."""
+    hd = c.hd
+    q = torch.randn(c.T, nh * hd, generator=c.gen).to(torch.bfloat16)
+    b = c.batch()
+    got = ops.quant_attention(q.cuda(), c.pages(), b, b.block_tables[0], nh, hd ** -0.5).cpu().double().view(c.T, nh, hd)
+    e = attention(q.view(c.T, nh, hd), c.k, c.v, c.k_scale, c.v_scale, c.cu, c.start, c.total, c.table, hd ** -0.5)
+    # a weight is within 2^-25 of the largest, p times a scale of at least 2^-102: p is at most 1, and the numbers of a channel as many as
+    # keys, at most 127 each
+    low = 2.0 ** -25 * 2.0 ** -102 * 127 * (c.pos + 1).double()[:, None, None]
+    tol = attention_bound(e, hd) - 1e-30 + 1.01 * low
+    over = ((got - e.out).abs() / tol).max().item()
+    assert torch.isfinite(got).all() and over <= 1.0, f"error {over:.2f} times the bound"
+    assert ops.attention_q8_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["tiny", "zeros", "wide"])
+@pytest.mark.parametrize("hd,nh,nkv,page", [(128, 8, 2, 16), (64, 7, 1, 8), (80, 16, 1, 24)])
+def test_value_scales_far_apart(kind, hd, nh, nkv, page):
+    """A few rows a request, one slice and many: what a scale of 2^-117 leaves, rows of zeros that keep their share, and both beside large ones."""
+    segs = [(1, 40, 41), (1, 699, 700), (1, 0, 1), (2 if nh // nkv <= 8 else 1, 30, 32 if nh // nkv <= 8 else 31)]
+    check_scales(scales_far_apart(Case(segs, nkv, hd, page, seed=hd + len(kind)).fill(), kind), nh)
+    check_scales(scales_far_apart(Case([(1, 9000, 9001)], nkv, hd, page, seed=hd + 1).fill(), kind), nh)
