@@ -219,7 +219,7 @@ __device__ __forceinline__ void some_keys(Queries<NB>& s, uint32_t k_rows, uint3
     for (int i = 0; i < 2; ++i) {
         // (a key that is no number, or whose value is none, has NaN as its score, and nothing else of it reaches who does not see it)
         const float k = ks[r + 8 * i], v = vs[r + 8 * i];
-        const bool fine = k < INFINITY && v < INFINITY;
+        const bool fine = max(__float_as_uint(k), __float_as_uint(v)) < 0x7f800000u;
         kk[i] = fine ? k : __uint_as_float(0x7fffffffu);
         vv[i] = fine ? v : 0.f;
         lv[i] = fmaxf(lg2(vv[i]), LEAST_LOG);

@@ -3,29 +3,33 @@
 //
 // A block works on 256 stacked rows (row = token * G + head of the group) of one (request, kv head) as two tiles of 128 (one, of head sizes
 // above 128: tensor memory holds no more) against tiles of 64 keys:
-//   * eight warps widen, four keys and four values: rows of whole numbers from the cache (16 bytes a load, straight into registers) become float16 times the row's scale
-//     over the largest scale of the 64 (a power of two, which goes back into the scores, and for the values into the exponent), and
-//     are written as the 128-byte-swizzled operands of the tensor cores.  Both tiles of rows use them: widening is a third of the
-//     block's instructions, and the reason why a block has 256 rows and is alone on its SM;
+//   * eight warps widen, four keys and four values: whole numbers from the cache (16 bytes a load, straight into registers) become bfloat16 (keys) and
+//     float16 (values), exact in both, and are written as the 128-byte-swizzled operands of the tensor cores.  Both tiles of rows use them:
+//     widening is a third of the block's instructions, and the reason why a block has 256 rows and is alone on its SM;
 //   * one warp issues S = Q K^T (M 128, N 64) into one of two buffers a tile of rows, another O += P V with P from tensor memory (one warp for
 //     both spent two thirds of its time between its products);
-//   * eight warps, one thread a row, make P: maximum, exponentials, sums; P is written over the S it came from as float16 pairs.
-// Roundings: K and V to float16, twice (their scale, and the product: 2^-11 of an element each; below 2^-14 of the tile's largest scale 2^-25 of that), P to float16 (the same,
-// beside the largest), and the result to bfloat16.  Scores, sums and outputs are float32; the queries are multiplied by a power of two a row
-// (attention_q8.cu) and exact.  The exponents' reference follows the largest t + log2 of the tile's value scale lazily (by steps of more than
-// 8), so O is seldom rescaled.
+//   * eight warps make P: products times the keys' scales, the values' scales inside the exponent, maximum, exponentials, sums; P is written as
+//     float16 pairs over the S that it came from.  A lane has 16 columns of four rows and not 64 of one: what it reads of the 64 keys' scales
+//     serves four rows (a row a thread would read four times as many bytes from shared memory).
+// Roundings: P to float16 (2^-11 of a weight, or 2^-25 of the row's largest), and the result to bfloat16.  Whole numbers and queries are exact, the
+// scales are multiplied or added in float32: a row's result has nothing of a key that the row does not see.  (Scales inside the operands, over
+// the largest scale of the 64 keys beside them, are a twentieth faster for 2,048 tokens and a tenth behind a long context, but a row then depends
+// on later tokens: one value 2^18 times as loud leaves float16's subnormals to those beside it.)  Scores, sums and outputs are float32.  Sums
+// of products stay below infinity for queries up to 2^112.  The exponents' reference follows the largest t + log2 vs that the row sees
+// lazily (RISE), so O is seldom rescaled.  With the scale inside the exponent, weights 2^126 below the reference vanish, and their part of the sum with
+// them: value scales that a row sees are to lie within 2^100 of each other (the key-slice kernel, which has instructions to spare, takes any).
 // A key that is no number (its scale, or its value's, is NaN) has NaN as its score: rows that see it become NaN, masked rows do not.  Keys behind
-// the request's end or on a page that is not held are zeros, and masked.
+// the request's end or on a page that is not held are masked, whatever stands in their place.
 //
 // Work is the list of all (rows, tile of keys) steps of the launch, cut into equal stretches, one a block, so that the last wave is not mostly
 // empty and a few rows over many keys still fill the GPU.  A stretch that begins or ends inside a block of rows leaves its sums in
 // memory; join_kernel adds them in the order of the keys.  Every wait is bounded (status word).
 //
-// 2,048 tokens of 32 heads of 128 on 8 kv heads: 71 us, 487 TFLOP/s; 2,048 behind 13,312 (40 heads on 8) 672 us, 895 of 1,652 that a large product
-// has.  A step (256 rows, 64 keys) takes 2,500 cycles, and nothing alone bounds it: the softmax's warps are busy for 2,000 of them, the products
-// need 1,500 (N 64 reads as many bytes of Q as it has work for), the widening 1,700.  Late piece without the exponentials 3 percent less,
-// without the widening's arithmetic 7, without seven eighths of Q K^T 10, without the softmax 15.  An item costs about five steps beside (its
-// queries come and are converted, the first scores, the outputs): of the 71 us a third.
+// 2,048 tokens of 32 heads of 128 on 8 kv heads: 73.5 us, 467 TFLOP/s; 2,048 behind 13,312 (40 heads on 8) 740 us, 812 of 1,652 that a large product
+// has, in bursts.  A step (256 rows, 64 keys) takes about 2,700 cycles, and nothing alone bounds it: the softmax's warps are busy for most of
+// them, the products need 1,500 (N 64 reads as many bytes of Q as it has work for).  Late piece without the exponentials 4 percent less, with
+// keys widened at the cost of values 2, where no reference ever moves 5.  An item costs about five steps beside (its queries come, the first
+// scores, the outputs): of the 74 us a third.
 #include "tcgen05.cuh"
 #include <cuda_fp16.h>
 
@@ -58,12 +62,19 @@ constexpr int THREADS = 32 * (QK_WARP + 4);
 constexpr int SOFTMAX_REGS = NQ == 2 ? 144 : 168, WIDEN_REGS = NQ == 2 ? 72 : 112, ISSUE_REGS = 48;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-constexpr int SMEM_BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + RING * 32 + 32 * 8 + 16;
+// What the softmax needs of a tile of keys.
+struct TileInfo {
+    float kl[BN / 2][4];            // of two neighbouring keys: ks, then lv; a weight in powers of two is the product times ks plus lv (a value's scale)
+    float per_v[BN];                // what makes of a weight its part of the sum: the scale comes off, and SUM_SHIFT
+    unsigned there[2], bad[2];      // bits: keys that are held, and that are no number
+};
+constexpr int SMEM_BYTES = NQ * Q_BYTES + 2 * STAGES * KV_BYTES + RING * (int)sizeof(TileInfo) + 32 * 8 + 16;
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t idesc_f16(int N, bool b_mn_major) {
-    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-}
-constexpr uint32_t IDESC_QK = idesc_f16(BN, false), IDESC_PV = idesc_f16(HD, true);
+// float16 operands, B's rows the keys (the values), beside bw::umma_idesc_bf16 (queries and keys)
+constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+constexpr float ZERO_LOG = -60.f;           // a value's scale of 0, in powers of two (its whole numbers are zeros)
+constexpr float SUM_SHIFT = -20.f, SUM_UNIT = 1.f / (1 << 20);          // sums are kept times 2^this: of scales of 2^-117 they would reach infinity
+constexpr float RISE = 14.f;                // a reference moves when a weight is 2^this times what it was taken from (float16 ends at 2^16)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MOST_BLOCKS = 160;            // blocks of a launch
 constexpr int MOST_PORTIONS = 16;           // requests of a launch
@@ -159,25 +170,59 @@ __device__ __forceinline__ bw::f32x2 add2(bw::f32x2 a, bw::f32x2 b) {
     return d;
 }
 
-// Two bytes of r (128 too large) times a row's factor (a float16 number, twice): 0x6400 | byte is 1024 + byte, 1152 less is the whole number,
-// exact; the product is rounded.
-template <int SEL>
-__device__ __forceinline__ uint32_t widen2(uint32_t r, uint32_t f) {
-    uint32_t n, d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(n) : "r"(__byte_perm(r, 0x64646464u, SEL)), "r"(0x64806480u));
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(n), "r"(f));
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two bytes of r (chosen by SEL) as bfloat16, exact: 0x4300 | the lower seven bits is 128 more than they are, and what comes off is 128, or with
+// the sign's bit 256 (0x4380).
+template <int SEL> __device__ __forceinline__ uint32_t key2(uint32_t r) {
+    const uint32_t x = __byte_perm(r, 0x43434343u, SEL);
+    uint32_t d;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x & 0xff7fff7fu), "r"(x & 0xff80ff80u));
     return d;
 }
-// 16 channels of a key, as the two units of its row of operands
-__device__ __forceinline__ void widen16(uint8_t* first, uint8_t* second, uint4 x, uint32_t f) {
-    const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-    *reinterpret_cast<uint4*>(first) = make_uint4(widen2<0x4140>(w[0], f), widen2<0x4342>(w[0], f), widen2<0x4140>(w[1], f), widen2<0x4342>(w[1], f));
-    *reinterpret_cast<uint4*>(second) = make_uint4(widen2<0x4140>(w[2], f), widen2<0x4342>(w[2], f), widen2<0x4140>(w[3], f), widen2<0x4342>(w[3], f));
+// As float16: a byte with its top bit turned over is 128 more, 0x6400 | byte 1024 more.
+template <int SEL> __device__ __forceinline__ uint32_t value2(uint32_t r) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(__byte_perm(r, 0x64646464u, SEL)), "r"(0x64806480u));
+    return d;
 }
-// The smallest power of two that is not below any finite one of a warp's non-negative numbers (bits of the largest); at least 2^-100.
-__device__ __forceinline__ float power_above(unsigned bits) {
-    const unsigned up = (bits + 0x7fffffu) & 0x7f800000u;
-    return __uint_as_float(max(up, 27u << 23));
+// 16 channels, as the two units of a row of operands
+__device__ __forceinline__ void widen_key(uint8_t* first, uint8_t* second, uint4 x) {
+    *reinterpret_cast<uint4*>(first) = make_uint4(key2<0x4140>(x.x), key2<0x4342>(x.x), key2<0x4140>(x.y), key2<0x4342>(x.y));
+    *reinterpret_cast<uint4*>(second) = make_uint4(key2<0x4140>(x.z), key2<0x4342>(x.z), key2<0x4140>(x.w), key2<0x4342>(x.w));
+}
+__device__ __forceinline__ void widen_value(uint8_t* first, uint8_t* second, uint4 x) {
+    const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+    *reinterpret_cast<uint4*>(first) = make_uint4(value2<0x4140>(w[0]), value2<0x4342>(w[0]), value2<0x4140>(w[1]), value2<0x4342>(w[1]));
+    *reinterpret_cast<uint4*>(second) = make_uint4(value2<0x4140>(w[2]), value2<0x4342>(w[2]), value2<0x4140>(w[3]), value2<0x4342>(w[3]));
+}
+
+// 16 lanes of tensor memory by 64 columns: a lane of the warp gets columns 8 j + 2 (lane & 3) and the next of row lane / 4 (v[4 j], v[4 j + 1]) and of
+// row lane / 4 + 8 (v[4 j + 2], v[4 j + 3]).
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(at) : "memory");
+}
+// The same lanes' float16 pairs: column 4 j + (lane & 3) of row lane / 4 from v[2 j], of row lane / 4 + 8 from v[2 j + 1].
+__device__ __forceinline__ void tmem_st_16x32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        :: "r"(at),
+           "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+           "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
 }
 
 template <int N>
@@ -185,9 +230,11 @@ __device__ __forceinline__ void outputs_at(uint32_t at, uint32_t (&o)[N]) {
     if constexpr (N == 32) bw::tmem_ld_32x32(at, o);
     else bw::tmem_ld_32x16(at, o);
 }
-
-// What the softmax needs of a tile of keys.
-struct TileInfo { float k_ref, log2_v, inv_v, pad; unsigned there[2]; unsigned pad2[2]; };
+template <int N>
+__device__ __forceinline__ void outputs_to(uint32_t at, const uint32_t (&o)[N]) {
+    if constexpr (N == 32) bw::tmem_st_32x32(at, o);
+    else bw::tmem_st_32x16(at, o);
+}
 
 __global__ void __launch_bounds__(THREADS, 1)
 attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work) {
@@ -268,7 +315,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ++ks)
                             bw::umma_bf16(tmem0 + 128 * q + 64 * b, behind(dq, (q * Q_BYTES + (ks >> 2) * Q_SLICE) / 16 + 2 * (ks & 3)),
-                                          behind(dks, (ks >> 2) * (KV_SLICE / 16) + 2 * (ks & 3)), IDESC_QK, ks != 0);
+                                          behind(dks, (ks >> 2) * (KV_SLICE / 16) + 2 * (ks & 3)), bw::umma_idesc_bf16(BM, BN), ks != 0);
                         bw::umma_commit(s_full + 8 * (2 * q + b));
                         if (q == tiles_q - 1) bw::umma_commit(k_empty + 8 * s);
                     }
@@ -348,14 +395,13 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             for (int i = 0; i < 2; ++i) got[i] = (unsigned)x.page[i] < (unsigned)p.num_pages ? (x.page[i] * p.nkv + x.g) * p.page_size + x.slot[i] : -1;
             return Rows{got[0], got[1]};
         };
-        auto scale = [&](const float* of, int row) { return row >= 0 ? of[row] : 0.f; };
         if (w.left > 0) {
             Walk ahead = w;
             Rows rows = rows_of(look_up(ahead));
             Pages next{{-1, -1}, {0, 0}, 0};
             if (ahead.left > 1) { ahead.step(p, work); next = look_up(ahead); }
             // A unit of the next step is loaded as soon as this step's is widened, into the same registers: it has a whole step to come.  Where no
-            // row is, the pool's first is read, and its factor is 0.
+            // row is, the pool's first is read, and masked.
             uint4 x[2][PER];
             const int8_t* base = from + 16 * (lane & 3);
             const int swap = SWAP && odd ? 1 : 0;            // slice j of this lane is slice j ^ swap of the row
@@ -368,7 +414,13 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
 #pragma unroll
                 for (int j = 0; j < PER; ++j) { x[0][j] = unit_of(a, j); x[1][j] = unit_of(b, j); }
             }
-            float ks[2] = {scale(p.k_scale, rows.a), scale(p.k_scale, rows.b)}, vs[2] = {scale(p.v_scale, rows.a), scale(p.v_scale, rows.b)};
+            // of the keys' warps: each looks after the scales of 16 keys, keys' in the lower lanes, values' in the upper ones
+            const int own_key = 16 * ww + (lane & 15);
+            auto scale_of = [&](const Rows& x) {
+                const int row = __shfl_sync(0xffffffffu, ww < 2 ? x.a : x.b, own_key & 31);
+                return keys && row >= 0 ? (lane < 16 ? p.k_scale : p.v_scale)[row] : 0.f;
+            };
+            float own = scale_of(rows);
             unsigned there0 = __ballot_sync(0xffffffffu, rows.a >= 0), there1 = __ballot_sync(0xffffffffu, rows.b >= 0);
             // where this lane's units go: rows mine and mine + 32, units 2 (lane & 3) and the next of every slice, permuted by the row
             uint8_t* first = tiles + mine * 128 + (((2 * (lane & 3)) ^ (mine & 7)) << 4);
@@ -379,50 +431,43 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 rows = rows_of(next);                                                     // of the next step (behind the last: none)
                 const int8_t *a = base + (size_t)max(__shfl_sync(0xffffffffu, rows.a, mine), 0) * HD, *b = base + (size_t)max(__shfl_sync(0xffffffffu, rows.b, mine), 0) * HD;
                 // (into the first-level cache now; loaded only behind the fence below, which waits for loads under way)
-                // references and factors
-                unsigned kb = 0, vb = 0;
-                bool bad[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const unsigned y = __float_as_uint(ks[i]), z = __float_as_uint(vs[i]);
-                    bad[i] = max(y, z) >= 0x7f800000u;
-                    kb = max(kb, bad[i] ? 0u : y);
-                    vb = max(vb, bad[i] ? 0u : z);
-                }
-                const float k_ref = power_above(__reduce_max_sync(0xffffffffu, kb)), v_ref = power_above(__reduce_max_sync(0xffffffffu, vb));
-                // (powers of two: the exponent turned around)
-                const float inv_v = __uint_as_float((254u << 23) - __float_as_uint(v_ref)),
-                            inv = keys ? __uint_as_float((254u << 23) - __float_as_uint(k_ref)) : inv_v;
-                uint32_t f[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float own = bad[i] ? (keys ? __uint_as_float(0x7fffffffu) : 0.f) : (keys ? ks[i] : vs[i]) * inv;
-                    f[i] = __shfl_sync(0xffffffffu, pack_f16x2(own, own), mine);
-                }
                 if (it >= STAGES && !all(bw::mbar_wait(empty + 8 * s, ((it / STAGES) - 1) & 1, &g_status, keys ? 37 : 38))) break;
-                if (warp == KEY_WARP && lane == 0) {
-                    TileInfo t;
-                    t.k_ref = k_ref; t.inv_v = inv_v;
-                    t.log2_v = (float)((int)(__float_as_uint(v_ref) >> 23) - 127);
-                    t.there[0] = there0; t.there[1] = there1;
-                    t.pad = 0.f; t.pad2[0] = t.pad2[1] = 0;
-                    info[it % RING] = t;
+                if (keys) {
+                    TileInfo& t = info[it % RING];
+                    const bool fine = __float_as_uint(own) < 0x7f800000u;
+                    const unsigned bad = __ballot_sync(0xffffffffu, !fine);
+                    float* kl = &t.kl[own_key >> 1][own_key & 1];
+                    // (ks positive and finite: a masked product, -infinity, stays that)
+                    if (lane < 16) kl[0] = fine ? fminf(fmaxf(own * p.scale_log2, 1.17549435e-38f), 3.402823466e38f) : 1.f;
+                    else {
+                        const float lv = fine && own > 0.f ? fmaxf(lg2(own), -126.f) : ZERO_LOG;
+                        kl[2] = lv;
+                        t.per_v[own_key] = ex2(SUM_SHIFT - lv);
+                    }
+                    if (lane == 0) {
+                        reinterpret_cast<unsigned short*>(t.bad)[ww] = (unsigned short)(bad | bad >> 16);
+                        if (ww == 0) { t.there[0] = there0; t.there[1] = there1; }
+                    }
+                    __syncwarp();
                 }
                 there0 = __ballot_sync(0xffffffffu, rows.a >= 0); there1 = __ballot_sync(0xffffffffu, rows.b >= 0);
-                // (one piece of code for keys and values: what an SM quarter's warps run over and over has to fit its instruction cache)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     if (!has(j)) continue;
                     const int to = s * KV_BYTES + j * KV_SLICE + (j & 1 ? -KV_SLICE : KV_SLICE) * swap;
-                    widen16(first + to, second + to, x[0][j], f[0]);
-                    widen16(first + to + 32 * 128, second + to + 32 * 128, x[1][j], f[1]);
+                    if (keys) {
+                        widen_key(first + to, second + to, x[0][j]);
+                        widen_key(first + to + 32 * 128, second + to + 32 * 128, x[1][j]);
+                    } else {
+                        widen_value(first + to, second + to, x[0][j]);
+                        widen_value(first + to + 32 * 128, second + to + 32 * 128, x[1][j]);
+                    }
                 }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(full + 8 * s);
                 __syncwarp();
-                ks[0] = scale(p.k_scale, rows.a); ks[1] = scale(p.k_scale, rows.b);
-                vs[0] = scale(p.v_scale, rows.a); vs[1] = scale(p.v_scale, rows.b);
+                own = scale_of(rows);
 #pragma unroll
                 for (int j = 0; j < PER; ++j) { x[0][j] = unit_of(a, j); x[1][j] = unit_of(b, j); }
                 next = Pages{{-1, -1}, {0, 0}, 0};
@@ -430,7 +475,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             }
         }
     } else {
-        // ---------------------------------------------------------------- softmax: tile of rows `q`, one thread a row
+        // ---------------------------------------------------------------- softmax: tile of rows `q`
         more_registers<SOFTMAX_REGS>();
         const int q = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -456,36 +501,16 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             const bool mine = q < q_tiles(item);
             const int gr = item.row0 + q * BM + row;                    // the row among the request's
             const bool row_ok = q * BM + row < item.n_rows;
-            const int tok = gr / p.G, head = item.g * p.G + gr - tok * p.G, qpos = item.q_pos0 + tok;
+            const int tok = gr / p.G, head = item.g * p.G + gr - tok * p.G;
             const int own_row = (item.tok + tok) * p.nh + head;         // of the queries and outputs
-            float sc = 0.f;             // what turns a product into a power of two, but for the tile's reference
             if (mine) {
                 // The warp's 32 rows come together (16 bytes a lane, neighbours of a row side by side: a row a lane would touch 32 lines with every
-                // load) and lie in their place in shared memory as they are; then every lane turns its row into float16 times a power of two.
+                // load) and lie in their place in shared memory as they are.
                 move_rows(own_row, row_ok, [&](int r, int u, size_t from, bool live) {
                     const int bytes = live ? 16 : 0;       // 0: zeros are written
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(bw::smem_u32(unit_at(r, u))), "l"(p.q + from), "r"(bytes) : "memory");
                 });
                 asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
-                __syncwarp();
-                unsigned most2 = 0;                       // of the even and of the odd channels, as 16-bit numbers
-#pragma unroll 4
-                for (int u = 0; u < UNITS; ++u) {
-                    const uint4 x = *unit_at(lane, u);
-                    most2 = __vmaxu2(__vmaxu2(most2, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
-                    most2 = __vmaxu2(__vmaxu2(most2, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
-                }
-                const unsigned most = max(most2 & 0xffffu, most2 >> 16);
-                unsigned ex = max(most >> 7, 15u);
-                if (ex == 255) ex = 141;                                // an infinity or NaN: as it is
-                const float up = __uint_as_float((268 - ex) << 23);
-                sc = __uint_as_float((ex - 14) << 23) * p.scale_log2;
-                auto two = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up); };
-#pragma unroll 4
-                for (int u = 0; u < UNITS; ++u) {
-                    const uint4 x = *unit_at(lane, u);
-                    *unit_at(lane, u) = make_uint4(two(x.x), two(x.y), two(x.z), two(x.w));
-                }
                 bw::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) bw::mbar_arrive(q_full + 8 * q);
@@ -496,82 +521,150 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
                 continue;
             }
 
-            const int lo = bw::first_visible(qpos, p.window, p.chunk);
             // the warp's rows that exist: positions of the first and the last
             const int warp_row = item.row0 + q * BM + (warp & 3) * 32, end_row = item.row0 + item.n_rows - 1;
             const int first_pos = item.q_pos0 + min(warp_row, end_row) / p.G, last_pos = item.q_pos0 + min(warp_row + 31, end_row) / p.G;
             const int see_all = bw::first_visible(last_pos, p.window, p.chunk);
-            float m = -INFINITY, l = 0.f;
+            // The lane's rows of the 32: lane / 4 and every eighth from there (columns: tmem_ld_16x64).  A row that does not exist stands against
+            // infinity: its weights are zeros, and no maximum moves it.
+            int pos[4];
+            float m4[4];
+            bw::f32x2 l4[4];            // this lane's columns only, even and odd ones
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = warp_row + 8 * i + (lane >> 2);
+                pos[i] = item.q_pos0 + r / p.G;
+                m4[i] = r <= end_row ? -INFINITY : INFINITY;
+                l4[i] = 0ull;
+            }
+            // from a lane's rows to row `lane` of the warp: row 8 i + k lies in lanes 4 k to 4 k + 3
+            auto own_row_of = [&](const float (&x)[4]) {
+                float got = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = __shfl_sync(0xffffffffu, x[i], 4 * (lane & 7));
+                    if (lane >> 3 == i) got = y;
+                }
+                return got;
+            };
             const int t_first = w.tile, t_end = w.end;
             for (int t = t_first; t < t_end; ++t, ++it, ++c) {
                 const int b = c & 1;
                 if (!all(bw::mbar_wait(s_full + 8 * (2 * q + b), (c >> 1) & 1, &g_status, 39))) { ok = false; break; }
                 bw::tc_fence_after();
-                const TileInfo ti = info[it % RING];
+                const TileInfo& ti = info[it % RING];
                 const int key0 = t * BN;
-                uint32_t v[BN];
-                bw::tmem_ld_32x32(tmem_S + 64 * b, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-                bw::tmem_ld_32x32(tmem_S + 64 * b + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+                uint32_t v[2][32];
+                tmem_ld_16x64(tmem_S + 64 * b, v[0]);
+                tmem_ld_16x64(tmem_S + 64 * b + (16u << 16), v[1]);
                 bw::tmem_ld_wait();
+                const unsigned bad = ti.bad[0] | ti.bad[1];
                 const bool gone = (ti.there[0] & ti.there[1]) != 0xffffffffu;
-                if (gone || key0 + BN - 1 > first_pos || key0 < see_all) {      // one branch a tile
-                    // key j is seen for j <= qpos - key0 and j >= lo - key0, if it is there: a mask of 64 bits
-                    const int hi_j = qpos - key0, lo_j = lo - key0;
-                    unsigned long long seen = (unsigned long long)ti.there[1] << 32 | ti.there[0];
-                    if (hi_j < 0 || lo_j > 63) seen = 0;
-                    else {
-                        if (hi_j < 63) seen &= (2ull << hi_j) - 1;
-                        if (lo_j > 0) seen &= ~0ull << lo_j;
-                    }
-                    const unsigned seen0 = (unsigned)seen, seen1 = (unsigned)(seen >> 32);
+                if (gone || bad || key0 + BN - 1 > first_pos || key0 < see_all) {      // one branch a tile
+                    const unsigned long long held = (unsigned long long)ti.there[1] << 32 | ti.there[0], none = (unsigned long long)ti.bad[1] << 32 | ti.bad[0];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (!(seen0 >> j & 1)) v[j] = 0xff800000u;
-                        if (!(seen1 >> j & 1)) v[32 + j] = 0xff800000u;
+                    for (int i = 0; i < 4; ++i) {
+                        // key j is seen for j <= position - key0 and j >= lo - key0, if it is there: a mask of 64 bits
+                        const int hi_j = pos[i] - key0, lo_j = bw::first_visible(pos[i], p.window, p.chunk) - key0;
+                        unsigned long long seen = held;
+                        if (hi_j < 0 || lo_j > 63) seen = 0;
+                        else {
+                            if (hi_j < 63) seen &= (2ull << hi_j) - 1;
+                            if (lo_j > 0) seen &= ~0ull << lo_j;
+                        }
+                        const unsigned long long mine = seen >> (2 * (lane & 3)), nan = none >> (2 * (lane & 3));
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t& x = v[i >> 1][4 * j + 2 * (i & 1) + e];
+                                if (!(mine >> (8 * j + e) & 1)) x = 0xff800000u;
+                                else if (nan >> (8 * j + e) & 1) x = 0x7fffffffu;
+                            }
                     }
                 }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // weights in powers of two, and the largest of each row
+                auto pair = [&](int i, int j) {
+                    const uint32_t* x = &v[i >> 1][4 * j + 2 * (i & 1)];
+                    return bw::pack2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < BN; j += 2)
-                    mx4[(j >> 1) & 3] = fmaxf(mx4[(j >> 1) & 3], fmaxf(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
-                const float f = fmaxf(sc * ti.k_ref, 1e-36f);     // (positive: the maximum commutes with it, and -infinity stays)
-                const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), f, ti.log2_v);
-                const bool grow = row_ok && mx > m + 8.f;
+                for (int j = 0; j < 8; ++j) {
+                    const ulonglong2 kl = *reinterpret_cast<const ulonglong2*>(ti.kl[4 * j + (lane & 3)]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float a, d;
+                        bw::unpack2(bw::fma2(pair(i, j), kl.x, kl.y), a, d);
+                        v[i >> 1][4 * j + 2 * (i & 1)] = __float_as_uint(a);
+                        v[i >> 1][4 * j + 2 * (i & 1) + 1] = __float_as_uint(d);
+                        mx[i] = fmaxf(mx[i], fmaxf(a, d));
+                    }
+                }
+                bool grow = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) grow |= mx[i] > m4[i] + RISE;
+                grow = __any_sync(0xffffffffu, grow);
                 float shrink = 1.f;
                 if (grow) {
-                    shrink = m == -INFINITY ? 1.f : ex2(m - mx);
-                    l *= shrink;
-                    m = mx;
+                    float factor[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+                        float root = 1.f;          // (attention_q8.cu: squares of roots)
+                        if (mx[i] > m4[i] + RISE) {
+                            if (m4[i] != -INFINITY) root = ex2(0.5f * (m4[i] - mx[i]));
+                            m4[i] = mx[i];
+                        }
+                        factor[i] = root * root;
+                        l4[i] = bw::mul2(bw::mul2(l4[i], bw::pack2(root, root)), bw::pack2(root, root));
+                    }
+                    shrink = own_row_of(factor);
                 }
-                if (t > t_first && __any_sync(0xffffffffu, grow)) {
-                    // O may be read once the P V of the step before is done
+                bw::f32x2 less[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = m4[i] == -INFINITY ? 0.f : -m4[i];
+                    less[i] = bw::pack2(x, x);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bw::f32x2 per_v = *reinterpret_cast<const bw::f32x2*>(ti.per_v + 8 * j + 2 * (lane & 3));
+#pragma unroll
+                        for (int i = 2 * h; i < 2 * h + 2; ++i) {
+                            float a, d;
+                            bw::unpack2(add2(pair(i, j), less[i]), a, d);
+                            a = ex2(a);
+                            d = ex2(d);
+                            l4[i] = bw::fma2(bw::pack2(a, d), per_v, l4[i]);
+                            v[h][2 * j + (i & 1)] = pack_f16x2(a, d);      // (a place whose score is done with)
+                        }
+                    }
+                    tmem_st_16x32(tmem_S + 64 * b + (uint32_t)h * (16u << 16), v[h]);
+                }
+                if (grow && t > t_first) {
+                    // O may be read once the P V of the step before is done; the next one waits for this warp.  (Behind the weights, whose registers are
+                    // free for 64 columns at a time; ahead of them, sixteen by sixteen, the late piece took 3 percent more.)
                     if (!all(bw::mbar_wait(pv_done + 8 * (2 * q + (b ^ 1)), ((c - 1) >> 1) & 1, &g_status, 40))) { ok = false; break; }
                     bw::tc_fence_after();
+                    constexpr int COLS = HD % 64 == 0 ? 2 : 1;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD; c0 += 16) {
-                        uint32_t o[16];
-                        bw::tmem_ld_32x16(tmem_Oq + c0, o);
+                    for (int c0 = 0; c0 < HD; c0 += COLS * O_STEP) {
+                        uint32_t o[COLS][O_STEP];
+#pragma unroll
+                        for (int h = 0; h < COLS; ++h) outputs_at(tmem_Oq + c0 + h * O_STEP, o[h]);
                         bw::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                        bw::tmem_st_32x16(tmem_Oq + c0, o);
-                    }
-                    bw::tmem_st_wait();
-                }
-                const float less = ti.log2_v - (m == -INFINITY ? 0.f : m);
-                const bw::f32x2 f2 = bw::pack2(f, f), less2 = bw::pack2(less, less);
-                bw::f32x2 sum2[2] = {0ull, 0ull};
+                        for (int h = 0; h < COLS; ++h) {
 #pragma unroll
-                for (int j = 0; j < BN; j += 2) {
-                    float a, d;
-                    bw::unpack2(bw::fma2(bw::pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f2, less2), a, d);
-                    a = ex2(a);
-                    d = ex2(d);
-                    sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], bw::pack2(a, d));
-                    v[j >> 1] = pack_f16x2(a, d);
+                            for (int j = 0; j < O_STEP; ++j) o[h][j] = __float_as_uint(__uint_as_float(o[h][j]) * shrink);
+                            outputs_to(tmem_Oq + c0 + h * O_STEP, o[h]);
+                        }
+                    }
                 }
-                bw::tmem_st_32x32(tmem_S + 64 * b, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-                l = fmaf(bw::sum2(add2(sum2[0], sum2[1])), ti.inv_v, l);
                 bw::tmem_st_wait();
                 bw::tc_fence_before();
                 __syncwarp();
@@ -580,9 +673,18 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             }
             if (!ok || !(ok = all(bw::mbar_wait(pv_done + 8 * (2 * q + ((c - 1) & 1)), ((c - 1) >> 1) & 1, &g_status, 41)))) break;
             bw::tc_fence_after();
+            float sums[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sums[i] = bw::sum2(l4[i]);
+                sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], 1);
+                sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], 2);
+            }
+            float l = own_row_of(sums);
+            const float m = own_row_of(m4);
             if (w.opens && w.closes) {
-                if (p.sink && row_ok) l += ex2(p.sink[head] * LOG2E - m);
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                if (p.sink && row_ok) l += ex2(p.sink[head] * LOG2E - m + SUM_SHIFT);
+                const float inv = l == 0.f ? 0.f : SUM_UNIT / l;
                 // (the queries are done with: the warp's outputs take their place, and go out 16 bytes a lane, a row's side by side)
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += O_STEP) {
@@ -657,19 +759,20 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (b + j <= to) most = fmaxf(most, x[j].x);
-        const float less = M == -INFINITY ? 0.f : ex2(M - most);
+        // (factors as the squares of their roots, which never vanish by themselves: attention_q8.cu)
+        const float root = M == -INFINITY ? 0.f : ex2(0.5f * (M - most)), less = root * root;
         M = most;
-        acc.x *= less; acc.y *= less; acc.z *= less; acc.w *= less; L *= less;
+        acc.x *= less; acc.y *= less; acc.z *= less; acc.w *= less; L = L * root * root;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float f = b + j > to || x[j].x == -INFINITY ? 0.f : ex2(x[j].x - M);
+            const float part = b + j > to || x[j].x == -INFINITY ? 0.f : ex2(0.5f * (x[j].x - M)), f = part * part;
             acc.x = fmaf(o[j].x, f, acc.x); acc.y = fmaf(o[j].y, f, acc.y); acc.z = fmaf(o[j].z, f, acc.z); acc.w = fmaf(o[j].w, f, acc.w);
-            L = fmaf(x[j].y, f, L);
+            L = fmaf(x[j].y * part, part, L);
         }
     }
     const int gr = it.row0 + r, tok = gr / p.G, head = it.g * p.G + gr - tok * p.G;
-    if (p.sink) L += ex2(p.sink[head] * LOG2E - M);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (p.sink) L += ex2(p.sink[head] * LOG2E - M + SUM_SHIFT);
+    const float inv = L == 0.f ? 0.f : SUM_UNIT / L;
     *reinterpret_cast<uint2*>(p.out + ((size_t)(it.tok + tok) * p.nh + head) * HD + 4 * quad) =
         make_uint2(bw::pack_bf16x2(acc.x * inv, acc.y * inv), bw::pack_bf16x2(acc.z * inv, acc.w * inv));
 }
@@ -677,7 +780,7 @@ join_kernel(const __grid_constant__ Params p, const __grid_constant__ Work work,
 // Blocks of a launch: one an SM, but no fewer steps a block than pay for its start (queries, tensor memory) and its part of the joining (100
 // tokens alone 21 us; with eight steps at least, and so fewer blocks, 28; two steps make no difference).
 constexpr int LEAST_STEPS = 4;
-// what an item costs beside its steps (its queries, the first scores, its outputs), in steps: 2,048 tokens 71 us counted as five, 73 as four, 72 as seven
+// what an item costs beside its steps (its queries, the first scores, its outputs), in steps: 2,048 tokens 74 us counted as five, 78 as four, 87 as three
 constexpr int ITEM_COST = 5;
 int blocks_for(long long cost) {
     const long long sms = bw::num_sms() < MOST_BLOCKS ? bw::num_sms() : MOST_BLOCKS;

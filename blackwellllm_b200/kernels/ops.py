@@ -1460,7 +1460,8 @@ def _loaded_libs():
 class QuantPages:
     """Pages of keys and values held in 8 bits: ``k`` and ``v`` int8 [num_pages, nkv, page_size, head_dim], whole numbers of -127 to 127, and
     ``k_scale``, ``v_scale`` float32 [num_pages, nkv, page_size], one scale per (token, kv head): a channel's value is number * scale.
-    Attention takes value scales of 0 (with numbers of 0 alone) and of 2^-117, the smallest that is written, to 2^100.
+    Attention takes value scales of 0 (with numbers of 0 alone) and of 2^-117, the smallest that is written, to 2^100.  Those of one
+    request lie within a factor of 2^100 of each other, 0 counting as 2^-60, where more than QUANT_FEW_ROWS rows of a step attend to it.
     Views of a pool are fine as long as each is contiguous."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale")
@@ -1609,8 +1610,8 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
                     chunk: Optional[int] = None, sink: Optional[torch.Tensor] = None, dealt: Optional[QuantDealt] = None) -> torch.Tensor:
     """:func:`paged_attention` over an 8-bit cache (which already holds this step's keys and values): bfloat16 queries [T, nh * head_dim],
     bfloat16 result.  A query sees the keys from ``first_visible(position, window, chunk)`` to its own position whose pages are
-    held; one that sees none gets zeros.  ``sink`` (float32 [nh]): one more term exp(sink) in a row's denominator.  ``dealt``: what
-    :func:`quant_attention_deal` made of the step.  In a graph that is replayed with other lengths (``static_bound``) every request has at most
+    held; one that sees none gets zeros.  Scores in powers of two stay below 2^27, queries below 2^112.  ``sink`` (float32 [nh]): one more
+    term exp(sink) in a row's denominator.  ``dealt``: what :func:`quant_attention_deal` made of the step.  In a graph that is replayed with other lengths (``static_bound``) every request has at most
     QUANT_FEW_ROWS tokens times heads of a group: longer portions stand where the host's positions were when they were recorded."""
     k = pages.k
     window, chunk = int(window or 0), int(chunk or 0)

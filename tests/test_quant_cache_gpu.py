@@ -498,8 +498,9 @@ def test_calls_on_two_streams_at_once_and_two_recorded_steps():
 
 
 def scales_far_apart(c, kind):
-    """The case's value rows again: ``tiny`` from what is barely written on, ``zeros`` rows of nothing beside loud ones, ``wide`` everything."""
-    lo, hi = {"tiny": (-117, -95), "zeros": (29, 31), "wide": (-117, 95)}[kind]
+    """The case's value rows again: ``tiny`` from what is barely written on, ``zeros`` rows of nothing beside loud ones, ``wide`` everything,
+    ``spread`` as far apart as portions of prompts take it."""
+    lo, hi = {"tiny": (-117, -95), "zeros": (29, 31), "wide": (-117, 95), "spread": (-60, 39)}[kind]
     draws = torch.rand(c.v_scale.shape, generator=c.gen)
     c.v_scale = torch.exp2(lo + 0.02 + (hi - lo) * draws).float()
     if kind == "zeros":
@@ -512,16 +513,16 @@ def scales_far_apart(c, kind):
     return c
 
 
-def check_scales(c, nh):
-    """As ``check_attention``, with the bound for the scales that the reference counts as 2^-102 and nothing absolute in it."""
+def check_scales(c, nh, counts=-102):
+    """As ``check_attention`` with nothing absolute in the bound, but for scales that count as 2^``counts`` in the reference of a row's weights."""
     hd = c.hd
     q = torch.randn(c.T, nh * hd, generator=c.gen).to(torch.bfloat16)
     b = c.batch()
     got = ops.quant_attention(q.cuda(), c.pages(), b, b.block_tables[0], nh, hd ** -0.5).cpu().double().view(c.T, nh, hd)
     e = attention(q.view(c.T, nh, hd), c.k, c.v, c.k_scale, c.v_scale, c.cu, c.start, c.total, c.table, hd ** -0.5)
-    # a weight is within 2^-25 of the largest, p times a scale of at least 2^-102: p is at most 1, and the numbers of a channel as many as
+    # a weight is within 2^-25 of the largest, p times a scale of at least that: p is at most 1, and the numbers of a channel as many as
     # keys, at most 127 each
-    low = 2.0 ** -25 * 2.0 ** -102 * 127 * (c.pos + 1).double()[:, None, None]
+    low = 2.0 ** -25 * 2.0 ** counts * 127 * (c.pos + 1).double()[:, None, None]
     tol = attention_bound(e, hd) - 1e-30 + 1.01 * low
     over = ((got - e.out).abs() / tol).max().item()
     assert torch.isfinite(got).all() and over <= 1.0, f"error {over:.2f} times the bound"
@@ -535,3 +536,42 @@ def test_value_scales_far_apart(kind, hd, nh, nkv, page):
     segs = [(1, 40, 41), (1, 699, 700), (1, 0, 1), (2 if nh // nkv <= 8 else 1, 30, 32 if nh // nkv <= 8 else 31)]
     check_scales(scales_far_apart(Case(segs, nkv, hd, page, seed=hd + len(kind)).fill(), kind), nh)
     check_scales(scales_far_apart(Case([(1, 9000, 9001)], nkv, hd, page, seed=hd + 1).fill(), kind), nh)
+
+
+@pytest.mark.parametrize("kind", ["plain", "tiny", "zeros", "spread"])
+@pytest.mark.parametrize("hd,nh,nkv,page", [(128, 8, 2, 16), (64, 7, 1, 8), (256, 4, 1, 24), (96, 6, 2, 16)])
+def test_portions_keep_what_the_bound_of_a_few_rows_grants(kind, hd, nh, nkv, page):
+    """Portions of prompts round weights and results alone: they are within the bound without anything for keys and values, whatever their scales."""
+    c = Case([(70, 0, 70), (41, 160, 201), (1, 99, 100), (130, 600, 730)], nkv, hd, page, seed=hd * 5 + len(kind)).fill()
+    # (scales of 0 count as 2^-60 there, others as they are)
+    check_scales(c if kind == "plain" else scales_far_apart(c, kind), nh, -60 if kind == "zeros" else -1000)
+
+
+@pytest.mark.parametrize("hd,nh,nkv", [(128, 8, 2), (64, 6, 1), (192, 2, 1)])
+@pytest.mark.parametrize("louder", [2.0 ** 14, 2.0 ** 20, 2.0 ** 30])
+def test_a_later_token_leaves_the_rows_before_it_alone(hd, nh, nkv, louder):
+    """Prompts whose tokens from some position on, in the tile of rows that do not see them, are far louder, or no numbers: the rows before
+    have the same bits, and those of the same prompt cut there within the bound."""
+    n, at = 230, 141
+    c = Case([(n, 0, n)], nkv, hd, 16, seed=hd).fill()
+    q = torch.randn(n, nh * hd, generator=c.gen).to(torch.bfloat16).cuda()
+    b = c.batch()
+    quiet = ops.quant_attention(q, c.pages(), b, b.block_tables[0], nh, 0.1)
+    page, slot = row_index(c.pos, c.req, c.table, c.page)
+    for factor in (louder, math.nan):
+        for scales in (c.k_scale, c.v_scale):
+            scales[page[at:], :, slot[at:]] *= factor
+        loud = ops.quant_attention(q, c.pages(), b, b.block_tables[0], nh, 0.1)
+        assert torch.equal(loud[:at], quiet[:at])
+        if factor == louder:
+            # (rows that see the loud keys have scores of up to 2^40: exponentials of their float32 errors have no bound, and there is none for them)
+            e = attention(q.cpu().view(n, nh, hd), c.k, c.v, c.k_scale, c.v_scale, c.cu, c.start, c.total, c.table, 0.1)
+            assert ((loud.cpu().double().view_as(e.out) - e.out).abs() <= attention_bound(e, hd))[:at].all()
+            cut = Case([(at, 0, at)], nkv, hd, 16, seed=hd)
+            cut.k, cut.v, cut.k_scale, cut.v_scale, cut.table = c.k, c.v, c.k_scale, c.v_scale, c.table
+            cb = cut.batch()
+            alone = ops.quant_attention(q[:at].contiguous(), cut.pages(), cb, cb.block_tables[0], nh, 0.1)
+            assert ((alone.cpu().double().view(at, nh, hd) - e.out[:at]).abs() <= attention_bound(e, hd)[:at]).all()
+        else:
+            assert torch.isnan(loud[at:]).all()
+    assert ops.attention_q8_status() == 0
