@@ -23,7 +23,8 @@
 //
 // Work is the list of all (rows, tile of keys) steps of the launch, cut into equal stretches, one a block, so that the last wave is not mostly
 // empty and a few rows over many keys still fill the GPU.  A stretch that begins or ends inside a block of rows leaves its sums in
-// memory; join_kernel adds them in the order of the keys.  Every wait is bounded (status word).
+// memory; join_kernel adds them in the order of the keys.  Every wait is bounded: one that gives up sets the status word, and the rows that it left out, and
+// all rows of later launches until the status is read, are NaN.
 //
 // 2,048 tokens of 32 heads of 128 on 8 kv heads: 73.5 us, 467 TFLOP/s; 2,048 behind 13,312 (40 heads on 8) 740 us, 812 of 1,652 that a large product
 // has, in bursts.  A step (256 rows, 64 keys) takes about 2,700 cycles, and nothing alone bounds it: the softmax's warps are busy for most of
@@ -274,7 +275,8 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
     Walk w;
     w.start(p, work);                                    // (of the launch's own numbers, while the kernel before is still at work)
     BW_PDL_WAIT();
-    if (tmem_slot[1] != 0) w.left = 0;                   // an earlier launch gave up: nothing is done
+    bool ok = tmem_slot[1] == 0;                         // else an earlier launch gave up: nothing is done, and the rows are no numbers
+    if (!ok && warp >= KEY_WARP) w.left = 0;
 
     if (warp >= QK_WARP) {
         fewer_registers<ISSUE_REGS>();
@@ -285,7 +287,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         if (warp == QK_WARP) {
             const uint64_t dq = bw::umma_smem_desc_sw128(bw::smem_u32(q_s)), dk = bw::umma_smem_desc_sw128(bw::smem_u32(k_s));
             int loaded[NQ] = {};                         // times that a tile's queries came
-            bool begins = true, ok = true;
+            bool begins = true;
             for (int it = 0; ok && w.left > 0; ++it) {
                 const int s = it % STAGES, tiles_q = q_tiles(w.it);
                 if (begins) {
@@ -326,7 +328,7 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             }
         } else if (warp == PV_WARP) {
             const uint64_t dv = bw::umma_smem_desc_mn_sw128(bw::smem_u32(v_s), KV_SLICE);
-            bool begins = true, ok = true;
+            bool begins = true;
             for (int it = 0; ok && w.left > 0; ++it) {
                 const int s = it % STAGES, tiles_q = q_tiles(w.it);
                 if (!all(bw::mbar_wait(v_full + 8 * s, (it / STAGES) & 1, &g_status, 34))) break;
@@ -481,7 +483,6 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tmem_S = tmem_base + 128 * q + lanes, tmem_Oq = tmem_O + q * O_COLS + lanes;
         int it = 0, c = 0;              // steps of the walk, and those of them that this tile of rows has
-        bool ok = true;
         constexpr int UNITS = HD / 8;   // of 16 bytes: a row of queries or outputs
         uint8_t* rows32 = q_s + q * Q_BYTES + (warp & 3) * 32 * 128;        // the warp's rows of the queries' tile
         auto unit_at = [&](int r, int u) { return reinterpret_cast<uint4*>(rows32 + (u >> 3) * Q_SLICE + r * 128 + (((u & 7) ^ (r & 7)) << 4)); };
@@ -722,6 +723,19 @@ attn_q8_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Work
             bw::tc_fence_before();
             w.pass(p, work);
         }
+        // a wait gave up, here or in a launch before: what is left of the stretch must not pass for a result
+        for (; w.left > 0; w.pass(p, work)) {
+            const Item item = w.it;
+            const int r = q * BM + row, gr = item.row0 + r, tok = gr / p.G;
+            if (q >= q_tiles(item) || r >= item.n_rows) continue;
+            if (w.opens && w.closes) {
+                uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)(item.tok + tok) * p.nh + item.g * p.G + gr - tok * p.G) * HD);
+#pragma unroll 1
+                for (int u = 0; u < UNITS; ++u) dst[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            } else {
+                reinterpret_cast<float2*>(p.part_ml)[(2 * (size_t)blockIdx.x + (w.opens ? 1 : 0)) * ROWS + r] = make_float2(0.f, __uint_as_float(0x7fffffffu));
+            }
+        }
     }
     bw::tc_fence_before();
     __syncthreads();
@@ -883,6 +897,9 @@ BW_EXPORT int bw_attention_q8_tc(const void* q, const void* k, const void* v, co
         return 0;
     });
 }
+
+// Sets the status as a wait that gives up does, for a test of what follows from that (synchronises the device).
+BW_EXPORT int bw_attention_q8_tc_give_up(int code) { return (int)cudaMemcpyToSymbol(g_status, &code, sizeof(int)); }
 
 // 0 if no bounded wait ever gave up; clears the status (synchronises the device).
 BW_EXPORT int bw_attention_q8_tc_status() {

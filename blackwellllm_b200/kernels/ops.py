@@ -1646,7 +1646,8 @@ def quant_attention(q: torch.Tensor, pages: QuantPages, batch, block_table: torc
 
 
 def attention_q8_status() -> int:
-    """0 if no bounded wait in the tcgen05 attention over an 8-bit cache ever gave up (synchronises the device)."""
+    """0 if no bounded wait in the tcgen05 attention over an 8-bit cache ever gave up (synchronises the device).  After one has, rows of
+    more than QUANT_FEW_ROWS a request are NaN, in later calls too, until this has been called."""
     total = 0
     for key, lib in list(_loaded_libs().items()):
         if key.startswith("attention_q8_tc"):

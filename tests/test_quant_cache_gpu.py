@@ -575,3 +575,20 @@ def test_a_later_token_leaves_the_rows_before_it_alone(hd, nh, nkv, louder):
         else:
             assert torch.isnan(loud[at:]).all()
     assert ops.attention_q8_status() == 0
+
+
+def test_after_a_wait_gave_up_rows_are_no_numbers():
+    """With the status set, as a wait that gives up sets it, nothing passes for a result: whole items and such as several blocks share (joined
+    from parts) are NaN until the status has been read; requests of few rows are another kernel's."""
+    from blackwellllm_b200.kernels.build import load_library
+    c = Case([(200, 0, 200), (1, 40, 41), (70, 3000, 3070)], 2, 64, 16, seed=3).fill()
+    b, pages = c.batch(), c.pages()
+    q = torch.randn(c.T, 4 * 64, generator=c.gen).to(torch.bfloat16).cuda()
+    want = ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.125)
+    assert ops.attention_q8_status() == 0 and torch.isfinite(want).all()
+    assert load_library("attention_q8_tc", {"HEAD_DIM": 64}).bw_attention_q8_tc_give_up(39) == 0
+    for _ in range(2):
+        got = ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.125)
+        assert torch.isnan(got[:200]).all() and torch.isnan(got[201:]).all() and torch.equal(got[200], want[200])
+    assert ops.attention_q8_status() == 39 and ops.attention_q8_status() == 0
+    assert torch.equal(ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.125), want)
