@@ -824,7 +824,8 @@ static int launches(const int* h_q_len, const int* h_q_start, int requests, int 
         if (n < 0 || h_q_start[r] < 0 || (long long)h_q_start[r] + n > 0x7fffff00ll) return BW_ERR_BAD_ARG;
         const long long rows = (long long)n * G, blocks = (rows + ROWS - 1) / ROWS;
         if (rows > min_rows) {
-            if (rows > 0x3fffffffll || items + blocks * nkv > 0x3fffffffll) return BW_ERR_UNSUPPORTED;
+            // (items, and rows of the queries, are counted in 32 bits)
+            if (rows > 0x3fffffffll || items + blocks * nkv > 0x3fffffffll || (tok + (long long)n) * G * nkv > 0x7fffffffll) return BW_ERR_UNSUPPORTED;
             work.portion[count] = {r, tok, n, h_q_start[r], items, (int)blocks};
             items += (int)blocks * nkv;
             if (++count == MOST_PORTIONS) if (const int e = flush()) return e;

@@ -249,3 +249,13 @@ def test_cached_rows_end_before_a_token_that_is_only_reserved(monkeypatch):
     eng.end_request("b")
     eng.step([StepEntry("b", [1] * 3, [])])
     assert rows() == [4, 4, 3, 3]
+
+
+@pytest.mark.parametrize("lens", [(1 << 24,), (1 << 23, 1 << 23), (1, 1 << 24)])
+def test_more_rows_of_queries_than_32_bits_count_are_refused(lens):
+    """2^24 tokens of 256 heads are 2^32 rows: places in the queries and outputs would wrap."""
+    room = entry("attention_q8_tc", "bw_attention_q8_tc_room", ctypes.c_longlong)
+    starts = [0] * len(lens)
+    assert room(ints(*lens), ints(*starts), len(lens), 16, 16, 16, 0, 0) == -2
+    few = [n >> 4 for n in lens]
+    assert room(ints(*few), ints(*starts), len(lens), 16, 16, 16, 0, 0) > 0
