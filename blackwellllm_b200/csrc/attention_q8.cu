@@ -61,6 +61,7 @@ struct Params {
     int cluster;                    // the slices of a (request, kv head) are one cluster of blocks and join there
     int shared;                     // > 0: the requests share `slices` slices by their lengths (see deal_kernel), none counted longer than this
     int* dealt;                     // then: which slice is whose
+    int slots;                      // slices of a kv head that run at once
     float scale_log2;
 };
 
@@ -385,9 +386,26 @@ template <typename T> __device__ __forceinline__ T read_block(uint32_t at, int r
     return v;
 }
 
-// Where only the device knows the lengths of a step (it was captured), `slices` blocks a kv head are dealt out by it: slices of one length for
-// all requests, the shortest of which there are not too many.  item: of which request a slice is, which one, how many the request has and where
-// they begin (x -1: there are fewer slices); first: where a request's slices begin, and how many.  One warp, 32 requests at a time.
+// Where only the device knows the lengths of a step (it was captured), and where lengths are so uneven that a place for every request's every
+// slice would be mostly empty, the slices are dealt out by it: of one length for all requests, the shortest with which all run at once, or
+// (slice_tiles) an even share of all tiles.  item: of which request a slice is, which one, how many the request has and where they
+// begin (x -1: there are fewer slices); first: where a request's slices begin, and how many.  One warp, 32 requests at a time.
+// Tiles of a slice, given all tiles of a step and `count(per)`, the slices that its requests have then: the shortest with which no more than
+// `slots` slices are made, and so run at once.  Many short requests make that many slices by themselves, and a long one beside them would stay in
+// few or one (one request at 65,536 keys beside 79 at 500: 512 tiles in a row): where it is more than twice an even share the share it is, and
+// slices run after one another.  count is at most slots + requests, and at most slots where requests are no more than half of that.
+#pragma nv_exec_check_disable      // (count is a lambda of the host's or of the device's)
+template <typename Int, typename Count>
+__host__ __device__ __forceinline__ Int slice_tiles(Int all, Int slots, Count count) {
+    const Int even = all > 0 ? (all - 1) / slots + 1 : 1;
+    if (const Int n = count(2 * even); n > slots) return n == count(all) ? 2 * even : even;      // (the same: none is longer than that)
+    Int lo = even, hi = 2 * even;
+    while (lo < hi) {
+        const Int mid = lo + (hi - lo) / 2;
+        if (count(mid) <= slots) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
 struct Dealt { int4* item; int2* first; };
 __host__ __device__ __forceinline__ Dealt dealt_at(int* at, int slices) { return {(int4*)at, (int2*)(at + 4 * (size_t)slices)}; }
 __global__ void __launch_bounds__(32)
@@ -407,14 +425,11 @@ deal_kernel(Params p) {
     int all = mine;
     for (int r = lane + 32; r < p.requests; r += 32) all += tiles_of(r);
     all = __reduce_add_sync(0xffffffffu, all);
-    // between the length that fills all slices and the one with which one slice more a request fits, too (the host: slices > requests)
-    int per = max((all - 1) / p.slices + 1, 1);
-    for (int hi = max((all - 1) / (p.slices - p.requests) + 1, 1); per < hi;) {
-        const int mid = (per + hi) >> 1;
-        int n = (mine + mid - 1) / mid;
-        for (int r = lane + 32; r < p.requests; r += 32) n += (tiles_of(r) + mid - 1) / mid;
-        if (__reduce_add_sync(0xffffffffu, n) <= p.slices) hi = mid; else per = mid + 1;
-    }
+    const int per = slice_tiles(all, p.slots, [&](int per) {
+        int n = (mine + per - 1) / per;
+        for (int r = lane + 32; r < p.requests; r += 32) n += (tiles_of(r) + per - 1) / per;
+        return __reduce_add_sync(0xffffffffu, n);
+    });
     int before = 0;
     for (int r0 = 0; r0 < p.requests; r0 += 32) {
         const int n = ((r0 ? tiles_of(r0 + lane) : mine) + per - 1) / per;
@@ -460,10 +475,11 @@ __global__ void __launch_bounds__(THREADS, FEW_BLOCKS<NB>)
 few_kernel(Params p) {
     BW_PDL_TRIGGER();
     extern __shared__ __align__(16) uint8_t smem[];
-    const int g = blockIdx.y;
+    // (dealt slices: a slice's kv heads one after the other, so that places left over come last)
+    const int g = p.shared ? blockIdx.x % p.nkv : blockIdx.y, place = p.shared ? blockIdx.x / p.nkv : blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     BW_PDL_WAIT();
-    const int4 item = p.shared ? dealt_at(p.dealt, p.slices).item[blockIdx.x] : make_int4(blockIdx.z, blockIdx.x, p.slices, 0);
+    const int4 item = p.shared ? dealt_at(p.dealt, p.slices).item[place] : make_int4(blockIdx.z, blockIdx.x, p.slices, 0);
     const int r = item.x, slice = item.y;
     if (r < 0) return;
     const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
@@ -548,7 +564,7 @@ few_kernel(Params p) {
             *reinterpret_cast<float4*>(os + row * JOIN_LD + c) = acc;
             if (c == 0) { ml[2 * row] = M; ml[2 * row + 1] = L; }
         } else {
-            const size_t at = (p.shared ? (size_t)blockIdx.x * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
+            const size_t at = (p.shared ? (size_t)place * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices + slice) * 16 + row;
             *reinterpret_cast<float4*>(p.part_o + at * HD + c) = acc;
             if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
         }
@@ -582,7 +598,7 @@ few_kernel(Params p) {
     cluster_sync();      // a block's shared memory stays until it has been read
 }
 
-// Joins the slices of every request that has more than one: a block per (row, kv head, request), groups of HD / 4 threads that take every
+// Joins the slices of every request that has more than one: blocks for the rows of a (kv head, request), groups of HD / 4 threads that take every
 // so many-th slice, then the groups' sums in order: the same sum whatever ran beside it.
 constexpr int QUADS = HD / 4;
 constexpr int JOIN_GROUPS = 256 / QUADS;
@@ -590,47 +606,51 @@ __global__ void __launch_bounds__(256)
 join_kernel(Params p) {
     BW_PDL_TRIGGER();
     BW_PDL_WAIT();
-    const int row = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
-    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
-    if (n_tok <= 0 || n_rows > 16 || row >= n_rows) return;
-    const int q_pos0 = p.q_start[r];
+    const int g = blockIdx.y, r = blockIdx.z;
     const int2 mine = p.shared ? dealt_at(p.dealt, p.slices).first[r] : make_int2(0, p.slices);
+    if (mine.y <= 1) return;        // (of many requests most have one slice)
+    const int tok = p.cu_q[r], n_tok = p.cu_q[r + 1] - tok, n_rows = n_tok * p.G;
+    if (n_tok <= 0 || n_rows > 16) return;
+    const int q_pos0 = p.q_start[r];
     const int live = walk_of(p, q_pos0, q_pos0 + n_tok - 1, mine.y).live;
     if (live <= 1) return;
     __shared__ float4 red[JOIN_GROUPS][QUADS];
     __shared__ float red_l[JOIN_GROUPS];
     __shared__ float scratch[32];
-    // from one slice's row to the next one's
-    const size_t step = p.shared ? (size_t)p.nkv * 16 : 16;
-    const size_t base = (p.shared ? (size_t)mine.x * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices) * 16 + row;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-    float M = -INFINITY;
-    for (int i = threadIdx.x; i < live; i += 256) M = fmaxf(M, ml[base + i * step].x);
-    M = bw::block_max(M, scratch);
-    const int group = threadIdx.x / QUADS, quad = threadIdx.x - group * QUADS;
-    if (group < JOIN_GROUPS) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float L = 0.f;
+    for (int row = blockIdx.x; row < n_rows; row += gridDim.x) {
+        // from one slice's row to the next one's
+        const size_t step = p.shared ? (size_t)p.nkv * 16 : 16;
+        const size_t base = (p.shared ? (size_t)mine.x * p.nkv + g : ((size_t)r * p.nkv + g) * p.slices) * 16 + row;
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+        float M = -INFINITY;
+        for (int i = threadIdx.x; i < live; i += 256) M = fmaxf(M, ml[base + i * step].x);
+        M = bw::block_max(M, scratch);
+        const int group = threadIdx.x / QUADS, quad = threadIdx.x - group * QUADS;
+        if (group < JOIN_GROUPS) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
 #pragma unroll 4
-        for (int i = group; i < live; i += JOIN_GROUPS) {
-            const float2 x = ml[base + i * step];
-            const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + i * step) * HD)[quad];
-            add_part(acc, L, v, x.x, x.y, M);
+            for (int i = group; i < live; i += JOIN_GROUPS) {
+                const float2 x = ml[base + i * step];
+                const float4 v = reinterpret_cast<const float4*>(p.part_o + (base + i * step) * HD)[quad];
+                add_part(acc, L, v, x.x, x.y, M);
+            }
+            red[group][quad] = acc;
+            if (quad == 0) red_l[group] = L;
         }
-        red[group][quad] = acc;
-        if (quad == 0) red_l[group] = L;
-    }
-    __syncthreads();
-    if (threadIdx.x < QUADS) {
-        float4 acc = red[0][threadIdx.x];
-        float L = red_l[0];
-        for (int i = 1; i < JOIN_GROUPS; ++i) {
-            const float4 v = red[i][threadIdx.x];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-            L += red_l[i];
+        __syncthreads();
+        if (threadIdx.x < QUADS) {
+            float4 acc = red[0][threadIdx.x];
+            float L = red_l[0];
+            for (int i = 1; i < JOIN_GROUPS; ++i) {
+                const float4 v = red[i][threadIdx.x];
+                acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+                L += red_l[i];
+            }
+            const int t = row / p.G, head = g * p.G + row - t * p.G;
+            write_row(p, (size_t)(tok + t), head, 4 * threadIdx.x, acc, L + sink_term(p, head, M));
         }
-        const int t = row / p.G, head = g * p.G + row - t * p.G;
-        write_row(p, (size_t)(tok + t), head, 4 * threadIdx.x, acc, L + sink_term(p, head, M));
+        __syncthreads();
     }
 }
 
@@ -663,9 +683,11 @@ static int clusters_at_once(int size) {
 // and a trip through memory: about a tile's time) serves more slices, and requests of many lengths, whose clusters would be half empty:
 // us with clusters and without, a token at 701 keys 6.2 and 7.6, 2 at 2,000 8.9 and 9.5, 4 at 4,000 15.9 and 14.0, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
 // them 63.5 and 55.8, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 11.8.
-// A step whose lengths only the device will know, and may be long, gets the slices that run at once, to share by what the lengths are then.
+// A step whose lengths only the device will know, and may be long, gets the slices that run at once, to share by what the lengths are then; and so does
+// one whose longest request has so many slices that a place for as many of each would be far more than there are (scratch, and blocks that
+// leave at once): 217 MB of scratch for one request at 131,072 keys and 50 short ones on 1 kv head of 128 are 5 so.
 constexpr int CLUSTER_EXTRA = 1;
-struct Plan { int per, slices, cluster, shared; };
+struct Plan { int per, slices, cluster, shared, slots; };
 static Plan plan_slices(const int* q_len, const int* q_start, int requests, int G, int nkv, int window, int chunk, int bound, bool whole) {
     auto tiles_of = [&](int r) -> long long {
         if (q_len[r] <= 0 || (long long)q_len[r] * G > 16) return 0;
@@ -680,25 +702,27 @@ static Plan plan_slices(const int* q_len, const int* q_start, int requests, int 
         }
         return n;
     };
-    long long most = 0, least = 0x7fffffff, few = 0;
+    long long most = 0, least = 0x7fffffff, few = 0, all = 0;
     bool wide = false;                        // more than eight rows: the larger kernel, of which fewer run at once
     for (int r = 0; r < requests; ++r) {
         const long long n = tiles_of(r);
         if (n == 0) continue;
         ++few;
+        all += n;
         wide |= q_len[r] * G > 8;
         if (n > most) most = n;
         if (n < least) least = n;
     }
-    if (most == 0) return {1, 0, 0, 0};
+    if (most == 0) return {1, 0, 0, 0, 0};
     const long long room = (long long)(wide ? FEW_BLOCKS<2> : FEW_BLOCKS<1>) * bw::num_sms();          // blocks that run at once
-    long long lo = 1, hi = most;
-    while (lo < hi) {
-        const long long mid = (lo + hi) / 2;
-        long long blocks = 0;
-        for (int r = 0; r < requests; ++r) blocks += (tiles_of(r) + mid - 1) / mid;
-        if (blocks * nkv <= room) hi = mid; else lo = mid + 1;
-    }
+    const long long slots = room > nkv ? room / nkv : 1;
+    auto count = [&](long long per) {
+        long long n = 0;
+        for (int r = 0; r < requests; ++r) n += (tiles_of(r) + per - 1) / per;
+        return n;
+    };
+    long long lo = slice_tiles(all, slots, count);
+    if (lo > most) lo = most;
     const long long slices = (most + lo - 1) / lo;
     if (slices > 1 && 4 * least >= 3 * most && (bound <= 0 || few == 1 || most <= MOST_CLUSTER)) {
         for (int size = slices < MOST_CLUSTER ? (int)slices : MOST_CLUSTER; size > 1; --size) {
@@ -706,12 +730,17 @@ static Plan plan_slices(const int* q_len, const int* q_start, int requests, int 
             if (per > lo + CLUSTER_EXTRA) break;
             const int at_once = wide ? (whole ? clusters_at_once<2, true>(size) : clusters_at_once<2, false>(size))
                                      : (whole ? clusters_at_once<1, true>(size) : clusters_at_once<1, false>(size));
-            if (few * nkv <= at_once) return {(int)per, (int)((most + per - 1) / per), 1, 0};
+            if (few * nkv <= at_once) return {(int)per, (int)((most + per - 1) / per), 1, 0, 0};
         }
     }
-    if (bound > 0 && slices > 1 && room / nkv > requests && most * requests <= 0x7fffffffll)
-        return {1, (int)(room / nkv), 0, requests > 1 ? (int)most : 0};
-    return {(int)lo, (int)slices, 0, 0};
+    if (bound > 0 && requests == 1 && slices > 1) return {1, (int)slots, 0, 0, 0};
+    // (what slice_tiles says of its count.  Captured requests of which as many run at once as there are stay whole while none is long)
+    const long long shared = 2LL * requests <= slots ? slots : slots + requests;
+    const bool captured = bound > 0 && requests > 1 && (slices > 1 || most > MOST_CLUSTER), 
+               uneven = bound <= 0 && requests * slices > 4 * count(lo) && requests * slices * nkv > 8 * room;
+    if ((captured || uneven) && most * requests <= 0x1fffffffll && shared * nkv <= 0x7fffffffll)
+        return {1, (int)shared, 0, (int)most, (int)slots};
+    return {(int)lo, (int)slices, 0, 0, 0};
 }
 
 template <int NB, bool WHOLE>
@@ -758,7 +787,7 @@ BW_EXPORT int bw_attention_q8_deal(const int* cu_q, const int* q_start, const in
     if ((uintptr_t)dealt & 15) return BW_ERR_BAD_ARG;
     Params p{};
     p.cu_q = cu_q; p.q_start = q_start; p.window = window; p.chunk = chunk; p.requests = requests; p.G = nh / nkv;
-    p.slices = plan.slices; p.shared = plan.shared; p.dealt = dealt;
+    p.slices = plan.slices; p.shared = plan.shared; p.dealt = dealt; p.slots = plan.slots;
     deal(p, (cudaStream_t)stream);
     BW_LAUNCH_CHECK();
     return 0;
@@ -788,7 +817,7 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (deal_here) dealt = reinterpret_cast<int*>(room + rows * (HD + 2));       // (rows is a multiple of 16)
     const int slices = plan.slices;
     Params p{(const bf16*)q, (bf16*)out, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, cu_q, q_start, kv_len, table, sink, room, room + rows * HD,
-             max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, plan.shared, dealt, scale * LOG2E};
+             max_blocks, nh, nkv, G, page_size, num_pages, window, chunk, requests, plan.per, slices, plan.cluster, plan.shared, dealt, plan.slots, scale * LOG2E};
     cudaStream_t s = (cudaStream_t)stream;
     int most_rows = 0;
     bool few1 = false, few2 = false;
@@ -800,7 +829,7 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     }
     if (!most_rows) return 0;
     if (slices < 1) return BW_ERR_BAD_ARG;
-    const dim3 grid((unsigned)slices, (unsigned)nkv, plan.shared ? 1u : (unsigned)requests);
+    const dim3 grid = plan.shared ? dim3((unsigned)slices * (unsigned)nkv) : dim3((unsigned)slices, (unsigned)nkv, (unsigned)requests);
     if (deal_here) {
         deal(p, s);
         BW_LAUNCH_CHECK();
@@ -808,7 +837,11 @@ BW_EXPORT int bw_attention_q8(const void* q, const void* k, const void* v, const
     if (few1) if (const int e = whole ? launch_few<1, true>(p, grid, s) : launch_few<1, false>(p, grid, s)) return e;
     if (few2) if (const int e = whole ? launch_few<2, true>(p, grid, s) : launch_few<2, false>(p, grid, s)) return e;
     if (slices > 1 && !plan.cluster) {
-        bw::launch(join_kernel, dim3((unsigned)most_rows, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
+        // (a block for every row, for few requests; for many, whose rows have mostly nothing to join, about 512 blocks: 64 at 2,048 keys, captured,
+        // 54.4 us with a block each and 51.2 so)
+        long long cols = 512 / ((long long)nkv * requests);
+        cols = cols < 1 ? 1 : cols > most_rows ? most_rows : cols;
+        bw::launch(join_kernel, dim3((unsigned)cols, (unsigned)nkv, (unsigned)requests), dim3(256), 0, s, p);
         BW_LAUNCH_CHECK();
     }
     return 0;

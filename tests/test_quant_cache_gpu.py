@@ -592,3 +592,38 @@ def test_after_a_wait_gave_up_rows_are_no_numbers():
         assert torch.isnan(got[:200]).all() and torch.isnan(got[201:]).all() and torch.equal(got[200], want[200])
     assert ops.attention_q8_status() == 39 and ops.attention_q8_status() == 0
     assert torch.equal(ops.quant_attention(q, pages, b, b.block_tables[0], 4, 0.125), want)
+
+
+def test_a_long_request_beside_two_hundred_short_ones():
+    """Slices dealt out on the device for a call of its own too, more of them than run at once: at the call's lengths, repeated on two streams, and
+    replayed at others (all short, the long one elsewhere, one longer than the bound)."""
+    lens = [21 + i % 7 for i in range(200)]
+    lens[37], lens[150] = 9001, 700
+    c = Case([(1, n - 1, n) for n in lens], 4, 64, 16, seed=12).fill()
+    got = c.check_attention(8)
+    b, pages = c.batch(), c.pages()
+    q = torch.randn(c.T, 8 * 64, generator=c.gen).to(torch.bfloat16).cuda()
+    want = ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125))
+    torch.cuda.synchronize()
+    assert got.shape[0] == 200 and all(torch.equal(o, want) for o in outs)
+    b = c.batch(bound=4096)
+    ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dealt = ops.quant_attention_deal(b, 8, 4, 64, 16)
+        out = ops.quant_attention(q, pages, b, b.block_tables[0], 8, 0.125, dealt=dealt)
+    assert dealt is not None
+    for long37, long150 in ((9001, 700), (20, 20), (3, 699), (5000, 1)):
+        ends = [min(n, 20) for n in lens]
+        ends[37], ends[150] = long37, long150
+        starts = [n - 1 for n in ends]
+        b.q_start.copy_(torch.tensor(starts)); b.kv_len.copy_(torch.tensor(ends))
+        out.fill_(float("nan"))
+        graph.replay()
+        e = attention(q.cpu().view(200, 8, 64), c.k, c.v, c.k_scale, c.v_scale, c.cu, starts, ends, c.table, 0.125)
+        assert ((out.cpu().double().view_as(e.out) - e.out).abs() <= attention_bound(e, 64)).all()

@@ -259,3 +259,36 @@ def test_more_rows_of_queries_than_32_bits_count_are_refused(lens):
     assert room(ints(*lens), ints(*starts), len(lens), 16, 16, 16, 0, 0) == -2
     few = [n >> 4 for n in lens]
     assert room(ints(*few), ints(*starts), len(lens), 16, 16, 16, 0, 0) > 0
+
+
+def scratch_of(lens, nkv, nh, bound=0):
+    """Floats of scratch that a call asks for (nothing is launched: it has none), for requests of one token each at these lengths."""
+    attend = entry("attention_q8", "bw_attention_q8")
+    p, ll, at = ctypes.c_void_p, ctypes.c_longlong, [ctypes.c_void_p(1 << 20)] * 9
+    need, R = ll(0), len(lens)
+    code = attend(*at, p(1 << 20), 9, ints(*[1] * R), ints(*[n - 1 for n in lens]), R, nh, nkv, 16, 1 << 10, 0, 0, bound, ctypes.c_float(0.1), None, None,
+                  ll(0), ctypes.byref(need), None, None)
+    assert code == -11
+    return need.value
+
+
+def test_a_long_request_beside_many_short_ones_is_divided():
+    """However many requests there are, one that is far longer than its share of the GPU is several blocks' work (and is joined from scratch): at the
+    lengths of the call, and in a step that is captured for lengths to come."""
+    deal = entry("attention_q8", "bw_attention_q8_deal")
+    for count in (40, 100, 200, 700):
+        assert scratch_of([131072] + [500] * (count - 1), 8, 32) > 0
+        need = ctypes.c_longlong(0)
+        assert deal(None, None, ints(*[1] * count), ints(*[0] * count), count, 32, 8, 16, 0, 0, 131072, None, ctypes.byref(need), None) == 0
+        assert need.value >= 4 * count
+
+
+def test_scratch_is_a_matter_of_the_slices_that_there_are():
+    """Not of as many for each request as the longest has: a slice is 16 rows of 64 channels and two numbers, and as many as four times the blocks
+    of a GPU (at most 32 an SM) beside one a request and kv head are room enough for any step."""
+    for nkv, nh in ((1, 8), (2, 8), (8, 32)):
+        for count in (20, 51, 256):
+            for longest in (30000, 131072, 1000000):
+                for lens in ([longest] + [300] * (count - 1), [300] * (count - 1) + [longest], [longest >> (i % 12) for i in range(count)]):
+                    need = scratch_of(lens, nkv, nh)
+                    assert need <= 16 * 66 * 4 * (148 * 32 + count * nkv) + 6 * (148 * 32 + count)
