@@ -192,15 +192,18 @@ class Engine:
 
     def cached_kv(self, rid, layer: int, start: int = 0, stop: Optional[int] = None):
         """The keys (as attention reads them: rotated) and values that the request's cache holds for positions ``start`` to
-        ``stop`` (None: all) of a layer that owns pages: two tensors [positions, kv heads, head size] in the model's dtype; of a cache in 8
-        bits the numbers times their scales.  Zeros at positions whose pages a window has given back.  A token that a step
+        ``stop`` (None: all) of a layer that owns pages (beside a state or not): two tensors [positions, kv heads, head size] in the
+        model's dtype; of a cache in 8 bits the numbers times their scales.  The head size is the pages': with the zeros of a mixer that
+        pads its heads; one whose values are a part of its keys' rows has the rows twice.  Zeros at positions whose pages a window has given back.  A token that a step
         prepared ahead has reserved counts from that step's launch on."""
         from ..kernels import ops
         if not self.cache.has(rid):
             raise EngineError(f"request {rid!r} is not live")
-        view = self.cache.views[layer] if 0 <= layer < len(self.cache.views) else None
-        if not isinstance(view, PagedKVView):
-            raise EngineError(f"layer {layer} owns no pages of keys and values")
+        views = self.cache.views[layer] if 0 <= layer < len(self.cache.views) else None
+        pages = [v for v in (views if isinstance(views, tuple) else (views,)) if isinstance(v, PagedKVView)]
+        if len(pages) != 1:
+            raise EngineError(f"layer {layer} owns " + ("no pages of keys and values" if not pages else "pages for more than one mixer"))
+        view = pages[0]
         n = self.cache.written(rid)
         stop = n if stop is None else stop
         if not 0 <= start <= stop <= n:

@@ -19,7 +19,7 @@ from blackwellllm_b200.engine.engine import Engine, EngineError, EngineOptions, 
 from blackwellllm_b200.kernels import ops
 from blackwellllm_b200.kernels.build import load_library
 from blackwellllm_b200.models.decoder import DecoderModel
-from blackwellllm_b200.parts.base import BuildContext, PagedKVRequest
+from blackwellllm_b200.parts.base import BuildContext, FixedStateRequest, PagedKVRequest
 from blackwellllm_b200.sampling.params import SamplingParams
 
 CPU = torch.device("cpu")
@@ -292,3 +292,27 @@ def test_scratch_is_a_matter_of_the_slices_that_there_are():
                 for lens in ([longest] + [300] * (count - 1), [300] * (count - 1) + [longest], [longest >> (i % 12) for i in range(count)]):
                     need = scratch_of(lens, nkv, nh)
                     assert need <= 16 * 66 * 4 * (148 * 32 + count * nkv) + 6 * (148 * 32 + count)
+
+
+def test_cached_rows_of_a_layer_that_owns_a_state_beside_its_pages(monkeypatch):
+    class PagesAndState(PagesOnly):
+        def cache_requests(self):
+            pages, state = PagedKVRequest(2, 16, None), FixedStateRequest((3,), torch.float32)
+            return [(pages, state), (state, pages), (state,), (pages, pages)]
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    cfg = parse_config(tiny.TINY_LLAMA)
+    eng = Engine(cfg, PagesAndState(cfg.vocab_size), EngineOptions(dtype="float32", page_size=8, num_pages=12, max_requests=3,
+                                                                   cuda_graphs=False, device="cpu"))
+    eng.step([StepEntry("a", [1] * 11, [])])
+    table = eng.cache.block_table("a", 0)
+    for layer, place in ((0, 0), (1, 1)):
+        v = eng.cache.views[layer][place]
+        v.k_pages.copy_(torch.randn(v.k_pages.shape))
+        k, val = eng.cached_kv("a", layer)
+        assert k.shape == val.shape == (11, 2, 16)
+        assert all(torch.equal(k[p], v.k_pages[table[p // 8], :, p % 8]) for p in range(11)) and not val.any()
+    with pytest.raises(EngineError, match="owns no pages"):
+        eng.cached_kv("a", 2)
+    with pytest.raises(EngineError, match="more than one"):
+        eng.cached_kv("a", 3)
