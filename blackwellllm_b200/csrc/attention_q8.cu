@@ -599,7 +599,8 @@ few_kernel(Params p) {
 }
 
 // Joins the slices of every request that has more than one: blocks for the rows of a (kv head, request), groups of HD / 4 threads that take every
-// so many-th slice, then the groups' sums in order: the same sum whatever ran beside it.
+// so many-th slice, then the groups' sums in order: the same sum in every run of a step.  (How long the slices are follows from the lengths of all the
+// step's requests: beside others a request's last bits may differ.)
 constexpr int QUADS = HD / 4;
 constexpr int JOIN_GROUPS = 256 / QUADS;
 __global__ void __launch_bounds__(256)

@@ -5,7 +5,8 @@
 //   log p_i = (x_i - m) - log1p(z),   entropy = log1p(z) - w / (1 + z).
 // The largest element's own term, 1, is left out of z so that a sharp distribution (z far below 1) keeps its bits.  Two such triples
 // of parts of a row join exactly as one element joins a part: the smaller maximum's element becomes an ordinary term.  All sums are float32,
-// in an order that depends on V alone (threads take every so many-th four elements; then trees).
+// in an order that follows from V and the number of blocks that share a row (threads take every so many-th four elements; then trees).  That number
+// goes by the call's rows and the GPU's SMs: a row by itself and the same row among hundreds may differ in last bits.
 //
 // The `top` (at most 32) most probable tokens, ties to the lowest id: a token is a 64-bit key, the logit's bits made ordered above, the
 // inverted id below; no two are equal.  Every thread knows the best key of its own elements from the pass.  The top-th best of the warps' best one,

@@ -881,7 +881,8 @@ TOKEN_LOG_PROBS_MAX_TOP = 32
 def token_log_probs(logits: torch.Tensor, target: torch.Tensor, top: int = 0) -> TokenLogProbs:
     """Log probability, rank, entropy and the ``top`` (at most 32) most probable tokens of every row of float32 ``logits`` [R, V] (rows may be
     apart), in one pass over them.  ``target`` int32 [R]; one outside [0, V) stands for none: log probability NaN, rank -1.  A row without a
-    distribution (a NaN or +infinity among its logits, or nothing but -infinity) gets NaN, and -1 for rank and ids."""
+    distribution (a NaN or +infinity among its logits, or nothing but -infinity) gets NaN, and -1 for rank and ids.  The sums' order, and so last
+    bits, goes by the number of rows (ids and ranks do not)."""
     if _pending is not None:
         _dev(logits, "logits", contiguous=False)
     got = _call("token_log_probs", _entry("token_probs", "bw_token_probs"), logits, target, top, TOKEN_LOG_PROBS_MAX_TOP) if logits.is_cuda else None
