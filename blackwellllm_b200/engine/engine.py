@@ -99,6 +99,8 @@ class Engine:
         self._graph_width = -(-longest // options.page_size)
         self.steps_run = 0
         self.tokens_run = 0
+        self._quant = any(g.request.quantized for g in self.cache.groups)
+        self._unchecked = False    # portions of prompts have run since check_portions
         self.native_steps = 0      # steps that went through the C entry point (csrc/decode_step.h)
 
     # ------------------------------------------------------------------ construction
@@ -516,6 +518,7 @@ class Engine:
                         batch.token_ids.copy_(token_source)
                     logits = self.model.forward(batch, self.cache.views)
                     T = batch.T
+                    self._unchecked |= self._quant and T > batch.R
         except BaseException:
             self._roll_back()
             raise
@@ -523,6 +526,18 @@ class Engine:
         self.steps_run += 1
         self.tokens_run += T
         return logits
+
+    def check_portions(self) -> None:
+        """Raises EngineError if the attention of a prompt's portion over an 8-bit cache gave up a wait in a step since the last call: the
+        rows of those steps are no results.  For where a step's tokens have been read back (it waits for the device); nothing to
+        look at costs nothing."""
+        if not self._unchecked:
+            return
+        self._unchecked = False
+        from ..kernels import ops
+        status = ops.attention_q8_status()
+        if status:
+            raise EngineError(f"attention over the 8-bit cache gave up a wait (status {status}): the prompts of this step were not computed")
 
     def _roll_back(self) -> None:
         """Puts every request of a failed step back to its length before the step; a request

@@ -228,7 +228,17 @@ class BlackwellEngine:
             logits = self.engine.step([StepEntry(rid, ids[at:at + n], [n - 1] if last else [])])
             at += n
         self._last_logits = {seq_id: logits[0]}
-        return self._pick(logits, [seq_id], temperature, top_p)[0]
+        token = self._pick(logits, [seq_id], temperature, top_p)[0]
+        try:
+            self.engine.check_portions()
+        except EngineError:
+            self._last_logits = {}
+            try:
+                self.engine.cache.truncate(rid, start_pos)
+            except ValueError:      # (into pages that a window has given back, or a state: nothing of it can stay)
+                self.release_sequence(seq_id)
+            raise
+        return token
 
     def forward_eval(self, token_id: int, pos: int, target_token_id: int, seq_id: int = 0) -> float:
         """Feeds ``token_id`` at ``pos`` and returns ln P(target_token_id) of the next token,
@@ -269,6 +279,7 @@ class BlackwellEngine:
                 given = ids[at + 1:at + 1 + n]
                 target = torch.tensor(given, dtype=torch.int32, device=logits.device)
                 out += _listed(ops.token_log_probs(logits, target, min(top, self.vocab_size)), given, range(n))
+                self.engine.check_portions()
                 at += n
         finally:
             if self.engine.cache.has(rid):
@@ -404,10 +415,14 @@ class BlackwellEngine:
         if picked is not None:
             sampled = {r.rid: t for r, t in zip(samplers, picked.tolist())}     # waits for the step
         try:
+            if picked is not None:
+                self.engine.check_portions()
             done = self.scheduler.commit(plan, sampled)
-        except BaseException:
+        except BaseException as e:
             if nxt is not None:
                 self.engine.cancel_prepared(nxt[1])
+            if isinstance(e, EngineError):
+                self.scheduler.start_over()     # (what the step left in the cache is no result)
             raise
         if nxt is not None:
             if done or self.scheduler.waiting:

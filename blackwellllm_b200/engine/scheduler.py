@@ -167,6 +167,11 @@ class Scheduler:
         self.stats.preemptions += 1
         self.waiting.appendleft(req)
 
+    def start_over(self) -> None:
+        """Every running request waits again, in the order of admission, and is computed from its first token."""
+        for r in sorted(self.running, key=lambda r: r.admitted_at, reverse=True):
+            self._preempt(r)
+
     def plan(self) -> StepPlan:
         """The next step.  If nothing can run although requests are running (every one of them is
         in its prompt and needs a page, and none is free), the most recently admitted one is

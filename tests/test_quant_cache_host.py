@@ -316,3 +316,71 @@ def test_cached_rows_of_a_layer_that_owns_a_state_beside_its_pages(monkeypatch):
         eng.cached_kv("a", 2)
     with pytest.raises(EngineError, match="more than one"):
         eng.cached_kv("a", 3)
+
+
+class Rule(PagesOnly):
+    """After a token t at position p comes (t + p) % vocab, over a cache in 8 bits that nobody writes."""
+
+    def cache_requests(self):
+        return [PagedKVRequest(2, 16, None, quantized=True)]
+
+    def forward(self, batch, views):
+        out = torch.zeros((len(batch.logit_rows), self.vocab), dtype=torch.float32)
+        for i, t in enumerate(batch.logit_rows.tolist()):
+            out[i, (int(batch.token_ids[t]) + int(batch.positions[t])) % self.vocab] = 1.0
+        return out
+
+
+def test_a_prompt_whose_attention_gave_up_is_an_error_and_computed_again(monkeypatch):
+    """The status is looked at with the tokens of a step that had a portion of a prompt, never for steps of single tokens; the requests of such
+    a step wait again, and what they generate then is what they would have."""
+    import dataclasses
+
+    from blackwellllm_b200 import BlackwellEngine, InferenceConfig
+    from blackwellllm_b200.engine import llm as llm_module
+
+    class Best:
+        def __init__(self, device):
+            pass
+
+        def sample_async(self, logits, *a):
+            return logits.argmax(dim=1)
+
+        def sample(self, logits, *a):
+            return logits.argmax(dim=1).tolist()
+
+    def from_config(raw, seed=0, std=0.02, options=None):
+        cfg = parse_config(raw)
+        return Engine(cfg, Rule(cfg.vocab_size), dataclasses.replace(options, device="cpu", cuda_graphs=False))
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(llm_module.Engine, "from_config", staticmethod(from_config))
+    monkeypatch.setattr(llm_module, "Sampler", Best)
+    answers, asked = [], []
+    monkeypatch.setattr(ops, "attention_q8_status", lambda: asked.append(1) or (answers.pop(0) if answers else 0))
+    llm = BlackwellEngine(None, InferenceConfig(max_context_length=96, max_batch_size=3), config=tiny.CONFIGS["llama"][0], page_size=8, max_batch_tokens=16)
+    prompts = [[3, 4, 5], list(range(10, 40)), [9, 8]]
+    params = SamplingParams(temperature=0.0, max_new_tokens=5, ignore_eos=True)
+    want = [r.token_ids for r in llm.generate(prompts, params)]
+    portions = len(asked)
+    assert 0 < portions < 6
+    for bad in range(portions):
+        answers[:] = [0] * bad + [39]
+        rids = [llm.add_request(p, params) for p in prompts]
+        done, failed = {}, 0
+        while llm.scheduler.has_work():
+            try:
+                done.update((r.request_id, r.token_ids) for r in llm.step())
+            except EngineError as e:
+                assert "gave up" in str(e)
+                failed += 1
+        assert failed == 1 and [done[r] for r in rids] == want
+        llm.engine.cache.check_invariants()
+    asked.clear()
+    first = llm.prefill([1, 2, 3], 0, 0.0, 1.0)
+    assert len(asked) == 1 and llm.forward(first, 3, 0.0, 1.0) == (first + 3) % llm.vocab_size and len(asked) == 1
+    answers[:] = [39]
+    with pytest.raises(EngineError, match="gave up"):
+        llm.prefill([4, 5, 6], 4, 0.0, 1.0)
+    assert llm.engine.cache.length(("seq", 0)) == 4 and llm.prefill([4, 5, 6], 4, 0.0, 1.0) == (6 + 6) % llm.vocab_size
+    assert llm.prefill([1, 2, 3], 0, 0.0, 1.0) == first

@@ -296,3 +296,24 @@ def test_half_the_bytes_hold_more_pages(folders):
     quant = Engine.from_config(raw, options=EngineOptions(kv_dtype="int8", **kw)).cache.groups[0].num_pages
     hd = raw["head_dim"]
     assert quant / plain == pytest.approx(2 * hd / (hd + 4), rel=0.1)
+
+
+def test_a_prompt_whose_attention_gave_up_is_an_error(folders):
+    """The status set as a wait that gives up sets it: the step's rows are no numbers and its caller hears of it, in every call that takes
+    prompts; afterwards all is as before."""
+    from blackwellllm_b200 import EngineError, SamplingParams
+    from blackwellllm_b200.kernels.build import load_library
+    raw, _, page = tiny.CONFIGS["llama"]
+    llm = make(folders[("llama", "bfloat16")], page_size=page, kv_dtype="int8")
+    ids, params = tiny.prompt(50, raw["vocab_size"], 4), SamplingParams(temperature=0.0, max_new_tokens=6, ignore_eos=True)
+    want, scored = llm.generate(ids, params)[0].token_ids, llm.score(ids)
+    hd = llm.engine.cache.groups[0].request.head_dim
+    give_up = load_library("attention_q8_tc", {"HEAD_DIM": hd}).bw_attention_q8_tc_give_up
+    for call in (lambda: llm.generate(ids, params), lambda: llm.prefill(ids, 0, 0.0, 1.0), lambda: llm.score(ids)):
+        assert give_up(39) == 0
+        with pytest.raises(EngineError, match="gave up"):
+            call()
+    while llm.scheduler.has_work():
+        for r in llm.step():
+            assert r.token_ids == want
+    assert llm.score(ids) == scored and llm.generate(ids, params)[0].token_ids == want
