@@ -355,8 +355,8 @@ struct Feed {
 // All (at most 16) rows of one (request, kv head) over one slice of the keys: the block's warps take sixteen keys each of every 64, each
 // with a ring of its own, and are joined at the end.  How many slices a request has follows from its length on the device, so the same launch
 // serves a captured step whatever the lengths become.
-// Bound by memory where there is much of it: 64 requests at 2,048 keys (8 kv heads of 128) 48.5 us, 5.7 TB/s of 6.5 that a copy has.  8 at 8,192
-// take 29.2, 4.7 TB/s: a block's start and the joining are a third of its eight tiles' time.  A token at 701 keys takes 6.3, the launch and
+// Bound by memory where there is much of it: 64 requests at 2,048 keys (8 kv heads of 128) 49.3 us, 5.6 TB/s of 6.5 that a copy has.  8 at 8,192
+// take 29.6, 4.7 TB/s: a block's start and the joining are a third of its eight tiles' time.  A token at 701 keys takes 6.2, the launch and
 // a chain of trips (lengths, page, keys, the other blocks).
 // (Two stages: other blocks' warps hide what a longer ring would, and there are more of them.  64 requests at 2,048 keys 48 us, with three
 // stages 50, with four 68.)
@@ -682,8 +682,8 @@ static int clusters_at_once(int size) {
 // most of any request (0: there is no such request).
 // Where requests are about equally long, up to eight slices that all run at once are a cluster and join there; a join of its own (a launch,
 // and a trip through memory: about a tile's time) serves more slices, and requests of many lengths, whose clusters would be half empty:
-// us with clusters and without, a token at 701 keys 6.2 and 7.6, 2 at 2,000 8.9 and 9.5, 4 at 4,000 15.9 and 14.0, 8 at 8,192 29.2 and 31.6; 31 at 512 to 4,096 with a prompt's portion beside
-// them 63.5 and 55.8, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 11.8.
+// us with clusters and without, a token at 701 keys 6.2 and 7.8, 2 at 2,000 9.0 and 10.3, 4 at 4,000 16.1 and 14.7, 8 at 8,192 29.6 and 32.5; 31 at 512 to 4,096
+// with a prompt's portion beside them 55.3 and 53.1, 8 at 8,192 with 2 kv heads of 64 (which want 32 slices) 16.1 and 12.0.
 // A step whose lengths only the device will know, and may be long, gets the slices that run at once, to share by what the lengths are then; and so does
 // one whose longest request has so many slices that a place for as many of each would be far more than there are (scratch, and blocks that
 // leave at once): 217 MB of scratch for one request at 131,072 keys and 50 short ones on 1 kv head of 128 are 5 so.

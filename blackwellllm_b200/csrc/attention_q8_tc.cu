@@ -27,7 +27,7 @@
 // all rows of later launches until the status is read, are NaN.
 //
 // 2,048 tokens of 32 heads of 128 on 8 kv heads: 73.5 us, 467 TFLOP/s; 2,048 behind 13,312 (40 heads on 8) 740 us, 812 of 1,652 that a large product
-// has, in bursts.  A step (256 rows, 64 keys) takes about 2,700 cycles, and nothing alone bounds it: the softmax's warps are busy for most of
+// has, in bursts (790 in a stream of calls, whose clock falls).  A step (256 rows, 64 keys) takes about 2,750 cycles, and nothing alone bounds it: the softmax's warps are busy for most of
 // them, the products need 1,500 (N 64 reads as many bytes of Q as it has work for).  Late piece without the exponentials 4 percent less, with
 // keys widened at the cost of values 2, where no reference ever moves 5.  An item costs about five steps beside (its queries come, the first
 // scores, the outputs): of the 74 us a third.

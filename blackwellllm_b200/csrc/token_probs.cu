@@ -364,7 +364,8 @@ BW_EXPORT int bw_token_probs(const float* logits, const int* target, float* log_
     const Args p{logits, target, log_prob, entropy, rank, top_ids, top_log_probs, V, top, (size_t)ld};
     const bool vec = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     // Few rows: as many blocks a row as run at once (two an SM), while each has a few thousand elements.  Many: a block a row; shared rows cost more in
-    // sorting than they even out (1,024 rows of 128,256 with one alternative: 100 us, as two blocks each 103, as four 133).
+    // sorting than they even out (1,024 rows of 128,256 with one alternative, in a graph: 101 us, as two blocks each 103, as four 133; 107 in a
+    // stream of calls).
     const long long sms = bw::num_sms();
     const bool few = R <= 2 * sms;
     int blocks = 1;
